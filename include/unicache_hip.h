@@ -45,6 +45,9 @@ extern "C" {
 #define UC_BF16 0
 #define UC_FP16 1
 #define UC_FP32 2
+/* code types of the 8-bit block-scaled cache (uc_block8_cache) */
+#define UC_INT8 3
+#define UC_E4M3 4
 
 /* return codes */
 #define UC_OK 0
@@ -715,6 +718,126 @@ int64_t uc_kivi_decode_workspace_bytes(int64_t n_items, int bits, int group_size
 int64_t uc_kivi_decode_preferred_workspace_bytes(int64_t n_items, int bits, int group_size, int64_t heads_q,
                                                  int64_t heads_kv, int64_t head_dim, int64_t query_len,
                                                  int64_t max_quantized_tokens, int64_t max_residual_tokens);
+
+/*
+ * The 8-bit block-scaled KV cache of one layer for a batch of S sequences (no
+ * reference counterpart).  A block is block_tokens consecutive tokens of one
+ * KV head; keys and values are held as 8-bit codes with one fp32 scale per
+ * block each, value = code * scale:
+ *   a = max(max |x| of the block, 2^-60 L), L = 127 (int8) or 448 (e4m3),
+ *   scale = a * (1/L), code = round(x * (L/a)), halves to even (fp32 steps).
+ * A block holding an infinity or a NaN gets that as its scale and codes 0, so
+ * all of it reads as NaN.  The last block of a sequence may be partial: it is
+ * quantized from the rows it has, its other codes are 0.  N blocks per
+ * sequence is the capacity.  All tensors are contiguous, 16-byte aligned.
+ */
+typedef struct uc_block8_cache {
+  void *key_code;      /* [S, Hkv, N * block_tokens, D] */
+  void *value_code;    /* [S, Hkv, N, D, block_tokens]: channels outermost in a block */
+  float *key_scale;    /* [S, Hkv, N] */
+  float *value_scale;  /* [S, Hkv, N] */
+  int8_t *key_bounds;  /* [S, Hkv, N, 2, D]: per channel the largest, then the smallest key code of the
+                          block's tokens in steps of a/127, rounded outwards (0 in a block without tokens) */
+  int32_t *lengths;    /* [S] tokens, on the device; read as 0 below 0 and as the capacity above it */
+  int64_t sequences;   /* S */
+  int64_t heads_kv;
+  int64_t head_dim;    /* 64 or 128 */
+  int64_t blocks;      /* N */
+  int32_t block_tokens; /* 32, 64 or 128 */
+  int32_t code_dtype;   /* UC_INT8 or UC_E4M3 */
+} uc_block8_cache;
+
+/*
+ * Quantize the first min(lengths[s], tokens) rows of each sequence of dense
+ * key / value [S, tokens, Hkv, D] (element (s, t, h, d) at s*ss + t*st + h*sh + d;
+ * strides multiples of 8, 16-byte aligned) into the cache's blocks
+ * 0 .. ceil(tokens / block_tokens) - 1; every code, scale and bound of those
+ * blocks is written.  `tail` (may be NULL) receives the dense rows of each
+ * sequence's partial last block for uc_block8_append: in_dtype
+ * [S, Hkv, 2 (key, value), block_tokens, D].  in_dtype: UC_BF16 or UC_FP16.
+ */
+int uc_block8_pack(const uc_block8_cache *cache, const void *key, int64_t k_ss, int64_t k_st, int64_t k_sh,
+                   const void *value, int64_t v_ss, int64_t v_st, int64_t v_sh, int in_dtype, int64_t tokens,
+                   void *tail, uc_stream_t stream);
+
+/*
+ * Append rows to every sequence and advance `lengths` on the device: sequence
+ * s takes the first min(counts[s], tokens) rows (counts NULL: all) of dense key / value
+ * [S, tokens, Hkv, D] as in uc_block8_pack.  The open block is quantized again from
+ * `tail` and the new rows, so the cache equals uc_block8_pack of all rows; a
+ * sequence's other blocks are not touched.  Rows that do not fit
+ * the capacity are dropped.
+ */
+int uc_block8_append(const uc_block8_cache *cache, void *tail, const void *key, int64_t k_ss, int64_t k_st,
+                     int64_t k_sh, const void *value, int64_t v_ss, int64_t v_st, int64_t v_sh, int in_dtype,
+                     int64_t tokens, const int32_t *counts, uc_stream_t stream);
+
+/*
+ * code * scale (one rounding to fp32, one to out_dtype: UC_BF16 or UC_FP16) of
+ * tokens 0 .. tokens - 1 of every sequence into contiguous [S, tokens, Hkv, D]; rows behind a
+ * sequence's length are 0.
+ */
+int uc_block8_dequant(const uc_block8_cache *cache, void *out_key, void *out_value, int out_dtype, int64_t tokens,
+                      uc_stream_t stream);
+
+/*
+ * Queries of an attention or selection call over a cache: element (s, i, h, d)
+ * of query at s*q_ss + i*q_st + h*q_sh + d, strides multiples of 8, 16-byte
+ * aligned, UC_BF16 or UC_FP16; query head h reads KV head h / (Hq / Hkv).
+ * Sequence s has query_lengths[s] queries (device int32, read into [0, query_len];
+ * NULL: query_len), rows behind them are no queries.  Causal calls take them for the sequence's last
+ * tokens: row i sees the keys up to lengths[s] - query_lengths[s] + i.
+ * max_tokens: how long the caller expects the longest sequence to be; it shapes the launch only.
+ */
+typedef struct uc_block8_query {
+  const void *query;
+  int64_t q_ss, q_st, q_sh;
+  int64_t query_len;
+  int64_t heads_q;
+  const int32_t *query_lengths;
+  int64_t max_tokens;
+  int32_t dtype;
+  int32_t causal;
+} uc_block8_query;
+
+/*
+ * out = softmax(sm_scale * q K^T) V over each row's visible keys, contiguous
+ * [S, Lq, Hq, D] of the query's dtype, and lse [S, Hq, Lq] (natural log, may be NULL).  Rows that
+ * see no key, and rows behind a sequence's queries, get 0 and -inf.  With `blocks`
+ * (int32 [S, ceil(Lq / query_block), Hkv, budget], ascending, -1 for none) each run of
+ * query_block rows sees the listed blocks of its KV head only.  sm_scale > 0.
+ * workspace: uc_block8_attn_workspace_bytes(cache, query, budget, query_block).
+ */
+int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_query *query, const int32_t *blocks, int64_t budget,
+                   int64_t query_block, float sm_scale, void *out, float *lse, void *workspace,
+                   int64_t workspace_bytes, uc_stream_t stream);
+
+/* Workspace of uc_block8_attn (budget 0: without a block list); -1 for bad arguments. */
+int64_t uc_block8_attn_workspace_bytes(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget,
+                                       int64_t query_block);
+
+/*
+ * The blocks that each run of query_block rows reads, for uc_block8_attn.  A
+ * row's score of a block is the most that its product with a key inside the
+ * block's bounds can be,
+ *   q.k <= sum_d max(c_d hi_d, c_d lo_d) * u * step,
+ * with the row as whole numbers c = round(q (127 / max|q|)), step = max|q| (1/127), u the
+ * bounds' step (the key scale, times 448/127 for e4m3), multiplied in that order in fp32;
+ * the whole-number sum is exact, so the choice does not depend on how it is computed.
+ * A run's score is the largest of its rows in the KV head's query heads (rows holding an infinity or
+ * a NaN do not count); a block whose scale is not finite scores highest.  Candidates are the blocks that the run's last row
+ * sees.  Chosen: the first `sink` blocks, the blocks from the one `recent` - 1 before the one that holds the first
+ * row's last key on, and then those of the highest score, the lower index of equals, up to `budget`
+ * in all; written ascending, then -1, to blocks int32 [S, ceil(Lq / query_block), Hkv, budget].
+ * budget >= sink + recent + (causal: ceil((min(query_block, Lq) - 1) / block_tokens)), recent >= 1.
+ */
+int uc_block8_select(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget, int64_t sink,
+                     int64_t recent, int64_t query_block, int32_t *blocks, void *workspace, int64_t workspace_bytes,
+                     uc_stream_t stream);
+
+/* Workspace of uc_block8_select; -1 for bad arguments. */
+int64_t uc_block8_select_workspace_bytes(const uc_block8_cache *cache, const uc_block8_query *query,
+                                         int64_t query_block);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,160 @@
+"""Refusals of the 8-bit block-scaled cache that need no GPU: the Python
+class's checks and the C ABI's, all before any launch."""
+
+import ctypes
+
+import pytest
+import torch
+
+from unicache_amd import _native as nat
+from unicache_amd.storage import Block8KVCache
+
+
+def test_cpu_tensors_fail_closed():
+    key = torch.randn(1, 64, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        Block8KVCache.from_dense(key, key)
+    with pytest.raises(RuntimeError, match="GPU"):
+        Block8KVCache.empty(1, 64, 4, 128, device="cpu")
+    with pytest.raises(RuntimeError, match="GPU"):
+        Block8KVCache(*_tensors())
+
+
+def _tensors(s=2, h=2, n=3, b=64, d=128, code=torch.int8):
+    return (torch.zeros(s, h, n * b, d, dtype=code), torch.zeros(s, h, n, d, b, dtype=code), torch.zeros(s, h, n),
+            torch.zeros(s, h, n), torch.zeros(s, h, n, 2, d, dtype=torch.int8), torch.zeros(s, dtype=torch.int32))
+
+
+def test_tensor_checks():
+    good = list(_tensors())
+    for i, bad, match in (
+            (0, good[0].float(), "codes must be"), (0, good[0][:, :, :-1], "key_code"), (1, good[1][..., :48], "blocks of"),
+            (1, good[1].transpose(3, 4), "blocks of|contiguous|expected"), (2, good[2].double(), "key_scale"),
+            (3, good[3][:, :1], "value_scale"), (4, good[4].to(torch.uint8), "key_bounds"),
+            (5, good[5].long(), "lengths"), (0, good[0][0], "expects"), (0, good[0][..., ::2], "blocks of|key_code|supports")):
+        with pytest.raises(ValueError, match=match):
+            Block8KVCache(*good[:i], bad, *good[i + 1:])
+    with pytest.raises(ValueError, match="tail"):
+        Block8KVCache(*good, tail=torch.zeros(2, 2, 2, 64, 128))
+    with pytest.raises(ValueError, match="tail"):
+        Block8KVCache(*good, tail=torch.zeros(2, 2, 2, 32, 128, dtype=torch.float16))
+
+
+def test_dense_checks():
+    key = torch.randn(1, 64, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="matching"):
+        Block8KVCache.from_dense(key, key[:, :32])
+    with pytest.raises(ValueError, match="one dtype"):
+        Block8KVCache.from_dense(key, key.half())
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        Block8KVCache.from_dense(key.float(), key.float())
+    with pytest.raises(ValueError, match="gradient"):
+        Block8KVCache.from_dense(key.requires_grad_(), key)
+
+
+def _cache(**kw):
+    f = dict(key_code=16, value_code=16, key_scale=16, value_scale=16, key_bounds=16, lengths=16, sequences=2,
+             heads_kv=4, head_dim=128, blocks=10, block_tokens=64, code_dtype=nat.UC_INT8)
+    f.update(kw)
+    return nat.Block8Cache(**f)
+
+
+def _query(**kw):
+    f = dict(query=16, q_ss=0, q_st=0, q_sh=0, query_len=2, heads_q=28, query_lengths=None, max_tokens=640,
+             dtype=nat.UC_BF16, causal=0)
+    f.update(kw)
+    return nat.Block8Query(**f)
+
+
+BAD_CACHES = [(dict(head_dim=96), "head_dim"), (dict(block_tokens=48), "block_tokens"), (dict(block_tokens=16), "block_tokens"),
+              (dict(code_dtype=nat.UC_FP16), "int8 or e4m3"), (dict(sequences=0), "empty"), (dict(blocks=0), "empty"),
+              (dict(heads_kv=-1), "empty"), (dict(blocks=1 << 40), "too large"), (dict(key_code=None), "NULL"),
+              (dict(value_code=24), "aligned"), (dict(lengths=2), "aligned"), (dict(sequences=1 << 23), "too many")]
+
+
+@pytest.mark.parametrize("fields,match", BAD_CACHES)
+def test_cache_validation(fields, match):
+    c, q = _cache(**fields), _query()
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_pack", c, 16, 0, 0, 0, 16, 0, 0, 0, nat.UC_BF16, 64, None, None)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_append", c, 16, 16, 0, 0, 0, 16, 0, 0, 0, nat.UC_BF16, 1, None, None)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_dequant", c, 16, 16, nat.UC_BF16, 64, None)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_attn", c, q, None, 0, 0, 0.1, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_select", c, q, 4, 1, 1, 1, 16, 16, 1 << 40, None)
+    assert nat.lib().uc_block8_attn_workspace_bytes(c, q, 0, 0) == -1
+    assert nat.lib().uc_block8_select_workspace_bytes(c, q, 1) == -1
+
+
+def test_row_validation():
+    c = _cache()
+    for bad in ((8, 0, 0, 0), (None, 0, 0, 0), (16, 4, 0, 0), (16, 0, 12, 0), (16, 0, 0, 1)):
+        with pytest.raises(ValueError, match="16-byte aligned"):
+            nat.call("uc_block8_pack", c, *bad, 16, 0, 0, 0, nat.UC_BF16, 64, None, None)
+        with pytest.raises(ValueError, match="16-byte aligned"):
+            nat.call("uc_block8_append", c, 16, 16, 0, 0, 0, *bad, nat.UC_BF16, 64, None, None)
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        nat.call("uc_block8_pack", c, 16, 0, 0, 0, 16, 0, 0, 0, nat.UC_FP32, 64, None, None)
+    with pytest.raises(ValueError, match="capacity"):
+        nat.call("uc_block8_pack", c, 16, 0, 0, 0, 16, 0, 0, 0, nat.UC_BF16, 641, None, None)
+    with pytest.raises(ValueError, match="capacity"):
+        nat.call("uc_block8_dequant", c, 16, 16, nat.UC_BF16, 641, None)
+    with pytest.raises(ValueError, match="tail"):
+        nat.call("uc_block8_append", c, None, 16, 0, 0, 0, 16, 0, 0, 0, nat.UC_BF16, 1, None, None)
+    with pytest.raises(ValueError, match="outputs"):
+        nat.call("uc_block8_dequant", c, 16, 24, nat.UC_BF16, 64, None)
+    nat.call("uc_block8_pack", c, None, 0, 0, 0, None, 0, 0, 0, nat.UC_BF16, 0, None, None)  # nothing to do
+
+
+BAD_QUERIES = [(dict(dtype=nat.UC_FP32), "bf16 or fp16"), (dict(heads_q=30), "multiple of KV heads"), (dict(heads_q=0), "multiple"),
+               (dict(query_len=-1), "query_len"), (dict(query_len=1 << 30), "query_len"), (dict(max_tokens=-1), "max_tokens")]
+
+
+@pytest.mark.parametrize("fields,match", BAD_QUERIES)
+def test_query_validation(fields, match):
+    c, q = _cache(), _query(**fields)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_attn", c, q, None, 0, 0, 0.1, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match=match):
+        nat.call("uc_block8_select", c, q, 4, 1, 1, 1, 16, 16, 1 << 40, None)
+
+
+def test_attention_and_selection_validation():
+    c = _cache()
+    for q, match in ((_query(query=8), "aligned"), (_query(q_st=4), "aligned")):
+        with pytest.raises(ValueError, match=match):
+            nat.call("uc_block8_attn", c, q, None, 0, 0, 0.1, 16, None, 16, 1 << 40, None)
+        with pytest.raises(ValueError, match=match):
+            nat.call("uc_block8_select", c, q, 4, 1, 1, 1, 16, 16, 1 << 40, None)
+    q = _query()
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="sm_scale"):
+            nat.call("uc_block8_attn", c, q, None, 0, 0, scale, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="belong together"):
+        nat.call("uc_block8_attn", c, q, 16, 0, 1, 0.1, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="belong together"):
+        nat.call("uc_block8_attn", c, q, None, 4, 1, 0.1, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="query_block"):
+        nat.call("uc_block8_attn", c, q, 16, 4, 0, 0.1, 16, None, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="out must be"):
+        nat.call("uc_block8_attn", c, q, None, 0, 0, 0.1, 8, None, 16, 1 << 40, None)
+    need = nat.lib().uc_block8_attn_workspace_bytes(c, q, 0, 0)
+    assert need > 0
+    with pytest.raises(ValueError, match="workspace"):
+        nat.call("uc_block8_attn", c, q, None, 0, 0, 0.1, 16, None, 16, need - 1, None)
+    need = nat.lib().uc_block8_select_workspace_bytes(c, q, 1)
+    with pytest.raises(ValueError, match="workspace"):
+        nat.call("uc_block8_select", c, q, 4, 1, 1, 1, 16, 16, need - 1, None)
+    for budget, sink, recent, block, match in ((0, 1, 1, 1, "budget"), (4, -1, 1, 1, "sink"), (4, 1, 0, 1, "recent"),
+                                               (4, 1, 1, 0, "query_block"), (4, 2, 3, 1, "always chosen")):
+        with pytest.raises(ValueError, match=match):
+            nat.call("uc_block8_select", c, q, budget, sink, recent, block, 16, 16, 1 << 40, None)
+    causal = _query(causal=1, query_len=200)  # 200 queries cover up to 1 + ceil(199 / 64) blocks
+    with pytest.raises(ValueError, match="6 blocks always chosen"):
+        nat.call("uc_block8_select", c, causal, 5, 1, 1, 200, 16, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="NULL"):
+        nat.call("uc_block8_attn", c, None, None, 0, 0, 0.1, 16, None, 16, 1 << 40, None)
+    assert ctypes.sizeof(nat.Block8Cache) == 88 and ctypes.sizeof(nat.Block8Query) == 72

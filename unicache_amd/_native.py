@@ -18,6 +18,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libunicache
 ABI_VERSION = 3
 
 UC_BF16, UC_FP16, UC_FP32 = 0, 1, 2
+UC_INT8, UC_E4M3 = 3, 4  # code types of the 8-bit block-scaled cache
 UC_OK, UC_EINVAL, UC_ERUNTIME = 0, -1, -2
 UC_OP_KIVI_AV, UC_OP_H2O_SCORES = 2, 3
 
@@ -98,6 +99,42 @@ class MqQuery(ctypes.Structure):
         ("n_packed", ctypes.c_int32),
         ("dense_begin", ctypes.c_int32),
         ("n_dense", ctypes.c_int32),
+    ]
+
+
+class Block8Cache(ctypes.Structure):
+    """Mirror of ``uc_block8_cache``."""
+
+    _fields_ = [
+        ("key_code", _P),
+        ("value_code", _P),
+        ("key_scale", _P),
+        ("value_scale", _P),
+        ("key_bounds", _P),
+        ("lengths", _P),
+        ("sequences", _L),
+        ("heads_kv", _L),
+        ("head_dim", _L),
+        ("blocks", _L),
+        ("block_tokens", ctypes.c_int32),
+        ("code_dtype", ctypes.c_int32),
+    ]
+
+
+class Block8Query(ctypes.Structure):
+    """Mirror of ``uc_block8_query`` (strides in elements)."""
+
+    _fields_ = [
+        ("query", _P),
+        ("q_ss", _L),
+        ("q_st", _L),
+        ("q_sh", _L),
+        ("query_len", _L),
+        ("heads_q", _L),
+        ("query_lengths", _P),
+        ("max_tokens", _L),
+        ("dtype", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
     ]
 
 
@@ -202,6 +239,19 @@ _SIGNATURES = {
         _I,
         [_P, _P, _L, _L, _L, _I, _L, _L, _P, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P],
     ),
+    "uc_block8_pack": (_I, [ctypes.POINTER(Block8Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _P]),
+    "uc_block8_append": (_I, [ctypes.POINTER(Block8Cache), _P, _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _P]),
+    "uc_block8_dequant": (_I, [ctypes.POINTER(Block8Cache), _P, _P, _I, _L, _P]),
+    "uc_block8_attn": (
+        _I,
+        [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _P, _L, _L, _F, _P, _P, _P, _L, _P],
+    ),
+    "uc_block8_attn_workspace_bytes": (_L, [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _L, _L]),
+    "uc_block8_select": (
+        _I,
+        [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _L, _L, _L, _L, _P, _P, _L, _P],
+    ),
+    "uc_block8_select_workspace_bytes": (_L, [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _L]),
     "uc_workspace_bytes": (_L, [_I, _L, _L, _L, _L, _L]),
     "uc_kivi_decode_workspace_bytes": (_L, [_L, _I, _I, _L, _L, _L, _L, _L, _L]),
     "uc_kivi_decode_preferred_workspace_bytes": (_L, [_L, _I, _I, _L, _L, _L, _L, _L, _L]),

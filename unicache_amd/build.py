@@ -30,6 +30,9 @@ SOURCES = [
     "uc_compact.hip",
     "uc_stream.hip",
     "uc_parts.hip",
+    "uc_block8.hip",
+    "uc_block8_attn.hip",
+    "uc_block8_select.hip",
 ]
 
 # -ffp-contract=off keeps the pack/dequant arithmetic bit-exact (no implicit

@@ -1,6 +1,7 @@
 """Physical storage of the UniCache engine on MI355X (drop-in for
 ``unicache.storage``'s physical layouts and tensor backend)."""
 
+from .block8 import Block8KVCache
 from .physical import (
     GQAH2OCache,
     PackedKIVICache,
@@ -13,6 +14,7 @@ from .physical import (
 from .tensor_backend import CacheMutationResult, TensorCacheStorageBackend
 
 __all__ = [
+    "Block8KVCache",
     "CacheMutationResult",
     "TensorCacheStorageBackend",
     "GQAH2OCache",
