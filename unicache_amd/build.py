@@ -32,6 +32,7 @@ SOURCES = [
     "uc_parts.hip",
     "uc_block8.hip",
     "uc_block8_attn.hip",
+    "uc_block8_mq.hip",
     "uc_block8_select.hip",
 ]
 

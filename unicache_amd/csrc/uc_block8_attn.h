@@ -1,0 +1,167 @@
+// What the attention kernels of the 8-bit block-scaled cache share: the query
+// and launch arguments, the rows and keys of a workgroup, and the arithmetic of the
+// scales (uc_block8_attn.hip has the mathematics).
+#pragma once
+#include "uc_block8.h"
+
+namespace uc {
+namespace b8 {
+
+constexpr int kTile = 64;                // keys of a tile
+constexpr int32_t kNone = 1 << 30;       // a half tile without keys: behind every length
+constexpr float kRaise = 8.0f;           // P stays below 2^8
+
+struct Query {
+  const uint16_t *p;
+  int64_t ss, st, sh;
+  const int32_t *lens;
+  int32_t len, heads, group;
+  int32_t fp16, causal;
+  float scale;  // sm_scale * log2(e)
+
+  __device__ __forceinline__ int32_t count(int32_t s) const {
+    if (lens == nullptr) return len;
+    const int32_t n = lens[s];
+    return n < 0 ? 0 : n > len ? len : n;
+  }
+};
+
+struct Plan {
+  const int32_t *list;  // block lists, or NULL: every block
+  int32_t budget;
+  int32_t run, runs;    // query tokens that share a list (without lists: all), and how many such runs
+  int32_t groups, rows; // row groups of a run, and their rows
+  int32_t splits, split_tiles;
+};
+
+// The rows of a workgroup: `first` + r / group is row r's query token.
+struct Rows {
+  int32_t s, h, length, count;
+  int32_t run0, run_rows, r0;  // first token and rows of the run, first row of the group
+  int32_t end_first, end_last; // keys that the first and the last row that counts see
+};
+
+__device__ __forceinline__ int32_t visible(const Query &q, int32_t length, int32_t count, int32_t token) {
+  if (!q.causal) return length;
+  const int32_t e = length - count + token + 1;
+  return e < 0 ? 0 : e;
+}
+
+__device__ __forceinline__ Rows rows_of(const Cache &c, const Query &q, const Plan &p, int32_t unit, int rows) {
+  Rows w;
+  const int32_t g = unit % p.groups, run = unit / p.groups % p.runs, sh = unit / p.groups / p.runs;
+  w.s = sh / c.heads;
+  w.h = sh % c.heads;
+  w.length = c.length(w.s);
+  w.count = q.count(w.s);
+  w.run0 = run * p.run;
+  const int32_t tokens = q.len - w.run0 < p.run ? q.len - w.run0 : p.run;
+  w.run_rows = tokens * q.group;
+  w.r0 = g * rows;
+  const int32_t t0 = w.run0 + w.r0 / q.group;
+  const int32_t r1 = (w.r0 + rows < w.run_rows ? w.r0 + rows : w.run_rows) - 1;
+  int32_t t1 = w.run0 + r1 / q.group;
+  t1 = t1 < w.count ? t1 : w.count - 1;
+  const bool none = w.r0 >= w.run_rows || t0 >= w.count;
+  w.end_first = none ? 0 : visible(q, w.length, w.count, t0);
+  w.end_last = none ? 0 : visible(q, w.length, w.count, t1);
+  return w;
+}
+
+// Tiles of a workgroup's rows, over all splits.
+__device__ __forceinline__ int32_t tiles_of(const Cache &c, const Plan &p, const Rows &w) {
+  if (p.list == nullptr) return (w.end_last + kTile - 1) / kTile;
+  return w.end_last == 0 ? 0 : (p.budget * c.block + kTile - 1) / kTile;
+}
+
+// Tiles of one split: the host's figure, or more where a sequence is longer than it expected.
+__device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) {
+  const int32_t least = (tiles + p.splits - 1) / p.splits;
+  return least > p.split_tiles ? least : p.split_tiles;
+}
+
+// First key of a half tile (32 keys); kNone where the list has none there.
+__device__ __forceinline__ int32_t half_of(const Cache &c, const Plan &p, const int32_t *list, int32_t half) {
+  if (list == nullptr) return half * 32;
+  const int32_t e = half >> (c.shift - 5), sub = half & ((c.block >> 5) - 1);
+  if (e >= p.budget) return kNone;
+  const int32_t b = list[e];
+  const bool again = e > 0 && list[e - 1] == b;  // an index given twice counts once
+  return b < 0 || b >= c.blocks || again ? kNone : (b << c.shift) + sub * 32;
+}
+
+// Keep the first n of 16 bytes.
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int32_t n) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int32_t k = n - 4 * i;
+    w[i] = k >= 4 ? w[i] : k <= 0 ? 0u : w[i] & ((1u << (8 * k)) - 1u);
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+
+// The value scale that a tile's keys count with; `most` is the largest so far.
+__device__ __forceinline__ float counted_scale(float vs, float &most) {
+  if (vs < __builtin_huge_valf()) most = fmaxf(most, vs);
+  const float least = most * 0x1p-60f;
+  return vs < least ? least : vs;  // a NaN stays
+}
+
+// l 2^d: in two steps, since 2^d may be below fp32's range where the product is not.
+__device__ __forceinline__ float rescaled(float l, float d) {
+  const float a = mf::fast_exp2(0.5f * d);
+  return l * a * a;
+}
+
+// One query row's fragments, scaled by a power of two into fp16; returns the
+// factor of its logits: sm_scale log2(e) / the power.  Lane quad x holds channels
+// 32 k + 8 x .. + 7 of fragment k; with PAIRS 64 (k / 2) + 16 x + 8 (k % 2) .. + 7, so that 16 bytes
+// of codes feed two fragments.
+template <int D, bool PAIRS>
+__device__ __forceinline__ float load_query(const Query &q, const Rows &w, int32_t r, h8 (&frag)[D / 32]) {
+  const int quad = (threadIdx.x & 63) >> 4;
+  const int32_t token = w.run0 + r / q.group;
+  uint4 raw[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) raw[k] = uint4{0, 0, 0, 0};
+  if (r < w.run_rows && token < w.count) {
+    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r % q.group) * q.sh;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      raw[k] = *reinterpret_cast<const uint4 *>(p + (PAIRS ? (k / 2) * 64 + quad * 16 + (k % 2) * 8 : k * 32 + quad * 8));
+    }
+  }
+  float x[D / 32][8], a = 0.0f;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+    const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = j % 2 ? u[j / 2] >> 16 : u[j / 2];
+      x[k][j] = q.fp16 ? f16_bits_to_f32(static_cast<uint16_t>(bits)) : bf16_bits_to_f32(bits & 0xffffu);
+      a = fmaxf(a, fabsf(x[k][j]));
+    }
+  }
+  a = mf::max_over_slices(a);
+  int e = static_cast<int>((__float_as_uint(a) >> 23) & 0xff) - 127;
+  // a row of zeros, or one with an infinity (whose logits are what they are); below 2^-100 the
+  // power stays in fp32's range
+  e = a == 0.0f || e == 128 ? 14 : e < -100 ? -100 : e;
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) frag[k][j] = mf::to_h(x[k][j] * up);
+  }
+  return q.scale * down;
+}
+
+// uc_block8_mq.hip: 128 rows a workgroup, keys staged through LDS.
+constexpr int kTileRows = 128;
+int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint32_t workgroups,
+                 uint16_t *out, float *lse, float *part, float *stat, hipStream_t stream);
+
+}  // namespace b8
+}  // namespace uc

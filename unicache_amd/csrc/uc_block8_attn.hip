@@ -25,96 +25,13 @@
 // consecutive keys of one query row, which is the operand that
 // O^T = V^T P^T takes, with no exchange between lanes: the values' blocks are
 // stored channel-major for that, 16 codes of a channel in one 16-byte load.
-#include "uc_block8.h"
+#include "uc_block8_attn.h"
 
 #include <type_traits>
 
 namespace uc {
 namespace b8 {
 namespace {
-
-constexpr int kTile = 64;                // keys of a tile
-constexpr int32_t kNone = 1 << 30;       // a half tile without keys: behind every length
-constexpr float kRaise = 8.0f;           // P stays below 2^8
-
-struct Query {
-  const uint16_t *p;
-  int64_t ss, st, sh;
-  const int32_t *lens;
-  int32_t len, heads, group;
-  int32_t fp16, causal;
-  float scale;  // sm_scale * log2(e)
-
-  __device__ __forceinline__ int32_t count(int32_t s) const {
-    if (lens == nullptr) return len;
-    const int32_t n = lens[s];
-    return n < 0 ? 0 : n > len ? len : n;
-  }
-};
-
-struct Plan {
-  const int32_t *list;  // block lists, or NULL: every block
-  int32_t budget;
-  int32_t run, runs;    // query tokens that share a list (without lists: all), and how many such runs
-  int32_t groups;       // row groups of a run
-  int32_t splits, split_tiles;
-};
-
-// The rows of a workgroup: `first` + r / group is row r's query token.
-struct Rows {
-  int32_t s, h, length, count;
-  int32_t run0, run_rows, r0;  // first token and rows of the run, first row of the group
-  int32_t end_first, end_last; // keys that the first and the last row that counts see
-};
-
-__device__ __forceinline__ int32_t visible(const Query &q, int32_t length, int32_t count, int32_t token) {
-  if (!q.causal) return length;
-  const int32_t e = length - count + token + 1;
-  return e < 0 ? 0 : e;
-}
-
-__device__ __forceinline__ Rows rows_of(const Cache &c, const Query &q, const Plan &p, int32_t unit, int rows) {
-  Rows w;
-  const int32_t g = unit % p.groups, run = unit / p.groups % p.runs, sh = unit / p.groups / p.runs;
-  w.s = sh / c.heads;
-  w.h = sh % c.heads;
-  w.length = c.length(w.s);
-  w.count = q.count(w.s);
-  w.run0 = run * p.run;
-  const int32_t tokens = q.len - w.run0 < p.run ? q.len - w.run0 : p.run;
-  w.run_rows = tokens * q.group;
-  w.r0 = g * rows;
-  const int32_t t0 = w.run0 + w.r0 / q.group;
-  const int32_t r1 = (w.r0 + rows < w.run_rows ? w.r0 + rows : w.run_rows) - 1;
-  int32_t t1 = w.run0 + r1 / q.group;
-  t1 = t1 < w.count ? t1 : w.count - 1;
-  const bool none = w.r0 >= w.run_rows || t0 >= w.count;
-  w.end_first = none ? 0 : visible(q, w.length, w.count, t0);
-  w.end_last = none ? 0 : visible(q, w.length, w.count, t1);
-  return w;
-}
-
-// Tiles of a workgroup's rows, over all splits.
-__device__ __forceinline__ int32_t tiles_of(const Cache &c, const Plan &p, const Rows &w) {
-  if (p.list == nullptr) return (w.end_last + kTile - 1) / kTile;
-  return w.end_last == 0 ? 0 : (p.budget * c.block + kTile - 1) / kTile;
-}
-
-// Tiles of one split: the host's figure, or more where a sequence is longer than it expected.
-__device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) {
-  const int32_t least = (tiles + p.splits - 1) / p.splits;
-  return least > p.split_tiles ? least : p.split_tiles;
-}
-
-// First key of a half tile (32 keys); kNone where the list has none there.
-__device__ __forceinline__ int32_t half_of(const Cache &c, const Plan &p, const int32_t *list, int32_t half) {
-  if (list == nullptr) return half * 32;
-  const int32_t e = half >> (c.shift - 5), sub = half & ((c.block >> 5) - 1);
-  if (e >= p.budget) return kNone;
-  const int32_t b = list[e];
-  const bool again = e > 0 && list[e - 1] == b;  // an index given twice counts once
-  return b < 0 || b >= c.blocks || again ? kNone : (b << c.shift) + sub * 32;
-}
 
 // Codes of one tile as they come from memory, with the scales of the lane's keys.
 template <int D>
@@ -155,72 +72,6 @@ __device__ __forceinline__ void load_values(Raw<D> &raw, const Cache &c, const L
   const int32_t step = 16 * c.block;
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) raw.v[n] = *reinterpret_cast<const uint4 *>(p + n * step);
-}
-
-// Keep the first n of 16 bytes.
-__device__ __forceinline__ uint4 first_bytes(uint4 v, int32_t n) {
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t k = n - 4 * i;
-    w[i] = k >= 4 ? w[i] : k <= 0 ? 0u : w[i] & ((1u << (8 * k)) - 1u);
-  }
-  return uint4{w[0], w[1], w[2], w[3]};
-}
-
-// One query row's fragments, scaled by a power of two into fp16; returns the
-// factor of its logits: sm_scale log2(e) / the power.
-template <int D>
-__device__ __forceinline__ float load_query(const Query &q, const Rows &w, int32_t r, h8 (&frag)[D / 32]) {
-  const int quad = (threadIdx.x & 63) >> 4;
-  const int32_t token = w.run0 + r / q.group;
-  uint4 raw[D / 32];
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) raw[k] = uint4{0, 0, 0, 0};
-  if (r < w.run_rows && token < w.count) {
-    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r % q.group) * q.sh;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      raw[k] = *reinterpret_cast<const uint4 *>(p + (k / 2) * 64 + quad * 16 + (k % 2) * 8);
-    }
-  }
-  float x[D / 32][8], a = 0.0f;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) {
-    const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t bits = j % 2 ? u[j / 2] >> 16 : u[j / 2];
-      x[k][j] = q.fp16 ? f16_bits_to_f32(static_cast<uint16_t>(bits)) : bf16_bits_to_f32(bits & 0xffffu);
-      a = fmaxf(a, fabsf(x[k][j]));
-    }
-  }
-  a = mf::max_over_slices(a);
-  int e = static_cast<int>((__float_as_uint(a) >> 23) & 0xff) - 127;
-  // a row of zeros, or one with an infinity (whose logits are what they are); below 2^-100 the
-  // power stays in fp32's range
-  e = a == 0.0f || e == 128 ? 14 : e < -100 ? -100 : e;
-  const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) frag[k][j] = mf::to_h(x[k][j] * up);
-  }
-  return q.scale * down;
-}
-
-// The value scale that a tile's keys count with; `most` is the largest so far.
-__device__ __forceinline__ float counted_scale(float vs, float &most) {
-  if (vs < __builtin_huge_valf()) most = fmaxf(most, vs);
-  const float least = most * 0x1p-60f;
-  return vs < least ? least : vs;  // a NaN stays
-}
-
-// l 2^d: in two steps, since 2^d may be below fp32's range where the product is not.
-__device__ __forceinline__ float rescaled(float l, float d) {
-  const float a = mf::fast_exp2(0.5f * d);
-  return l * a * a;
 }
 
 // State of 16 query rows in one wave: the lane's row is lane % 16.
@@ -285,7 +136,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const int32_t r = w.r0 + 16 * n + col;
-    factor[n] = load_query<D>(q, w, r, frag[n]);
+    factor[n] = load_query<D, true>(q, w, r, frag[n]);
     row_end[n] = visible(q, w.length, w.count, w.run0 + r / q.group);
     row_end[n] = row_end[n] < w.length ? row_end[n] : w.length;
     acc[n].m = mf::kNegInf;
@@ -421,49 +272,65 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
   }
 }
 
-// Join the splits of 16 NR rows: one wave per row.
-template <int D, int NR>
+// Join the splits: one workgroup per row, whose waves take every fourth split
+// (four loads of a wave in flight) and meet in LDS.
+template <int D>
 __global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                    const float *part, const float *stat) {
   constexpr int kC = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int32_t index = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int32_t unit = index / (16 * NR), rr = index % (16 * NR);
-  if (unit >= c.sequences * c.heads * p.runs * p.groups) return;
-  const Rows w = rows_of(c, q, p, unit, 16 * NR);
+  __shared__ float sh_o[4][D], sh_l[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int32_t unit = blockIdx.x / p.rows, rr = blockIdx.x % p.rows;
+  const Rows w = rows_of(c, q, p, unit, p.rows);
   const int32_t r = w.r0 + rr;
   if (r >= w.run_rows) return;
   const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
   const int32_t splits = tiles == 0 ? 1 : (tiles + per - 1) / per;
-  const int64_t base = int64_t(unit) * p.splits * (16 * NR) + rr;
+  const int64_t base = int64_t(unit) * p.splits * p.rows + rr;
   float m = mf::kNegInf;
-  for (int32_t i = lane; i < splits; i += 64) m = fmaxf(m, stat[2 * (base + int64_t(i) * (16 * NR))]);
+  for (int32_t i = lane; i < splits; i += 64) m = fmaxf(m, stat[2 * (base + int64_t(i) * p.rows)]);
   m = wave_max(m);
   float total = 0.0f, o[kC] = {};
-  for (int32_t i = 0; i < splits; ++i) {
-    const int64_t at = base + int64_t(i) * (16 * NR);
-    const float mi = stat[2 * at], li = stat[2 * at + 1];
-    if (mi == mf::kNegInf && !(li != 0.0f)) continue;
-    const float f = mf::fast_exp2(mi - m);
-    total += rescaled(li, mi - m);
+  for (int32_t i0 = wave; i0 < splits; i0 += 16) {
+    float mi[4], li[4], oi[4][kC];
 #pragma unroll
-    for (int j = 0; j < kC; ++j) o[j] += f * part[at * D + lane * kC + j];
+    for (int u = 0; u < 4; ++u) {
+      const int32_t i = i0 + 4 * u;
+      const int64_t at = base + int64_t(i < splits ? i : i0) * p.rows;
+      mi[u] = stat[2 * at];
+      li[u] = i < splits ? stat[2 * at + 1] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kC; ++j) oi[u][j] = part[at * D + lane * kC + j];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      // a split past the end, or one whose keys a row does not see
+      const bool live = i0 + 4 * u < splits && !(mi[u] == mf::kNegInf && !(li[u] != 0.0f));
+      const float d = live ? mi[u] - m : mf::kNegInf, f = mf::fast_exp2(d);
+      total += rescaled(li[u], d);
+#pragma unroll
+      for (int j = 0; j < kC; ++j) o[j] += live ? f * oi[u][j] : 0.0f;
+    }
   }
+#pragma unroll
+  for (int j = 0; j < kC; ++j) sh_o[wave][lane * kC + j] = o[j];
+  if (lane == 0) sh_l[wave] = total;
+  __syncthreads();
   const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
+  total = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
   const bool none = token >= w.count || total == 0.0f;
-  uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + lane * kC;
-#pragma unroll
-  for (int j = 0; j < kC; ++j) {
-    const float v = none ? 0.0f : o[j] / total;
-    dst[j] = q.fp16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
+  const int ch = threadIdx.x;
+  if (ch < D) {
+    const float v = none ? 0.0f : (sh_o[0][ch] + sh_o[1][ch] + sh_o[2][ch] + sh_o[3][ch]) / total;
+    out[((int64_t(w.s) * q.len + token) * q.heads + head) * D + ch] = q.fp16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
   }
-  if (lane == 0 && lse != nullptr) {
+  if (ch == 0 && lse != nullptr) {
     lse[(int64_t(w.s) * q.heads + head) * q.len + token] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(total));
   }
 }
 
 int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget, int64_t query_block,
-              const char *what, Query &q, Plan &p, int &nr) {
+              const char *what, Query &q, Plan &p) {
   UC_REQUIRE(query != nullptr, "%s: query is NULL", what);
   UC_REQUIRE(half_dtype(query->dtype), "%s: queries must be bf16 or fp16", what);
   UC_REQUIRE(query->heads_q > 0 && query->heads_q % cache->heads_kv == 0,
@@ -483,27 +350,28 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   p.run = static_cast<int32_t>(run);
   p.runs = static_cast<int32_t>(ceil_div(query->query_len, run));
   const int64_t rows = run * q.group;
-  nr = rows > 16 ? 2 : 1;
-  p.groups = static_cast<int32_t>(ceil_div(rows, 16 * nr));
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kTileRows;
+  p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
   // keys that the launch expects a row to read
   const int64_t capacity = cache->blocks * cache->block_tokens;
   int64_t keys = query->max_tokens < capacity ? query->max_tokens : capacity;
   if (budget > 0) keys = budget * cache->block_tokens;
   const int64_t tiles = keys > 0 ? ceil_div(keys, kTile) : 1;
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
-  // about 1024 workgroups (four a CU), each wave with a tile at least
-  int64_t splits = units > 0 ? 1024 / units : 1;
+  // about 1024 workgroups (four a CU) of few rows, each wave with a tile at least; 512 (two a CU) of
+  // many rows, each with four tiles
+  int64_t splits = units > 0 ? (p.rows == kTileRows ? 512 : 1024) / units : 1;
   const int64_t most = ceil_div(tiles, 4);
   splits = splits < 1 ? 1 : splits > most ? most : splits;
   p.split_tiles = static_cast<int32_t>(ceil_div(tiles, splits));
   p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
-  UC_REQUIRE(units * p.splits < (int64_t(1) << 31) / (16 * nr), "%s: too many query rows", what);
+  UC_REQUIRE(units * p.splits < (int64_t(1) << 31) / p.rows, "%s: too many query rows", what);
   return UC_OK;
 }
 
 // Floats of the splits' partial outputs and statistics.
-int64_t part_rows(const uc_block8_cache *cache, const Plan &p, int nr) {
-  return p.splits > 1 ? cache->sequences * cache->heads_kv * p.runs * p.groups * p.splits * 16 * nr : 0;
+int64_t part_rows(const uc_block8_cache *cache, const Plan &p) {
+  return p.splits > 1 ? cache->sequences * cache->heads_kv * p.runs * p.groups * p.splits * p.rows : 0;
 }
 
 }  // namespace
@@ -516,11 +384,10 @@ extern "C" int64_t uc_block8_attn_workspace_bytes(const uc_block8_cache *cache, 
   Cache c;
   Query q;
   Plan p;
-  int nr;
   if (check_cache(cache, "uc_block8_attn", c) ||
-      make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p, nr))
+      make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p))
     return -1;
-  return part_rows(cache, p, nr) * (cache->head_dim + 2) * int64_t(sizeof(float));
+  return part_rows(cache, p) * (cache->head_dim + 2) * int64_t(sizeof(float));
 }
 
 extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_query *query, const int32_t *blocks,
@@ -531,16 +398,15 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   Cache c;
   Query q;
   Plan p;
-  int nr;
   if (int rc = check_cache(cache, "uc_block8_attn", c)) return rc;
-  if (int rc = make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p, nr)) return rc;
+  if (int rc = make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p)) return rc;
   UC_REQUIRE((blocks != nullptr) == (budget > 0), "uc_block8_attn: a block list and its budget belong together");
   UC_REQUIRE(sm_scale > 0.0f && sm_scale < __builtin_huge_valf(), "uc_block8_attn: sm_scale must be positive");
   if (q.len == 0) return UC_OK;
   UC_REQUIRE(q.p != nullptr && (reinterpret_cast<uintptr_t>(q.p) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,
              "uc_block8_attn: query must be 16-byte aligned with strides that are multiples of 8");
   UC_REQUIRE(out != nullptr && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "uc_block8_attn: out must be 16-byte aligned");
-  const int64_t rows = part_rows(cache, p, nr);
+  const int64_t rows = part_rows(cache, p);
   UC_REQUIRE(rows == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                            workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "uc_block8_attn: workspace too small");
@@ -548,18 +414,30 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   q.scale = sm_scale * kLog2e;
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
-  return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
-    auto launch = [&](auto nr_tag) {
-      constexpr int NR = decltype(nr_tag)::value;
-      hipLaunchKernelGGL((rows_kernel<D, CODE, NR>), dim3(static_cast<uint32_t>(units * p.splits)), dim3(256), 0,
-                         as_stream(stream), c, q, p, static_cast<uint16_t *>(out), lse, part, stat);
-      int rc = check_launch("uc_block8_attn");
-      if (rc != UC_OK || p.splits == 1) return rc;
-      hipLaunchKernelGGL((join_kernel<D, NR>), dim3(static_cast<uint32_t>(ceil_div(units * 16 * NR, 4))), dim3(256), 0,
-                         as_stream(stream), c, q, p, static_cast<uint16_t *>(out), lse, part, stat);
-      return check_launch("uc_block8_attn (join)");
-    };
-    if (nr == 1) return launch(std::integral_constant<int, 1>());
-    return launch(std::integral_constant<int, 2>());
-  });
+  const uint32_t workgroups = static_cast<uint32_t>(units * p.splits);
+  int rc;
+  if (p.rows == kTileRows) {
+    rc = launch_tiles(cache, c, q, p, workgroups, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
+  } else {
+    rc = UC_B8_DISPATCH(cache, cache->head_dim, [&] {
+      if (p.rows == 16) {
+        hipLaunchKernelGGL((rows_kernel<D, CODE, 1>), dim3(workgroups), dim3(256), 0, as_stream(stream), c, q, p,
+                           static_cast<uint16_t *>(out), lse, part, stat);
+      } else {
+        hipLaunchKernelGGL((rows_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, as_stream(stream), c, q, p,
+                           static_cast<uint16_t *>(out), lse, part, stat);
+      }
+      return check_launch("uc_block8_attn");
+    });
+  }
+  if (rc != UC_OK || p.splits == 1) return rc;
+  const dim3 rows_grid(static_cast<uint32_t>(units * p.rows));
+  if (cache->head_dim == 128) {
+    hipLaunchKernelGGL((join_kernel<128>), rows_grid, dim3(256), 0, as_stream(stream), c, q, p,
+                       static_cast<uint16_t *>(out), lse, part, stat);
+  } else {
+    hipLaunchKernelGGL((join_kernel<64>), rows_grid, dim3(256), 0, as_stream(stream), c, q, p,
+                       static_cast<uint16_t *>(out), lse, part, stat);
+  }
+  return check_launch("uc_block8_attn (join)");
 }
