@@ -152,6 +152,8 @@ def test_attention_and_selection_validation():
                                                (4, 1, 1, 0, "query_block"), (4, 2, 3, 1, "always chosen")):
         with pytest.raises(ValueError, match=match):
             nat.call("uc_block8_select", c, q, budget, sink, recent, block, 16, 16, 1 << 40, None)
+    with pytest.raises(ValueError, match="too many blocks"):
+        nat.call("uc_block8_select", _cache(blocks=1 << 21), q, 4, 1, 1, 1, 16, 16, 1 << 60, None)
     causal = _query(causal=1, query_len=200)  # 200 queries cover up to 1 + ceil(199 / 64) blocks
     with pytest.raises(ValueError, match="6 blocks always chosen"):
         nat.call("uc_block8_select", c, causal, 5, 1, 1, 200, 16, 16, 1 << 40, None)

@@ -391,6 +391,18 @@ def test_sparse_attention(device, code, block, case):
     check((out, lse), reference(cache, q, lens, qlens, causal, 1 / math.sqrt(d), want, qb))
 
 
+@pytest.mark.parametrize("lq", [1, 40])
+def test_selection_among_more_blocks_than_lds_holds(device, lq):
+    lens = [300000, 262144 + 64]  # 9375 and 8194 blocks
+    g = torch.Generator(device="cuda").manual_seed(5)
+    key = torch.randn(2, 300000, 1, 64, generator=g, device="cuda", dtype=torch.bfloat16)
+    cache = Block8KVCache.from_dense(key, key, lengths=torch.tensor(lens, dtype=torch.int32, device=device),
+                                     block_tokens=32)
+    q = queries(2, lq, 2, 64, seed=6)
+    _, _, blocks = cache.sparse_attention(q, budget=50, query_block=40)
+    assert torch.equal(blocks.cpu(), chosen_blocks(cache, q, lens, [lq, lq], False, 50, 40, 1, 1))
+
+
 def test_selection_of_equal_scores_and_odd_queries(device):
     # equal blocks: the lower index; zero queries; a NaN query beside good ones; a block of NaN keys
     key, value = dense(1, 64 * 40, 1, 128, seed=60)

@@ -272,59 +272,79 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
   }
 }
 
-// Join the splits: one workgroup per row, whose waves take every fourth split
-// (four loads of a wave in flight) and meet in LDS.
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
+// Join the splits of the query rows.  WAVES == 1: a wave per row, for few splits; WAVES == 4: a
+// workgroup per row, whose waves take every fourth split and meet in LDS.  A
+// wave keeps four loads in flight.
+template <int D, int WAVES>
+__global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, int64_t rows, uint16_t *out, float *lse,
                                                    const float *part, const float *stat) {
   constexpr int kC = D / 64;
+  typedef float vec __attribute__((ext_vector_type(kC)));
   __shared__ float sh_o[4][D], sh_l[4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t unit = blockIdx.x / p.rows, rr = blockIdx.x % p.rows;
+  const int64_t index = WAVES == 1 ? int64_t(blockIdx.x) * 4 + wave : blockIdx.x;
+  if (index >= rows) return;
+  // rows of the runs in order: (sequence, head, run, row)
+  const int32_t full = p.run * q.group;
+  const int32_t r = static_cast<int32_t>(index % full), run = static_cast<int32_t>(index / full % p.runs);
+  const int64_t sh = index / full / p.runs;
+  const int32_t unit = static_cast<int32_t>((sh * p.runs + run) * p.groups + r / p.rows);
   const Rows w = rows_of(c, q, p, unit, p.rows);
-  const int32_t r = w.r0 + rr;
   if (r >= w.run_rows) return;
   const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
   const int32_t splits = tiles == 0 ? 1 : (tiles + per - 1) / per;
-  const int64_t base = int64_t(unit) * p.splits * p.rows + rr;
+  const int64_t base = int64_t(unit) * p.splits * p.rows + r % p.rows;
   float m = mf::kNegInf;
   for (int32_t i = lane; i < splits; i += 64) m = fmaxf(m, stat[2 * (base + int64_t(i) * p.rows)]);
   m = wave_max(m);
-  float total = 0.0f, o[kC] = {};
-  for (int32_t i0 = wave; i0 < splits; i0 += 16) {
-    float mi[4], li[4], oi[4][kC];
+  float total = 0.0f;
+  vec o = {};
+  for (int32_t i0 = WAVES == 1 ? 0 : wave; i0 < splits; i0 += 4 * WAVES) {
+    float mi[4], li[4];
+    vec oi[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int32_t i = i0 + 4 * u;
+      const int32_t i = i0 + WAVES * u;
       const int64_t at = base + int64_t(i < splits ? i : i0) * p.rows;
       mi[u] = stat[2 * at];
       li[u] = i < splits ? stat[2 * at + 1] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < kC; ++j) oi[u][j] = part[at * D + lane * kC + j];
+      oi[u] = *reinterpret_cast<const vec *>(part + at * D + lane * kC);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       // a split past the end, or one whose keys a row does not see
-      const bool live = i0 + 4 * u < splits && !(mi[u] == mf::kNegInf && !(li[u] != 0.0f));
+      const bool live = i0 + WAVES * u < splits && !(mi[u] == mf::kNegInf && !(li[u] != 0.0f));
       const float d = live ? mi[u] - m : mf::kNegInf, f = mf::fast_exp2(d);
       total += rescaled(li[u], d);
 #pragma unroll
       for (int j = 0; j < kC; ++j) o[j] += live ? f * oi[u][j] : 0.0f;
     }
   }
+  if constexpr (WAVES > 1) {
+    *reinterpret_cast<vec *>(&sh_o[wave][lane * kC]) = o;
+    if (lane == 0) sh_l[wave] = total;
+    __syncthreads();
+    if (wave > 0) return;
+    total = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
 #pragma unroll
-  for (int j = 0; j < kC; ++j) sh_o[wave][lane * kC + j] = o[j];
-  if (lane == 0) sh_l[wave] = total;
-  __syncthreads();
-  const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
-  total = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
-  const bool none = token >= w.count || total == 0.0f;
-  const int ch = threadIdx.x;
-  if (ch < D) {
-    const float v = none ? 0.0f : (sh_o[0][ch] + sh_o[1][ch] + sh_o[2][ch] + sh_o[3][ch]) / total;
-    out[((int64_t(w.s) * q.len + token) * q.heads + head) * D + ch] = q.fp16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
+    for (int j = 0; j < kC; ++j) o[j] = sh_o[0][lane * kC + j] + sh_o[1][lane * kC + j] + sh_o[2][lane * kC + j] + sh_o[3][lane * kC + j];
   }
-  if (ch == 0 && lse != nullptr) {
+  const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
+  const bool none = token >= w.count || total == 0.0f;
+  const float f = none ? 0.0f : 1.0f / total;
+  uint16_t v[kC];
+#pragma unroll
+  for (int j = 0; j < kC; ++j) {
+    const float x = none ? 0.0f : o[j] * f;
+    v[j] = q.fp16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
+  }
+  uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + lane * kC;
+  if constexpr (kC == 2) {
+    *reinterpret_cast<uint32_t *>(dst) = v[0] | (uint32_t(v[1]) << 16);
+  } else {
+    *dst = v[0];
+  }
+  if (lane == 0 && lse != nullptr) {
     lse[(int64_t(w.s) * q.heads + head) * q.len + token] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(total));
   }
 }
@@ -431,13 +451,17 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
     });
   }
   if (rc != UC_OK || p.splits == 1) return rc;
-  const dim3 rows_grid(static_cast<uint32_t>(units * p.rows));
-  if (cache->head_dim == 128) {
-    hipLaunchKernelGGL((join_kernel<128>), rows_grid, dim3(256), 0, as_stream(stream), c, q, p,
-                       static_cast<uint16_t *>(out), lse, part, stat);
-  } else {
-    hipLaunchKernelGGL((join_kernel<64>), rows_grid, dim3(256), 0, as_stream(stream), c, q, p,
-                       static_cast<uint16_t *>(out), lse, part, stat);
-  }
-  return check_launch("uc_block8_attn (join)");
+  const int64_t q_rows = cache->sequences * cache->heads_kv * p.runs * p.run * q.group;
+  auto join = [&](auto d_tag, auto waves_tag) {
+    constexpr int D = decltype(d_tag)::value, W = decltype(waves_tag)::value;
+    hipLaunchKernelGGL((join_kernel<D, W>), dim3(static_cast<uint32_t>(W == 1 ? ceil_div(q_rows, 4) : q_rows)), dim3(256),
+                       0, as_stream(stream), c, q, p, q_rows, static_cast<uint16_t *>(out), lse, part, stat);
+    return check_launch("uc_block8_attn (join)");
+  };
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 4> Four;
+  typedef std::integral_constant<int, 64> D64;
+  typedef std::integral_constant<int, 128> D128;
+  if (cache->head_dim == 128) return p.splits <= 8 ? join(D128(), One()) : join(D128(), Four());
+  return p.splits <= 8 ? join(D64(), One()) : join(D64(), Four());
 }

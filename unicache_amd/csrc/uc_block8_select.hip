@@ -45,35 +45,60 @@ struct Run {
   }
 };
 
-// One wave per query row: its codes and their step; step -1 marks a row that does not count.
+// Eight 16-bit values as floats.
+__device__ __forceinline__ void to_floats(uint4 raw, bool fp16, float (&x)[8]) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t bits = (j % 2 ? w[j / 2] >> 16 : w[j / 2]) & 0xffffu;
+    x[j] = fp16 ? f16_bits_to_f32(static_cast<uint16_t>(bits)) : bf16_bits_to_f32(bits);
+  }
+}
+
+// round(x inverse) of four values as bytes.
+__device__ __forceinline__ uint32_t four_codes(const float *x, float inverse) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float y = __builtin_amdgcn_fmed3f(rintf(mul_rn(x[j], inverse)), -127.0f, 127.0f);
+    w |= (static_cast<uint32_t>(static_cast<int>(y)) & 0xffu) << (8 * j);
+  }
+  return w;
+}
+
+// The codes' factor of a row with largest magnitude a, and their step.
+__device__ __forceinline__ float code_factor(float a) { return a > 0.0f ? div_rn(127.0f, a) : 0.0f; }
+__device__ __forceinline__ float code_step(float a) { return mul_rn(a, 1.0f / 127.0f); }
+
+// The codes and steps of all query rows, D / 8 lanes a row; step -1 marks a row that does not count.
 template <int D>
 __global__ __launch_bounds__(256) void codes_kernel(Cache c, Run q, int8_t *codes, float *steps, int64_t rows) {
-  constexpr int kE = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  constexpr int kLanes = D / 8;
+  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int part = threadIdx.x % kLanes;
   if (row >= rows) return;
   const int32_t h = static_cast<int32_t>(row % q.heads), t = static_cast<int32_t>(row / q.heads % q.len);
   const int32_t s = static_cast<int32_t>(row / q.heads / q.len);
-  float x[kE], a = 0.0f;
-  bool bad = t >= q.count(s);
-  if (!bad) {
-    const uint16_t *p = q.q + s * q.ss + t * q.st + h * q.sh + lane * kE;
+  const bool counts = t < q.count(s);
+  float x[8], a = 0.0f;
+  to_floats(counts ? *reinterpret_cast<const uint4 *>(q.q + s * q.ss + t * q.st + h * q.sh + part * 8) : uint4{0, 0, 0, 0},
+            q.fp16, x);
+  int bad = !counts;
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      x[j] = q.fp16 ? f16_bits_to_f32(p[j]) : bf16_bits_to_f32(p[j]);
-      a = fmaxf(a, fabsf(x[j]));
-      bad = bad || !(fabsf(x[j]) < __builtin_huge_valf());
-    }
-    a = wave_max(a);
+  for (int j = 0; j < 8; ++j) {
+    a = fmaxf(a, fabsf(x[j]));
+    bad |= !(fabsf(x[j]) < __builtin_huge_valf());
   }
-  bad = __any(bad);
-  const float inverse = bad || a == 0.0f ? 0.0f : div_rn(127.0f, a);
 #pragma unroll
-  for (int j = 0; j < kE; ++j) {
-    const float y = bad ? 0.0f : __builtin_amdgcn_fmed3f(rintf(mul_rn(x[j], inverse)), -127.0f, 127.0f);
-    codes[row * D + lane * kE + j] = static_cast<int8_t>(static_cast<int>(y));
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    a = fmaxf(a, __shfl_xor(a, o, kWave));
+    bad |= __shfl_xor(bad, o, kWave);
   }
-  if (lane == 0) steps[row] = bad ? -1.0f : mul_rn(a, 1.0f / 127.0f);
+  const float f = bad ? 0.0f : code_factor(a);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
+  *reinterpret_cast<uint2 *>(codes + row * D + part * 8) = uint2{four_codes(x, f), four_codes(x + 4, f)};
+  if (part == 0) steps[row] = bad ? -1.0f : code_step(a);
 }
 
 // The bytes of w that are positive, and those that are negative.
@@ -83,12 +108,78 @@ __device__ __forceinline__ void parts(int w, int &pos, int &neg) {
   pos = static_cast<int>(static_cast<uint32_t>(w) & ~m);
 }
 
-// A wave scores 16 blocks for one run: S = bounds x codes^T, so a lane holds
-// four blocks of one row, and the largest over the rows stays in its registers.
+// Codes of 16 rows as the B operand: lane % 16 is the row, lane / 16 and k name 16 channels.
+template <int D>
+struct RowCodes {
+  i4 pos[D / 64], neg[D / 64];
+  float step;  // -1: the row does not count
+
+  __device__ __forceinline__ void split(int k, i4 w) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int a, b;
+      parts(w[j], a, b);
+      pos[k][j] = a;
+      neg[k][j] = b;
+    }
+  }
+};
+
+// Bounds of 16 blocks as the A operand, and the steps of the lane's four of the results.
+template <int D>
+struct BlockBounds {
+  i4 hi[D / 64], lo[D / 64];
+  float u[4];
+};
+
+template <int D>
+__device__ __forceinline__ void load_bounds(BlockBounds<D> &x, const Cache &c, int64_t sh, int32_t b0, int32_t blocks,
+                                            float unit_factor) {
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int32_t mine = b0 + col < blocks ? b0 + col : blocks - 1;
+  const int8_t *p = c.bounds + (sh * c.blocks + mine) * 2 * D + quad * 16;
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    x.hi[k] = *reinterpret_cast<const i4 *>(p + k * 64);
+    x.lo[k] = *reinterpret_cast<const i4 *>(p + D + k * 64);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int32_t b = b0 + quad * 4 + i;
+    x.u[i] = mul_rn(c.key_scale[sh * c.blocks + (b < blocks ? b : blocks - 1)], unit_factor);
+  }
+}
+
+// best[i] = max(best[i], the lane's row's score of block 4 (lane / 16) + i)
+template <int D>
+__device__ __forceinline__ void score16(const BlockBounds<D> &x, const RowCodes<D> &r, float (&best)[4]) {
+  i4 acc = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) {
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[k], r.pos[k], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[k], r.neg[k], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = mul_rn(mul_rn(static_cast<float>(acc[i]), x.u[i]), r.step);
+    best[i] = r.step >= 0.0f ? fmaxf(best[i], v) : best[i];
+  }
+}
+
+// The largest over the 16 rows; a block whose scale is no finite number is
+// chosen, so that its NaN shows.
+__device__ __forceinline__ float over_rows(float best, float u) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) best = fmaxf(best, __shfl_xor(best, o, kWave));
+  return u < __builtin_huge_valf() ? best : __builtin_huge_valf();
+}
+
+// Scores for runs of many rows: a wave takes 64 blocks, whose bounds stay in registers, through all rows of
+// a run.
 template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t *codes, const float *steps,
                                                     float unit_factor, float *score, int32_t chunks) {
-  constexpr int kK = D / 64;
+  constexpr int kB = 4;  // 16-block groups
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int32_t unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;  // unit: (sequence, run, head)
   const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
@@ -99,55 +190,32 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
   const int32_t t0 = run * q.run;
   const int32_t rows = ((count - t0 < q.run) ? count - t0 : q.run) * q.group;
   const int64_t sh = int64_t(s) * c.heads + h;
-  for (int32_t b0 = (chunk * 4 + wave) * 16; b0 < blocks; b0 += chunks * 64) {
-    i4 hi[kK], lo[kK];
-    const int32_t mine = b0 + col < blocks ? b0 + col : blocks - 1;
-    const int8_t *p = c.bounds + (sh * c.blocks + mine) * 2 * D + quad * 16;
+  for (int32_t b0 = (chunk * 4 + wave) * 16 * kB; b0 < blocks; b0 += chunks * 64 * kB) {
+    BlockBounds<D> x[kB];
+    float best[kB][4];
 #pragma unroll
-    for (int k = 0; k < kK; ++k) {
-      hi[k] = *reinterpret_cast<const i4 *>(p + k * 64);
-      lo[k] = *reinterpret_cast<const i4 *>(p + D + k * 64);
-    }
-    float u[4], best[4];
+    for (int n = 0; n < kB; ++n) {
+      load_bounds<D>(x[n], c, sh, b0 + 16 * n, blocks, unit_factor);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int32_t b = b0 + quad * 4 + i;
-      u[i] = mul_rn(c.key_scale[sh * c.blocks + (b < blocks ? b : blocks - 1)], unit_factor);
-      best[i] = mf::kNegInf;
+      for (int i = 0; i < 4; ++i) best[n][i] = mf::kNegInf;
     }
     for (int32_t r0 = 0; r0 < rows; r0 += 16) {
       const int32_t r = r0 + col < rows ? r0 + col : rows - 1;  // the last row again: it changes no maximum
       const int64_t at = (int64_t(s) * q.len + t0 + r / q.group) * q.heads + h * q.group + r % q.group;
-      const float step = steps[at];
-      i4 acc = {0, 0, 0, 0};
+      RowCodes<D> rc;
+      rc.step = steps[at];
 #pragma unroll
-      for (int k = 0; k < kK; ++k) {
-        const i4 w = *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16);
-        i4 pos, neg;
+      for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          int a, b;
-          parts(w[j], a, b);
-          pos[j] = a;
-          neg[j] = b;
-        }
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(hi[k], pos, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(lo[k], neg, acc, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = mul_rn(mul_rn(static_cast<float>(acc[i]), u[i]), step);
-        best[i] = step >= 0.0f ? fmaxf(best[i], v) : best[i];
-      }
+      for (int n = 0; n < kB; ++n) score16<D>(x[n], rc, best[n]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int n = 0; n < kB; ++n) {
 #pragma unroll
-      for (int o = 1; o < 16; o <<= 1) best[i] = fmaxf(best[i], __shfl_xor(best[i], o, kWave));
-      const int32_t b = b0 + quad * 4 + i;
-      if (col == 0 && b < blocks) {
-        // a block whose scale is no finite number is chosen, so that its NaN shows
-        score[int64_t(unit) * c.blocks + b] = u[i] < __builtin_huge_valf() ? best[i] : __builtin_huge_valf();
+      for (int i = 0; i < 4; ++i) {
+        const float v = over_rows(best[n][i], x[n].u[i]);
+        const int32_t b = b0 + 16 * n + quad * 4 + i;
+        if (col == 0 && b < blocks) score[int64_t(unit) * c.blocks + b] = v;
       }
     }
   }
@@ -159,17 +227,26 @@ __device__ __forceinline__ uint32_t ordered(float v) {
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+constexpr int32_t kKept = 8192;  // scores that choose_kernel holds in LDS
+
 // One workgroup per (sequence, run, head).  Blocks before `low` and from
-// `high` on are chosen anyway; of the others the `want` highest.
-__global__ __launch_bounds__(256) void choose_kernel(Cache c, Run q, const float *score, int32_t *out) {
-  __shared__ int32_t hist[256];
-  __shared__ int32_t shared[4];
-  __shared__ int32_t wave_eq[4], wave_in[4];
+// `high` on are chosen anyway; of the others the `want` highest: their
+// smallest score is found two bits a round (each wave counts its keys by
+// ballots and adds three counts to one LDS word), then the chosen are written
+// by prefix sums.  With FUSED (runs of at most 16 rows) the scores are computed here, 16 blocks a
+// wave and step, so that a decode step's choice is one launch.
+template <int T, int D, bool FUSED>
+__global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_factor, float *score, int32_t *out) {
+  constexpr int kWaves = T / kWave;
+  __shared__ uint32_t kept[kKept];
+  __shared__ unsigned long long counts[3];
+  __shared__ int32_t wave_eq[kWaves], wave_in[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t unit = blockIdx.x;
-  const int32_t run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
+  const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
   const int32_t length = c.length(s), count = q.count(s);
-  const float *sc = score + int64_t(unit) * c.blocks;
+  const int64_t sh = int64_t(s) * c.heads + h;
+  float *sc = score + int64_t(unit) * c.blocks;
   int32_t *list = out + int64_t(unit) * q.budget;
   int32_t first, last, blocks = 0, low = 0, high = 0;
   if (q.keys(length, count, run, first, last)) {
@@ -178,65 +255,138 @@ __global__ __launch_bounds__(256) void choose_kernel(Cache c, Run q, const float
     low = q.sink < blocks ? q.sink : blocks;
     high = high < low ? low : high;
   }
+  const int32_t n = high - low;  // blocks to choose from
   const int32_t want = q.budget - low - (blocks - high);
+  const bool all = want >= n, held = n <= kKept;
+  if (!all) {
+    if constexpr (FUSED) {
+      const int col = lane & 15, quad = lane >> 4;
+      const int32_t t0 = run * q.run, rows = ((count - t0 < q.run) ? count - t0 : q.run) * q.group;
+      RowCodes<D> rc;
+      float x[D / 64][2][8], a = 0.0f;
+      int bad = col >= rows;
+      const int32_t r = bad ? 0 : col;
+      const uint16_t *p = q.q + s * q.ss + (t0 + r / q.group) * q.st + (h * q.group + r % q.group) * q.sh + quad * 16;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          to_floats(*reinterpret_cast<const uint4 *>(p + k * 64 + i * 8), q.fp16, x[k][i]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            a = fmaxf(a, fabsf(x[k][i][j]));
+            bad |= !(fabsf(x[k][i][j]) < __builtin_huge_valf());
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o < 64; o <<= 1) {
+        a = fmaxf(a, __shfl_xor(a, o, kWave));
+        bad |= __shfl_xor(bad, o, kWave);
+      }
+      const float f = bad ? 0.0f : code_factor(a);
+      rc.step = bad ? -1.0f : code_step(a);
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        i4 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[k][i][j] = bad ? 0.0f : x[k][i][j];
+          w[2 * i] = static_cast<int>(four_codes(x[k][i], f));
+          w[2 * i + 1] = static_cast<int>(four_codes(x[k][i] + 4, f));
+        }
+        rc.split(k, w);
+      }
+      for (int32_t b0 = low + wave * 16; b0 < high; b0 += kWaves * 16) {
+        BlockBounds<D> bb;
+        load_bounds<D>(bb, c, sh, b0, high, unit_factor);
+        float best[4] = {mf::kNegInf, mf::kNegInf, mf::kNegInf, mf::kNegInf};
+        score16<D>(bb, rc, best);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = over_rows(best[i], bb.u[i]);
+          const int32_t b = b0 + quad * 4 + i;
+          if (col == 0 && b < high) {
+            if (held) {
+              kept[b - low] = ordered(v);
+            } else {
+              sc[b] = v;
+            }
+          }
+        }
+      }
+    } else if (held) {
+      for (int32_t i = tid; i < n; i += T) kept[i] = ordered(sc[low + i]);
+    }
+  }
+  if (tid < 3) counts[tid] = 0;
+  __syncthreads();  // also orders this workgroup's writes of `score` before its reads
+  auto key = [&](int32_t i) { return held ? kept[i] : ordered(sc[low + i]); };
+
   uint32_t threshold = 0;
   int32_t equals = 0;  // blocks at the threshold that are chosen
-  if (want < high - low) {
-    // the want-th highest of [low, high), eight bits at a time
-    int32_t need = want > 0 ? want : 0;
-    if (need == 0) {
-      threshold = 0xffffffffu;
-    } else {
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int32_t b = low + tid; b < high; b += 256) {
-          const uint32_t key = ordered(sc[b]);
-          if (shift == 24 || (key >> (shift + 8)) == (threshold >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-        }
-        __syncthreads();
-        // thread i: keys in bins above i
-        int32_t above = 0;
-        for (int i = tid + 1; i < 256; ++i) above += hist[i];
-        if (above < need && above + hist[tid] >= need) {
-          shared[0] = tid;
-          shared[1] = above;
-        }
-        __syncthreads();
-        threshold |= static_cast<uint32_t>(shared[0]) << shift;
-        need -= shared[1];
-        __syncthreads();
+  if (!all && want > 0) {
+    int32_t need = want;
+    for (int round = 0; round < 16; ++round) {
+      const int shift = 30 - 2 * round;
+      // keys with the threshold's upper bits whose next two are 3, at least 2, at least 1
+      uint32_t c3 = 0, c2 = 0, c1 = 0;
+      for (int32_t i = tid; i - lane < n; i += T) {
+        const uint32_t k = i < n ? key(i) : 0;
+        const bool in = i < n && (round == 0 || (k >> (shift + 2)) == (threshold >> (shift + 2)));
+        const uint32_t digit = (k >> shift) & 3u;
+        c3 += __popcll(__ballot(in && digit == 3));
+        c2 += __popcll(__ballot(in && digit >= 2));
+        c1 += __popcll(__ballot(in && digit >= 1));
       }
-      equals = need;
+      if (lane == 0) {
+        atomicAdd(&counts[round % 3], c3 | (static_cast<unsigned long long>(c2) << 21) |
+                                          (static_cast<unsigned long long>(c1) << 42));
+      }
+      if (tid == 0) counts[(round + 1) % 3] = 0;  // last read two rounds ago
+      __syncthreads();
+      const unsigned long long sum = counts[round % 3];
+      const int32_t n3 = static_cast<int32_t>(sum & 0x1fffffu), n2 = static_cast<int32_t>((sum >> 21) & 0x1fffffu);
+      const int32_t n1 = static_cast<int32_t>(sum >> 42);
+      const uint32_t digit = need <= n3 ? 3u : need <= n2 ? 2u : need <= n1 ? 1u : 0u;
+      need -= digit == 3 ? 0 : digit == 2 ? n3 : digit == 1 ? n2 : n1;
+      threshold |= digit << shift;
+    }
+    equals = need;
+  }
+  for (int32_t i = tid; i < low; i += T) list[i] = i;
+  int32_t written = low, seen_equal = 0;
+  if (all) {
+    for (int32_t i = tid; i < n; i += T) list[low + i] = low + i;
+    written += n;
+  } else if (want > 0) {
+    for (int32_t i0 = 0; i0 < n; i0 += T) {
+      const int32_t i = i0 + tid;
+      const uint32_t k = i < n ? key(i) : 0;
+      const bool equal = i < n && k == threshold;
+      const uint64_t eq = __ballot(equal), before = (uint64_t(1) << lane) - 1;
+      if (lane == 0) wave_eq[wave] = __popcll(eq);
+      __syncthreads();
+      int32_t rank = seen_equal + __popcll(eq & before);
+      for (int v = 0; v < kWaves; ++v) {
+        if (v < wave) rank += wave_eq[v];
+        seen_equal += wave_eq[v];
+      }
+      const bool in = i < n && (k > threshold || (equal && rank < equals));
+      const uint64_t chosen = __ballot(in);
+      if (lane == 0) wave_in[wave] = __popcll(chosen);
+      __syncthreads();
+      int32_t at = written + __popcll(chosen & before);
+      for (int v = 0; v < kWaves; ++v) {
+        if (v < wave) at += wave_in[v];
+        written += wave_in[v];
+      }
+      if (in) list[at] = low + i;
     }
   }
-  const bool all = want >= high - low;
-  int32_t written = 0, seen_equal = 0;
-  for (int32_t b0 = 0; b0 < blocks; b0 += 256) {
-    const int32_t b = b0 + tid;
-    const bool live = b < blocks, must = live && (b < low || b >= high || all);
-    const uint32_t key = live && !must ? ordered(sc[b]) : 0;
-    const bool equal = live && !must && key == threshold;
-    const uint64_t eq = __ballot(equal);
-    if (lane == 0) wave_eq[wave] = __popcll(eq);
-    __syncthreads();
-    int32_t rank = seen_equal + __popcll(eq & ((uint64_t(1) << lane) - 1));
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) rank += wave_eq[w];
-      seen_equal += wave_eq[w];
-    }
-    const bool in = must || (live && (key > threshold || (equal && rank < equals)));
-    const uint64_t chosen = __ballot(in);
-    if (lane == 0) wave_in[wave] = __popcll(chosen);
-    __syncthreads();
-    int32_t at = written + __popcll(chosen & ((uint64_t(1) << lane) - 1));
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) at += wave_in[w];
-      written += wave_in[w];
-    }
-    if (in && at < q.budget) list[at] = b;
-  }
-  for (int32_t i = written + tid; i < q.budget; i += 256) list[i] = -1;
+  for (int32_t i = tid; i < blocks - high; i += T) list[written + i] = high + i;
+  for (int32_t i = written + blocks - high + tid; i < q.budget; i += T) list[i] = -1;
 }
 
 int make_run(const uc_block8_cache *cache, const uc_block8_query *query, int64_t query_block, const char *what, Run &q) {
@@ -299,6 +449,7 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t span = q.causal ? ceil_div(int64_t(q.run) - 1, int64_t(c.block)) : 0;
   UC_REQUIRE(sink + recent + span <= budget, "uc_block8_select: budget %lld is less than the %lld blocks always chosen",
              static_cast<long long>(budget), static_cast<long long>(sink + recent + span));
+  UC_REQUIRE(cache->blocks < (1 << 21), "uc_block8_select: too many blocks");  // counted in 21 bits
   if (q.len == 0) return UC_OK;
   UC_REQUIRE(q.q != nullptr && (reinterpret_cast<uintptr_t>(q.q) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,
              "uc_block8_select: query must be 16-byte aligned with strides that are multiples of 8");
@@ -315,22 +466,25 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t rows = cache->sequences * q.len * q.heads, units = cache->sequences * q.runs * cache->heads_kv;
   const int64_t capacity = cache->blocks * cache->block_tokens;
   const int64_t expected = query->max_tokens < capacity ? query->max_tokens : capacity;
-  const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 64) : 1;
+  const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 256) : 1;
   UC_REQUIRE(rows < (int64_t(1) << 32) && units * chunks < (int64_t(1) << 31), "uc_block8_select: too many query rows");
   const float factor = cache->code_dtype == UC_INT8 ? 1.0f : static_cast<float>(448.0 / 127.0);
   auto launch = [&](auto d_tag) {
     constexpr int D = decltype(d_tag)::value;
-    hipLaunchKernelGGL((codes_kernel<D>), dim3(static_cast<uint32_t>(ceil_div(rows, 4))), dim3(256), 0,
+    if (q.run * q.group <= 16) {
+      hipLaunchKernelGGL((choose_kernel<1024, D, true>), dim3(static_cast<uint32_t>(units)), dim3(1024), 0,
+                         as_stream(stream), c, q, factor, score, blocks);
+      return check_launch("uc_block8_select");
+    }
+    hipLaunchKernelGGL((codes_kernel<D>), dim3(static_cast<uint32_t>(ceil_div(rows, 256 / (D / 8)))), dim3(256), 0,
                        as_stream(stream), c, q, codes, steps, rows);
     if (int rc = check_launch("uc_block8_select (codes)")) return rc;
     hipLaunchKernelGGL((score_kernel<D>), dim3(static_cast<uint32_t>(units * chunks)), dim3(256), 0, as_stream(stream),
                        c, q, codes, steps, factor, score, static_cast<int32_t>(chunks));
-    return check_launch("uc_block8_select (scores)");
+    if (int rc = check_launch("uc_block8_select (scores)")) return rc;
+    hipLaunchKernelGGL((choose_kernel<256, D, false>), dim3(static_cast<uint32_t>(units)), dim3(256), 0,
+                       as_stream(stream), c, q, factor, score, blocks);
+    return check_launch("uc_block8_select");
   };
-  if (int rc = cache->head_dim == 128 ? launch(std::integral_constant<int, 128>())
-                                      : launch(std::integral_constant<int, 64>()))
-    return rc;
-  hipLaunchKernelGGL(choose_kernel, dim3(static_cast<uint32_t>(units)), dim3(256), 0, as_stream(stream), c, q, score,
-                     blocks);
-  return check_launch("uc_block8_select");
+  return cache->head_dim == 128 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 64>());
 }
