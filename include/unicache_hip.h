@@ -748,7 +748,8 @@ typedef struct uc_block8_cache {
 } uc_block8_cache;
 
 /*
- * Quantize the first min(lengths[s], tokens) rows of each sequence of dense
+ * Quantize the first rows of each sequence, row_counts[s] of them read into
+ * [0, tokens] (device int32; NULL: tokens), and set the cache's lengths to their number: dense
  * key / value [S, tokens, Hkv, D] (element (s, t, h, d) at s*ss + t*st + h*sh + d;
  * strides multiples of 8, 16-byte aligned) into the cache's blocks
  * 0 .. ceil(tokens / block_tokens) - 1; every code, scale and bound of those
@@ -758,7 +759,7 @@ typedef struct uc_block8_cache {
  */
 int uc_block8_pack(const uc_block8_cache *cache, const void *key, int64_t k_ss, int64_t k_st, int64_t k_sh,
                    const void *value, int64_t v_ss, int64_t v_st, int64_t v_sh, int in_dtype, int64_t tokens,
-                   void *tail, uc_stream_t stream);
+                   const int32_t *row_counts, void *tail, uc_stream_t stream);
 
 /*
  * Append rows to every sequence and advance `lengths` on the device: sequence

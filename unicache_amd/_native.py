@@ -239,7 +239,7 @@ _SIGNATURES = {
         _I,
         [_P, _P, _L, _L, _L, _I, _L, _L, _P, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P],
     ),
-    "uc_block8_pack": (_I, [ctypes.POINTER(Block8Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _P]),
+    "uc_block8_pack": (_I, [ctypes.POINTER(Block8Cache), _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _P, _P]),
     "uc_block8_append": (_I, [ctypes.POINTER(Block8Cache), _P, _P, _L, _L, _L, _P, _L, _L, _L, _I, _L, _P, _P]),
     "uc_block8_dequant": (_I, [ctypes.POINTER(Block8Cache), _P, _P, _I, _L, _P]),
     "uc_block8_attn": (

@@ -272,12 +272,14 @@ struct Dense {
 
 template <int D, int B, int CODE, int IN>
 __global__ __launch_bounds__((Shape<D, B>::kThreads)) void pack_kernel(Cache cache, Dense key, Dense value,
-                                                                       int32_t tokens, uint16_t *tail) {
+                                                                       int32_t tokens, const int32_t *row_counts,
+                                                                       int32_t *lengths, uint16_t *tail) {
   typedef Shape<D, B> S;
   __shared__ Shared<D, B> sh;
   const int32_t b = blockIdx.x, sequence = blockIdx.y / cache.heads, h = blockIdx.y % cache.heads;
-  int32_t length = cache.length(sequence);
-  length = length < tokens ? length : tokens;
+  int32_t length = row_counts != nullptr ? row_counts[sequence] : tokens;
+  length = length < 0 ? 0 : length > tokens ? tokens : length;
+  if (b == 0 && h == 0 && threadIdx.x == 0) lengths[sequence] = length;
   int rows = length - b * B;
   rows = rows < 0 ? 0 : rows > B ? B : rows;
   uint4 x[S::kPer][4], y[S::kPer][4];
@@ -473,7 +475,7 @@ int check_dense(const char *what, const void *p, int64_t ss, int64_t st, int64_t
 
 extern "C" int uc_block8_pack(const uc_block8_cache *cache, const void *key, int64_t k_ss, int64_t k_st, int64_t k_sh,
                               const void *value, int64_t v_ss, int64_t v_st, int64_t v_sh, int in_dtype,
-                              int64_t tokens, void *tail, uc_stream_t stream) {
+                              int64_t tokens, const int32_t *row_counts, void *tail, uc_stream_t stream) {
   using namespace uc;
   using namespace uc::b8;
   Cache c;
@@ -492,7 +494,7 @@ extern "C" int uc_block8_pack(const uc_block8_cache *cache, const void *key, int
       return UC_B8_DISPATCH_HALF(in_dtype, IN, [&] {
         const dim3 grid(static_cast<uint32_t>(ceil_div(tokens, B)), static_cast<uint32_t>(c.sequences * c.heads));
         hipLaunchKernelGGL((pack_kernel<D, B, CODE, IN>), grid, dim3(Shape<D, B>::kThreads), 0, as_stream(stream), c, k,
-                           v, static_cast<int32_t>(tokens), static_cast<uint16_t *>(tail));
+                           v, static_cast<int32_t>(tokens), row_counts, cache->lengths, static_cast<uint16_t *>(tail));
         return check_launch("uc_block8_pack");
       });
     });

@@ -18,6 +18,7 @@ struct Query {
   int32_t len, heads, group;
   int32_t fp16, causal;
   float scale;  // sm_scale * log2(e)
+  FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const {
     if (lens == nullptr) return len;
@@ -32,6 +33,7 @@ struct Plan {
   int32_t run, runs;    // query tokens that share a list (without lists: all), and how many such runs
   int32_t groups, rows; // row groups of a run, and their rows
   int32_t splits, split_tiles;
+  int32_t workgroups;   // few rows: workgroups that share all tiles; 0: one workgroup a unit
 };
 
 // The rows of a workgroup: `first` + r / group is row r's query token.
@@ -47,25 +49,36 @@ __device__ __forceinline__ int32_t visible(const Query &q, int32_t length, int32
   return e < 0 ? 0 : e;
 }
 
-__device__ __forceinline__ Rows rows_of(const Cache &c, const Query &q, const Plan &p, int32_t unit, int rows) {
+// Row r's token, counted from the run's first, and its head in the group.
+__device__ __forceinline__ int32_t token_of(const Query &q, int32_t r) { return static_cast<int32_t>(fast_div(r, q.by_group)); }
+
+// Rows of group g of a run, with its sequence's length and number of queries.
+__device__ __forceinline__ Rows rows_at(const Query &q, const Plan &p, int32_t s, int32_t h, int32_t run, int32_t g, int rows,
+                                        int32_t length, int32_t count) {
   Rows w;
-  const int32_t g = unit % p.groups, run = unit / p.groups % p.runs, sh = unit / p.groups / p.runs;
-  w.s = sh / c.heads;
-  w.h = sh % c.heads;
-  w.length = c.length(w.s);
-  w.count = q.count(w.s);
+  w.s = s;
+  w.h = h;
+  w.length = length;
+  w.count = count;
   w.run0 = run * p.run;
   const int32_t tokens = q.len - w.run0 < p.run ? q.len - w.run0 : p.run;
   w.run_rows = tokens * q.group;
   w.r0 = g * rows;
-  const int32_t t0 = w.run0 + w.r0 / q.group;
+  const int32_t t0 = w.run0 + token_of(q, w.r0);
   const int32_t r1 = (w.r0 + rows < w.run_rows ? w.r0 + rows : w.run_rows) - 1;
-  int32_t t1 = w.run0 + r1 / q.group;
+  int32_t t1 = w.run0 + token_of(q, r1);
   t1 = t1 < w.count ? t1 : w.count - 1;
   const bool none = w.r0 >= w.run_rows || t0 >= w.count;
   w.end_first = none ? 0 : visible(q, w.length, w.count, t0);
   w.end_last = none ? 0 : visible(q, w.length, w.count, t1);
   return w;
+}
+
+// Rows of unit ((sequence, head, run, group) in order).
+__device__ __forceinline__ Rows rows_of(const Cache &c, const Query &q, const Plan &p, int32_t unit, int rows) {
+  const int32_t g = unit % p.groups, run = unit / p.groups % p.runs, sh = unit / p.groups / p.runs;
+  const int32_t s = sh / c.heads;
+  return rows_at(q, p, s, sh % c.heads, run, g, rows, c.length(s), q.count(s));
 }
 
 // Tiles of a workgroup's rows, over all splits.
@@ -78,6 +91,52 @@ __device__ __forceinline__ int32_t tiles_of(const Cache &c, const Plan &p, const
 __device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) {
   const int32_t least = (tiles + p.splits - 1) / p.splits;
   return least > p.split_tiles ? least : p.split_tiles;
+}
+
+// Few rows: the tiles of all units ((sequence, head, run) in order) are cut into runs of equal
+// length for the workgroups, so that sequences of any lengths load them alike (32 sequences of 8k
+// tokens down to none: 74 us by equal splits of the longest, 65 so).  A unit's piece in workgroup g leaves its partial in slot
+// g + unit: of two pieces in order one of the two is larger.
+// Steps of one (head, run) of a sequence of so many keys: its tiles, rounded up to one for each of
+// the four waves.
+__device__ __forceinline__ int32_t steps_of(int32_t keys) { return (keys + 4 * kTile - 1) / (4 * kTile) * 4; }
+
+// Keys that a sequence's rows read.
+__device__ __forceinline__ int32_t keys_of(const Cache &c, const Plan &p, int32_t length, int32_t count) {
+  return p.list != nullptr ? p.budget * c.block : count > 0 ? length : 0;
+}
+
+__device__ __forceinline__ int32_t per_of(const Plan &p, int32_t total) {
+  return ((total + p.workgroups - 1) / p.workgroups + 3) / 4 * 4;
+}
+
+// A wave's sum, the same in every lane.
+__device__ __forceinline__ int32_t wave_total(int32_t v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
+
+// For a wave: steps of all sequences (of one head and run), of those before s, and of s.
+struct Steps {
+  int32_t total, before, mine;
+};
+
+__device__ __forceinline__ Steps steps_before(const Cache &c, const Query &q, const Plan &p, int32_t s) {
+  Steps w = {0, 0, 0};
+  if (p.list != nullptr) {
+    w.mine = steps_of(keys_of(c, p, 0, 0));
+    w.total = w.mine * c.sequences;
+    w.before = w.mine * s;
+    return w;
+  }
+  for (int32_t s0 = 0; s0 < c.sequences; s0 += 64) {
+    const int32_t i = s0 + (threadIdx.x & 63);
+    const int32_t n = i < c.sequences ? steps_of(keys_of(c, p, c.length(i), q.count(i))) : 0;
+    const int32_t sum = wave_prefix(n);
+    if (s >= s0 && s < s0 + 64) {
+      w.mine = __builtin_amdgcn_readlane(n, s - s0);
+      w.before = w.total + __builtin_amdgcn_readlane(sum, s - s0) - w.mine;
+    }
+    w.total += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return w;
 }
 
 // First key of a half tile (32 keys); kNone where the list has none there.
@@ -121,12 +180,12 @@ __device__ __forceinline__ float rescaled(float l, float d) {
 template <int D, bool PAIRS>
 __device__ __forceinline__ float load_query(const Query &q, const Rows &w, int32_t r, h8 (&frag)[D / 32]) {
   const int quad = (threadIdx.x & 63) >> 4;
-  const int32_t token = w.run0 + r / q.group;
+  const int32_t token = w.run0 + token_of(q, r);
   uint4 raw[D / 32];
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) raw[k] = uint4{0, 0, 0, 0};
   if (r < w.run_rows && token < w.count) {
-    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r % q.group) * q.sh;
+    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r - token_of(q, r) * q.group) * q.sh;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       raw[k] = *reinterpret_cast<const uint4 *>(p + (PAIRS ? (k / 2) * 64 + quad * 16 + (k % 2) * 8 : k * 32 + quad * 8));

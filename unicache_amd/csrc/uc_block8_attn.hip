@@ -1,7 +1,7 @@
-// Attention over the 8-bit block-scaled cache, by split keys: every workgroup
-// takes up to 16 NR query rows of one KV head (its query heads x query tokens)
-// and a run of 64-key tiles, its four waves alternate tiles, and what they hold is
-// joined at the end; a second launch joins the splits.
+// Attention over the 8-bit block-scaled cache for few query rows, by split keys:
+// a workgroup takes up to 16 NR query rows of one KV head (its query heads x
+// query tokens) and a run of 64-key tiles, its four waves alternate tiles, and what
+// they hold is joined at the end; a second launch joins the workgroups' parts.
 //
 // Mathematics, per row r and key t of block b, in base 2:
 //   x = (q_r . k_t) ks_b sm_scale log2(e) + log2(vs_b)
@@ -113,37 +113,24 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[4], floa
   acc.l += sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_rcpf(vs);
 }
 
+// LDS of the waves' join.
+template <int D>
+struct Joined {
+  float o[4][16][D + 4];
+  float m[4][16], l[4][16];
+};
+
+// Tiles begin .. end - 1 of the rows w, by a whole workgroup.  slot >= 0: the part goes there; else it
+// is all there is, and the rows are finished.
 template <int D, int CODE, int NR>
-__global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
-                                                      float *part, float *stat) {
-  constexpr int kPitch = D + 4;
-  __shared__ float sh_o[4][16][kPitch];
-  __shared__ float sh_m[4][16], sh_l[4][16];
+__device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan &p, const Rows &w, int32_t begin, int32_t end,
+                                      int32_t slot, Joined<D> &joined, uint16_t *out, float *lse, float *part,
+                                      float *stat) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
             quad = lane >> 4;
-  const int32_t split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
-  const Rows w = rows_of(c, q, p, unit, 16 * NR);
-  const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
-  const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
-  if (begin >= end && split > 0) return;  // the first split of rows without keys writes what they get
   const int64_t sh = int64_t(w.s) * c.heads + w.h;
   const int32_t *list = p.list == nullptr ? nullptr : p.list + ((int64_t(w.s) * p.runs + w.run0 / p.run) * c.heads + w.h) * p.budget;
 
-  h8 frag[NR][D / 32];
-  float factor[NR];
-  int32_t row_end[NR];
-  Acc<D> acc[NR];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int32_t r = w.r0 + 16 * n + col;
-    factor[n] = load_query<D, true>(q, w, r, frag[n]);
-    row_end[n] = visible(q, w.length, w.count, w.run0 + r / q.group);
-    row_end[n] = row_end[n] < w.length ? row_end[n] : w.length;
-    acc[n].m = mf::kNegInf;
-    acc[n].l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
-  }
   const int32_t tokens = c.blocks << c.shift;
   Lane<D> l;
   l.key = (quad & 1) * 16;
@@ -162,6 +149,21 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
     if (t1 >= tokens) t1 = kNone;
     load_keys(raw, c, l, t0, t1);
     load_values(raw, c, l, t0, t1);
+  }
+  h8 frag[NR][D / 32];
+  float factor[NR];
+  int32_t row_end[NR];
+  Acc<D> acc[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int32_t r = w.r0 + 16 * n + col;
+    factor[n] = load_query<D, true>(q, w, r, frag[n]);
+    row_end[n] = visible(q, w.length, w.count, w.run0 + token_of(q, r));
+    row_end[n] = row_end[n] < w.length ? row_end[n] : w.length;
+    acc[n].m = mf::kNegInf;
+    acc[n].l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
   }
   for (; t < end; t += 4) {
     int32_t n0 = kNone, n1 = kNone;
@@ -221,31 +223,32 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const float l_row = mf::sum_over_slices(acc[n].l);
-    if (n > 0) __syncthreads();
+    __syncthreads();  // what was joined before has been read
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(&sh_o[wave][col][16 * d + 4 * quad]) = acc[n].o[d];
+    for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(&joined.o[wave][col][16 * d + 4 * quad]) = acc[n].o[d];
     if (quad == 0) {
-      sh_m[wave][col] = acc[n].m;
-      sh_l[wave][col] = l_row;
+      joined.m[wave][col] = acc[n].m;
+      joined.l[wave][col] = l_row;
     }
     __syncthreads();
     float m = mf::kNegInf;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) m = fmaxf(m, sh_m[v][row]);
+    for (int v = 0; v < 4; ++v) m = fmaxf(m, joined.m[v][row]);
     float total = 0.0f, o[kC];
 #pragma unroll
     for (int j = 0; j < kC; ++j) o[j] = 0.0f;
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-      const float mv = sh_m[v][row];
-      const float d = mv == mf::kNegInf && !(sh_l[v][row] != 0.0f) ? mf::kNegInf : mv - m, f = mf::fast_exp2(d);
-      total += rescaled(sh_l[v][row], d);
+      const float mv = joined.m[v][row];
+      const float d = mv == mf::kNegInf && !(joined.l[v][row] != 0.0f) ? mf::kNegInf : mv - m, f = mf::fast_exp2(d);
+      total += rescaled(joined.l[v][row], d);
 #pragma unroll
-      for (int j = 0; j < kC; ++j) o[j] += f * sh_o[v][row][c0 + j];
+      for (int j = 0; j < kC; ++j) o[j] += f * joined.o[v][row][c0 + j];
     }
     const int32_t r = w.r0 + 16 * n + row;
-    if (p.splits > 1) {
-      const int64_t at = (int64_t(blockIdx.x) * (16 * NR) + 16 * n + row);
+    if (slot >= 0) {
+      if (r >= w.run_rows) continue;
+      const int64_t at = int64_t(slot) * (16 * NR) + 16 * n + row;
 #pragma unroll
       for (int j = 0; j < kC; j += 4) {
         *reinterpret_cast<f4 *>(part + at * D + c0 + j) = f4{o[j], o[j + 1], o[j + 2], o[j + 3]};
@@ -255,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
         stat[2 * at + 1] = total;
       }
     } else if (r < w.run_rows) {
-      const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
+      const int32_t token = w.run0 + token_of(q, r), head = w.h * q.group + r - token_of(q, r) * q.group;
       const bool none = token >= w.count || total == 0.0f;
       const float f = none ? 0.0f : 1.0f / total;
       uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + c0;
@@ -268,6 +271,71 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
         lse[(int64_t(w.s) * q.heads + head) * q.len + token] =
             none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(total));
       }
+    }
+  }
+}
+
+template <int D, int CODE, int NR>
+__global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
+                                                      float *part, float *stat) {
+  __shared__ Joined<D> joined;
+  if (p.workgroups == 0) {  // one workgroup a unit
+    const Rows w = rows_of(c, q, p, blockIdx.x, 16 * NR);
+    piece<D, CODE, NR>(c, q, p, w, 0, tiles_of(c, p, w), -1, joined, out, lse, part, stat);
+    return;
+  }
+  // this workgroup's steps, and the sequence, unit and step that they begin at
+  const int lane = threadIdx.x & 63;
+  const int32_t g = blockIdx.x, each = c.heads * p.runs;
+  int32_t s0 = 0, first = 0;  // sequences s0 .. s0 + 63 are in the lanes, `first` of them is the present one
+  int32_t length = 0, count = 0, steps = 0, sum = 0, total;
+  auto fill = [&] {
+    const int32_t i = s0 + lane;
+    length = i < c.sequences ? c.length(i) : 0;
+    count = i < c.sequences ? q.count(i) : 0;
+    steps = i < c.sequences ? steps_of(keys_of(c, p, length, count)) : 0;
+    sum = wave_prefix(steps);
+  };
+  fill();
+  total = c.sequences <= 64 ? __builtin_amdgcn_readlane(sum, 63) : steps_before(c, q, p, 0).total;
+  total *= each;
+  const int32_t per = per_of(p, total);
+  int32_t at = g * per;
+  const int32_t stop = at + per < total ? at + per : total;
+  if (at >= stop) return;
+  int32_t rest = at;  // steps of the present sequence before `at`
+  for (;;) {
+    const uint64_t past = __ballot(sum * each > rest);
+    if (past != 0) {
+      first = __builtin_ctzll(past);
+      break;
+    }
+    rest -= __builtin_amdgcn_readlane(sum, 63) * each;
+    s0 += 64;
+    fill();
+  }
+  int32_t now = __builtin_amdgcn_readlane(steps, first);  // steps of each of the sequence's units
+  rest -= (__builtin_amdgcn_readlane(sum, first) - now) * each;
+  int32_t n = rest / now, t = rest - n * now;  // the unit within the sequence, and its step
+  while (at < stop) {
+    const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
+    const int32_t h = p.runs == 1 ? n : n / p.runs, run = p.runs == 1 ? 0 : n % p.runs;
+    const Rows w = rows_at(q, p, s, h, run, 0, 16 * NR, __builtin_amdgcn_readlane(length, first),
+                           __builtin_amdgcn_readlane(count, first));
+    // (the step's end may lie behind the last tile)
+    piece<D, CODE, NR>(c, q, p, w, t, min(end, tiles_of(c, p, w)), g + s * each + n, joined, out, lse, part, stat);
+    at += end - t;
+    t = 0;
+    if (++n == each && at < stop) {
+      n = 0;
+      do {
+        if (++first == 64) {
+          first = 0;
+          s0 += 64;
+          fill();
+        }
+        now = __builtin_amdgcn_readlane(steps, first);
+      } while (now == 0);
     }
   }
 }
@@ -291,9 +359,20 @@ __global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, int
   const int32_t unit = static_cast<int32_t>((sh * p.runs + run) * p.groups + r / p.rows);
   const Rows w = rows_of(c, q, p, unit, p.rows);
   if (r >= w.run_rows) return;
-  const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
-  const int32_t splits = tiles == 0 ? 1 : (tiles + per - 1) / per;
-  const int64_t base = int64_t(unit) * p.splits * p.rows + r % p.rows;
+  // the parts of the row: consecutive slots
+  int32_t first, splits;
+  if (p.workgroups == 0) {
+    const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
+    first = unit * p.splits;
+    splits = tiles == 0 ? 1 : (tiles + per - 1) / per;
+  } else {
+    const Steps steps = steps_before(c, q, p, w.s);
+    const int32_t each = c.heads * p.runs, n = unit - w.s * each, per = per_of(p, steps.total * each);
+    const int32_t start = steps.before * each + n * steps.mine;
+    first = steps.mine == 0 ? 0 : start / per + unit;
+    splits = steps.mine == 0 ? 0 : (start + steps.mine - 1) / per + unit - first + 1;
+  }
+  const int64_t base = int64_t(first) * p.rows + r % p.rows;
   float m = mf::kNegInf;
   for (int32_t i = lane; i < splits; i += 64) m = fmaxf(m, stat[2 * (base + int64_t(i) * p.rows)]);
   m = wave_max(m);
@@ -329,7 +408,7 @@ __global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, int
 #pragma unroll
     for (int j = 0; j < kC; ++j) o[j] = sh_o[0][lane * kC + j] + sh_o[1][lane * kC + j] + sh_o[2][lane * kC + j] + sh_o[3][lane * kC + j];
   }
-  const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
+  const int32_t token = w.run0 + token_of(q, r), head = w.h * q.group + r - token_of(q, r) * q.group;
   const bool none = token >= w.count || total == 0.0f;
   const float f = none ? 0.0f : 1.0f / total;
   uint16_t v[kC];
@@ -349,6 +428,11 @@ __global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, int
   }
 }
 
+#ifndef KSHARE
+#define KSHARE 512
+#endif
+constexpr int64_t kShare = KSHARE;  // workgroups that share the tiles of few rows: two a CU
+
 int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget, int64_t query_block,
               const char *what, Query &q, Plan &p) {
   UC_REQUIRE(query != nullptr, "%s: query is NULL", what);
@@ -362,7 +446,8 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   UC_REQUIRE(budget == 0 || query_block > 0, "%s: query_block must be positive", what);
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q),
-            static_cast<int32_t>(query->heads_q / cache->heads_kv), query->dtype == UC_FP16, query->causal != 0, 0.0f};
+            static_cast<int32_t>(query->heads_q / cache->heads_kv), query->dtype == UC_FP16, query->causal != 0, 0.0f,
+            make_fastdiv(static_cast<uint32_t>(query->heads_q / cache->heads_kv))};
   p.list = nullptr;
   p.budget = static_cast<int32_t>(budget);
   const int64_t run = budget == 0 || query_block > query->query_len ? (query->query_len > 0 ? query->query_len : 1)
@@ -378,20 +463,31 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   if (budget > 0) keys = budget * cache->block_tokens;
   const int64_t tiles = keys > 0 ? ceil_div(keys, kTile) : 1;
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
-  // about 1024 workgroups (four a CU) of few rows, each wave with a tile at least; 512 (two a CU) of
-  // many rows, each with four tiles
-  int64_t splits = units > 0 ? (p.rows == kTileRows ? 512 : 1024) / units : 1;
-  const int64_t most = ceil_div(tiles, 4);
-  splits = splits < 1 ? 1 : splits > most ? most : splits;
-  p.split_tiles = static_cast<int32_t>(ceil_div(tiles, splits));
-  p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
+  p.workgroups = 0;
+  if (p.rows == kTileRows) {
+    // 512 workgroups (two a CU), each with four tiles at least
+    int64_t splits = units > 0 ? 512 / units : 1;
+    const int64_t most = ceil_div(tiles, 4);
+    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    p.split_tiles = static_cast<int32_t>(ceil_div(tiles, splits));
+    p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
+  } else {
+    p.splits = 1;
+    p.split_tiles = 0;
+    // lists are of one length, so many of them load the CUs alike
+    if (budget == 0 || units < 1024) {
+      const int64_t most = ceil_div(tiles, 4) * units;
+      p.workgroups = static_cast<int32_t>(most < kShare ? (most > 0 ? most : 1) : kShare);
+    }
+  }
   UC_REQUIRE(units * p.splits < (int64_t(1) << 31) / p.rows, "%s: too many query rows", what);
   return UC_OK;
 }
 
 // Floats of the splits' partial outputs and statistics.
 int64_t part_rows(const uc_block8_cache *cache, const Plan &p) {
-  return p.splits > 1 ? cache->sequences * cache->heads_kv * p.runs * p.groups * p.splits * p.rows : 0;
+  const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
+  return p.workgroups > 0 ? (units + p.workgroups) * p.rows : p.splits > 1 ? units * p.splits * p.rows : 0;
 }
 
 }  // namespace
@@ -434,7 +530,7 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   q.scale = sm_scale * kLog2e;
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
-  const uint32_t workgroups = static_cast<uint32_t>(units * p.splits);
+  const uint32_t workgroups = static_cast<uint32_t>(p.workgroups > 0 ? p.workgroups : units * p.splits);
   int rc;
   if (p.rows == kTileRows) {
     rc = launch_tiles(cache, c, q, p, workgroups, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
@@ -450,7 +546,7 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
       return check_launch("uc_block8_attn");
     });
   }
-  if (rc != UC_OK || p.splits == 1) return rc;
+  if (rc != UC_OK || (p.splits == 1 && p.workgroups == 0)) return rc;
   const int64_t q_rows = cache->sequences * cache->heads_kv * p.runs * p.run * q.group;
   auto join = [&](auto d_tag, auto waves_tag) {
     constexpr int D = decltype(d_tag)::value, W = decltype(waves_tag)::value;
@@ -462,6 +558,8 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 64> D64;
   typedef std::integral_constant<int, 128> D128;
-  if (cache->head_dim == 128) return p.splits <= 8 ? join(D128(), One()) : join(D128(), Four());
-  return p.splits <= 8 ? join(D64(), One()) : join(D64(), Four());
+  // parts of a row, if all sequences were of the expected length
+  const bool few = (p.workgroups > 0 ? ceil_div(p.workgroups, units) : p.splits) <= 8;
+  if (cache->head_dim == 128) return few ? join(D128(), One()) : join(D128(), Four());
+  return few ? join(D64(), One()) : join(D64(), Four());
 }

@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   for (int n = 0; n < 2; ++n) {
     const int32_t r = w.r0 + wave * 32 + n * 16 + col;
     factor[n] = load_query<D, false>(q, w, r, frag[n]);
-    const int32_t e = visible(q, w.length, w.count, w.run0 + r / q.group);
+    const int32_t e = visible(q, w.length, w.count, w.run0 + token_of(q, r));
     row_end[n] = e < w.length ? e : w.length;
     acc[n].m = mf::kNegInf;
     acc[n].l = 0.0f;
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         stat[2 * at + 1] = total;
       }
     } else if (r < w.run_rows) {
-      const int32_t token = w.run0 + r / q.group, head = w.h * q.group + r % q.group;
+      const int32_t token = w.run0 + token_of(q, r), head = w.h * q.group + r - token_of(q, r) * q.group;
       const bool none = token >= w.count || total == 0.0f;
       const float f = none ? 0.0f : 1.0f / total;
       uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + 4 * quad;

@@ -70,7 +70,8 @@ __device__ __forceinline__ uint32_t four_codes(const float *x, float inverse) {
 __device__ __forceinline__ float code_factor(float a) { return a > 0.0f ? div_rn(127.0f, a) : 0.0f; }
 __device__ __forceinline__ float code_step(float a) { return mul_rn(a, 1.0f / 127.0f); }
 
-// The codes and steps of all query rows, D / 8 lanes a row; step -1 marks a row that does not count.
+// The codes and steps of all query rows, D / 8 lanes a row; a NaN step marks a row that does not count
+// (no maximum takes it).
 template <int D>
 __global__ __launch_bounds__(256) void codes_kernel(Cache c, Run q, int8_t *codes, float *steps, int64_t rows) {
   constexpr int kLanes = D / 8;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256) void codes_kernel(Cache c, Run q, int8_t *code
 #pragma unroll
   for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
   *reinterpret_cast<uint2 *>(codes + row * D + part * 8) = uint2{four_codes(x, f), four_codes(x + 4, f)};
-  if (part == 0) steps[row] = bad ? -1.0f : code_step(a);
+  if (part == 0) steps[row] = bad ? __builtin_nanf("") : code_step(a);
 }
 
 // The bytes of w that are positive, and those that are negative.
@@ -108,11 +109,12 @@ __device__ __forceinline__ void parts(int w, int &pos, int &neg) {
   pos = static_cast<int>(static_cast<uint32_t>(w) & ~m);
 }
 
-// Codes of 16 rows as the B operand: lane % 16 is the row, lane / 16 and k name 16 channels.
+// Codes of 16 rows as the A operand: lane % 16 is the row, lane / 16 and k name 16 channels; and the
+// steps of the lane's four rows of the results, 4 (lane / 16) + i.
 template <int D>
 struct RowCodes {
   i4 pos[D / 64], neg[D / 64];
-  float step;  // -1: the row does not count
+  f4 step;
 
   __device__ __forceinline__ void split(int k, i4 w) {
 #pragma unroll
@@ -125,53 +127,80 @@ struct RowCodes {
   }
 };
 
-// Bounds of 16 blocks as the A operand, and the steps of the lane's four of the results.
+// Bounds of 16 blocks as the B operand, lane % 16 the block, and that block's step.
 template <int D>
 struct BlockBounds {
   i4 hi[D / 64], lo[D / 64];
-  float u[4];
+  float u;
 };
 
 template <int D>
 __device__ __forceinline__ void load_bounds(BlockBounds<D> &x, const Cache &c, int64_t sh, int32_t b0, int32_t blocks,
                                             float unit_factor) {
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-  const int32_t mine = b0 + col < blocks ? b0 + col : blocks - 1;
-  const int8_t *p = c.bounds + (sh * c.blocks + mine) * 2 * D + quad * 16;
+  const int64_t mine = sh * c.blocks + (b0 + col < blocks ? b0 + col : blocks - 1);
+  const int8_t *p = c.bounds + mine * 2 * D + quad * 16;
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) {
     x.hi[k] = *reinterpret_cast<const i4 *>(p + k * 64);
     x.lo[k] = *reinterpret_cast<const i4 *>(p + D + k * 64);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t b = b0 + quad * 4 + i;
-    x.u[i] = mul_rn(c.key_scale[sh * c.blocks + (b < blocks ? b : blocks - 1)], unit_factor);
-  }
+  x.u = mul_rn(c.key_scale[mine], unit_factor);
 }
 
-// best[i] = max(best[i], the lane's row's score of block 4 (lane / 16) + i)
+// best = max(best, the scores of the lane's block in its four rows)
 template <int D>
-__device__ __forceinline__ void score16(const BlockBounds<D> &x, const RowCodes<D> &r, float (&best)[4]) {
+__device__ __forceinline__ void score16(const BlockBounds<D> &x, const RowCodes<D> &r, float &best) {
   i4 acc = {0, 0, 0, 0};
 #pragma unroll
   for (int k = 0; k < D / 64; ++k) {
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.hi[k], r.pos[k], acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.lo[k], r.neg[k], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.pos[k], x.hi[k], acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(r.neg[k], x.lo[k], acc, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float v = mul_rn(mul_rn(static_cast<float>(acc[i]), x.u[i]), r.step);
-    best[i] = r.step >= 0.0f ? fmaxf(best[i], v) : best[i];
-  }
+  for (int i = 0; i < 4; ++i) best = fmaxf(best, mul_rn(mul_rn(static_cast<float>(acc[i]), x.u), r.step[i]));
 }
 
-// The largest over the 16 rows; a block whose scale is no finite number is
+// The largest over all rows; a block whose scale is no finite number is
 // chosen, so that its NaN shows.
 __device__ __forceinline__ float over_rows(float best, float u) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) best = fmaxf(best, __shfl_xor(best, o, kWave));
+  best = mf::max_over_slices(best);
   return u < __builtin_huge_valf() ? best : __builtin_huge_valf();
+}
+
+// The codes of a run's at most 16 rows into LDS, D / 8 lanes a row.
+template <int D>
+struct OwnCodes {
+  int8_t codes[16][D];
+  float step[16];
+};
+
+template <int D>
+__device__ __forceinline__ void own_codes(OwnCodes<D> &own, const Run &q, int32_t s, int32_t h, int32_t t0, int32_t rows) {
+  constexpr int kLanes = D / 8;
+  const int r = threadIdx.x / kLanes, part = threadIdx.x % kLanes;
+  if (r >= 16) return;
+  const bool counts = r < rows;
+  float x[8], a = 0.0f;
+  const int32_t token = t0 + r / q.group, head = h * q.group + r % q.group;
+  to_floats(counts ? *reinterpret_cast<const uint4 *>(q.q + s * q.ss + token * q.st + head * q.sh + part * 8)
+                   : uint4{0, 0, 0, 0}, q.fp16, x);
+  int bad = !counts;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a = fmaxf(a, fabsf(x[j]));
+    bad |= !(fabsf(x[j]) < __builtin_huge_valf());
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) {
+    a = fmaxf(a, __shfl_xor(a, o, kWave));
+    bad |= __shfl_xor(bad, o, kWave);
+  }
+  const float f = bad ? 0.0f : code_factor(a);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
+  *reinterpret_cast<uint2 *>(&own.codes[r][part * 8]) = uint2{four_codes(x, f), four_codes(x + 4, f)};
+  if (part == 0) own.step[r] = bad ? __builtin_nanf("") : code_step(a);
 }
 
 // Scores for runs of many rows: a wave takes 64 blocks, whose bounds stay in registers, through all rows of
@@ -192,18 +221,19 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
   const int64_t sh = int64_t(s) * c.heads + h;
   for (int32_t b0 = (chunk * 4 + wave) * 16 * kB; b0 < blocks; b0 += chunks * 64 * kB) {
     BlockBounds<D> x[kB];
-    float best[kB][4];
+    float best[kB];
 #pragma unroll
     for (int n = 0; n < kB; ++n) {
       load_bounds<D>(x[n], c, sh, b0 + 16 * n, blocks, unit_factor);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) best[n][i] = mf::kNegInf;
+      best[n] = mf::kNegInf;
     }
     for (int32_t r0 = 0; r0 < rows; r0 += 16) {
       const int32_t r = r0 + col < rows ? r0 + col : rows - 1;  // the last row again: it changes no maximum
       const int64_t at = (int64_t(s) * q.len + t0 + r / q.group) * q.heads + h * q.group + r % q.group;
       RowCodes<D> rc;
-      rc.step = steps[at];
+      const float step = steps[at];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rc.step[i] = __shfl(step, quad * 4 + i, kWave);
 #pragma unroll
       for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16));
 #pragma unroll
@@ -211,12 +241,9 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
     }
 #pragma unroll
     for (int n = 0; n < kB; ++n) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = over_rows(best[n][i], x[n].u[i]);
-        const int32_t b = b0 + 16 * n + quad * 4 + i;
-        if (col == 0 && b < blocks) score[int64_t(unit) * c.blocks + b] = v;
-      }
+      const float v = over_rows(best[n], x[n].u);
+      const int32_t b = b0 + 16 * n + col;
+      if (quad == 0 && b < blocks) score[int64_t(unit) * c.blocks + b] = v;
     }
   }
 }
@@ -231,15 +258,16 @@ constexpr int32_t kKept = 8192;  // scores that choose_kernel holds in LDS
 
 // One workgroup per (sequence, run, head).  Blocks before `low` and from
 // `high` on are chosen anyway; of the others the `want` highest: their
-// smallest score is found two bits a round (each wave counts its keys by
-// ballots and adds three counts to one LDS word), then the chosen are written
-// by prefix sums.  With FUSED (runs of at most 16 rows) the scores are computed here, 16 blocks a
+// smallest score is found eight bits a round by histograms in LDS, then the
+// chosen are written by prefix sums.  With FUSED (runs of at most 16 rows) the scores are computed here, 16 blocks a
 // wave and step, so that a decode step's choice is one launch.
 template <int T, int D, bool FUSED>
 __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_factor, float *score, int32_t *out) {
   constexpr int kWaves = T / kWave;
   __shared__ uint32_t kept[kKept];
-  __shared__ unsigned long long counts[3];
+  __shared__ __attribute__((aligned(16))) int32_t hist[256];
+  __shared__ __attribute__((aligned(16))) OwnCodes<D> own;
+  __shared__ int32_t found[2];
   __shared__ int32_t wave_eq[kWaves], wave_in[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int32_t unit = blockIdx.x;
@@ -260,54 +288,29 @@ __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_fa
   const bool all = want >= n, held = n <= kKept;
   if (!all) {
     if constexpr (FUSED) {
+      constexpr int kB = 4;  // 16-block groups of a wave in flight
       const int col = lane & 15, quad = lane >> 4;
-      const int32_t t0 = run * q.run, rows = ((count - t0 < q.run) ? count - t0 : q.run) * q.group;
+      BlockBounds<D> bb[kB];
+      const int32_t b0 = low + wave * 16 * kB;
+      if (b0 < high) {
+#pragma unroll
+        for (int g = 0; g < kB; ++g) load_bounds<D>(bb[g], c, sh, b0 + 16 * g, high, unit_factor);
+      }
+      const int32_t t0 = run * q.run;
+      own_codes<D>(own, q, s, h, t0, ((count - t0 < q.run) ? count - t0 : q.run) * q.group);
+      __syncthreads();
       RowCodes<D> rc;
-      float x[D / 64][2][8], a = 0.0f;
-      int bad = col >= rows;
-      const int32_t r = bad ? 0 : col;
-      const uint16_t *p = q.q + s * q.ss + (t0 + r / q.group) * q.st + (h * q.group + r % q.group) * q.sh + quad * 16;
+      rc.step = *reinterpret_cast<const f4 *>(&own.step[4 * quad]);
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
+      for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(&own.codes[col][k * 64 + quad * 16]));
+      for (int32_t b1 = b0; b1 < high; b1 += kWaves * 16 * kB) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          to_floats(*reinterpret_cast<const uint4 *>(p + k * 64 + i * 8), q.fp16, x[k][i]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            a = fmaxf(a, fabsf(x[k][i][j]));
-            bad |= !(fabsf(x[k][i][j]) < __builtin_huge_valf());
-          }
-        }
-      }
-#pragma unroll
-      for (int o = 16; o < 64; o <<= 1) {
-        a = fmaxf(a, __shfl_xor(a, o, kWave));
-        bad |= __shfl_xor(bad, o, kWave);
-      }
-      const float f = bad ? 0.0f : code_factor(a);
-      rc.step = bad ? -1.0f : code_step(a);
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) {
-        i4 w;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[k][i][j] = bad ? 0.0f : x[k][i][j];
-          w[2 * i] = static_cast<int>(four_codes(x[k][i], f));
-          w[2 * i + 1] = static_cast<int>(four_codes(x[k][i] + 4, f));
-        }
-        rc.split(k, w);
-      }
-      for (int32_t b0 = low + wave * 16; b0 < high; b0 += kWaves * 16) {
-        BlockBounds<D> bb;
-        load_bounds<D>(bb, c, sh, b0, high, unit_factor);
-        float best[4] = {mf::kNegInf, mf::kNegInf, mf::kNegInf, mf::kNegInf};
-        score16<D>(bb, rc, best);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = over_rows(best[i], bb.u[i]);
-          const int32_t b = b0 + quad * 4 + i;
-          if (col == 0 && b < high) {
+        for (int g = 0; g < kB; ++g) {
+          float best = mf::kNegInf;
+          score16<D>(bb[g], rc, best);
+          const float v = over_rows(best, bb[g].u);
+          const int32_t b = b1 + 16 * g + col;
+          if (quad == 0 && b < high) {
             if (held) {
               kept[b - low] = ordered(v);
             } else {
@@ -315,12 +318,15 @@ __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_fa
             }
           }
         }
+        if (b1 + kWaves * 16 * kB < high) {
+#pragma unroll
+          for (int g = 0; g < kB; ++g) load_bounds<D>(bb[g], c, sh, b1 + (kWaves * kB + g) * 16, high, unit_factor);
+        }
       }
     } else if (held) {
       for (int32_t i = tid; i < n; i += T) kept[i] = ordered(sc[low + i]);
     }
   }
-  if (tid < 3) counts[tid] = 0;
   __syncthreads();  // also orders this workgroup's writes of `score` before its reads
   auto key = [&](int32_t i) { return held ? kept[i] : ordered(sc[low + i]); };
 
@@ -328,30 +334,39 @@ __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_fa
   int32_t equals = 0;  // blocks at the threshold that are chosen
   if (!all && want > 0) {
     int32_t need = want;
-    for (int round = 0; round < 16; ++round) {
-      const int shift = 30 - 2 * round;
-      // keys with the threshold's upper bits whose next two are 3, at least 2, at least 1
-      uint32_t c3 = 0, c2 = 0, c1 = 0;
-      for (int32_t i = tid; i - lane < n; i += T) {
-        const uint32_t k = i < n ? key(i) : 0;
-        const bool in = i < n && (round == 0 || (k >> (shift + 2)) == (threshold >> (shift + 2)));
-        const uint32_t digit = (k >> shift) & 3u;
-        c3 += __popcll(__ballot(in && digit == 3));
-        c2 += __popcll(__ballot(in && digit >= 2));
-        c1 += __popcll(__ballot(in && digit >= 1));
-      }
-      if (lane == 0) {
-        atomicAdd(&counts[round % 3], c3 | (static_cast<unsigned long long>(c2) << 21) |
-                                          (static_cast<unsigned long long>(c1) << 42));
-      }
-      if (tid == 0) counts[(round + 1) % 3] = 0;  // last read two rounds ago
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 256; i += T) hist[i] = 0;
       __syncthreads();
-      const unsigned long long sum = counts[round % 3];
-      const int32_t n3 = static_cast<int32_t>(sum & 0x1fffffu), n2 = static_cast<int32_t>((sum >> 21) & 0x1fffffu);
-      const int32_t n1 = static_cast<int32_t>(sum >> 42);
-      const uint32_t digit = need <= n3 ? 3u : need <= n2 ? 2u : need <= n1 ? 1u : 0u;
-      need -= digit == 3 ? 0 : digit == 2 ? n3 : digit == 1 ? n2 : n1;
-      threshold |= digit << shift;
+      // bin 0 holds the highest digit
+      for (int32_t i = tid; i < n; i += T) {
+        const uint32_t k = key(i);
+        if (shift == 24 || (k >> (shift + 8)) == (threshold >> (shift + 8))) {
+          atomicAdd(&hist[255 - ((k >> shift) & 255u)], 1);
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {  // the bin that the need-th key falls into
+        const int4 v = *reinterpret_cast<const int4 *>(&hist[4 * lane]);
+        const int32_t mine = v.x + v.y + v.z + v.w;
+        const int32_t sum = wave_prefix(mine);
+        int32_t above = sum - mine;
+        if (above < need && sum >= need) {
+          int bin = 4 * lane;
+          const int32_t w[3] = {v.x, v.y, v.z};
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            if (bin == 4 * lane + i && above + w[i] < need) {
+              above += w[i];
+              ++bin;
+            }
+          }
+          found[0] = 255 - bin;
+          found[1] = above;
+        }
+      }
+      __syncthreads();
+      threshold |= static_cast<uint32_t>(found[0]) << shift;
+      need -= found[1];
     }
     equals = need;
   }
@@ -449,7 +464,6 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t span = q.causal ? ceil_div(int64_t(q.run) - 1, int64_t(c.block)) : 0;
   UC_REQUIRE(sink + recent + span <= budget, "uc_block8_select: budget %lld is less than the %lld blocks always chosen",
              static_cast<long long>(budget), static_cast<long long>(sink + recent + span));
-  UC_REQUIRE(cache->blocks < (1 << 21), "uc_block8_select: too many blocks");  // counted in 21 bits
   if (q.len == 0) return UC_OK;
   UC_REQUIRE(q.q != nullptr && (reinterpret_cast<uintptr_t>(q.q) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,
              "uc_block8_select: query must be 16-byte aligned with strides that are multiples of 8");
@@ -472,7 +486,7 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   auto launch = [&](auto d_tag) {
     constexpr int D = decltype(d_tag)::value;
     if (q.run * q.group <= 16) {
-      hipLaunchKernelGGL((choose_kernel<1024, D, true>), dim3(static_cast<uint32_t>(units)), dim3(1024), 0,
+      hipLaunchKernelGGL((choose_kernel<512, D, true>), dim3(static_cast<uint32_t>(units)), dim3(512), 0,
                          as_stream(stream), c, q, factor, score, blocks);
       return check_launch("uc_block8_select");
     }

@@ -43,11 +43,14 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
 
     if t.is_neg():
         t = t.resolve_neg()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 or s < 0 for s in t.stride()[:-1]):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        a, b, c, d = t.stride()
+        if d == 1 and not (a % 8 or b % 8 or c % 8):
+            return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 @functools.lru_cache(maxsize=256)
@@ -113,17 +116,21 @@ class Block8KVCache:
                                  f"{tuple(t.shape)} strides {tuple(t.stride())}")
         if not s or not h or not n:
             raise ValueError("Block8 cache needs a sequence, a KV head and a block at least")
-        self.device = nat.require_device(*(t for _, t, _, _ in expected), what="Block8 cache")
+        nat.require_device(*(t for _, t, _, _ in expected), what="Block8 cache")
         for name, t, _, _ in expected:
             if t.data_ptr() % (16 if name in ("key_code", "value_code", "key_bounds", "tail") else 4):
                 raise ValueError(f"Block8 cache {name} must be 16-byte aligned")
+        if max_tokens is not None and int(max_tokens) < 0:
+            raise ValueError("Block8 cache max_tokens must not be negative")
+        self._set(key_code, value_code, key_scale, value_scale, key_bounds, lengths, tail, (s, h, d, n, b), max_tokens)
+
+    def _set(self, key_code, value_code, key_scale, value_scale, key_bounds, lengths, tail, sizes, max_tokens) -> None:
         self.key_code, self.value_code = key_code, value_code
         self.key_scale, self.value_scale = key_scale, value_scale
         self.key_bounds, self.lengths, self.tail = key_bounds, lengths, tail
-        self.sequences, self.num_kv_heads, self.head_dim = s, h, d
-        self.blocks, self.block_tokens, self.code_dtype = n, b, key_code.dtype
-        if max_tokens is not None and int(max_tokens) < 0:
-            raise ValueError("Block8 cache max_tokens must not be negative")
+        self.sequences, self.num_kv_heads, self.head_dim, self.blocks, self.block_tokens = sizes
+        self.code_dtype, self.device = key_code.dtype, key_code.device
+        self._sizes = (*sizes, _CODES[key_code.dtype])
         self.max_tokens = self.capacity if max_tokens is None else min(int(max_tokens), self.capacity)
 
     @property
@@ -139,14 +146,16 @@ class Block8KVCache:
         """A cache without tokens, with room for `capacity` of them (rounded up
         to whole blocks) in every sequence, that takes dense rows of `dtype`."""
 
-        return cls._allocate(sequences, capacity, num_kv_heads, head_dim, block_tokens, code_dtype, dtype,
-                             torch.device(device), None, 0)
+        cache = cls._allocate(int(sequences), int(capacity), int(num_kv_heads), int(head_dim), int(block_tokens),
+                              code_dtype, dtype, torch.device(device), 0)
+        cache.lengths.zero_()
+        return cache
 
     @classmethod
-    def _allocate(cls, s, capacity, h, d, b, code_dtype, dtype, device, lengths, max_tokens) -> "Block8KVCache":
+    def _allocate(cls, s, capacity, h, d, b, code_dtype, dtype, device, max_tokens) -> "Block8KVCache":
         if device.type != "cuda":
             raise RuntimeError(f"Block8 cache requires a GPU (got {device})")
-        if int(capacity) <= 0 or int(s) <= 0 or int(h) <= 0:
+        if capacity <= 0 or s <= 0 or h <= 0:
             raise ValueError("Block8 cache needs a sequence, a KV head and a token of capacity at least")
         if b not in (32, 64, 128) or d not in (64, 128):
             raise ValueError("Block8 cache supports blocks of 32, 64 or 128 tokens and head_dim 64 or 128")
@@ -154,16 +163,17 @@ class Block8KVCache:
             raise ValueError("Block8 cache codes must be int8 or float8_e4m3fn")
         if dtype not in _HALVES:
             raise ValueError("Block8 cache tail must be bf16 or fp16")
-        n = -(-int(capacity) // b)
-        if lengths is None:
-            lengths = torch.zeros(s, dtype=torch.int32, device=device)
-        return cls(
+        n = -(-capacity // b)
+        cache = cls.__new__(cls)
+        cache._set(
             torch.empty((s, h, n * b, d), dtype=code_dtype, device=device),
             torch.empty((s, h, n, d, b), dtype=code_dtype, device=device),
             torch.empty((s, h, n), dtype=torch.float32, device=device),
             torch.empty((s, h, n), dtype=torch.float32, device=device),
-            torch.empty((s, h, n, 2, d), dtype=torch.int8, device=device), lengths, max_tokens=max_tokens,
-            tail=torch.empty((s, h, 2, b, d), dtype=dtype, device=device))
+            torch.empty((s, h, n, 2, d), dtype=torch.int8, device=device),
+            torch.empty((s,), dtype=torch.int32, device=device),
+            torch.empty((s, h, 2, b, d), dtype=dtype, device=device), (s, h, d, n, b), max_tokens)
+        return cache
 
     @classmethod
     def from_dense(cls, key: torch.Tensor, value: torch.Tensor, *, lengths: torch.Tensor | None = None,
@@ -182,33 +192,27 @@ class Block8KVCache:
         _check_half(key, "Block8 keys")
         _check_half(value, "Block8 values")
         device = nat.require_device(key, value, lengths, what="Block8 cache")
-        s, t, h, d = map(int, key.shape)
-        if capacity is None:
-            capacity = max(t, 1)
-        if int(capacity) < t:
+        s, t, h, d = key.shape
+        capacity = max(t, 1) if capacity is None else int(capacity)
+        if capacity < t:
             raise ValueError("Block8 cache capacity must cover the tokens")
-        if lengths is None:
-            lengths = torch.full((s,), t, dtype=torch.int32, device=device)
-        else:
-            if lengths.dtype != torch.int32 or tuple(lengths.shape) != (s,):
-                raise ValueError("Block8 cache lengths must be int32 [sequences]")
-            lengths = lengths.clamp(0, t)
-        cache = cls._allocate(s, capacity, h, d, int(block_tokens), code_dtype, key.dtype, device, lengths, t)
+        if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (s,)
+                                    or not lengths.is_contiguous()):
+            raise ValueError("Block8 cache lengths must be contiguous int32 [sequences]")
+        cache = cls._allocate(s, capacity, h, d, int(block_tokens), code_dtype, key.dtype, device, t)
         if t:
             key, value = _rows16(key), _rows16(value)
             cache._call("uc_block8_pack", cache._struct(), key.data_ptr(), *key.stride()[:3], value.data_ptr(),
-                     *value.stride()[:3], nat.dtype_code(key.dtype), t, cache.tail.data_ptr())
+                        *value.stride()[:3], nat.dtype_code(key.dtype), t, nat.ptr(lengths), cache.tail.data_ptr())
+        else:
+            cache.lengths.zero_()
         return cache
 
     # ------------------------------------------------------------- internals --
-    def _sizes(self) -> tuple:
-        return (self.sequences, self.num_kv_heads, self.head_dim, self.blocks, self.block_tokens,
-                _CODES[self.code_dtype])
-
     def _struct(self) -> "nat.Block8Cache":
         return nat.Block8Cache(self.key_code.data_ptr(), self.value_code.data_ptr(), self.key_scale.data_ptr(),
                                self.value_scale.data_ptr(), self.key_bounds.data_ptr(), self.lengths.data_ptr(),
-                               *self._sizes())
+                               *self._sizes)
 
     def _call(self, entry: str, *args) -> None:
         """An entry point on the current stream of the cache's device, whatever
@@ -226,10 +230,10 @@ class Block8KVCache:
 
         if query.dim() == 3 and self.sequences == 1:
             query = query.unsqueeze(0)
-        if query.dim() != 4 or int(query.shape[0]) != self.sequences or int(query.shape[3]) != self.head_dim:
+        if query.dim() != 4 or query.shape[0] != self.sequences or query.shape[3] != self.head_dim:
             raise ValueError(f"Block8 attention expects queries [{self.sequences}, tokens, heads, {self.head_dim}], "
                              f"got {tuple(query.shape)}")
-        hq = int(query.shape[2])
+        _, lq, hq, _ = query.shape
         if hq == 0 or hq % self.num_kv_heads:
             raise ValueError("Query heads must be divisible by the cache's KV heads")
         _check_half(query, "Block8 queries")
@@ -239,9 +243,8 @@ class Block8KVCache:
         if nat.require_device(query, query_lengths, what="Block8 attention") != self.device:
             raise RuntimeError("Block8 attention received tensors on different devices")
         query = _rows16(query)
-        sizes = (int(query.shape[1]), hq, self.max_tokens, nat.dtype_code(query.dtype), int(bool(causal)))
-        struct = nat.Block8Query(query.data_ptr(), *query.stride()[:3], sizes[0], hq, nat.ptr(query_lengths),
-                                 *sizes[2:])
+        sizes = (lq, hq, self.max_tokens, nat.dtype_code(query.dtype), 1 if causal else 0)
+        struct = nat.Block8Query(query.data_ptr(), *query.stride()[:3], lq, hq, nat.ptr(query_lengths), *sizes[2:])
         return query, struct, sizes
 
     def _attend(self, query, struct, sizes, blocks, budget, query_block, sm_scale):
@@ -249,9 +252,9 @@ class Block8KVCache:
         if not 0.0 < sm_scale < math.inf:
             raise ValueError("Block8 attention sm_scale must be positive")
         lq, hq = sizes[:2]
-        out = torch.empty((self.sequences, lq, hq, self.head_dim), dtype=query.dtype, device=self.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
         lse = torch.empty((self.sequences, hq, lq), dtype=torch.float32, device=self.device)
-        nbytes = _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes(), sizes, budget, query_block)
+        nbytes = _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes, sizes, budget, query_block)
         ws = nat.workspace(self.device, nbytes)
         self._call("uc_block8_attn", self._struct(), struct, nat.ptr(blocks), budget, query_block, sm_scale,
                  out.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes)
@@ -335,7 +338,7 @@ class Block8KVCache:
         q, struct, sizes = self._query(query, query_lengths, causal)
         runs = -(-sizes[0] // query_block)
         blocks = torch.empty((self.sequences, runs, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)
-        nbytes = _workspace_bytes("uc_block8_select_workspace_bytes", self._sizes(), sizes, query_block)
+        nbytes = _workspace_bytes("uc_block8_select_workspace_bytes", self._sizes, sizes, query_block)
         ws = nat.workspace(self.device, nbytes)
         self._call("uc_block8_select", self._struct(), struct, budget, sink, recent, query_block, blocks.data_ptr(),
                  ws.data_ptr(), nbytes)
