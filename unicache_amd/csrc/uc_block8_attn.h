@@ -173,6 +173,16 @@ __device__ __forceinline__ float rescaled(float l, float d) {
   return l * a * a;
 }
 
+template <int DT, int N>
+__device__ __forceinline__ void widen(const uint4 (&raw)[N], float (&x)[N][8]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[k][j] = half_bits_to_f32<DT>(j % 2 ? u[j / 2] >> 16 : u[j / 2]);
+  }
+}
+
 // One query row's fragments, scaled by a power of two into fp16; returns the
 // factor of its logits: sm_scale log2(e) / the power.  Lane quad x holds channels
 // 32 k + 8 x .. + 7 of fragment k; with PAIRS 64 (k / 2) + 16 x + 8 (k % 2) .. + 7, so that 16 bytes
@@ -192,15 +202,15 @@ __device__ __forceinline__ float load_query(const Query &q, const Rows &w, int32
     }
   }
   float x[D / 32][8], a = 0.0f;
+  if (q.fp16) {
+    widen<UC_FP16>(raw, x);
+  } else {
+    widen<UC_BF16>(raw, x);
+  }
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) {
-    const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t bits = j % 2 ? u[j / 2] >> 16 : u[j / 2];
-      x[k][j] = q.fp16 ? f16_bits_to_f32(static_cast<uint16_t>(bits)) : bf16_bits_to_f32(bits & 0xffffu);
-      a = fmaxf(a, fabsf(x[k][j]));
-    }
+    for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(x[k][j]));
   }
   a = mf::max_over_slices(a);
   int e = static_cast<int>((__float_as_uint(a) >> 23) & 0xff) - 127;
@@ -215,6 +225,13 @@ __device__ __forceinline__ float load_query(const Query &q, const Rows &w, int32
     for (int j = 0; j < 8; ++j) frag[k][j] = mf::to_h(x[k][j] * up);
   }
   return q.scale * down;
+}
+
+// Two outputs of the query's type.  (A select, not a branch: both are a few instructions.)
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool fp16) {
+  const uint32_t h = __builtin_bit_cast(uint32_t, h2{mf::to_h(a), mf::to_h(b)});
+  const uint32_t w = f32_to_bf16_bits(a) | (static_cast<uint32_t>(f32_to_bf16_bits(b)) << 16);
+  return fp16 ? h : w;
 }
 
 // uc_block8_mq.hip: 128 rows a workgroup, keys staged through LDS.

@@ -263,9 +263,8 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
       const float f = none ? 0.0f : 1.0f / total;
       uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + c0;
 #pragma unroll
-      for (int j = 0; j < kC; ++j) {
-        const float v = none ? 0.0f : o[j] * f;
-        dst[j] = q.fp16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v);
+      for (int j = 0; j < kC; j += 2) {
+        *reinterpret_cast<uint32_t *>(dst + j) = none ? 0u : pack2(o[j] * f, o[j + 1] * f, q.fp16);
       }
       if (c0 == 0 && lse != nullptr) {
         lse[(int64_t(w.s) * q.heads + head) * q.len + token] =

@@ -15,6 +15,8 @@
 // eight consecutive keys of its query row: the operand of O^T = V^T P^T.
 #include "uc_block8_attn.h"
 
+#include <type_traits>
+
 namespace uc {
 namespace b8 {
 namespace {
@@ -37,57 +39,76 @@ struct Staged {
   int32_t t[2];  // first keys of the halves
 };
 
+// What a thread loads.  A load's 256 threads take one half tile (at D = 64: the first two waves one
+// half, the last two the other), so its address is a scalar and a constant of the lane.
+template <int D>
+struct Loader {
+  int key, c16;       // keys: the key in its half, 16 channels
+  int channel, k16;   // values: the channel, 16 keys of its half
+  uint32_t koff, voff;
+
+  __device__ __forceinline__ explicit Loader(int32_t block) {
+    const int tid = threadIdx.x;
+    if constexpr (D == 128) {
+      // eight lanes write two keys' chunks to LDS, so that they meet no bank twice
+      c16 = (tid & 3) | ((tid >> 3) & 1) << 2;
+      key = ((tid >> 2) & 1) | (tid >> 4) << 1;
+    } else {
+      c16 = tid & 3;
+      key = (tid >> 2) & 31;
+    }
+    channel = (tid >> 1) & (D - 1);
+    k16 = tid & 1;
+    koff = key * D + c16 * 16;
+    voff = channel * block + k16 * 16;
+  }
+  // The half of load i: the same for a wave.
+  __device__ __forceinline__ int half(int i) const { return D == 128 ? i : __builtin_amdgcn_readfirstlane(threadIdx.x >> 7); }
+};
+
 template <int D>
 __device__ __forceinline__ void fetch(Staged<D> &st, const Cache &c, int64_t sh, const uint8_t *kbase,
-                                      const uint8_t *vbase, int32_t t0, int32_t t1) {
-  constexpr int kPerKey = D / 16;
+                                      const uint8_t *vbase, const Loader<D> &ld, int32_t t0, int32_t t1) {
   st.t[0] = t0;
   st.t[1] = t1;
-  const int32_t a0 = t0 == kNone ? 0 : t0, a1 = t1 == kNone ? 0 : t1;
+  const int32_t a[2] = {t0 == kNone ? 0 : t0, t1 == kNone ? 0 : t1};
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
-    const int key = threadIdx.x / kPerKey + i * (256 / kPerKey);
-    const int32_t t = (key < 32 ? a0 : a1 - 32) + key;
-    st.k[i] = *reinterpret_cast<const uint4 *>(kbase + int64_t(t) * D + threadIdx.x % kPerKey * 16);
-    const int channel = threadIdx.x / 4 + i * 64, k16 = threadIdx.x % 4;
-    const int32_t u = (k16 < 2 ? a0 : a1) + (k16 & 1) * 16;
-    st.v[i] = *reinterpret_cast<const uint4 *>(vbase + (int64_t(u >> c.shift) << c.shift) * D + channel * c.block +
-                                               (u & (c.block - 1)));
+    const int32_t t = ld.half(i) ? a[1] : a[0];
+    st.k[i] = *reinterpret_cast<const uint4 *>(kbase + int64_t(t) * D + ld.koff);
+    st.v[i] = *reinterpret_cast<const uint4 *>(vbase + ((int64_t(t >> c.shift) << c.shift) * D + (t & (c.block - 1))) + ld.voff);
   }
   const int64_t b = sh * c.blocks;
-  st.ks[0] = c.key_scale[b + (a0 >> c.shift)];
-  st.ks[1] = c.key_scale[b + (a1 >> c.shift)];
-  st.vs[0] = c.value_scale[b + (a0 >> c.shift)];
-  st.vs[1] = c.value_scale[b + (a1 >> c.shift)];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    st.ks[h] = c.key_scale[b + (a[h] >> c.shift)];
+    st.vs[h] = c.value_scale[b + (a[h] >> c.shift)];
+  }
 }
 
-// The order of a key's chunks in LDS.
+// The orders of a key's and of a channel's chunks in LDS.
 __device__ __forceinline__ int key_swizzle(int key) { return (key & 3) | ((key >> 3) & 3) << 2; }
+__device__ __forceinline__ int value_swizzle(int channel) {
+  return (channel & 1) | ((channel >> 2) & 1) << 1 | ((channel >> 1) & 1) << 2;
+}
 
 template <int D, int CODE>
-__device__ __forceinline__ void store(Staged<D> &st, char *buf, int32_t length) {
-  constexpr int kPerKey = D / 16, kChunks = D / 8;
+__device__ __forceinline__ void store(Staged<D> &st, char *buf, const Loader<D> &ld, int32_t length) {
   if (st.t[0] + 32 > length || st.t[1] + 32 > length) {  // codes behind the length are no values
-    const int32_t k16 = threadIdx.x % 4;
-    const int32_t u = (k16 < 2 ? st.t[0] : st.t[1]) + (k16 & 1) * 16;
 #pragma unroll
-    for (int i = 0; i < Tile<D>::kLoads; ++i) st.v[i] = first_bytes(st.v[i], length - u);
+    for (int i = 0; i < Tile<D>::kLoads; ++i) st.v[i] = first_bytes(st.v[i], length - (ld.half(i) ? st.t[1] : st.t[0]) - ld.k16 * 16);
   }
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
-    const int key = threadIdx.x / kPerKey + i * (256 / kPerKey), c16 = threadIdx.x % kPerKey;
-    char *row = buf + key * Tile<D>::kKeyRow;
-    const int sw = key_swizzle(key) & (kChunks - 1);
-    // eight lanes hold one key at D = 128: half of them write their second chunk first
-    const int odd = D == 128 ? (c16 >> 2) & 1 : 0;
-    const uint32_t x0 = odd ? st.k[i].z : st.k[i].x, y0 = odd ? st.k[i].w : st.k[i].y;
-    const uint32_t x1 = odd ? st.k[i].x : st.k[i].z, y1 = odd ? st.k[i].y : st.k[i].w;
-    *reinterpret_cast<h8 *>(row + 16 * ((2 * c16 + odd) ^ sw)) = codes_to_h8<CODE>(x0, y0);
-    *reinterpret_cast<h8 *>(row + 16 * ((2 * c16 + (odd ^ 1)) ^ sw)) = codes_to_h8<CODE>(x1, y1);
-    const int channel = threadIdx.x / 4 + i * 64, k16 = threadIdx.x % 4;
-    char *vrow = buf + Tile<D>::kKeyBytes + channel * Tile<D>::kValueRow;
-    *reinterpret_cast<h8 *>(vrow + 16 * ((2 * k16) ^ (channel & 7))) = codes_to_h8<CODE>(st.v[i].x, st.v[i].y);
-    *reinterpret_cast<h8 *>(vrow + 16 * ((2 * k16 + 1) ^ (channel & 7))) = codes_to_h8<CODE>(st.v[i].z, st.v[i].w);
+    const int h = ld.half(i);
+    char *row = buf + (ld.key + 32 * h) * Tile<D>::kKeyRow;
+    const int sw = key_swizzle(ld.key) & (D / 8 - 1);
+    *reinterpret_cast<h8 *>(row + 16 * ((2 * ld.c16) ^ sw)) = codes_to_h8<CODE>(st.k[i].x, st.k[i].y);
+    *reinterpret_cast<h8 *>(row + 16 * ((2 * ld.c16 + 1) ^ sw)) = codes_to_h8<CODE>(st.k[i].z, st.k[i].w);
+    char *vrow = buf + Tile<D>::kKeyBytes + ld.channel * Tile<D>::kValueRow;
+    const int chunk = 4 * h + 2 * ld.k16, vw = value_swizzle(ld.channel);
+    *reinterpret_cast<h8 *>(vrow + 16 * (chunk ^ vw)) = codes_to_h8<CODE>(st.v[i].x, st.v[i].y);
+    *reinterpret_cast<h8 *>(vrow + 16 * ((chunk + 1) ^ vw)) = codes_to_h8<CODE>(st.v[i].z, st.v[i].w);
   }
 }
 
@@ -114,9 +135,9 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float t = s[2 * h][0];
+      float t = mf::kNegInf;
 #pragma unroll
-      for (int j = 1; j < 8; ++j) t = fmaxf(t, s[2 * h + j / 4][j % 4]);
+      for (int j = 0; j < 8; ++j) t = fmaxf(t, s[2 * h + j / 4][j % 4]);
       top = fmaxf(top, __builtin_fmaf(t, c[h], lv[h]));
     }
   }
@@ -154,7 +175,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   typedef Tile<D> T;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-  const int32_t split = blockIdx.x % p.splits, unit = blockIdx.x / p.splits;
+  const int32_t split = blockIdx.x % p.splits;
+  int32_t unit = blockIdx.x / p.splits;
+  // the later rows of a causal run see more keys: the longest first
+  if (q.causal) unit += p.groups - 1 - 2 * (unit % p.groups);
   const Rows w = rows_of(c, q, p, unit, kTileRows);
   const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
   const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
@@ -186,29 +210,29 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) ka[k] = krow * T::kKeyRow + 16 * ((4 * k + quad) ^ (key_swizzle(krow) & (D / 8 - 1)));
 #pragma unroll
-  for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ (col & 7));
+  for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ value_swizzle(col));
 
   float most = 0.0f;
   Staged<D> st;
+  const Loader<D> ld(c.block);
   auto get = [&](int32_t t) {
     int32_t t0 = half_of(c, p, list, 2 * t), t1 = half_of(c, p, list, 2 * t + 1);
     if (t1 >= tokens) t1 = kNone;
-    fetch<D>(st, c, sh, kbase, vbase, t0, t1);
+    fetch<D>(st, c, sh, kbase, vbase, ld, t0, t1);
   };
-  if (begin < end) {
-    get(begin);
-    store<D, CODE>(st, lds, w.length);
-  }
-  __syncthreads();
-  for (int32_t t = begin; t < end; ++t) {
-    const char *buf = lds + ((t - begin) & 1) * T::kBytes;
-    char *other = lds + ((t - begin + 1) & 1) * T::kBytes;
+  // whether every row sees all keys of the staged tile
+  auto whole = [&] { return (st.t[0] > st.t[1] ? st.t[0] : st.t[1]) + 32 <= w.end_first; };
+  int32_t t = begin;
+  int present = 0;  // LDS offset of the tile's buffer
+  auto step = [&](auto mask_tag) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    const char *buf = lds + present;
     const int32_t t0 = st.t[0], t1 = st.t[1];
     float ks[2], vs[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       ks[h] = st.ks[h];
-      vs[h] = counted_scale(st.t[h] < w.length ? st.vs[h] : 1.0f, most);
+      vs[h] = counted_scale(!MASK || st.t[h] < w.length ? st.vs[h] : 1.0f, most);
     }
     const bool more = t + 1 < end;
     if (more) get(t + 1);
@@ -227,16 +251,11 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     h8 pr[2][2];
     const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
     const float inv[2] = {__builtin_amdgcn_rcpf(vs[0]), __builtin_amdgcn_rcpf(vs[1])};
-    const bool whole = (t0 > t1 ? t0 : t1) + 32 <= w.end_first;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const float cc[2] = {ks[0] * factor[n], ks[1] * factor[n]};
       const int32_t ends[2] = {row_end[n] - t0 - 8 * quad, row_end[n] - t1 - 8 * quad};
-      if (whole) {
-        weights<D, false>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
-      } else {
-        weights<D, true>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
-      }
+      weights<D, MASK>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
     }
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
@@ -247,16 +266,27 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         acc[1].o[d] = mf::mfma32(a, pr[1][h], acc[1].o[d]);
       }
     }
-    if (more) store<D, CODE>(st, other, w.length);
+    present ^= T::kBytes;
+    if (more) store<D, CODE>(st, lds + present, ld, w.length);
     __syncthreads();
+    ++t;
+  };
+  if (begin < end) {
+    get(begin);
+    store<D, CODE>(st, lds, ld, w.length);
   }
+  __syncthreads();
+  // tiles that every row sees come first; from the first other one on, every tile is masked
+  while (t < end && whole()) step(std::false_type());
+  while (t < end) step(std::true_type());
 
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
     const float total = mf::sum_over_slices(acc[n].l);
     if (p.splits > 1) {
-      const int64_t at = int64_t(blockIdx.x) * kTileRows + rr;
+      if (r >= w.run_rows) continue;
+      const int64_t at = (int64_t(unit) * p.splits + split) * kTileRows + rr;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(part + at * D + 16 * d + 4 * quad) = acc[n].o[d];
       if (quad == 0) {
@@ -270,13 +300,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + 4 * quad;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        uint16_t v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = none ? 0.0f : acc[n].o[d][i] * f;
-          v[i] = q.fp16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
-        }
-        *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{v[0] | (uint32_t(v[1]) << 16), v[2] | (uint32_t(v[3]) << 16)};
+        const f4 x = none ? f4{0, 0, 0, 0} : acc[n].o[d] * f;
+        *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2(x[0], x[1], q.fp16), pack2(x[2], x[3], q.fp16)};
       }
       if (quad == 0 && lse != nullptr) {
         lse[(int64_t(w.s) * q.heads + head) * q.len + token] =

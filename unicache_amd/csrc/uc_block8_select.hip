@@ -26,6 +26,7 @@ struct Run {
   int32_t len, heads, group, run, runs;
   int32_t fp16, causal;
   int32_t budget, sink, recent;
+  FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const {
     if (lens == nullptr) return len;
@@ -203,12 +204,13 @@ __device__ __forceinline__ void own_codes(OwnCodes<D> &own, const Run &q, int32_
   if (part == 0) own.step[r] = bad ? __builtin_nanf("") : code_step(a);
 }
 
-// Scores for runs of many rows: a wave takes 64 blocks, whose bounds stay in registers, through all rows of
-// a run.
+// Scores for runs of many rows: a wave takes 32 blocks, whose bounds stay in registers, through all rows
+// of a run, the next 16 rows' codes on their way.
+constexpr int kScored = 2;  // 16-block groups of a wave
+
 template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t *codes, const float *steps,
                                                     float unit_factor, float *score, int32_t chunks) {
-  constexpr int kB = 4;  // 16-block groups
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int32_t unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;  // unit: (sequence, run, head)
   const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
@@ -219,28 +221,38 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
   const int32_t t0 = run * q.run;
   const int32_t rows = ((count - t0 < q.run) ? count - t0 : q.run) * q.group;
   const int64_t sh = int64_t(s) * c.heads + h;
-  for (int32_t b0 = (chunk * 4 + wave) * 16 * kB; b0 < blocks; b0 += chunks * 64 * kB) {
-    BlockBounds<D> x[kB];
-    float best[kB];
+  const int64_t row0 = (int64_t(s) * q.len + t0) * q.heads + h * q.group;
+  for (int32_t b0 = (chunk * 4 + wave) * 16 * kScored; b0 < blocks; b0 += chunks * 64 * kScored) {
+    BlockBounds<D> x[kScored];
+    float best[kScored];
 #pragma unroll
-    for (int n = 0; n < kB; ++n) {
+    for (int n = 0; n < kScored; ++n) {
       load_bounds<D>(x[n], c, sh, b0 + 16 * n, blocks, unit_factor);
       best[n] = mf::kNegInf;
     }
-    for (int32_t r0 = 0; r0 < rows; r0 += 16) {
+    i4 next[D / 64];
+    float next_step;
+    auto fetch = [&](int32_t r0) {
       const int32_t r = r0 + col < rows ? r0 + col : rows - 1;  // the last row again: it changes no maximum
-      const int64_t at = (int64_t(s) * q.len + t0 + r / q.group) * q.heads + h * q.group + r % q.group;
+      const int32_t token = static_cast<int32_t>(fast_div(r, q.by_group));
+      const int64_t at = row0 + int64_t(token) * q.heads + (r - token * q.group);
+      next_step = steps[at];
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) next[k] = *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16);
+    };
+    fetch(0);
+    for (int32_t r0 = 0; r0 < rows; r0 += 16) {
       RowCodes<D> rc;
-      const float step = steps[at];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rc.step[i] = __shfl(step, quad * 4 + i, kWave);
+      for (int i = 0; i < 4; ++i) rc.step[i] = __shfl(next_step, quad * 4 + i, kWave);
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16));
+      for (int k = 0; k < D / 64; ++k) rc.split(k, next[k]);
+      if (r0 + 16 < rows) fetch(r0 + 16);
 #pragma unroll
-      for (int n = 0; n < kB; ++n) score16<D>(x[n], rc, best[n]);
+      for (int n = 0; n < kScored; ++n) score16<D>(x[n], rc, best[n]);
     }
 #pragma unroll
-    for (int n = 0; n < kB; ++n) {
+    for (int n = 0; n < kScored; ++n) {
       const float v = over_rows(best[n], x[n].u);
       const int32_t b = b0 + 16 * n + col;
       if (quad == 0 && b < blocks) score[int64_t(unit) * c.blocks + b] = v;
@@ -418,7 +430,8 @@ int make_run(const uc_block8_cache *cache, const uc_block8_query *query, int64_t
   q = Run{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
           static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q),
           static_cast<int32_t>(query->heads_q / cache->heads_kv), static_cast<int32_t>(run),
-          static_cast<int32_t>(ceil_div(query->query_len, run)), query->dtype == UC_FP16, query->causal != 0, 0, 0, 0};
+          static_cast<int32_t>(ceil_div(query->query_len, run)), query->dtype == UC_FP16, query->causal != 0, 0, 0, 0,
+          make_fastdiv(static_cast<uint32_t>(query->heads_q / cache->heads_kv))};
   return UC_OK;
 }
 
@@ -480,7 +493,7 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t rows = cache->sequences * q.len * q.heads, units = cache->sequences * q.runs * cache->heads_kv;
   const int64_t capacity = cache->blocks * cache->block_tokens;
   const int64_t expected = query->max_tokens < capacity ? query->max_tokens : capacity;
-  const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 256) : 1;
+  const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 64 * kScored) : 1;
   UC_REQUIRE(rows < (int64_t(1) << 32) && units * chunks < (int64_t(1) << 31), "uc_block8_select: too many query rows");
   const float factor = cache->code_dtype == UC_INT8 ? 1.0f : static_cast<float>(448.0 / 127.0);
   auto launch = [&](auto d_tag) {
