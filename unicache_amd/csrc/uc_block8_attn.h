@@ -113,7 +113,7 @@ __device__ __forceinline__ int32_t per_of(const Plan &p, int32_t total) {
 // A wave's sum, the same in every lane.
 __device__ __forceinline__ int32_t wave_total(int32_t v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
 
-// For a wave: steps of all sequences (of one head and run), of those before s, and of s.
+// For a whole wave: steps of all sequences (of one head and run), of those before a lane's s, and of s.
 struct Steps {
   int32_t total, before, mine;
 };
@@ -130,9 +130,10 @@ __device__ __forceinline__ Steps steps_before(const Cache &c, const Query &q, co
     const int32_t i = s0 + (threadIdx.x & 63);
     const int32_t n = i < c.sequences ? steps_of(keys_of(c, p, c.length(i), q.count(i))) : 0;
     const int32_t sum = wave_prefix(n);
+    const int32_t m = __shfl(n, s - s0, kWave), b = __shfl(sum, s - s0, kWave);
     if (s >= s0 && s < s0 + 64) {
-      w.mine = __builtin_amdgcn_readlane(n, s - s0);
-      w.before = w.total + __builtin_amdgcn_readlane(sum, s - s0) - w.mine;
+      w.mine = m;
+      w.before = w.total + b - m;
     }
     w.total += __builtin_amdgcn_readlane(sum, 63);
   }

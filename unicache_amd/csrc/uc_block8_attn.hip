@@ -339,98 +339,139 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, 
   }
 }
 
-// Join the splits of the query rows.  WAVES == 1: a wave per row, for few splits; WAVES == 4: a
-// workgroup per row, whose waves take every fourth split and meet in LDS.  A
-// wave keeps four loads in flight.
-template <int D, int WAVES>
-__global__ __launch_bounds__(256) void join_kernel(Cache c, Query q, Plan p, int64_t rows, uint16_t *out, float *lse,
-                                                   const float *part, const float *stat) {
-  constexpr int kC = D / 64;
-  typedef float vec __attribute__((ext_vector_type(kC)));
-  __shared__ float sh_o[4][D], sh_l[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t index = WAVES == 1 ? int64_t(blockIdx.x) * 4 + wave : blockIdx.x;
-  if (index >= rows) return;
+// Where a query row's parts are: `count` slots from `first` on.
+struct Parts {
+  Rows w;
+  int32_t r;
+  int32_t first, count;
+};
+
+__device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const Plan &p, int64_t index) {
+  Parts x;
   // rows of the runs in order: (sequence, head, run, row)
   const int32_t full = p.run * q.group;
-  const int32_t r = static_cast<int32_t>(index % full), run = static_cast<int32_t>(index / full % p.runs);
-  const int64_t sh = index / full / p.runs;
-  const int32_t unit = static_cast<int32_t>((sh * p.runs + run) * p.groups + r / p.rows);
-  const Rows w = rows_of(c, q, p, unit, p.rows);
-  if (r >= w.run_rows) return;
-  // the parts of the row: consecutive slots
-  int32_t first, splits;
+  const int64_t at = index / full;
+  x.r = static_cast<int32_t>(index - at * full);
+  const int32_t run = p.runs == 1 ? 0 : static_cast<int32_t>(at % p.runs);
+  const int32_t sh = static_cast<int32_t>(p.runs == 1 ? at : at / p.runs), s = sh / c.heads;
+  const int32_t group = p.groups == 1 ? 0 : x.r / p.rows;
+  x.w = rows_at(q, p, s, sh - s * c.heads, run, group, p.rows, c.length(s), q.count(s));
+  const int32_t unit = static_cast<int32_t>(at) * p.groups + group;
   if (p.workgroups == 0) {
-    const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
-    first = unit * p.splits;
-    splits = tiles == 0 ? 1 : (tiles + per - 1) / per;
+    const int32_t tiles = tiles_of(c, p, x.w), per = split_tiles_of(p, tiles);
+    x.first = unit * p.splits;
+    x.count = tiles == 0 ? 1 : (tiles + per - 1) / per;
   } else {
-    const Steps steps = steps_before(c, q, p, w.s);
-    const int32_t each = c.heads * p.runs, n = unit - w.s * each, per = per_of(p, steps.total * each);
+    const Steps steps = steps_before(c, q, p, s);
+    const int32_t each = c.heads * p.runs, n = unit - s * each, per = per_of(p, steps.total * each);
     const int32_t start = steps.before * each + n * steps.mine;
-    first = steps.mine == 0 ? 0 : start / per + unit;
-    splits = steps.mine == 0 ? 0 : (start + steps.mine - 1) / per + unit - first + 1;
+    x.first = steps.mine == 0 ? 0 : start / per + unit;
+    x.count = steps.mine == 0 ? 0 : (start + steps.mine - 1) / per + unit - x.first + 1;
   }
-  const int64_t base = int64_t(first) * p.rows + r % p.rows;
-  float m = mf::kNegInf;
-  for (int32_t i = lane; i < splits; i += 64) m = fmaxf(m, stat[2 * (base + int64_t(i) * p.rows)]);
-  m = wave_max(m);
-  float total = 0.0f;
-  vec o = {};
-  for (int32_t i0 = WAVES == 1 ? 0 : wave; i0 < splits; i0 += 4 * WAVES) {
-    float mi[4], li[4];
-    vec oi[4];
+  return x;
+}
+
+// Join the parts of a query row.  16 lanes take every STRIDE-th part from `begin` on, D / 16 channels each, two
+// parts' loads in flight; the outcome is relative to m, the largest reference of all.
+template <int D>
+struct Sum {
+  float o[D / 16];
+  float m, l;
+};
+
+template <int D, int STRIDE>
+__device__ __forceinline__ Sum<D> sum_parts(const Plan &p, const Parts &x, int32_t begin, const float *part, const float *stat) {
+  constexpr int kC = D / 16;
+  const int lane = threadIdx.x & 15;
+  const int64_t base = int64_t(x.first) * p.rows + (x.r - x.w.r0);
+  Sum<D> t;
+  t.m = mf::kNegInf;
+  t.l = 0.0f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int32_t i = i0 + WAVES * u;
-      const int64_t at = base + int64_t(i < splits ? i : i0) * p.rows;
+  for (int j = 0; j < kC; ++j) t.o[j] = 0.0f;
+  for (int32_t i = lane; i < x.count; i += 16) t.m = fmaxf(t.m, stat[2 * (base + int64_t(i) * p.rows)]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) t.m = fmaxf(t.m, __shfl_xor(t.m, o, kWave));
+  for (int32_t i0 = begin; i0 < x.count; i0 += 2 * STRIDE) {
+    float mi[2], li[2];
+    f4 oi[2][kC / 4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int32_t i = i0 + u * STRIDE;
+      const int64_t at = base + int64_t(i < x.count ? i : i0) * p.rows;
       mi[u] = stat[2 * at];
-      li[u] = i < splits ? stat[2 * at + 1] : 0.0f;
-      oi[u] = *reinterpret_cast<const vec *>(part + at * D + lane * kC);
+      li[u] = stat[2 * at + 1];
+#pragma unroll
+      for (int j = 0; j < kC / 4; ++j) oi[u][j] = *reinterpret_cast<const f4 *>(part + at * D + lane * kC + 4 * j);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      // a split past the end, or one whose keys a row does not see
-      const bool live = i0 + WAVES * u < splits && !(mi[u] == mf::kNegInf && !(li[u] != 0.0f));
-      const float d = live ? mi[u] - m : mf::kNegInf, f = mf::fast_exp2(d);
-      total += rescaled(li[u], d);
+    for (int u = 0; u < 2; ++u) {
+      // a part past the end, or one whose keys the row does not see
+      if (i0 + u * STRIDE >= x.count || (mi[u] == mf::kNegInf && !(li[u] != 0.0f))) continue;
+      const float d = mi[u] - t.m, f = mf::fast_exp2(d);
+      t.l += rescaled(li[u], d);
 #pragma unroll
-      for (int j = 0; j < kC; ++j) o[j] += live ? f * oi[u][j] : 0.0f;
+      for (int j = 0; j < kC; ++j) t.o[j] += f * oi[u][j / 4][j % 4];
     }
   }
-  if constexpr (WAVES > 1) {
-    *reinterpret_cast<vec *>(&sh_o[wave][lane * kC]) = o;
-    if (lane == 0) sh_l[wave] = total;
-    __syncthreads();
-    if (wave > 0) return;
-    total = sh_l[0] + sh_l[1] + sh_l[2] + sh_l[3];
+  return t;
+}
+
+template <int D>
+__device__ __forceinline__ void finish_row(const Query &q, const Parts &x, const Sum<D> &t, uint16_t *out, float *lse) {
+  constexpr int kC = D / 16;
+  const int lane = threadIdx.x & 15;
+  const int32_t g = token_of(q, x.r), token = x.w.run0 + g, head = x.w.h * q.group + x.r - g * q.group;
+  const bool none = token >= x.w.count || t.l == 0.0f;
+  const float f = 1.0f / t.l;
+  uint32_t v[kC / 2];
 #pragma unroll
-    for (int j = 0; j < kC; ++j) o[j] = sh_o[0][lane * kC + j] + sh_o[1][lane * kC + j] + sh_o[2][lane * kC + j] + sh_o[3][lane * kC + j];
-  }
-  const int32_t token = w.run0 + token_of(q, r), head = w.h * q.group + r - token_of(q, r) * q.group;
-  const bool none = token >= w.count || total == 0.0f;
-  const float f = none ? 0.0f : 1.0f / total;
-  uint16_t v[kC];
-#pragma unroll
-  for (int j = 0; j < kC; ++j) {
-    const float x = none ? 0.0f : o[j] * f;
-    v[j] = q.fp16 ? f32_to_f16_bits(x) : f32_to_bf16_bits(x);
-  }
-  uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + head) * D + lane * kC;
-  if constexpr (kC == 2) {
-    *reinterpret_cast<uint32_t *>(dst) = v[0] | (uint32_t(v[1]) << 16);
+  for (int j = 0; j < kC / 2; ++j) v[j] = none ? 0u : pack2(t.o[2 * j] * f, t.o[2 * j + 1] * f, q.fp16);
+  uint16_t *dst = out + ((int64_t(x.w.s) * q.len + token) * q.heads + head) * D + lane * kC;
+  if constexpr (kC == 8) {
+    *reinterpret_cast<uint4 *>(dst) = uint4{v[0], v[1], v[2], v[3]};
   } else {
-    *dst = v[0];
+    *reinterpret_cast<uint2 *>(dst) = uint2{v[0], v[1]};
   }
   if (lane == 0 && lse != nullptr) {
-    lse[(int64_t(w.s) * q.heads + head) * q.len + token] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(total));
+    lse[(int64_t(x.w.s) * q.heads + head) * q.len + token] = none ? mf::kNegInf : kLn2 * (t.m + __builtin_amdgcn_logf(t.l));
   }
 }
 
-#ifndef KSHARE
-#define KSHARE 512
-#endif
-constexpr int64_t kShare = KSHARE;  // workgroups that share the tiles of few rows: two a CU
+// Few parts a row: a wave joins four rows.
+template <int D>
+__global__ __launch_bounds__(256) void join_few_kernel(Cache c, Query q, Plan p, int64_t rows, uint16_t *out, float *lse,
+                                                       const float *part, const float *stat) {
+  const int64_t index = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const Parts x = parts_of(c, q, p, index < rows ? index : rows - 1);  // (whole waves: they sum up lengths)
+  if (index >= rows || x.r >= x.w.run_rows) return;
+  finish_row<D>(q, x, sum_parts<D, 1>(p, x, 0, part, stat), out, lse);
+}
+
+// Many: a workgroup joins one row, its 16-lane groups every 16th part.
+template <int D>
+__global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
+                                                        const float *part, const float *stat) {
+  constexpr int kC = D / 16;
+  __shared__ float sh_o[16][D], sh_l[16];
+  const Parts x = parts_of(c, q, p, blockIdx.x);
+  if (x.r >= x.w.run_rows) return;
+  const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  Sum<D> t = sum_parts<D, 16>(p, x, group, part, stat);
+#pragma unroll
+  for (int j = 0; j < kC; ++j) sh_o[group][lane * kC + j] = t.o[j];
+  if (lane == 0) sh_l[group] = t.l;
+  __syncthreads();
+  if (group > 0) return;
+  for (int g = 1; g < 16 && g < x.count; ++g) {
+    t.l += sh_l[g];
+#pragma unroll
+    for (int j = 0; j < kC; ++j) t.o[j] += sh_o[g][lane * kC + j];
+  }
+  finish_row<D>(q, x, t, out, lse);
+}
+
+constexpr int64_t kShare = 512;  // workgroups that share the tiles of few rows: two a CU
 
 int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget, int64_t query_block,
               const char *what, Query &q, Plan &p) {
@@ -547,18 +588,18 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   }
   if (rc != UC_OK || (p.splits == 1 && p.workgroups == 0)) return rc;
   const int64_t q_rows = cache->sequences * cache->heads_kv * p.runs * p.run * q.group;
-  auto join = [&](auto d_tag, auto waves_tag) {
-    constexpr int D = decltype(d_tag)::value, W = decltype(waves_tag)::value;
-    hipLaunchKernelGGL((join_kernel<D, W>), dim3(static_cast<uint32_t>(W == 1 ? ceil_div(q_rows, 4) : q_rows)), dim3(256),
-                       0, as_stream(stream), c, q, p, q_rows, static_cast<uint16_t *>(out), lse, part, stat);
-    return check_launch("uc_block8_attn (join)");
-  };
-  typedef std::integral_constant<int, 1> One;
-  typedef std::integral_constant<int, 4> Four;
-  typedef std::integral_constant<int, 64> D64;
-  typedef std::integral_constant<int, 128> D128;
   // parts of a row, if all sequences were of the expected length
   const bool few = (p.workgroups > 0 ? ceil_div(p.workgroups, units) : p.splits) <= 8;
-  if (cache->head_dim == 128) return few ? join(D128(), One()) : join(D128(), Four());
-  return few ? join(D64(), One()) : join(D64(), Four());
+  auto join = [&](auto d_tag) {
+    constexpr int D = decltype(d_tag)::value;
+    if (few) {
+      hipLaunchKernelGGL((join_few_kernel<D>), dim3(static_cast<uint32_t>(ceil_div(q_rows, 16))), dim3(256), 0,
+                         as_stream(stream), c, q, p, q_rows, static_cast<uint16_t *>(out), lse, part, stat);
+    } else {
+      hipLaunchKernelGGL((join_many_kernel<D>), dim3(static_cast<uint32_t>(q_rows)), dim3(256), 0, as_stream(stream), c,
+                         q, p, static_cast<uint16_t *>(out), lse, part, stat);
+    }
+    return check_launch("uc_block8_attn (join)");
+  };
+  return cache->head_dim == 128 ? join(std::integral_constant<int, 128>()) : join(std::integral_constant<int, 64>());
 }

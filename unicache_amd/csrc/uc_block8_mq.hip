@@ -92,23 +92,36 @@ __device__ __forceinline__ int value_swizzle(int channel) {
   return (channel & 1) | ((channel >> 2) & 1) << 1 | ((channel >> 1) & 1) << 2;
 }
 
-template <int D, int CODE>
-__device__ __forceinline__ void store(Staged<D> &st, char *buf, const Loader<D> &ld, int32_t length) {
-  if (st.t[0] + 32 > length || st.t[1] + 32 > length) {  // codes behind the length are no values
+// Codes behind the length are no values.
+template <int D>
+__device__ __forceinline__ void clear(Staged<D> &st, const Loader<D> &ld, int32_t length) {
+  if (st.t[0] + 32 > length || st.t[1] + 32 > length) {
 #pragma unroll
-    for (int i = 0; i < Tile<D>::kLoads; ++i) st.v[i] = first_bytes(st.v[i], length - (ld.half(i) ? st.t[1] : st.t[0]) - ld.k16 * 16);
+    for (int i = 0; i < Tile<D>::kLoads; ++i) {
+      st.v[i] = first_bytes(st.v[i], length - (ld.half(i) ? st.t[1] : st.t[0]) - ld.k16 * 16);
+    }
   }
+}
+
+template <int D, int CODE>
+__device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const Loader<D> &ld) {
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
-    const int h = ld.half(i);
-    char *row = buf + (ld.key + 32 * h) * Tile<D>::kKeyRow;
+    char *row = buf + (ld.key + 32 * ld.half(i)) * Tile<D>::kKeyRow;
     const int sw = key_swizzle(ld.key) & (D / 8 - 1);
     *reinterpret_cast<h8 *>(row + 16 * ((2 * ld.c16) ^ sw)) = codes_to_h8<CODE>(st.k[i].x, st.k[i].y);
     *reinterpret_cast<h8 *>(row + 16 * ((2 * ld.c16 + 1) ^ sw)) = codes_to_h8<CODE>(st.k[i].z, st.k[i].w);
-    char *vrow = buf + Tile<D>::kKeyBytes + ld.channel * Tile<D>::kValueRow;
-    const int chunk = 4 * h + 2 * ld.k16, vw = value_swizzle(ld.channel);
-    *reinterpret_cast<h8 *>(vrow + 16 * (chunk ^ vw)) = codes_to_h8<CODE>(st.v[i].x, st.v[i].y);
-    *reinterpret_cast<h8 *>(vrow + 16 * ((chunk + 1) ^ vw)) = codes_to_h8<CODE>(st.v[i].z, st.v[i].w);
+  }
+}
+
+template <int D, int CODE>
+__device__ __forceinline__ void store_values(const Staged<D> &st, char *buf, const Loader<D> &ld) {
+#pragma unroll
+  for (int i = 0; i < Tile<D>::kLoads; ++i) {
+    char *row = buf + Tile<D>::kKeyBytes + ld.channel * Tile<D>::kValueRow;
+    const int chunk = 4 * ld.half(i) + 2 * ld.k16, sw = value_swizzle(ld.channel);
+    *reinterpret_cast<h8 *>(row + 16 * (chunk ^ sw)) = codes_to_h8<CODE>(st.v[i].x, st.v[i].y);
+    *reinterpret_cast<h8 *>(row + 16 * ((chunk + 1) ^ sw)) = codes_to_h8<CODE>(st.v[i].z, st.v[i].w);
   }
 }
 
@@ -119,25 +132,27 @@ struct Acc16 {
   float m, l;
 };
 
-// Weights of one tile for 16 rows; ends[h]: keys of half h that the lane's row sees, from its own first key on.
-template <int D, bool MASK>
-__device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const float (&c)[2], const float (&lv)[2],
-                                        const float (&inv)[2], const int32_t (&ends)[2], h8 (&p)[2]) {
+// Weights of one tile for 16 rows.  N == 2: its halves are in two blocks; else one scale of each kind
+// is the tile's.  ends[h]: keys of half h that the lane's row sees, from its own first key on.
+template <int D, bool MASK, int N>
+__device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const float (&c)[N], const float (&lv)[N],
+                                        const float (&inv)[N], const int32_t (&ends)[2], h8 (&p)[2]) {
+  constexpr int kK = 16 / N;  // logits of a lane per scale
   float x[MASK ? 16 : 1];
   float top = mf::kNegInf;
   if constexpr (MASK) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const int h = j / 8;
-      x[j] = j % 8 < ends[h] ? __builtin_fmaf(s[j / 4][j % 4], c[h], lv[h]) : mf::kNegInf;
+      const int h = j / kK;
+      x[j] = j % 8 < ends[j / 8] ? __builtin_fmaf(s[j / 4][j % 4], c[h], lv[h]) : mf::kNegInf;
       top = fmaxf(top, x[j]);
     }
   } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < N; ++h) {
       float t = mf::kNegInf;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t = fmaxf(t, s[2 * h + j / 4][j % 4]);
+      for (int j = h * kK; j < (h + 1) * kK; ++j) t = fmaxf(t, s[j / 4][j % 4]);
       top = fmaxf(top, __builtin_fmaf(t, c[h], lv[h]));
     }
   }
@@ -152,14 +167,14 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
   }
   const float m = acc.m == mf::kNegInf ? 0.0f : acc.m;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < N; ++h) {
     float sum = 0.0f;
     const float shift = lv[h] - m;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = mf::fast_exp2(MASK ? x[MASK ? 8 * h + j : 0] - m : __builtin_fmaf(s[2 * h + j / 4][j % 4], c[h], shift));
-      sum += e;
-      p[h][j] = mf::to_h(e);
+    for (int j = h * kK; j < (h + 1) * kK; ++j) {
+      const float e = mf::fast_exp2(MASK ? x[MASK ? j : 0] - m : __builtin_fmaf(s[j / 4][j % 4], c[h], shift));
+      sum = j == h * kK ? e : sum + e;
+      p[j / 8][j % 8] = mf::to_h(e);
     }
     if constexpr (MASK) {
       acc.l += sum == 0.0f ? 0.0f : sum * inv[h];
@@ -169,8 +184,8 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
   }
 }
 
-template <int D, int CODE>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint32_t units, uint16_t *out, float *lse,
+template <int D, int CODE, int N>
+__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                       float *part, float *stat) {
   typedef Tile<D> T;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
@@ -228,15 +243,19 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     constexpr bool MASK = decltype(mask_tag)::value;
     const char *buf = lds + present;
     const int32_t t0 = st.t[0], t1 = st.t[1];
-    float ks[2], vs[2];
+    // (one block: the halves' scales are the same, and the first is there if any is)
+    float ks[N], lv[N], inv[N];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < N; ++h) {
       ks[h] = st.ks[h];
-      vs[h] = counted_scale(!MASK || st.t[h] < w.length ? st.vs[h] : 1.0f, most);
+      const float vs = counted_scale(!MASK || st.t[h] < w.length ? st.vs[h] : 1.0f, most);
+      lv[h] = __builtin_amdgcn_logf(vs);
+      inv[h] = __builtin_amdgcn_rcpf(vs);
     }
     const bool more = t + 1 < end;
     if (more) get(t + 1);
 
+    __builtin_amdgcn_s_setprio(3);
     f4 s[2][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -248,32 +267,46 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         s[1][j] = mf::mfma32(a, frag[1][k], s[1][j]);
       }
     }
+    __builtin_amdgcn_s_setprio(0);
     h8 pr[2][2];
-    const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
-    const float inv[2] = {__builtin_amdgcn_rcpf(vs[0]), __builtin_amdgcn_rcpf(vs[1])};
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const float cc[2] = {ks[0] * factor[n], ks[1] * factor[n]};
+      float cc[N];
+#pragma unroll
+      for (int h = 0; h < N; ++h) cc[h] = ks[h] * factor[n];
       const int32_t ends[2] = {row_end[n] - t0 - 8 * quad, row_end[n] - t1 - 8 * quad};
-      weights<D, MASK>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
+      weights<D, MASK, N>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
     }
+    // The next tile's codes become fp16 beside the P V products (after the last tile the present
+    // one's again, into the buffer that nobody reads): a few vector instructions per MFMA.
+    clear<D>(st, ld, w.length);
+    present ^= T::kBytes;
+    __builtin_amdgcn_s_setprio(3);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
+    for (int h = 0; h < 2; ++h) {
+      h8 a[D / 16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const h8 a = *reinterpret_cast<const h8 *>(buf + va[h] + d * 16 * T::kValueRow);
-        acc[0].o[d] = mf::mfma32(a, pr[0][h], acc[0].o[d]);
-        acc[1].o[d] = mf::mfma32(a, pr[1][h], acc[1].o[d]);
+      for (int d = 0; d < D / 16; ++d) a[d] = *reinterpret_cast<const h8 *>(buf + va[h] + d * 16 * T::kValueRow);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        acc[0].o[d] = mf::mfma32(a[d], pr[0][h], acc[0].o[d]);
+        acc[1].o[d] = mf::mfma32(a[d], pr[1][h], acc[1].o[d]);
+      }
+      if (h == 0) {
+        store_keys<D, CODE>(st, lds + present, ld);
+      } else {
+        store_values<D, CODE>(st, lds + present, ld);
       }
     }
-    present ^= T::kBytes;
-    if (more) store<D, CODE>(st, lds + present, ld, w.length);
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
     ++t;
   };
   if (begin < end) {
     get(begin);
-    store<D, CODE>(st, lds, ld, w.length);
+    clear<D>(st, ld, w.length);
+    store_keys<D, CODE>(st, lds, ld);
+    store_values<D, CODE>(st, lds, ld);
   }
   __syncthreads();
   // tiles that every row sees come first; from the first other one on, every tile is masked
@@ -316,8 +349,11 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint32_t workgroups,
                  uint16_t *out, float *lse, float *part, float *stat, hipStream_t stream) {
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
-    hipLaunchKernelGGL((tile_kernel<D, CODE>), dim3(workgroups), dim3(256), 0, stream, c, q, p, workgroups / p.splits, out,
-                       lse, part, stat);
+    if (c.block == 32) {
+      hipLaunchKernelGGL((tile_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, stream, c, q, p, out, lse, part, stat);
+    } else {
+      hipLaunchKernelGGL((tile_kernel<D, CODE, 1>), dim3(workgroups), dim3(256), 0, stream, c, q, p, out, lse, part, stat);
+    }
     return check_launch("uc_block8_attn");
   });
 }
