@@ -471,6 +471,27 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
   finish_row<D>(q, x, t, out, lse);
 }
 
+// Splits of 128-row workgroups: the least time in tiles.  Two (head_dim 128) or three workgroups share
+// a CU; up to one a CU takes 0.65 of the time a tile; the join takes two tiles and 0.006 for each part of
+// a workgroup.  Measured, one split -> the chosen: 112 units of 64 tiles 110 -> 56 us (4 splits), 28 of 256
+// 412 -> 59 (18), 572 of 64 247 -> 213 (4), 376 of 128 at head_dim 64 196 -> 151 (2); 512 of 64 stay at
+// one (206; two would take 224), as do 440 of 31 (66; 89).
+int64_t tile_splits(int64_t units, int64_t tiles, int64_t head_dim) {
+  const int64_t slots = head_dim == 128 ? 512 : 768;
+  int64_t best = 1;
+  double least = 1e300;
+  const int64_t most = ceil_div(tiles, 4) < 64 ? ceil_div(tiles, 4) : 64;
+  for (int64_t k = 1; k <= most; ++k) {
+    const double rounds = units * k <= slots / 2 ? 0.65 : static_cast<double>(ceil_div(units * k, slots));
+    const double time = rounds * static_cast<double>(ceil_div(tiles, k)) + (k > 1 ? 2.0 + 0.006 * static_cast<double>(units * k) : 0.0);
+    if (time < least) {
+      least = time;
+      best = k;
+    }
+  }
+  return best;
+}
+
 constexpr int64_t kShare = 512;  // workgroups that share the tiles of few rows: two a CU
 
 int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_t budget, int64_t query_block,
@@ -505,10 +526,7 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
   p.workgroups = 0;
   if (p.rows == kTileRows) {
-    // 512 workgroups (two a CU), each with four tiles at least
-    int64_t splits = units > 0 ? 512 / units : 1;
-    const int64_t most = ceil_div(tiles, 4);
-    splits = splits < 1 ? 1 : splits > most ? most : splits;
+    const int64_t splits = tile_splits(units, tiles, cache->head_dim);
     p.split_tiles = static_cast<int32_t>(ceil_div(tiles, splits));
     p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
   } else {
