@@ -85,15 +85,19 @@ template <int D, int CODE, bool MASK>
 __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[4], float factor, float ks, float vs,
                                              int32_t seen, h8 (&p)[2]) {
   const float c = ks * factor, lv = __builtin_amdgcn_logf(vs);
-  float x[16], top = mf::kNegInf;
+  float x[MASK ? 16 : 1], top = mf::kNegInf;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    x[j] = __builtin_fmaf(s[j / 4][j % 4], c, lv);
-    if constexpr (MASK) x[j] = j < seen ? x[j] : mf::kNegInf;
-    top = fmaxf(top, x[j]);
+    if constexpr (MASK) {
+      x[j] = j < seen ? __builtin_fmaf(s[j / 4][j % 4], c, lv) : mf::kNegInf;
+      top = fmaxf(top, x[j]);
+    } else {
+      top = fmaxf(top, s[j / 4][j % 4]);
+    }
   }
+  if constexpr (!MASK) top = __builtin_fmaf(top, c, lv);
   top = mf::max_over_slices(top);
-  if (__any(top > acc.m + kRaise || (acc.m == mf::kNegInf && top > acc.m))) {
+  if (__any(top > acc.m + kRaise)) {
     const float m = fmaxf(acc.m, top);
     const float d = m == mf::kNegInf ? 0.0f : acc.m - m, alpha = mf::fast_exp2(d);
     acc.m = m;
@@ -105,7 +109,7 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[4], floa
   float sum = 0.0f;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    const float e = mf::fast_exp2(x[j] - m);
+    const float e = mf::fast_exp2(MASK ? x[MASK ? j : 0] - m : __builtin_fmaf(s[j / 4][j % 4], c, lv - m));
     sum += e;
     p[j / 8][j % 8] = mf::to_h(e);
   }
@@ -113,18 +117,21 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[4], floa
   acc.l += sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_rcpf(vs);
 }
 
-// LDS of the waves' join.
-template <int D>
+// LDS of the waves' join; and with 32 rows of 128 channels the query fragments, which do not fit
+// the registers beside the rest (they spilled: 8 x 32k tokens, 28 rows, 149 us).
+template <int D, int NR>
 struct Joined {
+  static constexpr bool kHeld = D == 128 && NR == 2;
   float o[4][16][D + 4];
   float m[4][16], l[4][16];
+  h8 frag[kHeld ? NR * D / 32 : 1][64];
 };
 
 // Tiles begin .. end - 1 of the rows w, by a whole workgroup.  slot >= 0: the part goes there; else it
 // is all there is, and the rows are finished.
 template <int D, int CODE, int NR>
 __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan &p, const Rows &w, int32_t begin, int32_t end,
-                                      int32_t slot, Joined<D> &joined, uint16_t *out, float *lse, float *part,
+                                      int32_t slot, Joined<D, NR> &joined, uint16_t *out, float *lse, float *part,
                                       float *stat) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
             quad = lane >> 4;
@@ -165,7 +172,22 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
   }
-  for (; t < end; t += 4) {
+  if constexpr (Joined<D, NR>::kHeld) {
+    __syncthreads();  // the fragments of the piece before have been read
+    if (wave == 0) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) joined.frag[n * (D / 32) + k][lane] = frag[n][k];
+      }
+    }
+    __syncthreads();
+  }
+  auto step = [&](auto mask_tag) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    int at = lane;  // opaque, so that the fragments are read in every tile and not kept
+    if constexpr (Joined<D, NR>::kHeld) asm volatile("" : "+v"(at));
+    auto query = [&](int n, int k) { return Joined<D, NR>::kHeld ? joined.frag[n * (D / 32) + k][at] : frag[n][k]; };
     int32_t n0 = kNone, n1 = kNone;
     const bool more = t + 4 < end;
     if (more) {
@@ -183,22 +205,18 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
         const h8 a = codes_to_h8<CODE>(raw.k[j][x].x, raw.k[j][x].y), b = codes_to_h8<CODE>(raw.k[j][x].z, raw.k[j][x].w);
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-          s[n][j] = mf::mfma32(a, frag[n][2 * x], s[n][j]);
-          s[n][j] = mf::mfma32(b, frag[n][2 * x + 1], s[n][j]);
+          s[n][j] = mf::mfma32(a, query(n, 2 * x), s[n][j]);
+          s[n][j] = mf::mfma32(b, query(n, 2 * x + 1), s[n][j]);
         }
       }
     }
     const int32_t mine = ((quad & 2) ? t1 : t0) + l.key;  // the lane's first key
-    const float ks = raw.ks, vs = counted_scale(mine < w.length ? raw.vs : 1.0f, most);
+    const float ks = raw.ks, vs = counted_scale(!MASK || mine < w.length ? raw.vs : 1.0f, most);
     if (more) load_keys(raw, c, l, n0, n1);
     h8 pr[NR][2];
-    const int32_t last = t0 > t1 ? t0 : t1;
-    if (last + 32 <= w.end_first) {
 #pragma unroll
-      for (int n = 0; n < NR; ++n) softmax_step<D, CODE, false>(acc[n], s[n], factor[n], ks, vs, 16, pr[n]);
-    } else {
-#pragma unroll
-      for (int n = 0; n < NR; ++n) softmax_step<D, CODE, true>(acc[n], s[n], factor[n], ks, vs, row_end[n] - mine, pr[n]);
+    for (int n = 0; n < NR; ++n) softmax_step<D, CODE, MASK>(acc[n], s[n], factor[n], ks, vs, row_end[n] - mine, pr[n]);
+    if constexpr (MASK) {
       // codes behind the length are no values: a zero weight must not meet them
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) raw.v[d] = first_bytes(raw.v[d], w.length - mine);
@@ -215,7 +233,11 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
     if (more) load_values(raw, c, l, n0, n1);
     t0 = n0;
     t1 = n1;
-  }
+    t += 4;
+  };
+  // tiles that every row sees come first; from the first other one on, every tile is masked
+  while (t < end && (t0 > t1 ? t0 : t1) + 32 <= w.end_first) step(std::false_type());
+  while (t < end) step(std::true_type());
 
   // join the waves: 16 threads a row, D / 16 channels each
   constexpr int kC = D / 16;
@@ -277,7 +299,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
 template <int D, int CODE, int NR>
 __global__ __launch_bounds__(256, 2) void rows_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                       float *part, float *stat) {
-  __shared__ Joined<D> joined;
+  __shared__ Joined<D, NR> joined;
   if (p.workgroups == 0) {  // one workgroup a unit
     const Rows w = rows_of(c, q, p, blockIdx.x, 16 * NR);
     piece<D, CODE, NR>(c, q, p, w, 0, tiles_of(c, p, w), -1, joined, out, lse, part, stat);
