@@ -117,11 +117,11 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[4], floa
   acc.l += sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_rcpf(vs);
 }
 
-// LDS of the waves' join; and with 32 rows of 128 channels the query fragments, which do not fit
+// LDS of the waves' join; and with 32 rows of 128 channels or 48 of 64 the query fragments, which do not fit
 // the registers beside the rest (they spilled: 8 x 32k tokens, 28 rows, 149 us).
 template <int D, int NR>
 struct Joined {
-  static constexpr bool kHeld = D == 128 && NR == 2;
+  static constexpr bool kHeld = NR * D >= 192;
   float o[4][16][D + 4];
   float m[4][16], l[4][16];
   h8 frag[kHeld ? NR * D / 32 : 1][64];
@@ -493,6 +493,17 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
   finish_row<D>(q, x, t, out, lse);
 }
 
+template <int D, int CODE, class... Args>
+void launch_rows(int32_t rows, uint32_t workgroups, hipStream_t stream, const Args &...args) {
+  if (rows == 16) {
+    hipLaunchKernelGGL((rows_kernel<D, CODE, 1>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else if (rows == 32) {
+    hipLaunchKernelGGL((rows_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else if constexpr (D == 64) {
+    hipLaunchKernelGGL((rows_kernel<D, CODE, 3>), dim3(workgroups), dim3(256), 0, stream, args...);
+  }
+}
+
 // Splits of 128-row workgroups: the least time in tiles.  Two (head_dim 128) or three workgroups share
 // a CU; up to one a CU takes 0.65 of the time a tile; the join takes two tiles and 0.006 for each part of
 // a workgroup.  Measured, one split -> the chosen: 112 units of 64 tiles 110 -> 56 us (4 splits), 28 of 256
@@ -538,7 +549,7 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   p.run = static_cast<int32_t>(run);
   p.runs = static_cast<int32_t>(ceil_div(query->query_len, run));
   const int64_t rows = run * q.group;
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kTileRows;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 && cache->head_dim == 64 ? 48 : kTileRows;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
   // keys that the launch expects a row to read
   const int64_t capacity = cache->blocks * cache->block_tokens;
@@ -616,13 +627,7 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
     rc = launch_tiles(cache, c, q, p, workgroups, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
   } else {
     rc = UC_B8_DISPATCH(cache, cache->head_dim, [&] {
-      if (p.rows == 16) {
-        hipLaunchKernelGGL((rows_kernel<D, CODE, 1>), dim3(workgroups), dim3(256), 0, as_stream(stream), c, q, p,
-                           static_cast<uint16_t *>(out), lse, part, stat);
-      } else {
-        hipLaunchKernelGGL((rows_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, as_stream(stream), c, q, p,
-                           static_cast<uint16_t *>(out), lse, part, stat);
-      }
+      launch_rows<D, CODE>(p.rows, workgroups, as_stream(stream), c, q, p, static_cast<uint16_t *>(out), lse, part, stat);
       return check_launch("uc_block8_attn");
     });
   }
