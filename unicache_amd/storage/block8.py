@@ -37,6 +37,16 @@ def _check_half(t: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} requires a gradient, which the 8-bit cache does not give; detach it")
 
 
+def _check_tensor(name, t, dtype, shape, device, align) -> None:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"Block8 cache {name}: expected contiguous {dtype} {shape}, got {t.dtype} "
+                         f"{tuple(t.shape)} strides {tuple(t.stride())}")
+    if t.device != device:
+        raise RuntimeError("Block8 cache received tensors on different devices")
+    if t.data_ptr() & align:
+        raise ValueError(f"Block8 cache {name} must be {align + 1}-byte aligned")
+
+
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """`t` where the kernels can read it in place (unit channel stride, rows on
     16 bytes), a contiguous copy otherwise."""
@@ -92,34 +102,28 @@ class Block8KVCache:
                  tail=None) -> None:
         if key_code.dim() != 4 or value_code.dim() != 5:
             raise ValueError("Block8 cache expects key codes [S, Hkv, N * B, D] and value codes [S, Hkv, N, D, B]")
-        s, h, tokens, d = map(int, key_code.shape)
-        n, b = int(value_code.shape[2]), int(value_code.shape[4])
-        if key_code.dtype not in _CODES or value_code.dtype != key_code.dtype:
+        s, h, _, d = key_code.shape
+        n, b = value_code.shape[2], value_code.shape[4]
+        code_dtype = key_code.dtype
+        if code_dtype not in _CODES or value_code.dtype != code_dtype:
             raise ValueError("Block8 cache codes must be int8 or float8_e4m3fn, keys and values alike")
         if b not in (32, 64, 128) or d not in (64, 128):
             raise ValueError("Block8 cache supports blocks of 32, 64 or 128 tokens and head_dim 64 or 128")
-        expected = (
-            ("key_code", key_code, key_code.dtype, (s, h, n * b, d)),
-            ("value_code", value_code, key_code.dtype, (s, h, n, d, b)),
-            ("key_scale", key_scale, torch.float32, (s, h, n)),
-            ("value_scale", value_scale, torch.float32, (s, h, n)),
-            ("key_bounds", key_bounds, torch.int8, (s, h, n, 2, d)),
-            ("lengths", lengths, torch.int32, (s,)),
-        )
+        device = key_code.device
+        _check_tensor("key_code", key_code, code_dtype, (s, h, n * b, d), device, 15)
+        _check_tensor("value_code", value_code, code_dtype, (s, h, n, d, b), device, 15)
+        _check_tensor("key_scale", key_scale, torch.float32, (s, h, n), device, 3)
+        _check_tensor("value_scale", value_scale, torch.float32, (s, h, n), device, 3)
+        _check_tensor("key_bounds", key_bounds, torch.int8, (s, h, n, 2, d), device, 15)
+        _check_tensor("lengths", lengths, torch.int32, (s,), device, 3)
         if tail is not None:
             if tail.dtype not in _HALVES:
                 raise ValueError("Block8 cache tail must be bf16 or fp16")
-            expected += (("tail", tail, tail.dtype, (s, h, 2, b, d)),)
-        for name, t, dtype, shape in expected:
-            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-                raise ValueError(f"Block8 cache {name}: expected contiguous {dtype} {shape}, got {t.dtype} "
-                                 f"{tuple(t.shape)} strides {tuple(t.stride())}")
+            _check_tensor("tail", tail, tail.dtype, (s, h, 2, b, d), device, 15)
+        if device.type != "cuda":
+            raise RuntimeError(f"Block8 cache requires GPU tensors (got {device})")
         if not s or not h or not n:
             raise ValueError("Block8 cache needs a sequence, a KV head and a block at least")
-        nat.require_device(*(t for _, t, _, _ in expected), what="Block8 cache")
-        for name, t, _, _ in expected:
-            if t.data_ptr() % (16 if name in ("key_code", "value_code", "key_bounds", "tail") else 4):
-                raise ValueError(f"Block8 cache {name} must be 16-byte aligned")
         if max_tokens is not None and int(max_tokens) < 0:
             raise ValueError("Block8 cache max_tokens must not be negative")
         self._set(key_code, value_code, key_scale, value_scale, key_bounds, lengths, tail, (s, h, d, n, b), max_tokens)
@@ -240,24 +244,26 @@ class Block8KVCache:
         if query_lengths is not None and (query_lengths.dtype != torch.int32 or not query_lengths.is_contiguous()
                                           or tuple(query_lengths.shape) != (self.sequences,)):
             raise ValueError("Block8 query_lengths must be contiguous int32 [sequences]")
-        if nat.require_device(query, query_lengths, what="Block8 attention") != self.device:
-            raise RuntimeError("Block8 attention received tensors on different devices")
+        if query.device != self.device or (query_lengths is not None and query_lengths.device != self.device):
+            raise RuntimeError(f"Block8 attention requires GPU tensors on the cache's device {self.device}")
         query = _rows16(query)
-        sizes = (lq, hq, self.max_tokens, nat.dtype_code(query.dtype), 1 if causal else 0)
-        struct = nat.Block8Query(query.data_ptr(), *query.stride()[:3], lq, hq, nat.ptr(query_lengths), *sizes[2:])
-        return query, struct, sizes
+        a, b, c, _ = query.stride()
+        dtype, causal = nat.dtype_code(query.dtype), 1 if causal else 0
+        struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), self.max_tokens, dtype, causal)
+        return query, struct, (lq, hq, self.max_tokens, dtype, causal)
 
-    def _attend(self, query, struct, sizes, blocks, budget, query_block, sm_scale):
+    def _scale(self, sm_scale) -> float:
         sm_scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else float(sm_scale)
         if not 0.0 < sm_scale < math.inf:
             raise ValueError("Block8 attention sm_scale must be positive")
-        lq, hq = sizes[:2]
+        return sm_scale
+
+    def _attend(self, cache, query, struct, sizes, blocks, budget, query_block, sm_scale, ws, nbytes):
+        lq, hq = sizes[0], sizes[1]
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
         lse = torch.empty((self.sequences, hq, lq), dtype=torch.float32, device=self.device)
-        nbytes = _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes, sizes, budget, query_block)
-        ws = nat.workspace(self.device, nbytes)
-        self._call("uc_block8_attn", self._struct(), struct, nat.ptr(blocks), budget, query_block, sm_scale,
-                 out.data_ptr(), lse.data_ptr(), ws.data_ptr(), nbytes)
+        self._call("uc_block8_attn", cache, struct, nat.ptr(blocks), budget, query_block, sm_scale, out.data_ptr(),
+                   lse.data_ptr(), nat.ptr(ws), nbytes)
         return out, lse
 
     # ------------------------------------------------------------------ calls --
@@ -318,8 +324,11 @@ class Block8KVCache:
         to lengths[s] - query_lengths[s] + i.  Rows that see no key, and rows
         behind a sequence's queries, get 0 and -inf."""
 
+        sm_scale = self._scale(sm_scale)
         q, struct, sizes = self._query(query, query_lengths, causal)
-        return self._attend(q, struct, sizes, None, 0, 0, sm_scale)
+        nbytes = _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes, sizes, 0, 0)
+        ws = nat.workspace(self.device, nbytes) if nbytes else None
+        return self._attend(self._struct(), q, struct, sizes, None, 0, 0, sm_scale, ws, nbytes)
 
     def sparse_attention(self, query: torch.Tensor, *, budget: int, query_block: int = 1, sink: int = 1,
                          recent: int = 1, query_lengths: torch.Tensor | None = None, causal: bool = False,
@@ -335,14 +344,18 @@ class Block8KVCache:
         budget, query_block, sink, recent = int(budget), int(query_block), int(sink), int(recent)
         if budget <= 0 or query_block <= 0:
             raise ValueError("Block8 sparse attention needs a positive budget and query_block")
+        sm_scale = self._scale(sm_scale)
         q, struct, sizes = self._query(query, query_lengths, causal)
         runs = -(-sizes[0] // query_block)
         blocks = torch.empty((self.sequences, runs, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)
-        nbytes = _workspace_bytes("uc_block8_select_workspace_bytes", self._sizes, sizes, query_block)
+        # one workspace, for the one call and then for the other
+        nbytes = max(_workspace_bytes("uc_block8_select_workspace_bytes", self._sizes, sizes, query_block),
+                     _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes, sizes, budget, query_block))
         ws = nat.workspace(self.device, nbytes)
-        self._call("uc_block8_select", self._struct(), struct, budget, sink, recent, query_block, blocks.data_ptr(),
-                 ws.data_ptr(), nbytes)
-        out, lse = self._attend(q, struct, sizes, blocks, budget, query_block, sm_scale)
+        cache = self._struct()
+        self._call("uc_block8_select", cache, struct, budget, sink, recent, query_block, blocks.data_ptr(),
+                   ws.data_ptr(), nbytes)
+        out, lse = self._attend(cache, q, struct, sizes, blocks, budget, query_block, sm_scale, ws, nbytes)
         return out, lse, blocks
 
     # ------------------------------------------------------------------ bytes --
