@@ -237,8 +237,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool fp16) {
 
 // uc_block8_mq.hip: 128 rows a workgroup, keys staged through LDS.
 constexpr int kTileRows = 128;
-int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint32_t workgroups,
-                 uint16_t *out, float *lse, float *part, float *stat, hipStream_t stream);
+int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint16_t *out, float *lse, float *part, float *stat, hipStream_t stream);
 
 }  // namespace b8
 }  // namespace uc

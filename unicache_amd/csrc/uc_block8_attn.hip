@@ -624,7 +624,7 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   const uint32_t workgroups = static_cast<uint32_t>(p.workgroups > 0 ? p.workgroups : units * p.splits);
   int rc;
   if (p.rows == kTileRows) {
-    rc = launch_tiles(cache, c, q, p, workgroups, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
+    rc = launch_tiles(cache, c, q, p, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
   } else {
     rc = UC_B8_DISPATCH(cache, cache->head_dim, [&] {
       launch_rows<D, CODE>(p.rows, workgroups, as_stream(stream), c, q, p, static_cast<uint16_t *>(out), lse, part, stat);

@@ -190,10 +190,16 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   typedef Tile<D> T;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
-  const int32_t split = blockIdx.x % p.splits;
-  int32_t unit = blockIdx.x / p.splits;
+  // Workgroups go to the 8 XCDs in turn.  A list is one split of the keys of one (sequence, head, run);
+  // its row groups are dealt into `deal` hands so that 8 divides the number of hands, and an XCD plays whole hands:
+  // its L2 then holds the keys of few lists (8 heads of 16k tokens: 1011 -> 908 us).
+  const int32_t lists = c.sequences * c.heads * p.runs * p.splits, deal = 8 / (lists & 7 ? lists & -lists : 8);
+  const int32_t slots = (p.groups + deal - 1) / deal, x = blockIdx.x & 7, at = blockIdx.x >> 3, turn = at / slots;
+  const int32_t hand = x + 8 * turn, list_index = hand % lists, group = (at - turn * slots) * deal + hand / lists;
+  if (group >= p.groups) return;
+  const int32_t split = list_index % p.splits;
   // the later rows of a causal run see more keys: the longest first
-  if (q.causal) unit += p.groups - 1 - 2 * (unit % p.groups);
+  const int32_t unit = list_index / p.splits * p.groups + (q.causal ? p.groups - 1 - group : group);
   const Rows w = rows_of(c, q, p, unit, kTileRows);
   const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
   const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
@@ -346,8 +352,12 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 
 }  // namespace
 
-int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint32_t workgroups,
-                 uint16_t *out, float *lse, float *part, float *stat, hipStream_t stream) {
+int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint16_t *out, float *lse,
+                 float *part, float *stat, hipStream_t stream) {
+  // (the hands may be one row group longer than they need to be)
+  const int64_t lists = int64_t(c.sequences) * c.heads * p.runs * p.splits, deal = 8 / (lists & 7 ? lists & -lists : 8);
+  UC_REQUIRE(lists * deal * ceil_div(p.groups, deal) < (int64_t(1) << 31), "uc_block8_attn: too many query rows");
+  const uint32_t workgroups = static_cast<uint32_t>(lists * deal * ceil_div(p.groups, deal));
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
     if (c.block == 32) {
       hipLaunchKernelGGL((tile_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, stream, c, q, p, out, lse, part, stat);
