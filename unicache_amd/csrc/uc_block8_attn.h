@@ -140,14 +140,35 @@ __device__ __forceinline__ Steps steps_before(const Cache &c, const Query &q, co
   return w;
 }
 
-// First key of a half tile (32 keys); kNone where the list has none there.
-__device__ __forceinline__ int32_t half_of(const Cache &c, const Plan &p, const int32_t *list, int32_t half) {
-  if (list == nullptr) return half * 32;
-  const int32_t e = half >> (c.shift - 5), sub = half & ((c.block >> 5) - 1);
-  if (e >= p.budget) return kNone;
-  const int32_t b = list[e];
-  const bool again = e > 0 && list[e - 1] == b;  // an index given twice counts once
-  return b < 0 || b >= c.blocks || again ? kNone : (b << c.shift) + sub * 32;
+// A run's block list, 64 entries at a time in a wave's lanes, so that a tile's entry is no load that
+// its codes' loads would wait for.  An index that is none, that lies outside the cache or that is given twice in a row reads as -1.
+struct BlockList {
+  const int32_t *list;  // NULL: every block in turn
+  int32_t budget, blocks, chunk, held;
+
+  __device__ __forceinline__ BlockList(const Cache &c, const Plan &p, const Rows &w)
+      : list(p.list), budget(p.budget), blocks(c.blocks), chunk(-1), held(-1) {
+    if (list != nullptr) list += ((int64_t(w.s) * p.runs + w.run0 / p.run) * c.heads + w.h) * p.budget;
+  }
+
+  __device__ __forceinline__ int32_t entry(int32_t e) {
+    if (e >= budget) return -1;
+    if ((e >> 6) != chunk) {
+      chunk = e >> 6;
+      const int32_t i = chunk * 64 + (threadIdx.x & 63);
+      const int32_t b = i < budget ? list[i] : -1, before = i > 0 && i < budget ? list[i - 1] : -1;
+      held = b < 0 || b >= blocks || b == before ? -1 : b;
+    }
+    return __builtin_amdgcn_readlane(held, e & 63);
+  }
+};
+
+// First key of a half tile (32 keys); kNone where there is none.
+template <bool LISTED>
+__device__ __forceinline__ int32_t half_of(const Cache &c, BlockList &list, int32_t half) {
+  if constexpr (!LISTED) return half < c.blocks << (c.shift - 5) ? half * 32 : kNone;
+  const int32_t b = list.entry(half >> (c.shift - 5));
+  return b < 0 ? kNone : (b << c.shift) + (half & ((c.block >> 5) - 1)) * 32;
 }
 
 // Keep the first n of 16 bytes.

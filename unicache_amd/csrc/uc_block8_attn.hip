@@ -136,7 +136,8 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
             quad = lane >> 4;
   const int64_t sh = int64_t(w.s) * c.heads + w.h;
-  const int32_t *list = p.list == nullptr ? nullptr : p.list + ((int64_t(w.s) * p.runs + w.run0 / p.run) * c.heads + w.h) * p.budget;
+  BlockList list(c, p, w);
+  auto half = [&](int32_t i) { return p.list != nullptr ? half_of<true>(c, list, i) : half_of<false>(c, list, i); };
 
   const int32_t tokens = c.blocks << c.shift;
   Lane<D> l;
@@ -150,10 +151,8 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
   Raw<D> raw;
   int32_t t = begin + wave, t0 = 0, t1 = 0;
   if (t < end) {
-    t0 = half_of(c, p, list, 2 * t);
-    t1 = half_of(c, p, list, 2 * t + 1);
-    // a tile's second half may lie behind the capacity
-    if (t1 >= tokens) t1 = kNone;
+    t0 = half(2 * t);
+    t1 = half(2 * t + 1);
     load_keys(raw, c, l, t0, t1);
     load_values(raw, c, l, t0, t1);
   }
@@ -191,9 +190,8 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
     int32_t n0 = kNone, n1 = kNone;
     const bool more = t + 4 < end;
     if (more) {
-      n0 = half_of(c, p, list, 2 * (t + 4));
-      n1 = half_of(c, p, list, 2 * (t + 4) + 1);
-      if (n1 >= tokens) n1 = kNone;
+      n0 = half(2 * (t + 4));
+      n1 = half(2 * (t + 4) + 1);
     }
     f4 s[NR][4];
 #pragma unroll

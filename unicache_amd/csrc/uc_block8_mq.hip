@@ -184,7 +184,7 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
   }
 }
 
-template <int D, int CODE, int N>
+template <int D, int CODE, int N, bool LISTED>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                       float *part, float *stat) {
   typedef Tile<D> T;
@@ -205,8 +205,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
   if (begin >= end && split > 0) return;
   const int64_t sh = int64_t(w.s) * c.heads + w.h;
-  const int32_t *list =
-      p.list == nullptr ? nullptr : p.list + ((int64_t(w.s) * p.runs + w.run0 / p.run) * c.heads + w.h) * p.budget;
+  BlockList list(c, p, w);
   const int32_t tokens = c.blocks << c.shift;
   const uint8_t *kbase = c.key_code + sh * tokens * D, *vbase = c.value_code + sh * tokens * D;
 
@@ -237,8 +236,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   Staged<D> st;
   const Loader<D> ld(c.block);
   auto get = [&](int32_t t) {
-    int32_t t0 = half_of(c, p, list, 2 * t), t1 = half_of(c, p, list, 2 * t + 1);
-    if (t1 >= tokens) t1 = kNone;
+    const int32_t t0 = half_of<LISTED>(c, list, 2 * t), t1 = half_of<LISTED>(c, list, 2 * t + 1);
     fetch<D>(st, c, sh, kbase, vbase, ld, t0, t1);
   };
   // whether every row sees all keys of the staged tile
@@ -350,6 +348,19 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   }
 }
 
+template <int D, int CODE, class... Args>
+void launch_tile(bool two, bool listed, uint32_t workgroups, hipStream_t stream, const Args &...args) {
+  if (two && listed) {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, 2, true>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else if (two) {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, 2, false>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else if (listed) {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, 1, true>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, 1, false>), dim3(workgroups), dim3(256), 0, stream, args...);
+  }
+}
+
 }  // namespace
 
 int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, const Plan &p, uint16_t *out, float *lse,
@@ -359,11 +370,7 @@ int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, c
   UC_REQUIRE(lists * deal * ceil_div(p.groups, deal) < (int64_t(1) << 31), "uc_block8_attn: too many query rows");
   const uint32_t workgroups = static_cast<uint32_t>(lists * deal * ceil_div(p.groups, deal));
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
-    if (c.block == 32) {
-      hipLaunchKernelGGL((tile_kernel<D, CODE, 2>), dim3(workgroups), dim3(256), 0, stream, c, q, p, out, lse, part, stat);
-    } else {
-      hipLaunchKernelGGL((tile_kernel<D, CODE, 1>), dim3(workgroups), dim3(256), 0, stream, c, q, p, out, lse, part, stat);
-    }
+    launch_tile<D, CODE>(c.block == 32, p.list != nullptr, workgroups, stream, c, q, p, out, lse, part, stat);
     return check_launch("uc_block8_attn");
   });
 }

@@ -71,6 +71,13 @@ __device__ __forceinline__ uint32_t four_codes(const float *x, float inverse) {
 __device__ __forceinline__ float code_factor(float a) { return a > 0.0f ? div_rn(127.0f, a) : 0.0f; }
 __device__ __forceinline__ float code_step(float a) { return mul_rn(a, 1.0f / 127.0f); }
 
+// The bytes of w that are positive, and those that are negative.
+__device__ __forceinline__ void parts(int w, int &pos, int &neg) {
+  const uint32_t m = ((static_cast<uint32_t>(w) >> 7) & 0x01010101u) * 255u;
+  neg = static_cast<int>(static_cast<uint32_t>(w) & m);
+  pos = static_cast<int>(static_cast<uint32_t>(w) & ~m);
+}
+
 // The codes and steps of all query rows, D / 8 lanes a row; a NaN step marks a row that does not count
 // (no maximum takes it).
 template <int D>
@@ -101,13 +108,6 @@ __global__ __launch_bounds__(256) void codes_kernel(Cache c, Run q, int8_t *code
   for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
   *reinterpret_cast<uint2 *>(codes + row * D + part * 8) = uint2{four_codes(x, f), four_codes(x + 4, f)};
   if (part == 0) steps[row] = bad ? __builtin_nanf("") : code_step(a);
-}
-
-// The bytes of w that are positive, and those that are negative.
-__device__ __forceinline__ void parts(int w, int &pos, int &neg) {
-  const uint32_t m = ((static_cast<uint32_t>(w) >> 7) & 0x01010101u) * 255u;
-  neg = static_cast<int>(static_cast<uint32_t>(w) & m);
-  pos = static_cast<int>(static_cast<uint32_t>(w) & ~m);
 }
 
 // Codes of 16 rows as the A operand: lane % 16 is the row, lane / 16 and k name 16 channels; and the
@@ -204,13 +204,20 @@ __device__ __forceinline__ void own_codes(OwnCodes<D> &own, const Run &q, int32_
   if (part == 0) own.step[r] = bad ? __builtin_nanf("") : code_step(a);
 }
 
-// Scores for runs of many rows: a wave takes 32 blocks, whose bounds stay in registers, through all rows
-// of a run, the next 16 rows' codes on their way.
-constexpr int kScored = 2;  // 16-block groups of a wave
+// Scores for runs of many rows.  A wave takes 64 blocks, whose bounds stay in registers; a workgroup
+// takes 64 rows at a time into LDS, split into their positive and negative parts, for its four
+// waves, the next 64 on their way (each wave loading all rows for itself was bound by L2: 20 us for 28 x 2048 rows
+// by 512 blocks).
+constexpr int kScored = 4;      // 16-block groups of a wave
+constexpr int kStageRows = 64;
 
 template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t *codes, const float *steps,
                                                     float unit_factor, float *score, int32_t chunks) {
+  constexpr int kPitch = 2 * D + 16;  // bytes of a row: eight rows' chunks lie in different banks
+  constexpr int kLanes = D / 16, kLoads = kStageRows * kLanes / 256;
+  __shared__ __attribute__((aligned(16))) int8_t sh_codes[kStageRows * kPitch];
+  __shared__ __attribute__((aligned(16))) float sh_step[kStageRows];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int32_t unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;  // unit: (sequence, run, head)
   const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
@@ -222,7 +229,13 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
   const int32_t rows = ((count - t0 < q.run) ? count - t0 : q.run) * q.group;
   const int64_t sh = int64_t(s) * c.heads + h;
   const int64_t row0 = (int64_t(s) * q.len + t0) * q.heads + h * q.group;
-  for (int32_t b0 = (chunk * 4 + wave) * 16 * kScored; b0 < blocks; b0 += chunks * 64 * kScored) {
+  auto index_of = [&](int32_t r) {  // rows past the last are the last again: they change no maximum
+    r = r < rows ? r : rows - 1;
+    const int32_t token = static_cast<int32_t>(fast_div(r, q.by_group));
+    return row0 + int64_t(token) * q.heads + (r - token * q.group);
+  };
+  for (int32_t base = chunk * 64 * kScored; base < blocks; base += chunks * 64 * kScored) {
+    const int32_t b0 = base + wave * 16 * kScored;
     BlockBounds<D> x[kScored];
     float best[kScored];
 #pragma unroll
@@ -230,26 +243,49 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
       load_bounds<D>(x[n], c, sh, b0 + 16 * n, blocks, unit_factor);
       best[n] = mf::kNegInf;
     }
-    i4 next[D / 64];
-    float next_step;
+    i4 next[kLoads];
+    float next_step = 0.0f;
     auto fetch = [&](int32_t r0) {
-      const int32_t r = r0 + col < rows ? r0 + col : rows - 1;  // the last row again: it changes no maximum
-      const int32_t token = static_cast<int32_t>(fast_div(r, q.by_group));
-      const int64_t at = row0 + int64_t(token) * q.heads + (r - token * q.group);
-      next_step = steps[at];
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) next[k] = *reinterpret_cast<const i4 *>(codes + at * D + k * 64 + quad * 16);
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = threadIdx.x + i * 256;
+        next[i] = *reinterpret_cast<const i4 *>(codes + index_of(r0 + at / kLanes) * D + at % kLanes * 16);
+      }
+      if (threadIdx.x < kStageRows) next_step = steps[index_of(r0 + threadIdx.x)];
     };
     fetch(0);
-    for (int32_t r0 = 0; r0 < rows; r0 += 16) {
-      RowCodes<D> rc;
+    for (int32_t r0 = 0; r0 < rows; r0 += kStageRows) {
+      __syncthreads();  // the rows before have been read
 #pragma unroll
-      for (int i = 0; i < 4; ++i) rc.step[i] = __shfl(next_step, quad * 4 + i, kWave);
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = threadIdx.x + i * 256;
+        i4 pos, neg;
 #pragma unroll
-      for (int k = 0; k < D / 64; ++k) rc.split(k, next[k]);
-      if (r0 + 16 < rows) fetch(r0 + 16);
+        for (int j = 0; j < 4; ++j) {
+          int a, b;
+          parts(next[i][j], a, b);
+          pos[j] = a;
+          neg[j] = b;
+        }
+        int8_t *dst = sh_codes + at / kLanes * kPitch + at % kLanes * 16;
+        *reinterpret_cast<i4 *>(dst) = pos;
+        *reinterpret_cast<i4 *>(dst + D) = neg;
+      }
+      if (threadIdx.x < kStageRows) sh_step[threadIdx.x] = next_step;
+      __syncthreads();
+      if (r0 + kStageRows < rows) fetch(r0 + kStageRows);
+      for (int g = 0; g < kStageRows / 16 && r0 + 16 * g < rows; ++g) {
+        RowCodes<D> rc;
+        rc.step = *reinterpret_cast<const f4 *>(&sh_step[16 * g + 4 * quad]);
+        const int8_t *src = sh_codes + (16 * g + col) * kPitch + quad * 16;
 #pragma unroll
-      for (int n = 0; n < kScored; ++n) score16<D>(x[n], rc, best[n]);
+        for (int k = 0; k < D / 64; ++k) {
+          rc.pos[k] = *reinterpret_cast<const i4 *>(src + k * 64);
+          rc.neg[k] = *reinterpret_cast<const i4 *>(src + D + k * 64);
+        }
+#pragma unroll
+        for (int n = 0; n < kScored; ++n) score16<D>(x[n], rc, best[n]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < kScored; ++n) {
