@@ -320,6 +320,86 @@ def test_one_sequence_without_a_batch_axis(device):
     assert cache.lengths.tolist() == [153]
 
 
+def test_queries_of_no_tokens_and_odd_strides_of_single_dimensions(device):
+    key, value = dense(1, 64, 2, 64, seed=31)
+    cache = Block8KVCache.from_dense(key, value)
+    q = queries(1, 1, 4, 64, seed=32)
+    out, lse = cache.attention(q[:, :0])
+    assert out.shape == (1, 0, 4, 64) and lse.shape == (1, 4, 0)
+    out, lse, blocks = cache.sparse_attention(q[:, :0], budget=3)
+    assert out.shape == (1, 0, 4, 64) and blocks.shape == (1, 0, 2, 3)
+    odd = torch.empty_strided((1, 1, 4, 64), (7, 5, 64, 1), dtype=q.dtype, device=device).copy_(q)
+    assert torch.equal(cache.attention(odd)[0], cache.attention(q)[0])
+
+
+@pytest.mark.parametrize("lq,d", [(1, 128), (3, 64), (40, 64)])
+def test_more_sequences_than_a_wave_has_lanes(device, lq, d):
+    g = torch.Generator().manual_seed(33)
+    lens = torch.randint(0, 700, (150,), generator=g)
+    lens[::7] = 0
+    lens[60:70] = 0
+    lens = lens.tolist()
+    key, value = dense(150, 700, 2, d, seed=34)
+    cache = Block8KVCache.from_dense(key, value, lengths=torch.tensor(lens, dtype=torch.int32, device=device))
+    q = queries(150, lq, 6, d, seed=35)
+    check(cache.attention(q, causal=True), reference(cache, q, lens, [lq] * 150, True, 1 / math.sqrt(d)))
+    out, lse, blocks = cache.sparse_attention(q, budget=4, query_block=lq)
+    want = chosen_blocks(cache, q, lens, [lq] * 150, False, 4, lq, 1, 1)
+    assert torch.equal(blocks.cpu(), want)
+    check((out, lse), reference(cache, q, lens, [lq] * 150, False, 1 / math.sqrt(d), want, lq))
+
+
+@pytest.mark.parametrize("rows", [(8, 4, 64), (16, 3, 64), (16, 4, 64), (28, 4, 128), (4, 5, 128), (9, 7, 64)])
+def test_every_number_of_rows_of_a_head(device, rows):
+    # groups of 2 .. 28 query heads over one KV head x a few tokens, on both sides of 16, 32, 48 and 128 rows
+    hq, lq, d = rows
+    lens = [1500, 63]
+    key, value = dense(2, 1500, 1, d, seed=36)
+    cache = Block8KVCache.from_dense(key, value, lengths=torch.tensor(lens, dtype=torch.int32, device=device),
+                                     code_dtype=torch.int8)
+    q = queries(2, lq, hq, d, seed=37)
+    check(cache.attention(q, causal=True), reference(cache, q, lens, [lq] * 2, True, 1 / math.sqrt(d)))
+
+
+@pytest.mark.parametrize("lq", [1, 50])
+def test_scales_of_zero(device, lq):
+    # a cache that another program made, whose blocks of zeros have the scale 0
+    key, value = dense(1, 320, 2, 128, seed=38)
+    key[:, 64:128], value[:, :64], value[:, 192:256] = 0, 0, 0
+    cache = Block8KVCache.from_dense(key, value)
+    q = queries(1, lq, 4, 128, seed=39)
+    want = reference(cache, q, [320], [lq], False, 1 / math.sqrt(128))
+    cache.key_scale[:, :, 1] = 0
+    cache.value_scale[:, :, [0, 3]] = 0
+    check(cache.attention(q), want)
+
+
+@pytest.mark.parametrize("lq", [2, 60])
+@pytest.mark.parametrize("block", [32, 64, 128])
+def test_any_block_list_is_read_within_bounds(device, lq, block):
+    # the C entry point with indexes outside the cache, the same one twice in a row, none, and blocks behind the length
+    from unicache_amd import _native as nat
+
+    key, value = dense(1, 1000, 2, 128, seed=40)
+    cache = Block8KVCache.from_dense(key, value, block_tokens=block, capacity=1400)
+    q = queries(1, lq, 6, 128, seed=41)
+    lists = torch.full((1, 1, 2, 70), -1, dtype=torch.int32)
+    lists[0, 0, 0, :8] = torch.tensor([0, 0, 2, 2, 5, 10000, -7, 1 << 30])
+    lists[0, 0, 1, 60:70] = torch.tensor([1, 3, 3, 3, 6, cache.blocks - 1, cache.blocks, -1, -1, 7])
+    struct = cache._query(q, None, False)[1]
+    out, lse = torch.empty_like(q), torch.empty(1, 6, lq, device=device)
+    nbytes = nat.lib().uc_block8_attn_workspace_bytes(cache._struct(), struct, 70, lq)
+    ws = nat.workspace(device, nbytes)
+    there = lists.to(device)
+    nat.call("uc_block8_attn", cache._struct(), struct, there.data_ptr(), 70, lq, 0.1, out.data_ptr(), lse.data_ptr(),
+             ws.data_ptr(), nbytes, nat.stream(device))
+    last = -(-1000 // block) - 1
+    keep = torch.full((1, 1, 2, 4), -1, dtype=torch.int32)
+    keep[0, 0, 0, :3] = torch.tensor([0, 2, 5])
+    keep[0, 0, 1] = torch.tensor([1, 3, 6, 7])
+    check((out, lse), reference(cache, q, [1000], [lq], False, 0.1, keep.clamp_max(last + 1), lq))
+
+
 # --------------------------------------------------------------- selection --
 def chosen_blocks(cache, q, lens, qlens, causal, budget, query_block, sink, recent):
     s, lq, hq, d = q.shape
@@ -365,6 +445,9 @@ SPARSE = [
     dict(lens=[2100], hq=14, hkv=2, lq=150, budget=11, query_block=32, causal=True, sink=2, recent=3),
     dict(lens=[1300, 90], hq=8, hkv=4, lq=201, qlens=[201, 120], budget=8, query_block=100, causal=True, d=64),
     dict(lens=[640], hq=4, hkv=4, lq=77, budget=64, query_block=33, causal=False),
+    dict(lens=[20000, 9000], hq=8, hkv=2, lq=1, budget=150, recent=2),
+    dict(lens=[9000], hq=8, hkv=2, lq=48, budget=100, query_block=24, causal=True),
+    dict(lens=[1500], hq=8, hkv=4, lq=300, budget=5, causal=True),  # a list for each token
 ]
 
 
@@ -496,6 +579,71 @@ def test_captured_steps_replayed(device):
         if t % 7 == 0:
             torch.cuda.synchronize()
     assert cache.lengths.tolist() == [140, 140]
+
+
+def test_two_graphs_of_one_cache(device):
+    # decode and a sparse step captured apart, replayed in turn and over changed lengths
+    key, value = dense(3, 600, 2, 128, seed=92)
+    lens = torch.tensor([600, 100, 0], dtype=torch.int32, device=device)
+    cache = Block8KVCache.from_dense(key, value, lengths=lens)
+    q = queries(3, 1, 14, 128, seed=93)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attention(q), cache.sparse_attention(q, budget=3)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    with torch.cuda.graph(graphs[0]):
+        got.append(cache.attention(q))
+    with torch.cuda.graph(graphs[1]):
+        got.append(cache.sparse_attention(q, budget=3))
+    for n in (600, 64, 1, 0, 599, 300):
+        cache.lengths.copy_(torch.tensor([n, 600 - n, 7], dtype=torch.int32))
+        q.copy_(queries(3, 1, 14, 128, seed=n))
+        for g in graphs:
+            g.replay()
+        want = cache.attention(q), cache.sparse_attention(q, budget=3)
+        for a, b in zip(got[0] + got[1], want[0] + want[1]):
+            assert torch.equal(a, b), n
+
+
+def test_mixed_attention_over_a_block8_segment(device):
+    # the adapter's mixed call: dense rows, a packed KIVI segment, an H2O segment and an 8-bit one as one softmax
+    from unicache_amd.adapters.bagel import run_batched_physical_attention, run_fused_mixed_attention
+    from unicache_amd.storage import GQAH2OCache, PackedKIVICache
+
+    def rows(n, seed):
+        k, v = dense(1, n, 4, 128, seed=seed)
+        return k[0] * 0.3, v[0]
+
+    dk, dv = rows(90, 110)
+    pk, pv = rows(300, 111)
+    bk, bv = rows(333, 112)
+    hk, hv = rows(64, 113)
+    packed = PackedKIVICache.from_dense(pk, pv, logical_token_ids=torch.arange(300, device=device), token_type_id=0,
+                                        k_bits=4, v_bits=4, group_size=32, residual_length=10, backend="cuda")
+    h2o = GQAH2OCache.from_dense(hk, hv, logical_token_ids=torch.arange(64, device=device), token_type_id=0,
+                                 per_kv_head_scores=torch.rand(4, 64, device=device), target_tokens=20,
+                                 recent_tokens=5, selection_frozen=True)
+    block8 = Block8KVCache.from_dense(bk, bv)
+    rk, rv = packed.dequantize()
+    ek, ev = (t[0].float().double() for t in block8.dequantize(torch.float16))
+    for lq in (1, 200):
+        q = queries(1, lq, 28, 128, seed=114)[0]
+        for segments, keys, values in (
+                ([packed, block8, h2o], [dk, rk, h2o.key.transpose(0, 1)], [dv, rv, h2o.value.transpose(0, 1)]),
+                ([block8], [dk], [dv])):
+            out, lse = run_fused_mixed_attention(q, dk, dv, segments, return_lse=True)
+            k = torch.cat([*(t.double() for t in keys), ek]).repeat_interleave(7, dim=1)
+            v = torch.cat([*(t.double() for t in values), ev]).repeat_interleave(7, dim=1)
+            x = torch.einsum("rhd,thd->hrt", q.double(), k) / math.sqrt(128)
+            want = torch.einsum("hrt,thd->rhd", torch.softmax(x, dim=-1), v)
+            # the tolerances of the other mixed-attention tests: summaries are rounded to bf16 before they are merged
+            assert (out.double() - want).abs().max() < 2e-2 and (lse.double() - torch.logsumexp(x, dim=-1)).abs().max() < 5e-3
+            batched = run_batched_physical_attention(q, dk, dv, [0, lq], [0, 90], [segments])
+            assert torch.equal(batched, out)
+    with pytest.raises(ValueError, match="one sequence"):
+        run_fused_mixed_attention(q, dk, dv, [Block8KVCache.empty(2, 64, 4, 128, device=device)])
 
 
 def test_another_stream(device):

@@ -66,27 +66,39 @@ def run_fused_mixed_attention(
     UniCache's order [dense, H2O..., residuals...] and attended in the same
     fused pass as the first packed segment's prefix; further packed prefixes
     get their own pass (all passes in one batched launch for long queries) and
-    the summaries are merged by LSE.  Non-frozen H2O segments then receive
+    the summaries are merged by LSE.  Block8KVCache segments (one sequence each)
+    are summarised by Block8KVCache.attention and merged likewise; with one of
+    them no packed prefix is needed.  Non-frozen H2O segments then receive
     exp(logit - global LSE) as bf16 probabilities and are trimmed to their
     budget.  Returns the output (and the global LSE [Hq, Lq] with
     return_lse=True)."""
 
     from ..storage.kivi_cuda import (_max_decode_query_len, decode_segments_summary, decode_segments_supported,
-                                     packed_batch_with_dense, packed_kivi_quantized_attention_summary,
-                                     packed_segments_summary, packed_segments_supported, packed_summary_with_dense)
+                                     dense_attention_summary, packed_batch_with_dense,
+                                     packed_kivi_quantized_attention_summary, packed_segments_summary,
+                                     packed_segments_supported, packed_summary_with_dense)
+    from ..storage.block8 import Block8KVCache
     from ..storage.physical import GQAH2OCache, PackedKIVICache
 
     h2o = [s for s in physical_segments if isinstance(s, GQAH2OCache)]
     packed = [s for s in physical_segments if isinstance(s, PackedKIVICache)]
+    block8 = [s for s in physical_segments if isinstance(s, Block8KVCache)]
     with_prefix = [s for s in packed if s.quantized_tokens]
-    if not with_prefix:
+    if not with_prefix and not block8:
         raise RuntimeError("Fused mixed attention requires packed KIVI tokens")
+    if any(s.sequences != 1 for s in block8):
+        raise ValueError("Fused mixed attention takes Block8 segments of one sequence")
     lq, hq, d = map(int, query.shape)
-    first = with_prefix[0]
+    first = with_prefix[0] if with_prefix else None
     dense_parts = [(dense_key, dense_value)] + [(s.key.transpose(0, 1), s.value.transpose(0, 1)) for s in h2o] + [
         (s.residual_key, s.residual_value) for s in packed if not s.quantized_tokens and s.residual_tokens]
-    if dense_key.dtype in (torch.bfloat16, torch.float16) and packed_segments_supported(with_prefix, query,
-                                                                                      dense_parts):
+    if not with_prefix:
+        live = [(k, v) for k, v in dense_parts if k.shape[0]]
+        output, global_lse = dense_attention_summary(
+            query, torch.cat([k.to(dense_key.dtype) for k, _ in live], dim=0),
+            torch.cat([v.to(dense_value.dtype) for _, v in live], dim=0)) if live else (None, None)
+    elif dense_key.dtype in (torch.bfloat16, torch.float16) and packed_segments_supported(with_prefix, query,
+                                                                                        dense_parts):
         output, global_lse = packed_segments_summary(with_prefix, query, dense_parts, dense_dtype=dense_key.dtype)
     elif decode_segments_supported(with_prefix, query, dense_parts):
         output, global_lse = decode_segments_summary(with_prefix, query, dense_parts)
@@ -114,6 +126,13 @@ def run_fused_mixed_attention(
         else:
             summaries = [packed_summary_with_dense(first, query, all_key, all_value)]
             summaries += [packed_kivi_quantized_attention_summary(s, query) for s in with_prefix[1:]]
+        output, global_lse = summaries[0] if len(summaries) == 1 else merge_attention_summaries(summaries)
+    if block8:
+        q = query if query.dtype in (torch.bfloat16, torch.float16) else query.to(torch.bfloat16)
+        summaries = [] if output is None else [(output, global_lse)]
+        for segment in block8:
+            o, lse = segment.attention(q.unsqueeze(0))
+            summaries.append((o[0].to(query.dtype), lse[0]))
         output, global_lse = summaries[0] if len(summaries) == 1 else merge_attention_summaries(summaries)
     for segment in h2o:
         if segment.selection_frozen:
@@ -143,12 +162,13 @@ def run_batched_physical_attention(
     samples within the table limits): each sample's packed prefixes,
     residuals, current keys and H2O segments are read in place, no
     concatenation, and the rows of the output are written in place.  Other
-    samples with a packed prefix are one fused pass each
-    (run_fused_mixed_attention) and H2O-only samples one dense pass, so the
+    samples with a packed prefix, and those with Block8KVCache segments, are one
+    fused pass each (run_fused_mixed_attention) and H2O-only samples one dense pass, so the
     packed prefixes are never dequantised into a varlen workspace.  Returns
     [total queries, Hq, D] in q's dtype.  H2O segments must be frozen, as in the
     reference fast path."""
 
+    from ..storage.block8 import Block8KVCache
     from ..storage.kivi_cuda import dense_attention_summary, packed_segments_supported, packed_table_summaries
     from ..storage.physical import GQAH2OCache, PackedKIVICache
 
@@ -176,6 +196,9 @@ def run_batched_physical_attention(
             continue
         with_prefix = [s for s in packed if s.quantized_tokens]
         out_i = out[cu_q[i]:cu_q[i + 1]]
+        if any(isinstance(s, Block8KVCache) for s in segments):
+            out_i.copy_(run_fused_mixed_attention(q_i, k_i, v_i, list(segments)))
+            continue
         dense_parts = [(k_i, v_i)] + [(s.key.transpose(0, 1), s.value.transpose(0, 1)) for s in h2o] + [
             (s.residual_key, s.residual_value) for s in packed if not s.quantized_tokens and s.residual_tokens]
         if with_prefix and k.dtype in (torch.bfloat16, torch.float16) and packed_segments_supported(

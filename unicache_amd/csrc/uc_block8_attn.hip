@@ -147,7 +147,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
   l.kscale = c.key_scale + sh * c.blocks;
   l.vscale = c.value_scale + sh * c.blocks;
 
-  float most = 0.0f;  // the largest value scale so far
+  float most = kTiny;  // the largest value scale so far
   Raw<D> raw;
   int32_t t = begin + wave, t0 = 0, t1 = 0;
   if (t < end) {
@@ -605,9 +605,9 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   Plan p;
   if (int rc = check_cache(cache, "uc_block8_attn", c)) return rc;
   if (int rc = make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p)) return rc;
-  UC_REQUIRE((blocks != nullptr) == (budget > 0), "uc_block8_attn: a block list and its budget belong together");
   UC_REQUIRE(sm_scale > 0.0f && sm_scale < __builtin_huge_valf(), "uc_block8_attn: sm_scale must be positive");
   if (q.len == 0) return UC_OK;
+  UC_REQUIRE((blocks != nullptr) == (budget > 0), "uc_block8_attn: a block list and its budget belong together");
   UC_REQUIRE(q.p != nullptr && (reinterpret_cast<uintptr_t>(q.p) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,
              "uc_block8_attn: query must be 16-byte aligned with strides that are multiples of 8");
   UC_REQUIRE(out != nullptr && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "uc_block8_attn: out must be 16-byte aligned");

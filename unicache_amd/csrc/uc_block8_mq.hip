@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
   for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ value_swizzle(col));
 
-  float most = 0.0f;
+  float most = kTiny;
   Staged<D> st;
   const Loader<D> ld(c.block);
   auto get = [&](int32_t t) {

@@ -47,20 +47,24 @@ def _check_tensor(name, t, dtype, shape, device, align) -> None:
         raise ValueError(f"Block8 cache {name} must be {align + 1}-byte aligned")
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """`t` where the kernels can read it in place (unit channel stride, rows on
-    16 bytes), a contiguous copy otherwise."""
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """A [S, T, H, D] tensor as the kernels can read it -- in place where its
+    channels are adjacent and its rows on 16 bytes, else a contiguous copy --
+    and its first three strides."""
 
     if t.is_neg():
         t = t.resolve_neg()
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
-            return t
+    aligned = t.data_ptr() % 16 == 0
+    if not (aligned and t.is_contiguous()):
         a, b, c, d = t.stride()
-        if d == 1 and not (a % 8 or b % 8 or c % 8):
-            return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+        if aligned and d == 1 and not (a % 8 or b % 8 or c % 8):
+            return t, a, b, c
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+    # (a contiguous tensor's strides of dimensions of size 1 may be anything)
+    _, n, h, d = t.shape
+    return t, n * h * d, h * d, d
 
 
 @functools.lru_cache(maxsize=256)
@@ -88,7 +92,8 @@ class Block8KVCache:
       channel, in steps of the block's largest key / 127, rounded outwards
     - ``lengths``     [S] int32, tokens held by each sequence, on the device
 
-    D is 64 or 128, B 32, 64 or 128.  ``tail`` ([S, Hkv, 2, B, D] in the dense
+    D is 64 or 128, B 32, 64 or 128.  Scales are not negative (0 will do for a
+    block of zeros).  ``tail`` ([S, Hkv, 2, B, D] in the dense
     dtype, or None) holds the dense rows of each sequence's open block for
     append.  ``max_tokens`` is how long the caller takes the longest sequence
     to be (default: the capacity, raised by append); it shapes launches, and no
@@ -205,9 +210,9 @@ class Block8KVCache:
             raise ValueError("Block8 cache lengths must be contiguous int32 [sequences]")
         cache = cls._allocate(s, capacity, h, d, int(block_tokens), code_dtype, key.dtype, device, t)
         if t:
-            key, value = _rows16(key), _rows16(value)
-            cache._call("uc_block8_pack", cache._struct(), key.data_ptr(), *key.stride()[:3], value.data_ptr(),
-                        *value.stride()[:3], nat.dtype_code(key.dtype), t, nat.ptr(lengths), cache.tail.data_ptr())
+            (key, *k_strides), (value, *v_strides) = _rows16(key), _rows16(value)
+            cache._call("uc_block8_pack", cache._struct(), key.data_ptr(), *k_strides, value.data_ptr(), *v_strides,
+                        nat.dtype_code(key.dtype), t, nat.ptr(lengths), cache.tail.data_ptr())
         else:
             cache.lengths.zero_()
         return cache
@@ -246,8 +251,7 @@ class Block8KVCache:
             raise ValueError("Block8 query_lengths must be contiguous int32 [sequences]")
         if query.device != self.device or (query_lengths is not None and query_lengths.device != self.device):
             raise RuntimeError(f"Block8 attention requires GPU tensors on the cache's device {self.device}")
-        query = _rows16(query)
-        a, b, c, _ = query.stride()
+        query, a, b, c = _rows16(query)
         dtype, causal = nat.dtype_code(query.dtype), 1 if causal else 0
         struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), self.max_tokens, dtype, causal)
         return query, struct, (lq, hq, self.max_tokens, dtype, causal)
@@ -270,9 +274,8 @@ class Block8KVCache:
     def append(self, key: torch.Tensor, value: torch.Tensor, *, counts: torch.Tensor | None = None) -> None:
         """Append dense rows [S, n, Hkv, D] ([n, Hkv, D] for one sequence) to
         the sequences: the first counts[s] of them (int32 on the device; default all n).  The
-        result equals from_dense of all rows.  `lengths` advances on the device;
-        rows past the capacity are dropped there, and refused here as far as
-        the host knows the lengths (max_tokens)."""
+        result equals from_dense of all rows.  `lengths` advances on the device,
+        which alone knows them: rows past the capacity are dropped there."""
 
         if self.tail is None:
             raise RuntimeError("Block8 append needs the open blocks' dense rows (tail)")
@@ -293,9 +296,9 @@ class Block8KVCache:
         n = int(key.shape[1])
         if n == 0:
             return
-        key, value = _rows16(key), _rows16(value)
-        self._call("uc_block8_append", self._struct(), self.tail.data_ptr(), key.data_ptr(), *key.stride()[:3],
-                 value.data_ptr(), *value.stride()[:3], nat.dtype_code(key.dtype), n, nat.ptr(counts))
+        (key, *k_strides), (value, *v_strides) = _rows16(key), _rows16(value)
+        self._call("uc_block8_append", self._struct(), self.tail.data_ptr(), key.data_ptr(), *k_strides,
+                   value.data_ptr(), *v_strides, nat.dtype_code(key.dtype), n, nat.ptr(counts))
         self.max_tokens = min(self.max_tokens + n, self.capacity)
 
     def dequantize(self, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
