@@ -33,6 +33,7 @@ struct Plan {
   int32_t run, runs;    // query tokens that share a list (without lists: all), and how many such runs
   int32_t groups, rows; // row groups of a run, and their rows
   int32_t splits, split_tiles;
+  int32_t key_groups;   // many rows: 1, or 2 groups of waves in a workgroup that share its tiles
   int32_t workgroups;   // few rows: workgroups that share all tiles; 0: one workgroup a unit
 };
 

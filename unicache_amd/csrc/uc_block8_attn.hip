@@ -502,25 +502,35 @@ void launch_rows(int32_t rows, uint32_t workgroups, hipStream_t stream, const Ar
   }
 }
 
-// Splits of 128-row workgroups: the least time in tiles.  Two (head_dim 128) or three workgroups share
-// a CU; up to one a CU takes 0.65 of the time a tile; the join takes two tiles and 0.006 for each part of
+// Splits of 128-row workgroups, and how many groups of four waves they have: the least time in tiles.  Of one
+// group, two (head_dim 128) or three workgroups share a CU, and up to one a CU takes 0.65 of the time a tile; of
+// two groups one, each with half of the tiles, joined in LDS (one tile).  The launch that joins splits takes two tiles and 0.006 for each part of
 // a workgroup.  Measured, one split -> the chosen: 112 units of 64 tiles 110 -> 56 us (4 splits), 28 of 256
 // 412 -> 59 (18), 572 of 64 247 -> 213 (4), 376 of 128 at head_dim 64 196 -> 151 (2); 512 of 64 stay at
 // one (206; two would take 224), as do 440 of 31 (66; 89).
-int64_t tile_splits(int64_t units, int64_t tiles, int64_t head_dim) {
+void split_tiles(int64_t units, int64_t tiles, int64_t head_dim, bool listed, Plan &p) {
   const int64_t slots = head_dim == 128 ? 512 : 768;
   int64_t best = 1;
   double least = 1e300;
   const int64_t most = ceil_div(tiles, 4) < 64 ? ceil_div(tiles, 4) : 64;
   for (int64_t k = 1; k <= most; ++k) {
+    const double join = k > 1 ? 2.0 + 0.006 * static_cast<double>(units * k) : 0.0;
     const double rounds = units * k <= slots / 2 ? 0.65 : static_cast<double>(ceil_div(units * k, slots));
-    const double time = rounds * static_cast<double>(ceil_div(tiles, k)) + (k > 1 ? 2.0 + 0.006 * static_cast<double>(units * k) : 0.0);
-    if (time < least) {
-      least = time;
+    const double one = rounds * static_cast<double>(ceil_div(tiles, k)) + join;
+    const double two = static_cast<double>(ceil_div(units * k, 256) * ceil_div(tiles, 2 * k)) + 1.0 + join;
+    if (one < least) {
+      least = one;
       best = k;
+      p.key_groups = 1;
+    }
+    if (two < least && !listed) {
+      least = two;
+      best = k;
+      p.key_groups = 2;
     }
   }
-  return best;
+  p.split_tiles = static_cast<int32_t>(ceil_div(tiles, best));
+  p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
 }
 
 constexpr int64_t kShare = 512;  // workgroups that share the tiles of few rows: two a CU
@@ -556,10 +566,9 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   const int64_t tiles = keys > 0 ? ceil_div(keys, kTile) : 1;
   const int64_t units = cache->sequences * cache->heads_kv * p.runs * p.groups;
   p.workgroups = 0;
+  p.key_groups = 1;
   if (p.rows == kTileRows) {
-    const int64_t splits = tile_splits(units, tiles, cache->head_dim);
-    p.split_tiles = static_cast<int32_t>(ceil_div(tiles, splits));
-    p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
+    split_tiles(units, tiles, cache->head_dim, budget > 0, p);
   } else {
     p.splits = 1;
     p.split_tiles = 0;

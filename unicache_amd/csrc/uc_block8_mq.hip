@@ -48,7 +48,7 @@ struct Loader {
   uint32_t koff, voff;
 
   __device__ __forceinline__ explicit Loader(int32_t block) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x & 255;
     if constexpr (D == 128) {
       // eight lanes write two keys' chunks to LDS, so that they meet no bank twice
       c16 = (tid & 3) | ((tid >> 3) & 1) << 2;
@@ -63,7 +63,7 @@ struct Loader {
     voff = channel * block + k16 * 16;
   }
   // The half of load i: the same for a wave.
-  __device__ __forceinline__ int half(int i) const { return D == 128 ? i : __builtin_amdgcn_readfirstlane(threadIdx.x >> 7); }
+  __device__ __forceinline__ int half(int i) const { return D == 128 ? i : __builtin_amdgcn_readfirstlane((threadIdx.x >> 7) & 1); }
 };
 
 template <int D>
@@ -184,12 +184,48 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
   }
 }
 
-template <int D, int CODE, int N, bool LISTED>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
+// The second group's rows join the first's, lane by lane, through LDS (which nobody reads any more).
+template <int D>
+__device__ __forceinline__ void join_groups(Acc16<D> (&acc)[2], f4 *sh, int part_of, int wave) {
+  constexpr int kO = D / 16;
+  const int lane = threadIdx.x & 63;
+  f4 *at = sh + wave * 2 * (kO + 1) * 64 + lane;
+  if (part_of == 1) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int d = 0; d < kO; ++d) at[(n * (kO + 1) + d) * 64] = acc[n].o[d];
+      at[(n * (kO + 1) + kO) * 64] = f4{acc[n].m, acc[n].l, 0, 0};
+    }
+  }
+  __syncthreads();
+  if (part_of == 1) return;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const f4 s = at[(n * (kO + 1) + kO) * 64];
+    const float m = fmaxf(acc[n].m, s[0]);
+    const float d0 = m == mf::kNegInf ? 0.0f : acc[n].m - m, d1 = m == mf::kNegInf ? 0.0f : s[0] - m;
+    const float f0 = mf::fast_exp2(d0), f1 = mf::fast_exp2(d1);
+    acc[n].m = m;
+    acc[n].l = rescaled(acc[n].l, d0) + rescaled(s[1], d1);
+#pragma unroll
+    for (int d = 0; d < kO; ++d) {
+      const f4 o = at[(n * (kO + 1) + d) * 64];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n].o[d][i] = acc[n].o[d][i] * f0 + o[i] * f1;
+    }
+  }
+}
+
+template <int D, int CODE, int N, bool LISTED, int G>
+__global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                       float *part, float *stat) {
   typedef Tile<D> T;
-  __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  __shared__ __attribute__((aligned(16))) char lds_all[2 * G * T::kBytes];
+  // G == 2: two groups of four waves hold the same rows and take half of the tiles each
+  const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  char *const lds = lds_all + part_of * 2 * T::kBytes;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, col = lane & 15, quad = lane >> 4;
   // Workgroups go to the 8 XCDs in turn.  A list is one split of the keys of one (sequence, head, run);
   // its row groups are dealt into `deal` hands so that 8 divides the number of hands, and an XCD plays whole hands:
   // its L2 then holds the keys of few lists (8 heads of 16k tokens: 1011 -> 908 us).
@@ -202,8 +238,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   const int32_t unit = list_index / p.splits * p.groups + (q.causal ? p.groups - 1 - group : group);
   const Rows w = rows_of(c, q, p, unit, kTileRows);
   const int32_t tiles = tiles_of(c, p, w), per = split_tiles_of(p, tiles);
-  const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
-  if (begin >= end && split > 0) return;
+  const int32_t begin0 = split * per, end0 = begin0 + per < tiles ? begin0 + per : tiles;
+  if (begin0 >= end0 && split > 0) return;
+  const int32_t steps = end0 > begin0 ? (end0 - begin0 + G - 1) / G : 0;  // of a group; the second may have one less
+  const int32_t begin = begin0 + part_of * steps, end = begin + steps < end0 ? begin + steps : end0;
   const int64_t sh = int64_t(w.s) * c.heads + w.h;
   BlockList list(c, p, w);
   const int32_t tokens = c.blocks << c.shift;
@@ -316,6 +354,11 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   // tiles that every row sees come first; from the first other one on, every tile is masked
   while (t < end && whole()) step(std::false_type());
   while (t < end) step(std::true_type());
+  if constexpr (G == 2) {
+    if (end - begin < steps) __syncthreads();  // the other group's last tile
+    join_groups<D>(acc, reinterpret_cast<f4 *>(lds_all), part_of, wave);
+    if (part_of == 1) return;
+  }
 
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -348,16 +391,14 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   }
 }
 
-template <int D, int CODE, class... Args>
-void launch_tile(bool two, bool listed, uint32_t workgroups, hipStream_t stream, const Args &...args) {
-  if (two && listed) {
-    hipLaunchKernelGGL((tile_kernel<D, CODE, 2, true>), dim3(workgroups), dim3(256), 0, stream, args...);
-  } else if (two) {
-    hipLaunchKernelGGL((tile_kernel<D, CODE, 2, false>), dim3(workgroups), dim3(256), 0, stream, args...);
-  } else if (listed) {
-    hipLaunchKernelGGL((tile_kernel<D, CODE, 1, true>), dim3(workgroups), dim3(256), 0, stream, args...);
+template <int D, int CODE, int N, class... Args>
+void launch_tile(bool listed, int groups, uint32_t workgroups, hipStream_t stream, const Args &...args) {
+  if (listed) {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, N, true, 1>), dim3(workgroups), dim3(256), 0, stream, args...);
+  } else if (groups == 2) {
+    hipLaunchKernelGGL((tile_kernel<D, CODE, N, false, 2>), dim3(workgroups), dim3(512), 0, stream, args...);
   } else {
-    hipLaunchKernelGGL((tile_kernel<D, CODE, 1, false>), dim3(workgroups), dim3(256), 0, stream, args...);
+    hipLaunchKernelGGL((tile_kernel<D, CODE, N, false, 1>), dim3(workgroups), dim3(256), 0, stream, args...);
   }
 }
 
@@ -370,7 +411,11 @@ int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, c
   UC_REQUIRE(lists * deal * ceil_div(p.groups, deal) < (int64_t(1) << 31), "uc_block8_attn: too many query rows");
   const uint32_t workgroups = static_cast<uint32_t>(lists * deal * ceil_div(p.groups, deal));
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
-    launch_tile<D, CODE>(c.block == 32, p.list != nullptr, workgroups, stream, c, q, p, out, lse, part, stat);
+    if (c.block == 32) {
+      launch_tile<D, CODE, 2>(p.list != nullptr, p.key_groups, workgroups, stream, c, q, p, out, lse, part, stat);
+    } else {
+      launch_tile<D, CODE, 1>(p.list != nullptr, p.key_groups, workgroups, stream, c, q, p, out, lse, part, stat);
+    }
     return check_launch("uc_block8_attn");
   });
 }
