@@ -158,3 +158,31 @@ def test_attention_and_selection_validation():
     with pytest.raises(ValueError, match="NULL"):
         nat.call("uc_block8_attn", c, None, None, 0, 0, 0.1, 16, None, 16, 1 << 40, None)
     assert ctypes.sizeof(nat.Block8Cache) == 88 and ctypes.sizeof(nat.Block8Query) == 72
+
+
+def test_launches_that_are_too_large():
+    many = _query(query_len=1 << 21, heads_q=4)  # 2 x 4 x 2^21 runs of one query, a workgroup each
+    with pytest.raises(ValueError, match="too many query rows"):
+        nat.call("uc_block8_select", _cache(), many, 4, 1, 1, 1, 16, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="too many query rows"):
+        nat.call("uc_block8_attn", _cache(), many, 16, 4, 1, 0.1, 16, None, 16, 1 << 50, None)
+    # 2^28 rows of 16 lanes
+    with pytest.raises(ValueError, match="too many query rows"):
+        nat.call("uc_block8_select", _cache(heads_kv=16), _query(query_len=1 << 23, heads_q=16), 4, 1, 1, 1 << 23, 16, 16,
+                 1 << 50, None)
+    # one workgroup of 128 rows a head, and each head's dealt to eight XCDs
+    with pytest.raises(ValueError, match="too many query rows"):
+        nat.call("uc_block8_attn", _cache(sequences=(1 << 22) - 1, heads_kv=1), _query(query_len=64, heads_q=2), None, 0,
+                 0, 0.1, 16, None, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="budget"):
+        nat.call("uc_block8_attn", _cache(), _query(), 16, (1 << 24) + 1, 1, 0.1, 16, None, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="budget"):
+        nat.call("uc_block8_select", _cache(), _query(), (1 << 24) + 1, 1, 1, 1, 16, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="too many keys"):
+        nat.call("uc_block8_attn", _cache(), _query(query_len=100), 16, 1 << 24, 1, 0.1, 16, None, 16, 1 << 50, None)
+
+
+def test_decode_selection_needs_no_score_workspace():
+    small = _query(query_len=1)
+    assert nat.lib().uc_block8_select_workspace_bytes(_cache(blocks=8192), small, 1) == 256
+    assert nat.lib().uc_block8_select_workspace_bytes(_cache(blocks=8193), small, 1) >= 2 * 4 * 8193 * 4

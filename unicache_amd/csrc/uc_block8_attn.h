@@ -96,8 +96,9 @@ __device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) 
 
 // Few rows: the tiles of all units ((sequence, head, run) in order) are cut into runs of equal
 // length for the workgroups, so that sequences of any lengths load them alike (32 sequences of 8k
-// tokens down to none: 74 us by equal splits of the longest, 65 so).  A unit's piece in workgroup g leaves its partial in slot
-// g + unit: of two pieces in order one of the two is larger.
+// tokens down to none: 74 us by equal splits of the longest, 59 so).  A unit's piece in
+// workgroup g leaves its partial in slot g + unit: of two pieces in order one of the two is larger.
+
 // Steps of one (head, run) of a sequence of so many keys: its tiles, rounded up to one for each of
 // the four waves.
 __device__ __forceinline__ int32_t steps_of(int32_t keys) { return (keys + 4 * kTile - 1) / (4 * kTile) * 4; }

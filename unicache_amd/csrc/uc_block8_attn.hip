@@ -25,6 +25,12 @@
 // consecutive keys of one query row, which is the operand that
 // O^T = V^T P^T takes, with no exchange between lanes: the values' blocks are
 // stored channel-major for that, 16 codes of a channel in one 16-byte load.
+//
+// Bound by HBM: each code is read once, straight into registers, a wave's next 64 keys (16 KB at 128
+// channels) on their way while it computes on the present ones, 128 KB in flight a CU.  Of 8 sequences
+// of 32k tokens (28/4 heads, 269 MB) the first launch takes 42 us from back to back calls (6.4 TB/s,
+// part of it from the last-level cache), both 56 over changing inputs (4.8 TB/s; a large copy
+// 4.9).  Small calls are two launches: 2k tokens 7.1 + 5.7 us.
 #include "uc_block8_attn.h"
 
 #include <type_traits>
@@ -502,10 +508,10 @@ void launch_rows(int32_t rows, uint32_t workgroups, hipStream_t stream, const Ar
   }
 }
 
-// Splits of 128-row workgroups, and how many groups of four waves they have: the least time in tiles.  Of one
-// group, two (head_dim 128) or three workgroups share a CU, and up to one a CU takes 0.65 of the time a tile; of
-// two groups one, each with half of the tiles, joined in LDS (one tile).  The launch that joins splits takes two tiles and 0.006 for each part of
-// a workgroup.  Measured, one split -> the chosen: 112 units of 64 tiles 110 -> 56 us (4 splits), 28 of 256
+// Splits of 128-row workgroups, and how many groups of four waves they have: the least time in
+// tiles.  Of one group, two (head_dim 128) or three workgroups share a CU, and up to one a CU takes
+// 0.65 of the time a tile; of two groups one, each with half of the tiles, joined in LDS (one
+// tile).  The launch that joins splits takes two tiles and 0.006 for each part of a workgroup.  Measured, one split -> the chosen: 112 units of 64 tiles 110 -> 56 us (4 splits), 28 of 256
 // 412 -> 59 (18), 572 of 64 247 -> 213 (4), 376 of 128 at head_dim 64 196 -> 151 (2); 512 of 64 stay at
 // one (206; two would take 224), as do 440 of 31 (66; 89).
 void split_tiles(int64_t units, int64_t tiles, int64_t head_dim, bool listed, Plan &p) {
@@ -544,7 +550,7 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
   UC_REQUIRE(query->query_len >= 0 && query->query_len < (1 << 24), "%s: bad query_len", what);
   UC_REQUIRE(query->heads_q / cache->heads_kv * query->query_len < (int64_t(1) << 30), "%s: too many query rows", what);
   UC_REQUIRE(query->max_tokens >= 0, "%s: negative max_tokens", what);
-  UC_REQUIRE(budget >= 0 && budget < (1 << 24), "%s: bad budget", what);
+  UC_REQUIRE(budget >= 0 && budget <= (1 << 30) / cache->block_tokens, "%s: bad budget", what);
   UC_REQUIRE(budget == 0 || query_block > 0, "%s: query_block must be positive", what);
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q),
@@ -578,7 +584,13 @@ int make_plan(const uc_block8_cache *cache, const uc_block8_query *query, int64_
       p.workgroups = static_cast<int32_t>(most < kShare ? (most > 0 ? most : 1) : kShare);
     }
   }
-  UC_REQUIRE(units * p.splits < (int64_t(1) << 31) / p.rows, "%s: too many query rows", what);
+  // a launch has less than 2^32 threads, and 32-bit counts of tiles
+  const bool joins = p.splits > 1 || p.workgroups > 0;
+  UC_REQUIRE(units * p.splits < (1 << 24) &&
+                 (!joins || cache->sequences * cache->heads_kv * p.runs * p.run * q.group < (1 << 28)),
+             "%s: too many query rows", what);
+  const int64_t longest = budget > 0 ? keys : capacity;
+  UC_REQUIRE(p.workgroups == 0 || units * ceil_div(longest, 4 * kTile) < (1 << 28), "%s: too many keys in all", what);
   return UC_OK;
 }
 

@@ -13,6 +13,15 @@
 // order, so that the fragments' 16-byte reads meet no bank twice.  Key tile j's row r is key
 // 32 (j / 2) + 8 (r / 4) + 4 (j % 2) + r % 4, so that a lane's logits of two tiles are
 // eight consecutive keys of its query row: the operand of O^T = V^T P^T.
+//
+// Bound by the vector instructions beside the matrix cores: at D = 128 a wave's tile is 64 MFMAs
+// (1,024 cycles) and about 235 other vector instructions (the exponentials and what leads to
+// them, the maxima, the casts, the next tile's conversion).  The cores are busy about 40 % of the
+// time, the LDS 30 %, without a bank conflict.  4096 causal queries behind 12k tokens of 32/8 heads:
+// 921 us, 1,045 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
+// LDS reads but need twice the accumulators.  The matrix phases run at raised priority, so that
+// the wave that is in one keeps the cores fed; forcing vector instructions between the MFMAs by
+// scheduling barriers was slower than that.
 #include "uc_block8_attn.h"
 
 #include <type_traits>
@@ -408,7 +417,7 @@ int launch_tiles(const uc_block8_cache *cache, const Cache &c, const Query &q, c
                  float *part, float *stat, hipStream_t stream) {
   // (the hands may be one row group longer than they need to be)
   const int64_t lists = int64_t(c.sequences) * c.heads * p.runs * p.splits, deal = 8 / (lists & 7 ? lists & -lists : 8);
-  UC_REQUIRE(lists * deal * ceil_div(p.groups, deal) < (int64_t(1) << 31), "uc_block8_attn: too many query rows");
+  UC_REQUIRE(lists * deal * ceil_div(p.groups, deal) < (1 << 24) / p.key_groups, "uc_block8_attn: too many query rows");
   const uint32_t workgroups = static_cast<uint32_t>(lists * deal * ceil_div(p.groups, deal));
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
     if (c.block == 32) {

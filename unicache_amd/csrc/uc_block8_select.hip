@@ -5,10 +5,12 @@
 // with a key inside a block's bounds (c+ and c- its positive and negative parts), so the scores
 // of all rows and blocks are one int8 matrix product over 2 D, exact in
 // int32; a score is fp32(I) u step, two roundings, whatever the order of the sum.
-// Three launches: the rows' codes, the scores (16 blocks x 16 rows per
-// MFMA tile, the largest over a run's rows kept in registers), and
-// the choice of the `budget` highest (radix selection on the scores' ordered
-// bit patterns).
+// Runs of at most 16 rows (decode) take one launch, a workgroup per run and
+// head: scores into LDS, then the `budget` highest by histograms of eight bits of their ordered
+// patterns.  512 blocks 9.4 us (latency: lengths, rows, bounds, four histogram rounds), 2048
+// blocks of 128 heads 26 us (67 MB of bounds on 128 CUs).  Longer runs take three: the rows' codes, the
+// scores (MFMA tiles of 16 rows x 16 blocks, the largest over a run's rows kept in registers), and the
+// choice; 2048 tokens of 28/4 heads by 512 blocks 7.4 + 14.5 + 5.6 us.
 #include "uc_block8.h"
 
 #include <type_traits>
@@ -471,18 +473,22 @@ int make_run(const uc_block8_cache *cache, const uc_block8_query *query, int64_t
   return UC_OK;
 }
 
+// One launch computes the scores and chooses.
+bool fused(const Run &q) { return q.run * q.group <= 16; }
+
 struct Space {
   int64_t codes, steps, scores, total;  // byte offsets
 };
 
 Space space_of(const uc_block8_cache *cache, const Run &q) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  const int64_t rows = cache->sequences * q.len * q.heads;
+  const int64_t rows = fused(q) ? 0 : cache->sequences * q.len * q.heads;
+  const bool scores = !fused(q) || cache->blocks > kKept;
   Space w;
   w.codes = 0;
   w.steps = up(rows * cache->head_dim);
   w.scores = w.steps + up(rows * 4);
-  w.total = w.scores + up(cache->sequences * q.runs * cache->heads_kv * cache->blocks * 4);
+  w.total = w.scores + up(scores ? cache->sequences * q.runs * cache->heads_kv * cache->blocks * 4 : 1);
   return w;
 }
 
@@ -508,7 +514,7 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   Run q;
   if (int rc = check_cache(cache, "uc_block8_select", c)) return rc;
   if (int rc = make_run(cache, query, query_block, "uc_block8_select", q)) return rc;
-  UC_REQUIRE(budget > 0 && budget < (1 << 24), "uc_block8_select: budget must be positive");
+  UC_REQUIRE(budget > 0 && budget <= (1 << 30) / cache->block_tokens, "uc_block8_select: bad budget");
   UC_REQUIRE(sink >= 0 && recent >= 1, "uc_block8_select: sink must not be negative and recent must be positive");
   const int64_t span = q.causal ? ceil_div(int64_t(q.run) - 1, int64_t(c.block)) : 0;
   UC_REQUIRE(sink + recent + span <= budget, "uc_block8_select: budget %lld is less than the %lld blocks always chosen",
@@ -530,11 +536,14 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t capacity = cache->blocks * cache->block_tokens;
   const int64_t expected = query->max_tokens < capacity ? query->max_tokens : capacity;
   const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 64 * kScored) : 1;
-  UC_REQUIRE(rows < (int64_t(1) << 32) && units * chunks < (int64_t(1) << 31), "uc_block8_select: too many query rows");
+  // a launch has less than 2^32 threads
+  UC_REQUIRE(fused(q) ? units < (1 << 23)
+                      : rows * (cache->head_dim / 8) < (int64_t(1) << 32) - 256 && units * chunks < (1 << 24),
+             "uc_block8_select: too many query rows");
   const float factor = cache->code_dtype == UC_INT8 ? 1.0f : static_cast<float>(448.0 / 127.0);
   auto launch = [&](auto d_tag) {
     constexpr int D = decltype(d_tag)::value;
-    if (q.run * q.group <= 16) {
+    if (fused(q)) {
       hipLaunchKernelGGL((choose_kernel<512, D, true>), dim3(static_cast<uint32_t>(units)), dim3(512), 0,
                          as_stream(stream), c, q, factor, score, blocks);
       return check_launch("uc_block8_select");
