@@ -180,6 +180,9 @@ def test_launches_that_are_too_large():
         nat.call("uc_block8_select", _cache(), _query(), (1 << 24) + 1, 1, 1, 1, 16, 16, 1 << 50, None)
     with pytest.raises(ValueError, match="too many keys"):
         nat.call("uc_block8_attn", _cache(), _query(query_len=100), 16, 1 << 24, 1, 0.1, 16, None, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="too many rows"):  # 2^13 x 8 x 257 workgroups
+        nat.call("uc_block8_append", _cache(sequences=1 << 13, heads_kv=8, blocks=300), 16, 16, 0, 0, 0, 16, 0, 0, 0,
+                 nat.UC_BF16, 1 << 14, None, None)
 
 
 def test_decode_selection_needs_no_score_workspace():

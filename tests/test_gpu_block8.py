@@ -122,6 +122,25 @@ def test_append_equals_from_dense(device, code, block, d):
     assert cache.lengths.tolist() == [cache.capacity] * s
 
 
+@pytest.mark.parametrize("code", CODES)
+def test_chunked_prefill_equals_from_dense(device, code):
+    # chunks of many blocks, each from an open block into another
+    t, h, s, d, block = 2500, 3, 2, 64, 32
+    key, value = dense(s, t, h, d, seed=4)
+    cache = Block8KVCache.empty(s, t, h, d, block_tokens=block, code_dtype=code)
+    start = 0
+    for n in (700, 1024, 3, 512, 261):
+        cache.append(key[:, start:start + n], value[:, start:start + n])
+        start += n
+    assert start == t
+    want = Block8KVCache.from_dense(key, value, block_tokens=block, code_dtype=code)
+    for name in ("key_code", "value_code", "key_scale", "value_scale", "key_bounds"):
+        assert torch.equal(getattr(cache, name).float(), getattr(want, name).float()), name
+    rows = t % block
+    assert torch.equal(cache.tail[:, :, 0, :rows], key[:, -rows:].transpose(1, 2))
+    assert torch.equal(cache.tail[:, :, 1, :rows], value[:, -rows:].transpose(1, 2))
+
+
 def test_a_block_with_infinities_reads_as_nan(device):
     key, value = dense(1, 200, 2, 128)
     key[0, 70, 1, 3] = math.inf

@@ -16,6 +16,8 @@
 // which they leave in 16-byte stores.
 #include "uc_block8.h"
 
+#include <algorithm>
+
 namespace uc {
 namespace b8 {
 
@@ -326,47 +328,64 @@ __device__ __forceinline__ int32_t appended(const Cache &cache, const int32_t *c
   return n < room ? n : room;
 }
 
-// One workgroup per (sequence, KV head) walks the blocks that the new rows
-// touch: the first holds rows of `tail`, the last leaves its rows there.  A
+// One workgroup per (sequence, KV head) and block that the new rows may touch, `most` of them (one
+// after the other, 4096 tokens of 8 heads took 210 us; so, 19).  The first block may hold rows of `tail`; its
+// workgroup leaves the last block's rows there too, once it has read what was there: a
 // thread reads and writes the same tail elements, so no barrier orders them.
 template <int D, int B, int CODE, int IN>
 __global__ __launch_bounds__((Shape<D, B>::kThreads)) void append_kernel(Cache cache, Dense key, Dense value,
                                                                          int32_t tokens, const int32_t *counts,
-                                                                         uint16_t *tail) {
+                                                                         uint16_t *tail, int32_t most) {
   typedef Shape<D, B> S;
   __shared__ Shared<D, B> sh;
-  const int32_t sequence = blockIdx.x / cache.heads, h = blockIdx.x % cache.heads;
+  const int32_t unit = blockIdx.x / most, index = blockIdx.x % most;
+  const int32_t sequence = unit / cache.heads, h = unit % cache.heads;
   const int32_t length = cache.length(sequence);
   const int32_t n = appended(cache, counts, sequence, tokens, length);
-  if (n <= 0) return;
-  uint16_t *t = tail + int64_t(blockIdx.x) * 2 * B * D;
-  const int32_t end = length + n;
-  for (int32_t b = length / B; b * B < end; ++b) {
-    const int rows = end - b * B < B ? end - b * B : B;
-    uint4 x[S::kPer][4], y[S::kPer][4];
+  const int32_t end = length + n, b = length / B + index;
+  if (n <= 0 || b * B >= end) return;
+  const int32_t last = (end - 1) / B;
+  uint16_t *t = tail + int64_t(unit) * 2 * B * D;
+  const int rows = end - b * B < B ? end - b * B : B;
+  uint4 x[S::kPer][4], y[S::kPer][4];
+#pragma unroll
+  for (int u = 0; u < S::kPer; ++u) {
+    const int at = threadIdx.x + u * S::kThreads, c = at % S::kChunks, g = at / S::kChunks;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * g + i;
+      const int32_t token = b * B + r;
+      x[u][i] = y[u][i] = uint4{0, 0, 0, 0};
+      if (token < length) {
+        x[u][i] = *reinterpret_cast<const uint4 *>(t + r * D + 8 * c);
+        y[u][i] = *reinterpret_cast<const uint4 *>(t + (B + r) * D + 8 * c);
+      } else if (token < end) {
+        x[u][i] = *reinterpret_cast<const uint4 *>(key.row(sequence, token - length, h) + 8 * c);
+        y[u][i] = *reinterpret_cast<const uint4 *>(value.row(sequence, token - length, h) + 8 * c);
+      }
+    }
+  }
+  // the rows of the block that stays open
+  if (index == 0 && end % B != 0) {
 #pragma unroll
     for (int u = 0; u < S::kPer; ++u) {
-      const int unit = threadIdx.x + u * S::kThreads, c = unit % S::kChunks, g = unit / S::kChunks;
+      const int at = threadIdx.x + u * S::kThreads, c = at % S::kChunks, g = at / S::kChunks;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 4 * g + i;
-        const int32_t at = b * B + r;
-        x[u][i] = y[u][i] = uint4{0, 0, 0, 0};
-        if (at < length) {
-          x[u][i] = *reinterpret_cast<const uint4 *>(t + r * D + 8 * c);
-          y[u][i] = *reinterpret_cast<const uint4 *>(t + (B + r) * D + 8 * c);
-        } else if (at < end) {
-          x[u][i] = *reinterpret_cast<const uint4 *>(key.row(sequence, at - length, h) + 8 * c);
-          y[u][i] = *reinterpret_cast<const uint4 *>(value.row(sequence, at - length, h) + 8 * c);
-          if (rows < B) {  // the block that stays open
-            *reinterpret_cast<uint4 *>(t + r * D + 8 * c) = x[u][i];
-            *reinterpret_cast<uint4 *>(t + (B + r) * D + 8 * c) = y[u][i];
-          }
+        const int32_t token = last * B + r;
+        if (token < length || token >= end) continue;
+        uint4 kr = x[u][i], vr = y[u][i];
+        if (last != b) {
+          kr = *reinterpret_cast<const uint4 *>(key.row(sequence, token - length, h) + 8 * c);
+          vr = *reinterpret_cast<const uint4 *>(value.row(sequence, token - length, h) + 8 * c);
         }
+        *reinterpret_cast<uint4 *>(t + r * D + 8 * c) = kr;
+        *reinterpret_cast<uint4 *>(t + (B + r) * D + 8 * c) = vr;
       }
     }
-    quantize_block<D, B, CODE, IN>(x, y, rows, cache, int64_t(blockIdx.x) * cache.blocks + b, sh);
   }
+  quantize_block<D, B, CODE, IN>(x, y, rows, cache, int64_t(unit) * cache.blocks + b, sh);
 }
 
 __global__ void advance_kernel(Cache cache, int32_t *lengths, int32_t tokens, const int32_t *counts) {
@@ -519,12 +538,15 @@ extern "C" int uc_block8_append(const uc_block8_cache *cache, void *tail, const 
   if (int rc = check_dense("uc_block8_append", value, v_ss, v_st, v_sh, "value")) return rc;
   const Dense k{static_cast<const uint16_t *>(key), k_ss, k_st, k_sh};
   const Dense v{static_cast<const uint16_t *>(value), v_ss, v_st, v_sh};
+  // blocks that the rows may touch
+  const int64_t most = std::min<int64_t>(ceil_div(tokens - 1, int64_t(c.block)) + 1, c.blocks);
+  UC_REQUIRE(int64_t(c.sequences) * c.heads * most < (1 << 24), "uc_block8_append: too many rows");
   const int rc = UC_B8_DISPATCH(cache, cache->head_dim, [&] {
     return UC_B8_DISPATCH_BLOCK(cache, [&] {
       return UC_B8_DISPATCH_HALF(in_dtype, IN, [&] {
-        hipLaunchKernelGGL((append_kernel<D, B, CODE, IN>), dim3(static_cast<uint32_t>(c.sequences * c.heads)),
+        hipLaunchKernelGGL((append_kernel<D, B, CODE, IN>), dim3(static_cast<uint32_t>(c.sequences * c.heads * most)),
                            dim3(Shape<D, B>::kThreads), 0, as_stream(stream), c, k, v, static_cast<int32_t>(tokens),
-                           counts, static_cast<uint16_t *>(tail));
+                           counts, static_cast<uint16_t *>(tail), static_cast<int32_t>(most));
         return check_launch("uc_block8_append");
       });
     });
