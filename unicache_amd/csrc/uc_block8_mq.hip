@@ -16,12 +16,12 @@
 //
 // Bound by the vector instructions beside the matrix cores: at D = 128 a wave's tile is 64 MFMAs
 // (1,024 cycles) and about 235 other vector instructions (the exponentials and what leads to
-// them, the maxima, the casts, the next tile's conversion).  The cores are busy about 40 % of the
-// time, the LDS 30 %, without a bank conflict.  4096 causal queries behind 12k tokens of 32/8 heads:
-// 921 us, 1,045 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
+// them, the maxima, the casts, the next tile's conversion).  The cores are busy about 47 % of the
+// time, the LDS 35 %, without a bank conflict.  4096 causal queries behind 12k tokens of 32/8 heads:
+// 859 to 892 us on two cards, 1,079 to 1,120 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
 // LDS reads but need twice the accumulators.  The matrix phases run at raised priority, so that
-// the wave that is in one keeps the cores fed; forcing vector instructions between the MFMAs by
-// scheduling barriers was slower than that.
+// the wave that is in one keeps the cores fed.  Codes converted a tile earlier, beside the Q K
+// products, were 7 % slower.
 #include "uc_block8_attn.h"
 
 #include <type_traits>
@@ -141,20 +141,25 @@ struct Acc16 {
   float m, l;
 };
 
-// Weights of one tile for 16 rows.  N == 2: its halves are in two blocks; else one scale of each kind
-// is the tile's.  ends[h]: keys of half h that the lane's row sees, from its own first key on.
+// A logit of one row, as the exponent of its weight.
+template <bool MASK>
+__device__ __forceinline__ float exponent(float s, float c, float shift, bool seen) {
+  const float x = __builtin_fmaf(s, c, shift);
+  return MASK && !seen ? mf::kNegInf : x;
+}
+
+// The reference of 16 rows' weights, raised where one of the tile's logits asks for it.  N == 2: its halves are
+// in two blocks; else one scale of each kind is the tile's.  ends[h]: keys of half h that the lane's
+// row sees, from its own first key on.
 template <int D, bool MASK, int N>
-__device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const float (&c)[N], const float (&lv)[N],
-                                        const float (&inv)[N], const int32_t (&ends)[2], h8 (&p)[2]) {
+__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], const float (&c)[N], const float (&lv)[N],
+                                           const int32_t (&ends)[2]) {
   constexpr int kK = 16 / N;  // logits of a lane per scale
-  float x[MASK ? 16 : 1];
   float top = mf::kNegInf;
   if constexpr (MASK) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      const int h = j / kK;
-      x[j] = j % 8 < ends[j / 8] ? __builtin_fmaf(s[j / 4][j % 4], c[h], lv[h]) : mf::kNegInf;
-      top = fmaxf(top, x[j]);
+      top = fmaxf(top, exponent<true>(s[j / 4][j % 4], c[j / kK], lv[j / kK], j % 8 < ends[j / 8]));
     }
   } else {
 #pragma unroll
@@ -174,23 +179,23 @@ __device__ __forceinline__ void weights(Acc16<D> &acc, const f4 (&s)[4], const f
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) acc.o[n] *= alpha;
   }
-  const float m = acc.m == mf::kNegInf ? 0.0f : acc.m;
+  return acc.m == mf::kNegInf ? 0.0f : acc.m;
+}
+
+// The weights of half a tile, and their sum.
+template <bool MASK>
+__device__ __forceinline__ float weights(const f4 (&s)[4], int half, float c, float lv, float inv, float m,
+                                         int32_t end, float l, h8 &p) {
+  float sum = 0.0f;
+  const float shift = lv - m;
 #pragma unroll
-  for (int h = 0; h < N; ++h) {
-    float sum = 0.0f;
-    const float shift = lv[h] - m;
-#pragma unroll
-    for (int j = h * kK; j < (h + 1) * kK; ++j) {
-      const float e = mf::fast_exp2(MASK ? x[MASK ? j : 0] - m : __builtin_fmaf(s[j / 4][j % 4], c[h], shift));
-      sum = j == h * kK ? e : sum + e;
-      p[j / 8][j % 8] = mf::to_h(e);
-    }
-    if constexpr (MASK) {
-      acc.l += sum == 0.0f ? 0.0f : sum * inv[h];
-    } else {
-      acc.l = __builtin_fmaf(sum, inv[h], acc.l);
-    }
+  for (int j = 0; j < 8; ++j) {
+    const float e = mf::fast_exp2(exponent<MASK>(s[2 * half + j / 4][j % 4], c, shift, j < end));
+    sum = j == 0 ? e : sum + e;
+    p[j] = mf::to_h(e);
   }
+  if constexpr (MASK) return l + (sum == 0.0f ? 0.0f : sum * inv);
+  return __builtin_fmaf(sum, inv, l);
 }
 
 // The second group's rows join the first's, lane by lane, through LDS (which nobody reads any more).
@@ -235,6 +240,17 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
   const int part_of = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   char *const lds = lds_all + part_of * 2 * T::kBytes;
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, col = lane & 15, quad = lane >> 4;
+  // Two waves share a SIMD: of two groups, or in slots of the SIMD that differ in their last bit (HW_ID's first four bits).
+  // One goes before the other in its vector phases, so that they do not reach the matrix cores
+  // together (without: prefill 4k 914 us, edit 50.6; with: 894, 48.5).
+  const bool before = (G == 2 ? part_of : __builtin_amdgcn_s_getreg((3 << 11) | 4) & 1) != 0;
+  auto vector_phase = [&] {
+    if (before) {
+      __builtin_amdgcn_s_setprio(1);
+    } else {
+      __builtin_amdgcn_s_setprio(0);
+    }
+  };
   // Workgroups go to the 8 XCDs in turn.  A list is one split of the keys of one (sequence, head, run);
   // its row groups are dealt into `deal` hands so that 8 divides the number of hands, and an XCD plays whole hands:
   // its L2 then holds the keys of few lists (8 heads of 16k tokens: 1011 -> 908 us).
@@ -318,18 +334,33 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
         s[1][j] = mf::mfma32(a, frag[1][k], s[1][j]);
       }
     }
-    __builtin_amdgcn_s_setprio(0);
+    vector_phase();
     h8 pr[2][2];
+    float cc[2][N], m[2];
+    int32_t ends[2][2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      float cc[N];
 #pragma unroll
-      for (int h = 0; h < N; ++h) cc[h] = ks[h] * factor[n];
-      const int32_t ends[2] = {row_end[n] - t0 - 8 * quad, row_end[n] - t1 - 8 * quad};
-      weights<D, MASK, N>(acc[n], s[n], cc, lv, inv, ends, pr[n]);
+      for (int h = 0; h < N; ++h) cc[n][h] = ks[h] * factor[n];
+      ends[n][0] = row_end[n] - t0 - 8 * quad;
+      ends[n][1] = row_end[n] - t1 - 8 * quad;
+      m[n] = reference<D, MASK, N>(acc[n], s[n], cc[n], lv, ends[n]);
     }
-    // The next tile's codes become fp16 beside the P V products (after the last tile the present
-    // one's again, into the buffer that nobody reads): a few vector instructions per MFMA.
+    auto weigh = [&](int h) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        acc[n].l = weights<MASK>(s[n], h, cc[n][h * (N - 1)], lv[h * (N - 1)], inv[h * (N - 1)], m[n], ends[n][h],
+                                 acc[n].l, pr[n][h]);
+      }
+    };
+    weigh(0);
+    // The second half's weights take their turns beside the first's P V products, and the next tile's
+    // codes become fp16 beside the second's (after the last tile the present one's again, into the
+    // buffer that nobody reads): prefill 4k 859 us, 898 with the weights before the products and codes beside
+    // both.  Lists and 64 channels, whose workgroups are few or have half the products, do better the
+    // second way (sparse prefill 164, 167; 3 x 777 tokens 47.3, 48.4).
+    constexpr bool kEarly = D == 64 || LISTED;
+    if constexpr (kEarly) weigh(1);
     clear<D>(st, ld, w.length);
     present ^= T::kBytes;
     __builtin_amdgcn_s_setprio(3);
@@ -343,13 +374,22 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
         acc[0].o[d] = mf::mfma32(a[d], pr[0][h], acc[0].o[d]);
         acc[1].o[d] = mf::mfma32(a[d], pr[1][h], acc[1].o[d]);
       }
-      if (h == 0) {
-        store_keys<D, CODE>(st, lds + present, ld);
-      } else {
-        store_values<D, CODE>(st, lds + present, ld);
+      if (!kEarly && h == 0) {
+        weigh(1);
+        if constexpr (!MASK) {  // (masked tiles have more vector instructions than this order provides for)
+          __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);  // the values
+#pragma unroll
+          for (int d = 0; d < D / 8; ++d) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product,
+            __builtin_amdgcn_sched_group_barrier(0x400, 1, 0);  // an exponential
+            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);    // and other vector instructions
+          }
+        }
       }
+      if (kEarly ? h == 0 : h == 1) store_keys<D, CODE>(st, lds + present, ld);
+      if (h == 1) store_values<D, CODE>(st, lds + present, ld);
     }
-    __builtin_amdgcn_s_setprio(0);
+    vector_phase();
     __syncthreads();
     ++t;
   };
