@@ -185,7 +185,10 @@ def test_launches_that_are_too_large():
                  nat.UC_BF16, 1 << 14, None, None)
 
 
-def test_decode_selection_needs_no_score_workspace():
-    small = _query(query_len=1)
-    assert nat.lib().uc_block8_select_workspace_bytes(_cache(blocks=8192), small, 1) == 256
-    assert nat.lib().uc_block8_select_workspace_bytes(_cache(blocks=8193), small, 1) >= 2 * 4 * 8193 * 4
+def test_decode_selection_asks_for_scores_where_it_keeps_them_in_memory():
+    need = nat.lib().uc_block8_select_workspace_bytes
+    one = _query(query_len=1)
+    assert need(_cache(blocks=512), one, 1) == 256
+    for sequences, blocks in ((2, 513), (32, 513), (33, 8193)):  # 8, 128 and 132 runs
+        assert need(_cache(sequences=sequences, blocks=blocks), one, 1) >= sequences * 4 * blocks * 4
+    assert need(_cache(sequences=33, blocks=8192), one, 1) == 256

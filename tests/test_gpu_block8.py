@@ -505,6 +505,22 @@ def test_selection_among_more_blocks_than_lds_holds(device, lq):
     assert torch.equal(blocks.cpu(), chosen_blocks(cache, q, lens, [lq, lq], False, 50, 40, 1, 1))
 
 
+@pytest.mark.parametrize("lens,lq,run", [([262200], 130, 1), ([40000, 100, 25000], 7, 2), ([17000], 12, 5)])
+def test_selection_of_few_rows_among_many_blocks(device, lens, lq, run):
+    # many runs of more blocks than LDS holds; causal runs whose sequences end differently
+    causal = run > 1
+    g = torch.Generator(device="cuda").manual_seed(7)
+    key = torch.randn(len(lens), max(lens), 1, 64, generator=g, device="cuda", dtype=torch.bfloat16)
+    cache = Block8KVCache.from_dense(key, key, lengths=torch.tensor(lens, dtype=torch.int32, device=device),
+                                     block_tokens=32)
+    q = queries(len(lens), lq, 3, 64, seed=8)
+    _, _, blocks = cache.sparse_attention(q, budget=50, query_block=run, sink=3, recent=2, causal=causal)
+    assert torch.equal(blocks.cpu(), chosen_blocks(cache, q, lens, [lq] * len(lens), causal, 50, run, 3, 2))
+    # a launch that expects shorter sequences
+    cache.max_tokens = 600 * 32
+    assert torch.equal(cache.sparse_attention(q, budget=50, query_block=run, sink=3, recent=2, causal=causal)[2], blocks)
+
+
 def test_selection_of_equal_scores_and_odd_queries(device):
     # equal blocks: the lower index; zero queries; a NaN query beside good ones; a block of NaN keys
     key, value = dense(1, 64 * 40, 1, 128, seed=60)

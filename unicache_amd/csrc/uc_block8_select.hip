@@ -7,8 +7,9 @@
 // int32; a score is fp32(I) u step, two roundings, whatever the order of the sum.
 // Runs of at most 16 rows (decode) take one launch, a workgroup per run and
 // head: scores into LDS, then the `budget` highest by histograms of eight bits of their ordered
-// patterns.  512 blocks 9.4 us (latency: lengths, rows, bounds, four histogram rounds), 2048
-// blocks of 128 heads 26 us (67 MB of bounds on 128 CUs).  Longer runs take three: the rows' codes, the
+// patterns; or, few runs of many blocks, one for the scores and one for the choice.  512 blocks 9.4 us
+// (latency: lengths, rows, bounds, four histogram rounds), 2048 blocks of 128 heads 24 us (67 MB
+// of bounds: 11 us of HBM, and the choice).  Longer runs take three: the rows' codes, the
 // scores (MFMA tiles of 16 rows x 16 blocks, the largest over a run's rows kept in registers), and the
 // choice; 2048 tokens of 28/4 heads by 512 blocks 7.4 + 14.5 + 5.6 us.
 #include "uc_block8.h"
@@ -211,6 +212,7 @@ __device__ __forceinline__ void own_codes(OwnCodes<D> &own, const Run &q, int32_
 // waves, the next 64 on their way (each wave loading all rows for itself was bound by L2: 20 us for 28 x 2048 rows
 // by 512 blocks).
 constexpr int kScored = 4;      // 16-block groups of a wave
+constexpr int kFewBlocks = 256; // blocks of a workgroup and step of score_few_kernel
 constexpr int kStageRows = 64;
 
 template <int D>
@@ -298,6 +300,77 @@ __global__ __launch_bounds__(256) void score_kernel(Cache c, Run q, const int8_t
   }
 }
 
+// The blocks of a run: those before `low` and from `high` on (up to `blocks`) are chosen anyway, of the
+// others the `want` highest.
+struct Candidates {
+  int32_t blocks, low, high, want;
+  __device__ __forceinline__ bool all() const { return want >= high - low; }
+};
+
+__device__ __forceinline__ Candidates candidates(const Cache &c, const Run &q, int32_t length, int32_t count, int32_t run) {
+  Candidates x = {0, 0, 0, 0};
+  int32_t first, last;
+  if (q.keys(length, count, run, first, last)) {
+    x.blocks = (last >> c.shift) + 1;
+    x.high = (first >> c.shift) - q.recent + 1;
+    x.low = q.sink < x.blocks ? q.sink : x.blocks;
+    x.high = x.high < x.low ? x.low : x.high;
+  }
+  x.want = q.budget - x.low - (x.blocks - x.high);
+  return x;
+}
+
+// Scores of a run's at most 16 rows by 16 * GROUPS blocks a wave and step, for the blocks from b0 on below
+// `high` in steps of `stride`: the rows' codes go through `own`, take(block, score) gets the outcomes.
+template <int D, int GROUPS, class Take>
+__device__ __forceinline__ void score_run(const Cache &c, const Run &q, int32_t s, int32_t h, int32_t run, int32_t count,
+                                          int32_t b0, int32_t high, int32_t stride, float unit_factor, OwnCodes<D> &own,
+                                          const Take &take) {
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int64_t sh = int64_t(s) * c.heads + h;
+  BlockBounds<D> bb[GROUPS];
+  if (b0 < high) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) load_bounds<D>(bb[g], c, sh, b0 + 16 * g, high, unit_factor);
+  }
+  const int32_t t0 = run * q.run;
+  own_codes<D>(own, q, s, h, t0, ((count - t0 < q.run) ? count - t0 : q.run) * q.group);
+  __syncthreads();
+  RowCodes<D> rc;
+  rc.step = *reinterpret_cast<const f4 *>(&own.step[4 * quad]);
+#pragma unroll
+  for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(&own.codes[col][k * 64 + quad * 16]));
+  for (int32_t b1 = b0; b1 < high; b1 += stride) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      float best = mf::kNegInf;
+      score16<D>(bb[g], rc, best);
+      const float v = over_rows(best, bb[g].u);
+      const int32_t b = b1 + 16 * g + col;
+      if (quad == 0 && b < high) take(b, v);
+    }
+    if (b1 + stride < high) {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) load_bounds<D>(bb[g], c, sh, b1 + stride + 16 * g, high, unit_factor);
+    }
+  }
+}
+
+// The scores of a run of at most 16 rows by `chunks` workgroups, for choose_kernel.
+template <int D>
+__global__ __launch_bounds__(256) void score_few_kernel(Cache c, Run q, float unit_factor, float *score, int32_t chunks) {
+  __shared__ __attribute__((aligned(16))) OwnCodes<D> own;
+  const int32_t unit = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
+  const int32_t count = q.count(s);
+  const Candidates x = candidates(c, q, c.length(s), count, run);
+  const int32_t begin = x.low + chunk * kFewBlocks;
+  if (x.all() || begin >= x.high) return;
+  float *sc = score + int64_t(unit) * c.blocks;
+  score_run<D, kFewBlocks / 64>(c, q, s, h, run, count, begin + (threadIdx.x >> 6) * (kFewBlocks / 4), x.high,
+                                chunks * kFewBlocks, unit_factor, own, [&](int32_t b, float v) { sc[b] = v; });
+}
+
 // Bits of a score that order as it does.
 __device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);
@@ -306,11 +379,9 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 
 constexpr int32_t kKept = 8192;  // scores that choose_kernel holds in LDS
 
-// One workgroup per (sequence, run, head).  Blocks before `low` and from
-// `high` on are chosen anyway; of the others the `want` highest: their
-// smallest score is found eight bits a round by histograms in LDS, then the
-// chosen are written by prefix sums.  With FUSED (runs of at most 16 rows) the scores are computed here, 16 blocks a
-// wave and step, so that a decode step's choice is one launch.
+// One workgroup per (sequence, run, head).  The smallest of the `want` highest scores is found eight
+// bits a round by histograms in LDS, then the chosen are written by prefix sums.  With FUSED (runs of
+// at most 16 rows) the scores are computed here, so that a decode step's choice is one launch.
 template <int T, int D, bool FUSED>
 __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_factor, float *score, int32_t *out) {
   constexpr int kWaves = T / kWave;
@@ -323,56 +394,22 @@ __global__ __launch_bounds__(T) void choose_kernel(Cache c, Run q, float unit_fa
   const int32_t unit = blockIdx.x;
   const int32_t h = unit % c.heads, run = unit / c.heads % q.runs, s = unit / c.heads / q.runs;
   const int32_t length = c.length(s), count = q.count(s);
-  const int64_t sh = int64_t(s) * c.heads + h;
   float *sc = score + int64_t(unit) * c.blocks;
   int32_t *list = out + int64_t(unit) * q.budget;
-  int32_t first, last, blocks = 0, low = 0, high = 0;
-  if (q.keys(length, count, run, first, last)) {
-    blocks = (last >> c.shift) + 1;
-    high = (first >> c.shift) - q.recent + 1;
-    low = q.sink < blocks ? q.sink : blocks;
-    high = high < low ? low : high;
-  }
+  const Candidates x = candidates(c, q, length, count, run);
+  const int32_t blocks = x.blocks, low = x.low, high = x.high, want = x.want;
   const int32_t n = high - low;  // blocks to choose from
-  const int32_t want = q.budget - low - (blocks - high);
-  const bool all = want >= n, held = n <= kKept;
+  const bool all = x.all(), held = n <= kKept;
   if (!all) {
     if constexpr (FUSED) {
-      constexpr int kB = 4;  // 16-block groups of a wave in flight
-      const int col = lane & 15, quad = lane >> 4;
-      BlockBounds<D> bb[kB];
-      const int32_t b0 = low + wave * 16 * kB;
-      if (b0 < high) {
-#pragma unroll
-        for (int g = 0; g < kB; ++g) load_bounds<D>(bb[g], c, sh, b0 + 16 * g, high, unit_factor);
-      }
-      const int32_t t0 = run * q.run;
-      own_codes<D>(own, q, s, h, t0, ((count - t0 < q.run) ? count - t0 : q.run) * q.group);
-      __syncthreads();
-      RowCodes<D> rc;
-      rc.step = *reinterpret_cast<const f4 *>(&own.step[4 * quad]);
-#pragma unroll
-      for (int k = 0; k < D / 64; ++k) rc.split(k, *reinterpret_cast<const i4 *>(&own.codes[col][k * 64 + quad * 16]));
-      for (int32_t b1 = b0; b1 < high; b1 += kWaves * 16 * kB) {
-#pragma unroll
-        for (int g = 0; g < kB; ++g) {
-          float best = mf::kNegInf;
-          score16<D>(bb[g], rc, best);
-          const float v = over_rows(best, bb[g].u);
-          const int32_t b = b1 + 16 * g + col;
-          if (quad == 0 && b < high) {
-            if (held) {
-              kept[b - low] = ordered(v);
-            } else {
-              sc[b] = v;
-            }
-          }
-        }
-        if (b1 + kWaves * 16 * kB < high) {
-#pragma unroll
-          for (int g = 0; g < kB; ++g) load_bounds<D>(bb[g], c, sh, b1 + (kWaves * kB + g) * 16, high, unit_factor);
-        }
-      }
+      score_run<D, 4>(c, q, s, h, run, count, low + wave * 64, high, kWaves * 64, unit_factor, own,
+                      [&](int32_t b, float v) {
+                        if (held) {
+                          kept[b - low] = ordered(v);
+                        } else {
+                          sc[b] = v;
+                        }
+                      });
     } else if (held) {
       for (int32_t i = tid; i < n; i += T) kept[i] = ordered(sc[low + i]);
     }
@@ -473,8 +510,15 @@ int make_run(const uc_block8_cache *cache, const uc_block8_query *query, int64_t
   return UC_OK;
 }
 
-// One launch computes the scores and chooses.
-bool fused(const Run &q) { return q.run * q.group <= 16; }
+// Runs whose rows fit one product: their codes need no memory.
+bool few(const Run &q) { return q.run * q.group <= 16; }
+
+// Whether a launch of its own computes their scores, with a workgroup per 256 blocks: where a workgroup per
+// run would take more than one step over its 512 blocks and leave half of the CUs idle (a CU takes
+// in 24 bytes a ns at most, 6 TB/s in all).  One launch, then two, us: 8 runs of 512 blocks 9.2, 9.9; 1024 14.5, 11.6; 8192
+// 80, 30; 128 runs of 512 10.0, 11.2; 1024 16.9, 16.0; 2048 29.2, 24.3; 256 runs of 1024 19.8, 21.7; 4096
+// 60, 65.
+bool scored_apart(int64_t units, int64_t blocks) { return blocks > 512 && units <= 128; }
 
 struct Space {
   int64_t codes, steps, scores, total;  // byte offsets
@@ -482,13 +526,14 @@ struct Space {
 
 Space space_of(const uc_block8_cache *cache, const Run &q) {
   auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-  const int64_t rows = fused(q) ? 0 : cache->sequences * q.len * q.heads;
-  const bool scores = !fused(q) || cache->blocks > kKept;
+  const int64_t rows = few(q) ? 0 : cache->sequences * q.len * q.heads;
+  const int64_t units = cache->sequences * q.runs * cache->heads_kv;
+  const bool scores = !few(q) || cache->blocks > kKept || scored_apart(units, cache->blocks);
   Space w;
   w.codes = 0;
   w.steps = up(rows * cache->head_dim);
   w.scores = w.steps + up(rows * 4);
-  w.total = w.scores + up(scores ? cache->sequences * q.runs * cache->heads_kv * cache->blocks * 4 : 1);
+  w.total = w.scores + up(scores ? units * cache->blocks * 4 : 1);
   return w;
 }
 
@@ -537,13 +582,21 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   const int64_t expected = query->max_tokens < capacity ? query->max_tokens : capacity;
   const int64_t chunks = expected > 0 ? ceil_div(ceil_div(expected, int64_t(c.block)), 64 * kScored) : 1;
   // a launch has less than 2^32 threads
-  UC_REQUIRE(fused(q) ? units < (1 << 23)
+  UC_REQUIRE(few(q) ? units < (1 << 23)
                       : rows * (cache->head_dim / 8) < (int64_t(1) << 32) - 256 && units * chunks < (1 << 24),
              "uc_block8_select: too many query rows");
   const float factor = cache->code_dtype == UC_INT8 ? 1.0f : static_cast<float>(448.0 / 127.0);
   auto launch = [&](auto d_tag) {
     constexpr int D = decltype(d_tag)::value;
-    if (fused(q)) {
+    if (few(q)) {
+      if (scored_apart(units, ceil_div(expected, int64_t(c.block)))) {
+        hipLaunchKernelGGL((score_few_kernel<D>), dim3(static_cast<uint32_t>(units * chunks)), dim3(256), 0,
+                           as_stream(stream), c, q, factor, score, static_cast<int32_t>(chunks));
+        if (int rc = check_launch("uc_block8_select (scores)")) return rc;
+        hipLaunchKernelGGL((choose_kernel<512, D, false>), dim3(static_cast<uint32_t>(units)), dim3(512), 0,
+                           as_stream(stream), c, q, factor, score, blocks);
+        return check_launch("uc_block8_select");
+      }
       hipLaunchKernelGGL((choose_kernel<512, D, true>), dim3(static_cast<uint32_t>(units)), dim3(512), 0,
                          as_stream(stream), c, q, factor, score, blocks);
       return check_launch("uc_block8_select");
