@@ -18,7 +18,7 @@
 // (1,024 cycles) and about 235 other vector instructions (the exponentials and what leads to
 // them, the maxima, the casts, the next tile's conversion).  The cores are busy about 47 % of the
 // time, the LDS 35 %, without a bank conflict.  4096 causal queries behind 12k tokens of 32/8 heads:
-// 859 to 892 us on two cards, 1,079 to 1,120 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
+// 859 to 899 us by card, 1,071 to 1,120 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
 // LDS reads but need twice the accumulators.  The matrix phases run at raised priority, so that
 // the wave that is in one keeps the cores fed.  Codes converted a tile earlier, beside the Q K
 // products, were 7 % slower.

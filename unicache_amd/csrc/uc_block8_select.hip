@@ -8,8 +8,8 @@
 // Runs of at most 16 rows (decode) take one launch, a workgroup per run and
 // head: scores into LDS, then the `budget` highest by histograms of eight bits of their ordered
 // patterns; or, few runs of many blocks, one for the scores and one for the choice.  512 blocks 9.4 us
-// (latency: lengths, rows, bounds, four histogram rounds), 2048 blocks of 128 heads 24 us (67 MB
-// of bounds: 11 us of HBM, and the choice).  Longer runs take three: the rows' codes, the
+// (latency: lengths, rows, bounds, four histogram rounds), 2048 blocks of 128 heads 14.2 + 9.6 us
+// (67 MB of bounds at 4.7 TB/s, and the choice).  Longer runs take three: the rows' codes, the
 // scores (MFMA tiles of 16 rows x 16 blocks, the largest over a run's rows kept in registers), and the
 // choice; 2048 tokens of 28/4 heads by 512 blocks 7.4 + 14.5 + 5.6 us.
 #include "uc_block8.h"
