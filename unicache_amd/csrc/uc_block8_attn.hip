@@ -30,7 +30,7 @@
 // channels) on their way while it computes on the present ones, 128 KB in flight a CU.  Of 8 sequences
 // of 32k tokens (28/4 heads, 269 MB) the first launch takes 42 us from back to back calls (6.4 TB/s,
 // part of it from the last-level cache), both 56 over changing inputs (4.8 TB/s; a large copy
-// 4.9).  Small calls are two launches: 2k tokens 7.1 + 5.7 us.
+// 4.9).  Small calls are two launches: 2k tokens 7.1 + 4.8 us.
 #include "uc_block8_attn.h"
 
 #include <type_traits>
@@ -415,12 +415,9 @@ __device__ __forceinline__ Sum<D> sum_parts(const Plan &p, const Parts &x, int32
   t.l = 0.0f;
 #pragma unroll
   for (int j = 0; j < kC; ++j) t.o[j] = 0.0f;
-  for (int32_t i = lane; i < x.count; i += 16) t.m = fmaxf(t.m, stat[2 * (base + int64_t(i) * p.rows)]);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) t.m = fmaxf(t.m, __shfl_xor(t.m, o, kWave));
-  for (int32_t i0 = begin; i0 < x.count; i0 += 2 * STRIDE) {
-    float mi[2], li[2];
-    f4 oi[2][kC / 4];
+  float mi[2], li[2];
+  f4 oi[2][kC / 4];
+  auto load = [&](int32_t i0) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int32_t i = i0 + u * STRIDE;
@@ -430,6 +427,12 @@ __device__ __forceinline__ Sum<D> sum_parts(const Plan &p, const Parts &x, int32
 #pragma unroll
       for (int j = 0; j < kC / 4; ++j) oi[u][j] = *reinterpret_cast<const f4 *>(part + at * D + lane * kC + 4 * j);
     }
+  };
+  if (begin < x.count) load(begin);  // on their way while the largest reference is found
+  for (int32_t i = lane; i < x.count; i += 16) t.m = fmaxf(t.m, stat[2 * (base + int64_t(i) * p.rows)]);
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) t.m = fmaxf(t.m, __shfl_xor(t.m, o, kWave));
+  for (int32_t i0 = begin; i0 < x.count;) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       // a part past the end, or one whose keys the row does not see
@@ -439,6 +442,8 @@ __device__ __forceinline__ Sum<D> sum_parts(const Plan &p, const Parts &x, int32
 #pragma unroll
       for (int j = 0; j < kC; ++j) t.o[j] += f * oi[u][j / 4][j % 4];
     }
+    i0 += 2 * STRIDE;
+    if (i0 < x.count) load(i0);
   }
   return t;
 }
