@@ -804,7 +804,8 @@ typedef struct uc_block8_query {
 /*
  * out = softmax(sm_scale * q K^T) V over each row's visible keys, contiguous
  * [S, Lq, Hq, D] of the query's dtype, and lse [S, Hq, Lq] (natural log, may be NULL).  Rows that
- * see no key, and rows behind a sequence's queries, get 0 and -inf.  With `blocks`
+ * see no key, and rows behind a sequence's queries, get 0 and -inf.  Value scales below 2^-88, or below
+ * 2^-60 of a larger one that the row has seen (0 for a block of zeros among them), count as that.  With `blocks`
  * (int32 [S, ceil(Lq / query_block), Hkv, budget], ascending, -1 for none) each run of
  * query_block rows sees the listed blocks of its KV head only.  sm_scale > 0.
  * workspace: uc_block8_attn_workspace_bytes(cache, query, budget, query_block).

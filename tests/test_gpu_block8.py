@@ -733,3 +733,91 @@ def test_a_long_cache_past_32_bit_offsets(device):
     assert (dense_lse[2].double().cpu() - want).abs().max() < 1e-4
     share = torch.exp(el[0] - want).reshape(1, -1, 1)
     assert (dense_out[2].double().cpu() - eo[0] * share).abs().max() <= 2.0 ** -7 * eo.abs().max()
+
+
+def zero_region(region, *, block, code, s=1, n=2048, h=4, d=128, seed=130):
+    """A cache as another program may have made it: values of zero and value scales of 0 in the blocks
+    for which region(first token) holds."""
+
+    key, value = dense(s, n, h, d, seed=seed)
+    at = torch.tensor([region(b * block) for b in range(-(-n // block))])
+    value[:, at.repeat_interleave(block)[:n].to(value.device)] = 0
+    cache = Block8KVCache.from_dense(key, value, block_tokens=block, code_dtype=code)
+    cache.value_scale[:, :, at.to(value.device)] = 0
+    return cache
+
+
+# alone, before real values (a padded sequence), between them, behind them, and every second block
+ZERO_REGIONS = [lambda t: True, lambda t: t < 256, lambda t: t < 1024, lambda t: 256 <= t < 512, lambda t: t >= 1024,
+                lambda t: t // 128 % 2 == 0, lambda t: t // 32 % 2 == 0, lambda t: t // 32 % 2 == 1]
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("lq", [1, 50])
+@pytest.mark.parametrize("region", range(len(ZERO_REGIONS)))
+def test_many_blocks_of_zeros_with_scales_of_zero(device, region, lq, code):
+    # logits that are equal (zero queries) and random ones; d products at most, so the tolerances of reference() hold
+    for block in (32, 128):
+        print(f"zero region {region} block {block} rows {lq}", flush=True)
+        cache = zero_region(ZERO_REGIONS[region], block=block, code=code)
+        for q in (queries(1, lq, 28, 128, seed=131, scale=0.0), queries(1, lq, 28, 128, seed=132)):
+            got = cache.attention(q)
+            assert torch.isfinite(got[0]).all() and torch.isfinite(got[1]).all()
+            check(got, reference(cache, q, [2048], [lq], False, 1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("lq", [1, 50])
+@pytest.mark.parametrize("tokens", [256, 1024, 30000])
+def test_a_sequence_of_zeros_alone(device, tokens, lq):
+    # ragged: as many keys as one workgroup takes, and many times that; out is 0, lse that of the keys
+    cache = zero_region(lambda t: True, block=64, code=torch.int8, s=2, n=tokens, h=2, d=64, seed=133)
+    cache.lengths[1] = tokens // 2 + 5
+    q = queries(2, lq, 8, 64, seed=134)
+    check(cache.attention(q), reference(cache, q, [tokens, tokens // 2 + 5], [lq] * 2, False, 1 / math.sqrt(64)))
+
+
+@pytest.mark.parametrize("lq", [1, 50])
+@pytest.mark.parametrize("power", [70, 100])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_blocks_of_zeros_beside_very_large_values(device, odd, power, lq):
+    # from_dense's own scales: every second half of a 64-key tile holds zeros (scale 2^-60), the others values of 2^power
+    for code in CODES:
+        key, value = dense(1, 640, 2, 128, seed=135)
+        value = value * 2.0 ** power
+        value[:, torch.arange(640, device=device) // 32 % 2 == odd] = 0
+        cache = Block8KVCache.from_dense(key, value, block_tokens=32, code_dtype=code)
+        for q in (queries(1, lq, 8, 128, seed=136, scale=0.0), queries(1, lq, 8, 128, seed=137)):
+            for causal in (False, True):
+                check(cache.attention(q, causal=causal),
+                      reference(cache, q, [640], [lq], causal, 1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("lq", [1, 50])
+def test_small_value_scales(device, lq):
+    # another program's values far below the quantizer's smallest, behind blocks of zeros: kept down to scales of 2^-88
+    for block in (32, 64):
+        cache = zero_region(lambda t: t < 512, block=block, code=torch.float8_e4m3fn, n=1000, h=2)
+        q = queries(1, lq, 8, 128, seed=138)
+        cache.value_scale.mul_(2.0 ** -66)  # dense() has scales of 2^-13 to 2^-6
+        check(cache.attention(q), reference(cache, q, [1000], [lq], False, 1 / math.sqrt(128)))
+        # below that the weights stay right, and what the values add is less than 448 * 2^-88
+        _, want, _, tol = reference(cache, q, [1000], [lq], False, 1 / math.sqrt(128))
+        cache.value_scale.mul_(2.0 ** -60)
+        out, lse = cache.attention(q)
+        assert ((lse.double().cpu() - want).abs() <= tol).all() and (out.abs() <= 448 * 2.0 ** -88).all()
+
+
+@pytest.mark.parametrize("lq", [3, 50])
+def test_rows_that_do_not_see_a_tiles_larger_scale(device, lq):
+    # causal rows whose last key is in the first half of a tile, whose second half holds values 2^70 times as large
+    key, value = dense(1, 64 + lq, 2, 128, seed=139)
+    for code in CODES:
+        cache = Block8KVCache.from_dense(key[:, :64], value[:, :64], block_tokens=32, code_dtype=code, capacity=128)
+        cache.value_scale[:, :, 0] *= 2.0 ** -70
+        q = queries(1, 64, 8, 128, seed=140)[:, 32 - lq // 2:32 - lq // 2 + lq]
+        cache.lengths.fill_(32 - lq // 2 + lq)
+        out, lse = cache.attention(q, causal=True)
+        seen = lq // 2  # rows whose last key is token 31 or one before it
+        first = Block8KVCache(*(getattr(cache, n) for n in ("key_code", "value_code", "key_scale", "value_scale", "key_bounds")),
+                              torch.full_like(cache.lengths, 32))
+        check((out[:, :seen], lse[..., :seen]), reference(first, q[:, :seen], [32], [seen], True, 1 / math.sqrt(128)))

@@ -184,10 +184,20 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int32_t n) {
   return uint4{w[0], w[1], w[2], w[3]};
 }
 
-// The value scale that a tile's keys count with; `most` is the largest so far.
-__device__ __forceinline__ float counted_scale(float vs, float &most) {
-  if (vs < __builtin_huge_valf()) most = fmaxf(most, vs);
-  const float least = most * 0x1p-60f;
+// The value scale that keys count with in their weights' exponents.  A weight is relative to the largest
+// logit + log2(scale) of its row, so a scale far below another's would leave fp32's range there: it counts as
+// 2^-60 of `most`, the largest scale of the blocks that the row has seen, the present tile's among them
+// (its weights then keep their place in l, whose terms are P / scale).  And where no larger one has been seen it counts as
+// 2^-88 at least: a key adds 2^88 to l at most, a raised reference 2^8, so the 2^30 keys of the
+// longest sequence stay below 2^128.  (A scale of 0 comes from another program; the quantizer's smallest is 2^-60.)
+constexpr float kLeastScale = 0x1p-88f;
+
+__device__ __forceinline__ float larger_scale(float most, float vs) {
+  return vs < __builtin_huge_valf() ? fmaxf(most, vs) : most;  // an infinity or a NaN is no scale to go by
+}
+
+__device__ __forceinline__ float counted_scale(float vs, float most) {
+  const float least = fmaxf(most * 0x1p-60f, kLeastScale);
   return vs < least ? least : vs;  // a NaN stays
 }
 

@@ -11,8 +11,8 @@
 // running reference of x (not of the logit): P stays in fp16's range
 // whatever the blocks' scales are, and its rounding (half a step, 2^-11) is
 // relative to the largest contribution.  Sums, m and O are fp32.  A block whose
-// value scale is less than 2^-60 of one read before it (a block of zeros has
-// 2^-60) counts as 2^-60 of that one: its weights then keep their place in l, and
+// value scale is less than 2^-60 of another that the row has seen (a block of zeros has
+// 2^-60, another program's 0) counts as 2^-60 of that one: its weights then keep their place in l, and
 // what its values add is below 2^-51 of the head's largest either way.
 //
 // Codes become fp16 exactly (int8 and e4m3 both fit); a query row is
@@ -153,7 +153,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
   l.kscale = c.key_scale + sh * c.blocks;
   l.vscale = c.value_scale + sh * c.blocks;
 
-  float most = kTiny;  // the largest value scale so far
+  float most = 0.0f;  // the largest value scale so far
   Raw<D> raw;
   int32_t t = begin + wave, t0 = 0, t1 = 0;
   if (t < end) {
@@ -214,12 +214,30 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Plan
         }
       }
     }
-    const int32_t mine = ((quad & 2) ? t1 : t0) + l.key;  // the lane's first key
-    const float ks = raw.ks, vs = counted_scale(!MASK || mine < w.length ? raw.vs : 1.0f, most);
+    const int32_t half0 = (quad & 2) ? t1 : t0, other0 = (quad & 2) ? t0 : t1;  // first keys of the lane's half and of the other
+    const int32_t mine = half0 + l.key;                                        // the lane's first key
+    const float ks = raw.ks, vs = raw.vs;
+    // the scale of the other half, whose lanes share the rows' references
+    float vo = vs;
+    if (c.shift == 5) vo = __shfl_xor(vs, 32, kWave);
     if (more) load_keys(raw, c, l, n0, n1);
     h8 pr[NR][2];
+    if constexpr (!MASK) most = larger_scale(larger_scale(most, vs), vo);
 #pragma unroll
-    for (int n = 0; n < NR; ++n) softmax_step<D, CODE, MASK>(acc[n], s[n], factor[n], ks, vs, row_end[n] - mine, pr[n]);
+    for (int n = 0; n < NR; ++n) {
+      float counted = counted_scale(vs, most);
+      if constexpr (MASK) {
+        // blocks that the row does not see are nothing to go by (later tiles are for rows that see all of this one)
+        float seen = half0 < row_end[n] ? larger_scale(most, vs) : most;
+        seen = other0 < row_end[n] ? larger_scale(seen, vo) : seen;
+        counted = half0 < row_end[n] ? counted_scale(vs, seen) : 1.0f;
+      }
+      softmax_step<D, CODE, MASK>(acc[n], s[n], factor[n], ks, counted, row_end[n] - mine, pr[n]);
+    }
+    if constexpr (MASK) {
+      most = half0 < w.length ? larger_scale(most, vs) : most;
+      most = other0 < w.length ? larger_scale(most, vo) : most;
+    }
     if constexpr (MASK) {
       // codes behind the length are no values: a zero weight must not meet them
 #pragma unroll

@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
 #pragma unroll
   for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ value_swizzle(col));
 
-  float most = kTiny;
+  float most = 0.0f;  // the largest value scale so far
   Staged<D> st;
   const Loader<D> ld(c.block);
   auto get = [&](int32_t t) {
@@ -311,13 +311,28 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
     const char *buf = lds + present;
     const int32_t t0 = st.t[0], t1 = st.t[1];
     // (one block: the halves' scales are the same, and the first is there if any is)
-    float ks[N], lv[N], inv[N];
+    // Masked halves of two blocks: a row goes by the scales that it sees, so they count for each row by itself.
+    constexpr int R = MASK && N == 2 ? 2 : 1;
+    float ks[N], lv[R][N], inv[R][N];
 #pragma unroll
-    for (int h = 0; h < N; ++h) {
-      ks[h] = st.ks[h];
-      const float vs = counted_scale(!MASK || st.t[h] < w.length ? st.vs[h] : 1.0f, most);
-      lv[h] = __builtin_amdgcn_logf(vs);
-      inv[h] = __builtin_amdgcn_rcpf(vs);
+    for (int h = 0; h < N; ++h) ks[h] = st.ks[h];
+    const float before = most;
+#pragma unroll
+    for (int h = 0; h < N; ++h) most = !MASK || st.t[h] < w.length ? larger_scale(most, st.vs[h]) : most;
+#pragma unroll
+    for (int n = 0; n < R; ++n) {
+      float seen = most;
+      if constexpr (R == 2) {
+        seen = t0 < row_end[n] ? larger_scale(before, st.vs[0]) : before;
+        seen = t1 < row_end[n] ? larger_scale(seen, st.vs[N - 1]) : seen;
+      }
+#pragma unroll
+      for (int h = 0; h < N; ++h) {
+        const bool there = !MASK || st.t[h] < (R == 2 ? row_end[n] : w.length);
+        const float vs = there ? counted_scale(st.vs[h], seen) : 1.0f;
+        lv[n][h] = __builtin_amdgcn_logf(vs);
+        inv[n][h] = __builtin_amdgcn_rcpf(vs);
+      }
     }
     const bool more = t + 1 < end;
     if (more) get(t + 1);
@@ -344,13 +359,13 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
       for (int h = 0; h < N; ++h) cc[n][h] = ks[h] * factor[n];
       ends[n][0] = row_end[n] - t0 - 8 * quad;
       ends[n][1] = row_end[n] - t1 - 8 * quad;
-      m[n] = reference<D, MASK, N>(acc[n], s[n], cc[n], lv, ends[n]);
+      m[n] = reference<D, MASK, N>(acc[n], s[n], cc[n], lv[n % R], ends[n]);
     }
     auto weigh = [&](int h) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        acc[n].l = weights<MASK>(s[n], h, cc[n][h * (N - 1)], lv[h * (N - 1)], inv[h * (N - 1)], m[n], ends[n][h],
-                                 acc[n].l, pr[n][h]);
+        const int b = h * (N - 1);
+        acc[n].l = weights<MASK>(s[n], h, cc[n][b], lv[n % R][b], inv[n % R][b], m[n], ends[n][h], acc[n].l, pr[n][h]);
       }
     };
     weigh(0);

@@ -93,7 +93,8 @@ class Block8KVCache:
     - ``lengths``     [S] int32, tokens held by each sequence, on the device
 
     D is 64 or 128, B 32, 64 or 128.  Scales are not negative (0 will do for a
-    block of zeros).  ``tail`` ([S, Hkv, 2, B, D] in the dense
+    block of zeros; attention takes value scales below 2^-88, or below 2^-60 of a
+    larger one that the row has seen, for that).  ``tail`` ([S, Hkv, 2, B, D] in the dense
     dtype, or None) holds the dense rows of each sequence's open block for
     append.  ``max_tokens`` is how long the caller takes the longest sequence
     to be (default: the capacity, raised by append); it shapes launches, and no
