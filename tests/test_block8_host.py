@@ -192,3 +192,38 @@ def test_decode_selection_asks_for_scores_where_it_keeps_them_in_memory():
     for sequences, blocks in ((2, 513), (32, 513), (33, 8193)):  # 8, 128 and 132 runs
         assert need(_cache(sequences=sequences, blocks=blocks), one, 1) >= sequences * 4 * blocks * 4
     assert need(_cache(sequences=33, blocks=8192), one, 1) == 256
+
+
+@pytest.mark.parametrize("sink,recent", [(1 << 62, 1 << 62), ((1 << 62) + 100, (1 << 62) + 100), ((1 << 63) - 1, 1),
+                                         (1, (1 << 63) - 1), (5, 1), (0, 5)])
+def test_always_chosen_blocks_whose_sum_passes_64_bits(sink, recent):
+    with pytest.raises(ValueError, match="always chosen"):
+        nat.call("uc_block8_select", _cache(), _query(), 4, sink, recent, 1, 16, 16, 1 << 40, None)
+
+
+def _cpu_cache(monkeypatch):
+    """A cache object over CPU tensors, and the calls that it would make."""
+
+    tensors = _tensors()
+    cache = Block8KVCache.__new__(Block8KVCache)
+    cache._set(*tensors, None, (2, 2, 128, 3, 64), None)
+    calls = []
+    monkeypatch.setattr(cache, "_call", lambda entry, *args: calls.append((entry, args)))
+    return cache, calls
+
+
+def test_sparse_attention_numbers_that_do_not_fit_the_c_types(monkeypatch):
+    # ctypes cuts whole numbers to 64 bits without a word
+    cache, calls = _cpu_cache(monkeypatch)
+    q = torch.randn(2, 10, 4, 128, dtype=torch.bfloat16)
+    for kw in (dict(budget=(1 << 64) + 5), dict(budget=1 << 40), dict(budget=(1 << 24) + 1), dict(budget=4, sink=1 << 64),
+               dict(budget=4, sink=-1), dict(budget=4, recent=(1 << 64) + 1), dict(budget=4, recent=0)):
+        with pytest.raises(ValueError):
+            cache.sparse_attention(q, **kw)
+    assert not calls
+    for block in (10, 11, (1 << 64) + 3):
+        _, _, blocks = cache.sparse_attention(q, budget=4, query_block=block)
+        assert blocks.shape == (2, 1, 2, 4)
+    assert [c[1][5] for c in calls if c[0] == "uc_block8_select"] == [10] * 3
+    assert [c[1][4] for c in calls if c[0] == "uc_block8_attn"] == [10] * 3
+    cache.sparse_attention(q[:, :0], budget=4, query_block=1 << 64)

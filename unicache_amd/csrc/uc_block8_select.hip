@@ -562,6 +562,9 @@ extern "C" int uc_block8_select(const uc_block8_cache *cache, const uc_block8_qu
   UC_REQUIRE(budget > 0 && budget <= (1 << 30) / cache->block_tokens, "uc_block8_select: bad budget");
   UC_REQUIRE(sink >= 0 && recent >= 1, "uc_block8_select: sink must not be negative and recent must be positive");
   const int64_t span = q.causal ? ceil_div(int64_t(q.run) - 1, int64_t(c.block)) : 0;
+  // (each by itself first: the sum of large ones would pass 64 bits)
+  UC_REQUIRE(sink <= budget && recent <= budget, "uc_block8_select: budget %lld is less than the blocks always chosen",
+             static_cast<long long>(budget));
   UC_REQUIRE(sink + recent + span <= budget, "uc_block8_select: budget %lld is less than the %lld blocks always chosen",
              static_cast<long long>(budget), static_cast<long long>(sink + recent + span));
   if (q.len == 0) return UC_OK;

@@ -348,13 +348,19 @@ class Block8KVCache:
         budget, query_block, sink, recent = int(budget), int(query_block), int(sink), int(recent)
         if budget <= 0 or query_block <= 0:
             raise ValueError("Block8 sparse attention needs a positive budget and query_block")
+        if budget > (1 << 30) // self.block_tokens:
+            raise ValueError("Block8 sparse attention: a budget of more than 2^30 tokens")
+        if not 0 <= sink <= budget or not 1 <= recent <= budget:
+            raise ValueError("Block8 sparse attention: sink must not be negative, recent must be positive, and neither "
+                             "more than the budget")
         sm_scale = self._scale(sm_scale)
         q, struct, sizes = self._query(query, query_lengths, causal)
-        runs = -(-sizes[0] // query_block)
-        blocks = torch.empty((self.sequences, runs, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)
+        query_block = min(query_block, max(sizes[0], 1))
         # one workspace, for the one call and then for the other
         nbytes = max(_workspace_bytes("uc_block8_select_workspace_bytes", self._sizes, sizes, query_block),
                      _workspace_bytes("uc_block8_attn_workspace_bytes", self._sizes, sizes, budget, query_block))
+        runs = -(-sizes[0] // query_block)
+        blocks = torch.empty((self.sequences, runs, self.num_kv_heads, budget), dtype=torch.int32, device=self.device)
         ws = nat.workspace(self.device, nbytes)
         cache = self._struct()
         self._call("uc_block8_select", cache, struct, budget, sink, recent, query_block, blocks.data_ptr(),
