@@ -227,3 +227,15 @@ def test_sparse_attention_numbers_that_do_not_fit_the_c_types(monkeypatch):
     assert [c[1][5] for c in calls if c[0] == "uc_block8_select"] == [10] * 3
     assert [c[1][4] for c in calls if c[0] == "uc_block8_attn"] == [10] * 3
     cache.sparse_attention(q[:, :0], budget=4, query_block=1 << 64)
+
+
+@pytest.mark.parametrize("heads,lq", [(1 << 62, 4), (1 << 61, 8), (1 << 32, 1 << 20), (1 << 34, 0)])
+def test_query_heads_whose_rows_pass_64_bits(heads, lq):
+    # heads_q x query_len is 2^64: as a 64-bit number no row at all
+    q = _query(heads_q=heads, query_len=lq)
+    with pytest.raises(ValueError, match="query heads|query rows"):
+        nat.call("uc_block8_attn", _cache(), q, None, 0, 0, 0.1, 16, None, 16, 1 << 50, None)
+    with pytest.raises(ValueError, match="query heads|query rows"):
+        nat.call("uc_block8_select", _cache(), q, 4, 1, 1, 1, 16, 16, 1 << 50, None)
+    assert nat.lib().uc_block8_attn_workspace_bytes(_cache(), q, 0, 0) == -1
+    assert nat.lib().uc_block8_select_workspace_bytes(_cache(), q, 1) == -1

@@ -497,6 +497,7 @@ int make_run(const uc_block8_cache *cache, const uc_block8_query *query, int64_t
   UC_REQUIRE(query->heads_q > 0 && query->heads_q % cache->heads_kv == 0,
              "%s: query heads must be a multiple of KV heads", what);
   UC_REQUIRE(query->query_len >= 0 && query->query_len < (1 << 24), "%s: bad query_len", what);
+  UC_REQUIRE(query->heads_q < (1 << 24), "%s: too many query heads", what);  // (the products below stay in 64 bits)
   UC_REQUIRE(query->heads_q / cache->heads_kv * query->query_len < (int64_t(1) << 30), "%s: too many query rows", what);
   UC_REQUIRE(query->max_tokens >= 0, "%s: negative max_tokens", what);
   UC_REQUIRE(query_block > 0, "%s: query_block must be positive", what);
