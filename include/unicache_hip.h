@@ -807,7 +807,7 @@ typedef struct uc_block8_query {
  * see no key, and rows behind a sequence's queries, get 0 and -inf.  Value scales below 2^-88, or below
  * 2^-60 of a larger one that the row has seen (0 for a block of zeros among them), count as that.  With `blocks`
  * (int32 [S, ceil(Lq / query_block), Hkv, budget], ascending, -1 for none) each run of
- * query_block rows sees the listed blocks of its KV head only.  sm_scale > 0.
+ * query_block rows sees the listed blocks of its KV head only.  0 < sm_scale <= 2^127.
  * workspace: uc_block8_attn_workspace_bytes(cache, query, budget, query_block).
  */
 int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_query *query, const int32_t *blocks, int64_t budget,

@@ -239,3 +239,17 @@ def test_query_heads_whose_rows_pass_64_bits(heads, lq):
         nat.call("uc_block8_select", _cache(), q, 4, 1, 1, 1, 16, 16, 1 << 50, None)
     assert nat.lib().uc_block8_attn_workspace_bytes(_cache(), q, 0, 0) == -1
     assert nat.lib().uc_block8_select_workspace_bytes(_cache(), q, 1) == -1
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.4e38, 1e39, 1e-46, 0.0, -1.0, float("nan"), float("inf")])
+def test_logit_scales_that_fp32_does_not_hold(monkeypatch, scale):
+    # times log2(e), as the kernels take them; before any launch
+    with pytest.raises(ValueError, match="sm_scale"):
+        nat.call("uc_block8_attn", _cache(), _query(), None, 0, 0, scale, 16, None, 16, 1 << 40, None)
+    cache, calls = _cpu_cache(monkeypatch)
+    q = torch.randn(2, 3, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="sm_scale"):
+        cache.attention(q, sm_scale=scale)
+    with pytest.raises(ValueError, match="sm_scale"):
+        cache.sparse_attention(q, budget=3, sm_scale=scale)
+    assert not calls

@@ -650,7 +650,8 @@ extern "C" int uc_block8_attn(const uc_block8_cache *cache, const uc_block8_quer
   Plan p;
   if (int rc = check_cache(cache, "uc_block8_attn", c)) return rc;
   if (int rc = make_plan(cache, query, budget, query_block, "uc_block8_attn", q, p)) return rc;
-  UC_REQUIRE(sm_scale > 0.0f && sm_scale < __builtin_huge_valf(), "uc_block8_attn: sm_scale must be positive");
+  // (times log2(e) it stays in fp32's range)
+  UC_REQUIRE(sm_scale > 0.0f && sm_scale <= 0x1p127f, "uc_block8_attn: sm_scale must be positive, and 2^127 at most");
   if (q.len == 0) return UC_OK;
   UC_REQUIRE((blocks != nullptr) == (budget > 0), "uc_block8_attn: a block list and its budget belong together");
   UC_REQUIRE(q.p != nullptr && (reinterpret_cast<uintptr_t>(q.p) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,

@@ -258,9 +258,9 @@ class Block8KVCache:
         return query, struct, (lq, hq, self.max_tokens, dtype, causal)
 
     def _scale(self, sm_scale) -> float:
-        sm_scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else float(sm_scale)
-        if not 0.0 < sm_scale < math.inf:
-            raise ValueError("Block8 attention sm_scale must be positive")
+        sm_scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else ctypes.c_float(float(sm_scale)).value
+        if not 0.0 < sm_scale <= 2.0 ** 127:
+            raise ValueError("Block8 attention sm_scale must be positive, and 2^127 at most (as fp32)")
         return sm_scale
 
     def _attend(self, cache, query, struct, sizes, blocks, budget, query_block, sm_scale, ws, nbytes):
