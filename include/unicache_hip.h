@@ -452,6 +452,7 @@ int uc_kivi_attn_mq_table(const uc_mq_query *queries_host, int n_queries,
  * Merge normalised attention summaries of n_segments disjoint key segments:
  *   lse = logsumexp_s lse_s;  out = sum_s out_s * exp(lse_s - lse)
  * outs[s] are [Lq, Hq, D] of out_dtype (contiguous), lses[s] fp32 [Hq, Lq].
+ * Rows whose lse_s are all -inf (no key anywhere) are weighted by 0: 0 and -inf.
  * `outs` and `lses` are HOST arrays of n_segments device pointers
  * (n_segments <= 16).  out_lse may be NULL.
  * Replaces: merge_attention_summaries (adapters/bagel.py:57-72).

@@ -696,3 +696,23 @@ def test_batched_decode_doubled_split(device):
         out, lse = packed_kivi_attention_summary(caches[i], qs[i])
         assert_close(f32(batch.outputs[i]), f32(out), max_abs=5e-3, mean_abs=2e-4, what=f"item {i}")
         assert_close(f32(batch.lses[i]), f32(lse), max_abs=1e-4, mean_abs=1e-5, what=f"lse {i}")
+
+
+def test_merge_of_rows_that_see_nothing(device):
+    # a row without keys in any segment is 0 and -inf, by either kernel; other rows and NaN are what they were
+    for dtype, d in ((torch.bfloat16, 128), (torch.float32, 64), (torch.float16, 100)):
+        g = torch.Generator().manual_seed(60)
+        outs = [torch.randn(5, 4, d, generator=g).to(dtype).to(device) for _ in range(3)]
+        lses = [torch.randn(4, 5, generator=g).to(device) for _ in range(3)]
+        want, want_lse = merge_attention_summaries(list(zip(outs, lses)))
+        for o, l in zip(outs, lses):
+            o[2], l[:, 2] = 0, -math.inf
+        lses[1][0, 4] = math.nan
+        outs[0][1, 3], lses[0][3, 1] = 0, -math.inf  # one empty segment beside others
+        lses[0][1, 3] = lses[1][1, 3] = -math.inf  # all but one
+        out, lse = merge_attention_summaries(list(zip(outs, lses)))
+        assert not out[2].any() and (lse[:, 2] == -math.inf).all()
+        assert torch.isnan(out[4, 0]).all() and torch.isnan(lse[0, 4])
+        assert torch.equal(out[3, 1], outs[2][3, 1]) and lse[1, 3] == lses[2][1, 3]
+        assert torch.equal(out[0], want[0]) and torch.equal(lse[:, 0], want_lse[:, 0])
+        assert torch.isfinite(out[1]).all()

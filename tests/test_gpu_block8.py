@@ -821,3 +821,27 @@ def test_rows_that_do_not_see_a_tiles_larger_scale(device, lq):
         first = Block8KVCache(*(getattr(cache, n) for n in ("key_code", "value_code", "key_scale", "value_scale", "key_bounds")),
                               torch.full_like(cache.lengths, 32))
         check((out[:, :seen], lse[..., :seen]), reference(first, q[:, :seen], [32], [seen], True, 1 / math.sqrt(128)))
+
+
+@pytest.mark.parametrize("lq", [1, 70])
+def test_mixed_attention_over_empty_segments(device, lq):
+    # no dense rows and 8-bit segments of which none, one or all hold tokens
+    from unicache_amd.adapters.bagel import run_batched_physical_attention, run_fused_mixed_attention
+
+    key, value = dense(1, 100, 4, 128, seed=115)
+    none = key[0, :0]
+    q = queries(1, lq, 28, 128, seed=116)[0]
+
+    def empty():
+        return Block8KVCache.empty(1, 200, 4, 128, device=device)
+
+    for segments in ([empty()], [empty(), empty()], [empty(), empty(), empty()]):
+        out, lse = run_fused_mixed_attention(q, none, none, segments, return_lse=True)
+        assert not out.any() and (lse == -math.inf).all()
+        assert not run_batched_physical_attention(q, none, none, [0, lq], [0, 0], [segments]).any()
+    full = Block8KVCache.from_dense(key, value)
+    want, want_lse = run_fused_mixed_attention(q, none, none, [full], return_lse=True)
+    out, lse = run_fused_mixed_attention(q, none, none, [empty(), full, empty()], return_lse=True)
+    # weights of 0 and 1, and 1 again for the logarithm's half step
+    assert (out.float() - want.float()).abs().max() <= 2.0 ** -8 * want.float().abs().max()
+    assert (lse - want_lse).abs().max() <= 2.0 ** -22 * (1 + want_lse.abs().max())

@@ -16,7 +16,8 @@ def merge_attention_summaries(
     """Merge normalised segment outputs [Lq, Hq, D] by their per-row LSE
     [Hq, Lq] (adapters/bagel.py:57-72): lse = logsumexp_s lse_s and
     out = sum_s out_s * exp(lse_s - lse), accumulated in fp32 and returned in
-    the first output's dtype."""
+    the first output's dtype.  Rows whose LSE is -inf in every summary (no key
+    anywhere) are 0 and -inf."""
 
     if not summaries:
         raise ValueError("At least one attention summary is required")

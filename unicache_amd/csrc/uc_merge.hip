@@ -19,7 +19,8 @@ struct MergeArgs {
 // One workgroup per (query head, query row).  Follows torch.logsumexp: the
 // max is taken over segments and replaced by 0 when infinite, then
 // lse = log(sum exp(l_s - m)) + m; the output accumulates
-// out_s * exp(l_s - lse) in segment order starting from zero.
+// out_s * exp(l_s - lse) in segment order starting from zero.  A row that sees no
+// key in any segment (all l_s and so lse -inf) has weights of 0: exp(-inf + inf) would be NaN.
 template <int OD>
 __global__ __launch_bounds__(128) void lse_merge_kernel(MergeArgs a) {
   const int64_t hq = blockIdx.x / a.Lq, i = blockIdx.x % a.Lq;
@@ -34,7 +35,7 @@ __global__ __launch_bounds__(128) void lse_merge_kernel(MergeArgs a) {
   for (int s = 0; s < a.n; ++s) sum = add_rn(sum, expf(sub_rn(l[s], m)));
   const float total = add_rn(logf(sum), m);
   float w[kMaxSegments];
-  for (int s = 0; s < a.n; ++s) w[s] = expf(sub_rn(l[s], total));
+  for (int s = 0; s < a.n; ++s) w[s] = total == -__builtin_huge_valf() ? 0.0f : expf(sub_rn(l[s], total));
   for (int64_t d = threadIdx.x; d < a.D; d += blockDim.x) {
     const int64_t off = (i * a.Hq + hq) * a.D + d;
     float o = 0.0f;
@@ -56,7 +57,7 @@ __device__ __forceinline__ float merge_weights(const MergeArgs &a, int64_t li, f
   float sum = 0.0f;
   for (int s = 0; s < a.n; ++s) sum = add_rn(sum, expf(sub_rn(l[s], m)));
   const float total = add_rn(logf(sum), m);
-  for (int s = 0; s < a.n; ++s) w[s] = expf(sub_rn(l[s], total));
+  for (int s = 0; s < a.n; ++s) w[s] = total == -__builtin_huge_valf() ? 0.0f : expf(sub_rn(l[s], total));
   return total;
 }
 
