@@ -824,8 +824,8 @@ int64_t uc_block8_attn_workspace_bytes(const uc_block8_cache *cache, const uc_bl
  * row's score of a block is the most that its product with a key inside the
  * block's bounds can be,
  *   q.k <= sum_d max(c_d hi_d, c_d lo_d) * u * step,
- * with the row as whole numbers c = round(q (127 / max|q|)), step = max|q| (1/127), u the
- * bounds' step (the key scale, times 448/127 for e4m3), multiplied in that order in fp32;
+ * with the row as whole numbers c = round(q (127 / max|q|)) (of 2^64 q where max|q| < 2^-100, for fp32's
+ * range), step = max|q| (1/127), u the bounds' step (the key scale, times 448/127 for e4m3), multiplied in that order in fp32;
  * the whole-number sum is exact, so the choice does not depend on how it is computed.
  * A run's score is the largest of its rows in the KV head's query heads (rows holding an infinity or
  * a NaN do not count); a block whose scale is not finite scores highest.  Candidates are the blocks that the run's last row

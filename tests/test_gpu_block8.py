@@ -845,3 +845,32 @@ def test_mixed_attention_over_empty_segments(device, lq):
     # weights of 0 and 1, and 1 again for the logarithm's half step
     assert (out.float() - want.float()).abs().max() <= 2.0 ** -8 * want.float().abs().max()
     assert (lse - want_lse).abs().max() <= 2.0 ** -22 * (1 + want_lse.abs().max())
+
+
+@pytest.mark.parametrize("lq", [1, 5, 40])
+def test_selection_by_very_small_queries(device, lq):
+    # bf16 rows down to subnormals: 127 / max|q| is past fp32's range below 2^-121, the codes are what they are of 2^64 q
+    key, value = dense(1, 64 * 40, 2, 128, seed=62)
+    q = queries(1, lq, 4, 128, seed=63)
+    q[..., ::5] = 0
+    for power in (-90, -110, -122, -126, -131):
+        small = (q.float() * 2.0 ** power).to(torch.bfloat16)
+        for code in CODES:
+            cache = Block8KVCache.from_dense(key * 2.0 ** 100, value, block_tokens=64, code_dtype=code)
+            blocks = cache.sparse_attention(small, budget=6, query_block=lq)[2]
+            x = small[0].float().cpu().numpy()
+            a = np.abs(x).max(axis=-1, keepdims=True)
+            y, b = x * np.float32(2.0 ** 64), a * np.float32(2.0 ** 64)
+            with np.errstate(divide="ignore", invalid="ignore"):
+                c = np.where(b > 0, np.rint(y * (np.float32(127) / b)), 0).astype(np.float64)
+            step = a[..., 0] * np.float32(1.0 / 127.0)
+            for j in range(2):
+                bounds = cache.key_bounds[0, j].cpu().numpy().astype(np.float64)
+                unit = cache.key_scale[0, j].cpu().numpy()
+                if code != torch.int8:
+                    unit = unit * np.float32(448.0 / 127.0)
+                rows, s = c[:, 2 * j:2 * j + 2].reshape(-1, 128), step[:, 2 * j:2 * j + 2].reshape(-1, 1)
+                whole = np.maximum(rows[:, None] * bounds[None, :, 0], rows[:, None] * bounds[None, :, 1]).sum(axis=2)
+                score = (whole.astype(np.float32) * unit * s).max(axis=0)
+                order = sorted(range(40), key=lambda t: (t not in (0, 39), -score[t], t))[:6]
+                assert blocks[0, 0, j].tolist() == sorted(order), (power, code, j)

@@ -1,6 +1,6 @@
 // Block selection for sparse attention over the 8-bit block-scaled cache.
 //
-// A row q as whole numbers c = round(q (127 / max|q|)) can have at most
+// A row q as whole numbers c = round(q (127 / max|q|)) (of 2^64 q for rows below 2^-100) can have at most
 //   I = sum_d max(c_d hi_d, c_d lo_d) = sum_d c+_d hi_d + c-_d lo_d
 // with a key inside a block's bounds (c+ and c- its positive and negative parts), so the scores
 // of all rows and blocks are one int8 matrix product over 2 D, exact in
@@ -72,6 +72,8 @@ __device__ __forceinline__ uint32_t four_codes(const float *x, float inverse) {
 
 // The codes' factor of a row with largest magnitude a, and their step.
 __device__ __forceinline__ float code_factor(float a) { return a > 0.0f ? div_rn(127.0f, a) : 0.0f; }
+// Rows below 2^-100 are multiplied by this first, exactly: 127 / a is past fp32's range below 2^-121.
+__device__ __forceinline__ float code_lift(float a) { return a < 0x1p-100f ? 0x1p64f : 1.0f; }
 __device__ __forceinline__ float code_step(float a) { return mul_rn(a, 1.0f / 127.0f); }
 
 // The bytes of w that are positive, and those that are negative.
@@ -106,9 +108,9 @@ __global__ __launch_bounds__(256) void codes_kernel(Cache c, Run q, int8_t *code
     a = fmaxf(a, __shfl_xor(a, o, kWave));
     bad |= __shfl_xor(bad, o, kWave);
   }
-  const float f = bad ? 0.0f : code_factor(a);
+  const float up = code_lift(a), f = bad ? 0.0f : code_factor(mul_rn(a, up));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
+  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : mul_rn(x[j], up);
   *reinterpret_cast<uint2 *>(codes + row * D + part * 8) = uint2{four_codes(x, f), four_codes(x + 4, f)};
   if (part == 0) steps[row] = bad ? __builtin_nanf("") : code_step(a);
 }
@@ -200,9 +202,9 @@ __device__ __forceinline__ void own_codes(OwnCodes<D> &own, const Run &q, int32_
     a = fmaxf(a, __shfl_xor(a, o, kWave));
     bad |= __shfl_xor(bad, o, kWave);
   }
-  const float f = bad ? 0.0f : code_factor(a);
+  const float up = code_lift(a), f = bad ? 0.0f : code_factor(mul_rn(a, up));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : x[j];
+  for (int j = 0; j < 8; ++j) x[j] = bad ? 0.0f : mul_rn(x[j], up);
   *reinterpret_cast<uint2 *>(&own.codes[r][part * 8]) = uint2{four_codes(x, f), four_codes(x + 4, f)};
   if (part == 0) own.step[r] = bad ? __builtin_nanf("") : code_step(a);
 }
