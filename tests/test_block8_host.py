@@ -253,3 +253,37 @@ def test_logit_scales_that_fp32_does_not_hold(monkeypatch, scale):
     with pytest.raises(ValueError, match="sm_scale"):
         cache.sparse_attention(q, budget=3, sm_scale=scale)
     assert not calls
+
+
+def test_tracked_tensors_are_refused(monkeypatch):
+    # by autograd or by forward mode: a gradient would be lost without a word
+    from torch.autograd import forward_ad
+
+    dense = torch.randn(2, 64, 2, 128, dtype=torch.bfloat16)
+    q = torch.randn(2, 3, 4, 128, dtype=torch.bfloat16)
+    cache, calls = _cpu_cache(monkeypatch)
+    cache.tail = torch.zeros(2, 2, 2, 64, 128, dtype=torch.bfloat16)
+
+    def refuses(track):
+        for call in (lambda t: Block8KVCache.from_dense(t, dense), lambda t: Block8KVCache.from_dense(dense, t),
+                     lambda t: cache.append(t, dense), lambda t: cache.append(dense, t)):
+            with pytest.raises(ValueError, match="gradient"):
+                call(track(dense))
+        for call in (cache.attention, lambda t: cache.sparse_attention(t, budget=3)):
+            with pytest.raises(ValueError, match="gradient"):
+                call(track(q))
+        for i in (2, 3):  # another program's scales
+            tensors = list(_tensors())
+            tensors[i] = track(tensors[i])
+            with pytest.raises(ValueError, match="gradient"):
+                Block8KVCache(*tensors)
+        with pytest.raises(ValueError, match="gradient"):
+            Block8KVCache(*_tensors(), tail=track(cache.tail))
+
+    refuses(lambda t: t.clone().requires_grad_())
+    with forward_ad.dual_level():
+        refuses(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+        cache.attention(q)  # no tangent of its own
+    with torch.no_grad():
+        cache.attention(q.clone().requires_grad_())
+    assert [c[0] for c in calls] == ["uc_block8_attn"] * 2

@@ -22,6 +22,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 from .physical import tensor_bytes
@@ -30,17 +31,25 @@ _CODES = {torch.int8: nat.UC_INT8, torch.float8_e4m3fn: nat.UC_E4M3}
 _HALVES = (torch.bfloat16, torch.float16)
 
 
+def _check_untracked(t: torch.Tensor, what: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which the 8-bit cache does not give; detach it")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} carries a forward-mode gradient, which the 8-bit cache does not give; detach it")
+
+
 def _check_half(t: torch.Tensor, what: str) -> None:
     if t.dtype not in _HALVES:
         raise ValueError(f"{what} must be bf16 or fp16 (got {t.dtype})")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{what} requires a gradient, which the 8-bit cache does not give; detach it")
+    _check_untracked(t, what)
 
 
 def _check_tensor(name, t, dtype, shape, device, align) -> None:
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"Block8 cache {name}: expected contiguous {dtype} {shape}, got {t.dtype} "
                          f"{tuple(t.shape)} strides {tuple(t.stride())}")
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _check_untracked(t, f"Block8 cache {name}")
     if t.device != device:
         raise RuntimeError("Block8 cache received tensors on different devices")
     if t.data_ptr() & align:
@@ -101,8 +110,9 @@ class Block8KVCache:
     result depends on its being right, so a captured graph that appends may
     outgrow it.  Only dequantize returns that many rows.
 
-    Calls enqueue work on the current stream of the cache's device, allocate
-    their outputs and workspaces from torch's allocator and never wait for the GPU."""
+    Tensors that track a gradient, backward or forward, are refused.  Calls
+    enqueue work on the current stream of the cache's device, allocate their
+    outputs and workspaces from torch's allocator and never wait for the GPU."""
 
     def __init__(self, key_code, value_code, key_scale, value_scale, key_bounds, lengths, *, max_tokens=None,
                  tail=None) -> None:
