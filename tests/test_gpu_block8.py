@@ -874,3 +874,30 @@ def test_selection_by_very_small_queries(device, lq):
                 score = (whole.astype(np.float32) * unit * s).max(axis=0)
                 order = sorted(range(40), key=lambda t: (t not in (0, 39), -score[t], t))[:6]
                 assert blocks[0, 0, j].tolist() == sorted(order), (power, code, j)
+
+
+def test_more_sequences_and_heads_than_a_grid_dimension_holds(device):
+    # packed at once, appended, restored: 65,535 is the most in a launch's second dimension
+    s, h = 33000, 2
+    g = torch.Generator(device="cuda").manual_seed(17)
+    key = torch.randn(s, 3, h, 64, generator=g, device="cuda", dtype=torch.bfloat16)
+    value = torch.randn(s, 3, h, 64, generator=g, device="cuda", dtype=torch.bfloat16)
+    lengths = torch.randint(0, 4, (s,), generator=g, device="cuda", dtype=torch.int32)
+    packed = Block8KVCache.from_dense(key, value, lengths=lengths, block_tokens=32, code_dtype=torch.int8)
+    grown = Block8KVCache.empty(s, 3, h, 64, block_tokens=32, code_dtype=torch.int8)
+    grown.append(key, value, counts=lengths)
+    assert torch.equal(packed.lengths, lengths) and torch.equal(grown.lengths, lengths)
+    some = lengths > 0
+    for name in ("key_code", "value_code", "key_scale", "value_scale", "key_bounds"):
+        assert torch.equal(getattr(packed, name)[some], getattr(grown, name)[some]), name
+    small = Block8KVCache.from_dense(key[-9:], value[-9:], lengths=lengths[-9:].clone(), block_tokens=32, code_dtype=torch.int8)
+    want = small.dequantize()
+    for cache in (packed, grown):
+        k, v = cache.dequantize()
+        assert torch.equal(k[-9:, :3], want[0]) and torch.equal(v[-9:, :3], want[1])
+        # codes are within half a step of the rows: amax / 254, and half a step of bf16
+        live = torch.arange(3, device=device) < lengths[:, None]
+        for rows, restored in ((key, k), (value, v)):
+            bound = rows.float().abs().amax(dim=(1, 3), keepdim=True) * (1 / 254 + 2.0 ** -8)
+            assert ((rows.float() - restored[:, :3].float()).abs()[live] <= bound.expand_as(rows)[live]).all()
+            assert not restored[:, :3][~live].any()

@@ -274,13 +274,25 @@ struct Dense {
   }
 };
 
+// A workgroup per block of every (sequence, head): blocks along x, these pairs along y and, past the most
+// that y holds, z.
+constexpr int64_t kGridY = 65535;
+
+dim3 block_grid(const Cache &c, int64_t blocks) {
+  const int64_t pairs = int64_t(c.sequences) * c.heads, y = pairs < kGridY ? pairs : kGridY;
+  return dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(y), static_cast<uint32_t>(ceil_div(pairs, y)));
+}
+
+__device__ __forceinline__ int32_t pair_of_grid() { return blockIdx.z * gridDim.y + blockIdx.y; }
+
 template <int D, int B, int CODE, int IN>
 __global__ __launch_bounds__((Shape<D, B>::kThreads)) void pack_kernel(Cache cache, Dense key, Dense value,
                                                                        int32_t tokens, const int32_t *row_counts,
                                                                        int32_t *lengths, uint16_t *tail) {
   typedef Shape<D, B> S;
   __shared__ Shared<D, B> sh;
-  const int32_t b = blockIdx.x, sequence = blockIdx.y / cache.heads, h = blockIdx.y % cache.heads;
+  const int32_t b = blockIdx.x, pair = pair_of_grid(), sequence = pair / cache.heads, h = pair % cache.heads;
+  if (sequence >= cache.sequences) return;
   int32_t length = row_counts != nullptr ? row_counts[sequence] : tokens;
   length = length < 0 ? 0 : length > tokens ? tokens : length;
   if (b == 0 && h == 0 && threadIdx.x == 0) lengths[sequence] = length;
@@ -300,10 +312,10 @@ __global__ __launch_bounds__((Shape<D, B>::kThreads)) void pack_kernel(Cache cac
       }
     }
   }
-  quantize_block<D, B, CODE, IN>(x, y, rows, cache, int64_t(blockIdx.y) * cache.blocks + b, sh);
+  quantize_block<D, B, CODE, IN>(x, y, rows, cache, int64_t(pair) * cache.blocks + b, sh);
   // the open block's rows, for append
   if (tail != nullptr && rows > 0 && rows < B) {
-    uint16_t *t = tail + int64_t(blockIdx.y) * 2 * B * D;
+    uint16_t *t = tail + int64_t(pair) * 2 * B * D;
 #pragma unroll
     for (int u = 0; u < S::kPer; ++u) {
       const int unit = threadIdx.x + u * S::kThreads, c = unit % S::kChunks, g = unit / S::kChunks;
@@ -402,8 +414,9 @@ __global__ __launch_bounds__((Shape<D, B>::kThreads)) void dequant_kernel(Cache 
                                                                           int32_t tokens) {
   typedef Shape<D, B> S;
   __shared__ uint8_t codes[D * S::kPitch];
-  const int32_t b = blockIdx.x, sequence = blockIdx.y / cache.heads, h = blockIdx.y % cache.heads;
-  const int64_t block_index = int64_t(blockIdx.y) * cache.blocks + b;
+  const int32_t b = blockIdx.x, pair = pair_of_grid(), sequence = pair / cache.heads, h = pair % cache.heads;
+  if (sequence >= cache.sequences) return;
+  const int64_t block_index = int64_t(pair) * cache.blocks + b;
   const int32_t length = cache.length(sequence);
   const bool any = b * B < length;
   const float ks = any ? cache.key_scale[block_index] : 0.0f, vs = any ? cache.value_scale[block_index] : 0.0f;
@@ -507,13 +520,12 @@ extern "C" int uc_block8_pack(const uc_block8_cache *cache, const void *key, int
   if (int rc = check_dense("uc_block8_pack", key, k_ss, k_st, k_sh, "key")) return rc;
   if (int rc = check_dense("uc_block8_pack", value, v_ss, v_st, v_sh, "value")) return rc;
   UC_REQUIRE((reinterpret_cast<uintptr_t>(tail) & 15) == 0, "uc_block8_pack: tail must be 16-byte aligned");
-  UC_REQUIRE(cache->sequences * cache->heads_kv <= 65535, "uc_block8_pack: too many sequences x heads");
   const Dense k{static_cast<const uint16_t *>(key), k_ss, k_st, k_sh};
   const Dense v{static_cast<const uint16_t *>(value), v_ss, v_st, v_sh};
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
     return UC_B8_DISPATCH_BLOCK(cache, [&] {
       return UC_B8_DISPATCH_HALF(in_dtype, IN, [&] {
-        const dim3 grid(static_cast<uint32_t>(ceil_div(tokens, B)), static_cast<uint32_t>(c.sequences * c.heads));
+        const dim3 grid = block_grid(c, ceil_div(tokens, int64_t(B)));
         hipLaunchKernelGGL((pack_kernel<D, B, CODE, IN>), grid, dim3(Shape<D, B>::kThreads), 0, as_stream(stream), c, k,
                            v, static_cast<int32_t>(tokens), row_counts, cache->lengths, static_cast<uint16_t *>(tail));
         return check_launch("uc_block8_pack");
@@ -571,11 +583,10 @@ extern "C" int uc_block8_dequant(const uc_block8_cache *cache, void *out_key, vo
   UC_REQUIRE(out_key && out_value &&
                  ((reinterpret_cast<uintptr_t>(out_key) | reinterpret_cast<uintptr_t>(out_value)) & 15) == 0,
              "uc_block8_dequant: outputs must be 16-byte aligned");
-  UC_REQUIRE(cache->sequences * cache->heads_kv <= 65535, "uc_block8_dequant: too many sequences x heads");
   return UC_B8_DISPATCH(cache, cache->head_dim, [&] {
     return UC_B8_DISPATCH_BLOCK(cache, [&] {
       return UC_B8_DISPATCH_HALF(out_dtype, OUT, [&] {
-        const dim3 grid(static_cast<uint32_t>(ceil_div(tokens, B)), static_cast<uint32_t>(c.sequences * c.heads));
+        const dim3 grid = block_grid(c, ceil_div(tokens, int64_t(B)));
         hipLaunchKernelGGL((dequant_kernel<D, B, CODE, OUT>), grid, dim3(Shape<D, B>::kThreads), 0, as_stream(stream),
                            c, static_cast<uint16_t *>(out_key), static_cast<uint16_t *>(out_value),
                            static_cast<int32_t>(tokens));
