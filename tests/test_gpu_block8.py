@@ -901,3 +901,35 @@ def test_more_sequences_and_heads_than_a_grid_dimension_holds(device):
             bound = rows.float().abs().amax(dim=(1, 3), keepdim=True) * (1 / 254 + 2.0 ** -8)
             assert ((rows.float() - restored[:, :3].float()).abs()[live] <= bound.expand_as(rows)[live]).all()
             assert not restored[:, :3][~live].any()
+
+
+@pytest.mark.parametrize("lq", [1, 3, 100])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_mixed_attention_over_heads_of_64_channels(device, lq, dtype):
+    # dense rows and 8-bit segments, few and many query rows of a KV head
+    from unicache_amd.adapters.bagel import run_batched_physical_attention, run_fused_mixed_attention
+
+    dk, dv = (t[0] for t in dense(1, 130, 4, 64, seed=117, dtype=dtype))
+    bk, bv = dense(1, 200, 4, 64, seed=118, dtype=dtype)
+    block8 = Block8KVCache.from_dense(bk, bv)
+    ek, ev = ((c.float().double() * sc.double().repeat_interleave(64, dim=2)[..., None])[0, :, :200].transpose(0, 1)
+              for c, sc in ((block8.key_code, block8.key_scale),
+                            (block8.value_code.float().transpose(3, 4).reshape(1, 4, -1, 64), block8.value_scale)))
+    q = queries(1, lq, 28, 64, seed=119, dtype=dtype)[0] * 0.3
+    out, lse = run_fused_mixed_attention(q, dk, dv, [block8], return_lse=True)
+    k = torch.cat([dk.double(), ek]).repeat_interleave(7, dim=1)
+    v = torch.cat([dv.double(), ev]).repeat_interleave(7, dim=1)
+    x = torch.einsum("rhd,thd->hrt", q.double(), k) / 8
+    p = torch.softmax(x, dim=-1)
+    want, spread = (torch.einsum("hrt,thd->rhd", p, t) for t in (v, v.abs()))
+    # weights rounded to 16 bits (half a step of the type at most), each summary's output and the merged one
+    # likewise, and fp32 sums: three roundings relative to the sum of magnitudes, and a fourth for their products
+    assert ((out.double() - want).abs() <= 4 * EPS[dtype] * spread + 1e-6).all()
+    # logits: 64 products and as many sums in fp32, over the largest sum of magnitudes; the sums of weights.  Of many
+    # rows the dense kernel sums the weights that it has rounded to the rows' type, (1 + e) p with |e| <= EPS for each:
+    # their sum is within EPS of the exact one, relatively, so its logarithm within -log(1 - EPS) <= 1.01 EPS, and the
+    # merged one, in which the dense part weighs 1 at most, no farther
+    size = (torch.einsum("rhd,thd->hrt", q.double().abs(), k.abs()) / 8).amax(dim=-1)
+    off = 72 * 2.0 ** -24 * size + 400 * 2.0 ** -23 + 64 * 2.0 ** -23 + (1.01 * EPS[dtype] if lq * 7 > 16 else 0)
+    assert ((lse.double() - torch.logsumexp(x, dim=-1)).abs() <= off).all()
+    assert torch.equal(run_batched_physical_attention(q, dk, dv, [0, lq], [0, 130], [[block8]]), out)

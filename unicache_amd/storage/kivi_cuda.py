@@ -608,7 +608,8 @@ def dense_attention_summary(
     """Softmax attention of query [Lq, Hq, D] over dense 16-bit keys/values
     [T, Hkv, D] in one pass of the packed kernels with an empty packed prefix:
     the bf16-only summary (flash_attention_summary, adapters/bagel.py:75-95).
-    (out [Lq, Hq, D] in the query dtype, lse [Hq, Lq])."""
+    More than 16 query rows per KV head of a head_dim below 128 go through copies
+    padded to it.  (out [Lq, Hq, D] in the query dtype, lse [Hq, Lq])."""
 
     if key.shape != value.shape or key.dim() != 3 or query.dim() != 3:
         raise ValueError("Dense attention expects query [Lq, Hq, D] and matching [T, Hkv, D] keys/values")
@@ -636,11 +637,17 @@ def dense_attention_summary(
                  nat.dtype_code(dk.dtype), nat.dtype_code(q.dtype), 1.0 / math.sqrt(d), 0, 0, ws.data_ptr(), ws_bytes,
                  nat.stream(device))
         return out, lse
-    if d != 128:
-        raise ValueError("Dense attention over more than 16 query rows per KV head needs head_dim 128")
-    nat.call("uc_kivi_attn_mq", item, bits, group, hq, hkv, d, lq, nat.dtype_code(q.dtype), nat.dtype_code(dk.dtype),
+    if d > 128:
+        raise ValueError("Dense attention over more than 16 query rows per KV head needs head_dim 128 at most")
+    wide = out
+    if d < 128:  # channels of zeros change no logit
+        q, dk, dv = (torch.nn.functional.pad(t, (0, 128 - d)) for t in (q, dk, dv))
+        wide = torch.empty_like(q)
+        item = nat.KiviItem(None, None, None, None, None, None, dk.data_ptr(), dv.data_ptr(), q.data_ptr(),
+                            wide.data_ptr(), lse.data_ptr(), 0, tokens, 0)
+    nat.call("uc_kivi_attn_mq", item, bits, group, hq, hkv, 128, lq, nat.dtype_code(q.dtype), nat.dtype_code(dk.dtype),
              nat.dtype_code(q.dtype), 1.0 / math.sqrt(d), None, 0, nat.stream(device))  # no workspace
-    return out, lse
+    return (out if wide is out else wide[..., :d].contiguous()), lse
 
 
 def packed_kivi_quantized_attention_summary(
