@@ -716,3 +716,26 @@ def test_merge_of_rows_that_see_nothing(device):
         assert torch.equal(out[3, 1], outs[2][3, 1]) and lse[1, 3] == lses[2][1, 3]
         assert torch.equal(out[0], want[0]) and torch.equal(lse[:, 0], want_lse[:, 0])
         assert torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("n", [16, 17, 31, 32, 50])
+def test_merge_of_many_summaries(device, n):
+    # more than one launch takes, ones without keys among them
+    g = torch.Generator().manual_seed(61)
+    outs = [torch.randn(3, 4, 64, generator=g).to(torch.bfloat16).to(device) for _ in range(n)]
+    lses = [(torch.randn(4, 3, generator=g) * 2).to(device) for _ in range(n)]
+    for s in range(0, n, 7):
+        outs[s][1], lses[s][:, 1] = 0, -math.inf
+    for s in range(n):
+        outs[s][2, 0], lses[s][0, 2] = 0, -math.inf  # a row without keys anywhere
+    out, lse = merge_attention_summaries(list(zip(outs, lses)))
+    l = torch.stack(lses).double()
+    total = torch.logsumexp(l, dim=0)
+    w = torch.exp(l - total.clamp_min(-1e300)).transpose(1, 2)[..., None]
+    parts = w * torch.stack(outs).double()
+    want = parts.sum(dim=0)
+    assert out.dtype == torch.bfloat16 and not out[2, 0].any() and lse[0, 2] == -math.inf
+    # fp32 weights and sums: 2^-24 a term, and the exponents' rounding of logs up to 8, twice; then half a step of bf16
+    assert ((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + (n + 32) * 2.0 ** -23 * parts.abs().sum(dim=0)).all()
+    live = torch.isfinite(total)
+    assert ((lse.double() - total)[live].abs() <= (n + 32) * 2.0 ** -23).all()

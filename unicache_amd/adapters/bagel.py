@@ -9,6 +9,8 @@ import torch
 
 from .. import _native as nat
 
+_MERGED = 16  # summaries of one uc_lse_merge launch
+
 
 def merge_attention_summaries(
     summaries: list[tuple[torch.Tensor, torch.Tensor]],
@@ -24,6 +26,10 @@ def merge_attention_summaries(
     out0 = summaries[0][0]
     device = nat.require_device(*[o for o, _ in summaries], *[l for _, l in summaries],
                                 what="Attention summary merge")
+    if len(summaries) > _MERGED:  # more than one launch takes: the first ones' sum, in fp32, is one of the others
+        wide = [(o.float(), l) for o, l in summaries]
+        merged, total = merge_attention_summaries([merge_attention_summaries(wide[:_MERGED]), *wide[_MERGED:]])
+        return merged.to(out0.dtype), total
     lq, hq, d = map(int, out0.shape)
     same = all(o.dtype == out0.dtype for o, _ in summaries)
     work_dtype = out0.dtype if same else torch.float32
