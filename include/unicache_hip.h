@@ -754,7 +754,7 @@ typedef struct uc_block8_cache {
  * key / value [S, tokens, Hkv, D] (element (s, t, h, d) at s*ss + t*st + h*sh + d;
  * strides multiples of 8, 16-byte aligned) into the cache's blocks
  * 0 .. ceil(tokens / block_tokens) - 1; every code, scale and bound of those
- * blocks is written.  `tail` (may be NULL) receives the dense rows of each
+ * blocks is written.  With tokens 0 nothing is done, lengths included.  `tail` (may be NULL) receives the dense rows of each
  * sequence's partial last block for uc_block8_append: in_dtype
  * [S, Hkv, 2 (key, value), block_tokens, D].  in_dtype: UC_BF16 or UC_FP16.
  */
@@ -805,8 +805,8 @@ typedef struct uc_block8_query {
 /*
  * out = softmax(sm_scale * q K^T) V over each row's visible keys, contiguous
  * [S, Lq, Hq, D] of the query's dtype, and lse [S, Hq, Lq] (natural log, may be NULL).  Rows that
- * see no key, and rows behind a sequence's queries, get 0 and -inf.  Value scales below 2^-88, or below
- * 2^-60 of a larger one that the row has seen (0 for a block of zeros among them), count as that.  With `blocks`
+ * see no key, and rows behind a sequence's queries, get 0 and -inf.  A value scale below 2^-88, or
+ * below 2^-60 of a larger one that the row has seen, counts as that (0 will do for a block of zeros).  With `blocks`
  * (int32 [S, ceil(Lq / query_block), Hkv, budget], ascending, -1 for none) each run of
  * query_block rows sees the listed blocks of its KV head only.  0 < sm_scale <= 2^127.
  * workspace: uc_block8_attn_workspace_bytes(cache, query, budget, query_block).

@@ -7,7 +7,9 @@
 // each, 16 in all at D = 128) while the present one is computed, turn them into
 // fp16 once for all rows, and write the other of two LDS buffers: one barrier a
 // tile.  The scales of a tile are two scalars (its halves may lie in two
-// blocks), so the codes are never multiplied.
+// blocks), so the codes are never multiplied; only in masked tiles of two blocks each row has value scales
+// of its own (3 x 777 padded prompts 47.9 us without that, which lost keys beside very large values, and 48.9).
+// At D = 64 a tile has half the MFMAs and the same weights: 8.8 other vector instructions a MFMA, 3.7 at 128.
 //
 // LDS rows (a key's channels, a channel's keys) hold 16-byte chunks in swizzled
 // order, so that the fragments' 16-byte reads meet no bank twice.  Key tile j's row r is key
@@ -18,7 +20,7 @@
 // (1,024 cycles) and about 235 other vector instructions (the exponentials and what leads to
 // them, the maxima, the casts, the next tile's conversion).  The cores are busy about 47 % of the
 // time, the LDS 35 %, without a bank conflict.  4096 causal queries behind 12k tokens of 32/8 heads:
-// 859 to 899 us by card, 1,071 to 1,120 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
+// 859 to 908 us by card, 1,060 to 1,120 TFLOP/s; a large library product reaches 1,355.  64 rows a wave would halve the
 // LDS reads but need twice the accumulators.  The matrix phases run at raised priority, so that
 // the wave that is in one keeps the cores fed.  Codes converted a tile earlier, beside the Q K
 // products, were 7 % slower.
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(256 * G, 2) void tile_kernel(Cache c, Query q, Plan
     // codes become fp16 beside the second's (after the last tile the present one's again, into the
     // buffer that nobody reads): prefill 4k 859 us, 898 with the weights before the products and codes beside
     // both.  Lists and 64 channels, whose workgroups are few or have half the products, do better the
-    // second way (sparse prefill 164, 167; 3 x 777 tokens 47.3, 48.4).
+    // second way (sparse prefill 164, 167; 3 x 777 tokens 48.9, 49.6).
     constexpr bool kEarly = D == 64 || LISTED;
     if constexpr (kEarly) weigh(1);
     clear<D>(st, ld, w.length);

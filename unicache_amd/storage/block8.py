@@ -102,8 +102,8 @@ class Block8KVCache:
     - ``lengths``     [S] int32, tokens held by each sequence, on the device
 
     D is 64 or 128, B 32, 64 or 128.  Scales are not negative (0 will do for a
-    block of zeros; attention takes value scales below 2^-88, or below 2^-60 of a
-    larger one that the row has seen, for that).  ``tail`` ([S, Hkv, 2, B, D] in the dense
+    block of zeros: to attention a value scale below 2^-88, or below 2^-60 of a
+    larger one that the row has seen, counts as that).  ``tail`` ([S, Hkv, 2, B, D] in the dense
     dtype, or None) holds the dense rows of each sequence's open block for
     append.  ``max_tokens`` is how long the caller takes the longest sequence
     to be (default: the capacity, raised by append); it shapes launches, and no
@@ -352,7 +352,8 @@ class Block8KVCache:
         the one `recent` - 1 before the run's own first block on, and of the
         others those in which a key inside the bounds can have the largest
         product with one of the run's rows (queries rounded to 8 bits; the lower
-        index of equals).  Returns out, lse and the chosen blocks, int32
+        index of equals).  A run takes the time of `budget` blocks, whether its
+        sequence has as many or not.  Returns out, lse and the chosen blocks, int32
         [S, ceil(Lq / query_block), Hkv, budget], ascending, then -1."""
 
         budget, query_block, sink, recent = int(budget), int(query_block), int(sink), int(recent)
