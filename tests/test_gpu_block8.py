@@ -933,3 +933,28 @@ def test_mixed_attention_over_heads_of_64_channels(device, lq, dtype):
     off = 72 * 2.0 ** -24 * size + 400 * 2.0 ** -23 + 64 * 2.0 ** -23 + (1.01 * EPS[dtype] if lq * 7 > 16 else 0)
     assert ((lse.double() - torch.logsumexp(x, dim=-1)).abs() <= off).all()
     assert torch.equal(run_batched_physical_attention(q, dk, dv, [0, lq], [0, 130], [[block8]]), out)
+
+
+@pytest.mark.parametrize("lq", [1, 40])
+def test_a_long_context_of_zeros_before_a_few_values(device, lq):
+    # 2^21 keys in blocks whose value scale is 0, then 64 real ones; zero queries, so that every key weighs the same
+    n, d = (1 << 21) + 64, 64
+    cache = Block8KVCache.empty(1, n, 1, d, block_tokens=64, code_dtype=torch.int8)
+    key, value = dense(1, 64, 1, d, seed=141)
+    last = Block8KVCache.from_dense(key, value, block_tokens=64, code_dtype=torch.int8)
+    for name in ("key_code", "value_code", "key_scale", "value_scale", "key_bounds"):
+        getattr(cache, name).zero_()
+    cache.key_code[:, :, -64:] = last.key_code
+    for name in ("value_code", "key_scale", "value_scale", "key_bounds"):
+        getattr(cache, name)[:, :, -1] = getattr(last, name)[:, :, 0]
+    q = torch.zeros(1, lq, 8, d, dtype=torch.bfloat16, device=device)
+    values = (last.value_code[0, 0, 0].double() * last.value_scale[0, 0, 0].double()).cpu()  # [D, 64]
+    for tokens in (n, n - 64):
+        cache.lengths.fill_(tokens)
+        out, lse = cache.attention(q)
+        # fp32 sums in one lane: 2^15 tiles at most, and 2^10 terms of a tile and of the joins; the logarithm's half steps
+        off = (2 ** 15 + 2 ** 10) * 2.0 ** -24 + 2.0 ** -16
+        assert (lse.double() - math.log(tokens)).abs().max() <= off
+        want, size = (t.sum(dim=1) / tokens if tokens == n else torch.zeros(d).double() for t in (values, values.abs()))
+        err = (out.double().cpu() - want).abs()
+        assert (err <= 2.0 ** -8 * want.abs() + (off + 2.0 ** -11) * size + 448 * 2.0 ** -88).all()
