@@ -842,6 +842,126 @@ int uc_block8_select(const uc_block8_cache *cache, const uc_block8_query *query,
 int64_t uc_block8_select_workspace_bytes(const uc_block8_cache *cache, const uc_block8_query *query,
                                          int64_t query_block);
 
+/*
+ * The paged KV cache: the 16-bit keys and values of up to S sequences over L layers, in
+ * pages of page_tokens tokens from a common pool of P pages (no reference counterpart).
+ * Token t of sequence s is row t % page_tokens of page table[s, t / page_tokens] in
+ * every layer.  Whole pages may be held by several sequences; a sequence's last, partly
+ * filled page (its open page) is held by no other.  Lengths outside [0, M * page_tokens]
+ * read as the nearer end; table entries outside [0, P) are no pages: their tokens are not
+ * seen and not written.  All tensors are contiguous, key and value 16-byte aligned.
+ * granted, references and free_pages (all three or none) are what uc_paged_reserve, uc_paged_reorder and
+ * uc_paged_compact need; the other calls do without.  Bits of free_pages past P are ignored.
+ */
+typedef struct uc_paged_cache {
+  void *key;            /* [L, P, Hkv, page_tokens, D] */
+  void *value;          /* the same */
+  int32_t *table;       /* [S, M] */
+  int32_t *lengths;     /* [S] tokens held */
+  int32_t *granted;     /* [S] tokens that the last uc_paged_reserve added */
+  int32_t *references;  /* [P] sequences that hold a page */
+  uint32_t *free_pages; /* [ceil(P / 32)] bit p % 32 of word p / 32: page p is free (references 0) */
+  int64_t layers;
+  int64_t pages;          /* P */
+  int64_t sequences;      /* S <= 4096 */
+  int64_t sequence_pages; /* M */
+  int64_t heads_kv;
+  int64_t head_dim;       /* 64 or 128 */
+  int32_t page_tokens;    /* 16, 32, 64, 128 or 256 */
+  int32_t dtype;          /* UC_BF16 or UC_FP16 */
+} uc_paged_cache;
+
+/*
+ * out = softmax(sm_scale * q K^T) V of one layer over each row's visible keys, contiguous [S, Lq, Hq, D], and lse
+ * [S, Hq, Lq] (natural log, may be NULL).  query as in uc_block8_attn, its dtype the cache's.  Rows that
+ * see no key, and rows behind a sequence's queries, get 0 and -inf.  What a row does not see never
+ * reaches it, whatever it holds.  0 < sm_scale <= 2^127.
+ * workspace: uc_paged_attn_workspace_bytes(cache, query).
+ */
+int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const uc_block8_query *query, float sm_scale, void *out,
+                  float *lse, void *workspace, int64_t workspace_bytes, uc_stream_t stream);
+
+/* Workspace of uc_paged_attn; -1 for bad arguments. */
+int64_t uc_paged_attn_workspace_bytes(const uc_paged_cache *cache, const uc_block8_query *query);
+
+/*
+ * Rotary positions of several axes: pair i of a head's channels -- (i, i + pairs), or (2 i, 2 i + 1) with
+ * `adjacent` -- turns by positions[axis[i]] * turns[i] revolutions (a product of 64 bits, whole
+ * revolutions taken off): (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  Channels from 2 pairs
+ * on stay.  `inverse` turns back.  An axis outside [0, axes) reads as 0.
+ */
+typedef struct uc_rotary_plan {
+  const double *turns;   /* device [pairs] revolutions per position */
+  const int32_t *axis;   /* device [pairs] */
+  const void *positions; /* device [axes, S, tokens], contiguous; NULL (uc_paged_write only): each token's place in its
+                            sequence, on every axis */
+  int64_t axes;
+  int64_t pairs;         /* a multiple of 8, 2 pairs <= head_dim */
+  int32_t position_bytes; /* 4 or 8: signed whole numbers, below 2^31 in magnitude */
+  int32_t adjacent;
+  int32_t inverse;
+  int32_t reserved;
+} uc_rotary_plan;
+
+/*
+ * Rotate dense rows [S, tokens, heads, head_dim] (element (s, t, h, d) at s*ss + t*st + h*sh + d; strides
+ * multiples of 8, 16-byte aligned) of queries and, with heads_k > 0, keys into contiguous outputs of the same dtype
+ * (UC_BF16 or UC_FP16).  An output may be its input where that is contiguous.  head_dim: a multiple of 16, 512 at most.
+ */
+int uc_rotary(const uc_rotary_plan *plan, int64_t sequences, int64_t tokens, int64_t head_dim, int dtype,
+              const void *query, int64_t q_ss, int64_t q_st, int64_t q_sh, int64_t heads_q, void *out_query,
+              const void *key, int64_t k_ss, int64_t k_st, int64_t k_sh, int64_t heads_k, void *out_key,
+              uc_stream_t stream);
+
+/*
+ * Write new rows into the pages of one layer: sequence s's first counts[s] rows (read into
+ * [0, tokens]; NULL: tokens) of dense key / value [S, tokens, Hkv, D] (as in uc_rotary) are its last
+ * counts[s] tokens, the lengths being raised already (uc_paged_reserve).  With a plan (else NULL) the keys are rotated,
+ * and so are all rows of query [S, tokens, heads_q, D] (may be NULL) into contiguous out_query.
+ */
+int uc_paged_write(const uc_paged_cache *cache, int64_t layer, const void *key, int64_t k_ss, int64_t k_st, int64_t k_sh,
+                   const void *value, int64_t v_ss, int64_t v_st, int64_t v_sh, int64_t tokens, const int32_t *counts,
+                   const uc_rotary_plan *plan, const void *query, int64_t q_ss, int64_t q_st, int64_t q_sh,
+                   int64_t heads_q, void *out_query, uc_stream_t stream);
+
+/*
+ * The first `tokens` rows of every sequence of one layer as contiguous [S, tokens, Hkv, D], zeros behind its length.
+ */
+int uc_paged_dense(const uc_paged_cache *cache, int64_t layer, void *out_key, void *out_value, int64_t tokens,
+                   uc_stream_t stream);
+
+/*
+ * Room for counts[s] more tokens of each sequence (read into [0, tokens]; NULL: tokens): the pages they need are taken
+ * from the free ones, the lowest first, by the sequences in order; lengths are raised, and granted[s] is what sequence s
+ * got, less than asked for where the table or the pool has no more room.
+ */
+int uc_paged_reserve(const uc_paged_cache *cache, int64_t tokens, const int32_t *counts, uc_stream_t stream);
+
+/*
+ * Sequence s becomes what sequence parents[s] was before the call (NULL: itself; outside [0, S): empty), cut to
+ * lengths[s] tokens where that is less (NULL: uncut).  Pages are shared, not copied, but for open pages: of the
+ * sequences that hold one as their open page the lowest keeps it, unless another holds it whole, and the
+ * others get copies of its rows in free pages, the lowest first, in order.  Pages held no more are freed before that.
+ * A sequence for which no free page is left ends with its whole pages.
+ */
+int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *parents, const int32_t *lengths, void *workspace,
+                     int64_t workspace_bytes, uc_stream_t stream);
+
+/* Workspace of uc_paged_reorder; -1 for bad arguments. */
+int64_t uc_paged_reorder_workspace_bytes(const uc_paged_cache *cache);
+
+/*
+ * Each sequence keeps the tokens t with keep[s * keep_stride + t] != 0 (bytes) and those from `tokens` on, in order.
+ * Pages before the first that loses a token stay; the kept rows behind them move into free pages, the
+ * lowest first, by the sequences in order, and the pages they leave are released after that.  Where the free pages
+ * do not suffice, that sequence and those after it keep all their tokens.
+ */
+int uc_paged_compact(const uc_paged_cache *cache, const uint8_t *keep, int64_t keep_stride, int64_t tokens,
+                     void *workspace, int64_t workspace_bytes, uc_stream_t stream);
+
+/* Workspace of uc_paged_compact; -1 for bad arguments. */
+int64_t uc_paged_compact_workspace_bytes(const uc_paged_cache *cache);
+
 #ifdef __cplusplus
 }
 #endif

@@ -138,6 +138,44 @@ class Block8Query(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of ``uc_paged_cache``."""
+
+    _fields_ = [
+        ("key", _P),
+        ("value", _P),
+        ("table", _P),
+        ("lengths", _P),
+        ("granted", _P),
+        ("references", _P),
+        ("free_pages", _P),
+        ("layers", _L),
+        ("pages", _L),
+        ("sequences", _L),
+        ("sequence_pages", _L),
+        ("heads_kv", _L),
+        ("head_dim", _L),
+        ("page_tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class RotaryPlan(ctypes.Structure):
+    """Mirror of ``uc_rotary_plan``."""
+
+    _fields_ = [
+        ("turns", _P),
+        ("axis", _P),
+        ("positions", _P),
+        ("axes", _L),
+        ("pairs", _L),
+        ("position_bytes", ctypes.c_int32),
+        ("adjacent", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "uc_abi_version": (_I, []),
@@ -252,6 +290,26 @@ _SIGNATURES = {
         [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _L, _L, _L, _L, _P, _P, _L, _P],
     ),
     "uc_block8_select_workspace_bytes": (_L, [ctypes.POINTER(Block8Cache), ctypes.POINTER(Block8Query), _L]),
+    "uc_paged_attn": (
+        _I,
+        [ctypes.POINTER(PagedCache), _L, ctypes.POINTER(Block8Query), _F, _P, _P, _P, _L, _P],
+    ),
+    "uc_paged_attn_workspace_bytes": (_L, [ctypes.POINTER(PagedCache), ctypes.POINTER(Block8Query)]),
+    "uc_rotary": (
+        _I,
+        [ctypes.POINTER(RotaryPlan), _L, _L, _L, _I, _P, _L, _L, _L, _L, _P, _P, _L, _L, _L, _L, _P, _P],
+    ),
+    "uc_paged_write": (
+        _I,
+        [ctypes.POINTER(PagedCache), _L, _P, _L, _L, _L, _P, _L, _L, _L, _L, _P, ctypes.POINTER(RotaryPlan),
+         _P, _L, _L, _L, _L, _P, _P],
+    ),
+    "uc_paged_dense": (_I, [ctypes.POINTER(PagedCache), _L, _P, _P, _L, _P]),
+    "uc_paged_reserve": (_I, [ctypes.POINTER(PagedCache), _L, _P, _P]),
+    "uc_paged_reorder": (_I, [ctypes.POINTER(PagedCache), _P, _P, _P, _L, _P]),
+    "uc_paged_reorder_workspace_bytes": (_L, [ctypes.POINTER(PagedCache)]),
+    "uc_paged_compact": (_I, [ctypes.POINTER(PagedCache), _P, _L, _L, _P, _L, _P]),
+    "uc_paged_compact_workspace_bytes": (_L, [ctypes.POINTER(PagedCache)]),
     "uc_workspace_bytes": (_L, [_I, _L, _L, _L, _L, _L]),
     "uc_kivi_decode_workspace_bytes": (_L, [_L, _I, _I, _L, _L, _L, _L, _L, _L]),
     "uc_kivi_decode_preferred_workspace_bytes": (_L, [_L, _I, _I, _L, _L, _L, _L, _L, _L]),
@@ -343,6 +401,16 @@ def stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """An entry point on the current stream of `device`, whatever the current device is."""
+
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream(device))
+
+
 def require_device(*tensors: torch.Tensor | None, what: str) -> torch.device:
     """All given tensors must live on one GPU; returns that device."""
 
@@ -359,6 +427,26 @@ def require_device(*tensors: torch.Tensor | None, what: str) -> torch.device:
     if device is None:
         raise RuntimeError(f"{what} received no GPU tensor")
     return device
+
+
+def rows16(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """A [S, T, H, D] tensor as the kernels can read it -- in place where its
+    channels are adjacent and its rows on 16 bytes, else a contiguous copy --
+    and its first three strides."""
+
+    if t.is_neg():
+        t = t.resolve_neg()
+    aligned = t.data_ptr() % 16 == 0
+    if not (aligned and t.is_contiguous()):
+        a, b, c, d = t.stride()
+        if aligned and d == 1 and not (a % 8 or b % 8 or c % 8):
+            return t, a, b, c
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+    # (a contiguous tensor's strides of dimensions of size 1 may be anything)
+    _, n, h, d = t.shape
+    return t, n * h * d, h * d, d
 
 
 @functools.lru_cache(maxsize=256)

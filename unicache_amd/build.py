@@ -34,6 +34,9 @@ SOURCES = [
     "uc_block8_attn.hip",
     "uc_block8_mq.hip",
     "uc_block8_select.hip",
+    "uc_paged.hip",
+    "uc_paged_attn.hip",
+    "uc_rotary.hip",
 ]
 
 # -ffp-contract=off keeps the pack/dequant arithmetic bit-exact (no implicit

@@ -71,17 +71,6 @@ __device__ __forceinline__ void codes_to_f4(uint32_t w, float *out) {
   out[3] = static_cast<float>(b[1]);
 }
 
-// Inclusive prefix sum over a wave, without LDS.
-__device__ __forceinline__ int32_t wave_prefix(int32_t v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below in the row of 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // rows 1 and 3: the row below's last
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 2 and 3: lane 31
-  return v;
-}
-
 #define UC_B8_DISPATCH(cache, head_dim, ...)                                             \
   [&] {                                                                                  \
     if ((cache)->code_dtype == UC_INT8) {                                                \

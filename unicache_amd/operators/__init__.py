@@ -7,11 +7,13 @@ from .physical import (
     per_kv_head_scores_from_probs,
     per_kv_head_scores_from_qk,
 )
+from .rotary import MultiAxisRotary
 
 __all__ = [
     "H2OPhysicalGQAOperator",
     "KIVIPackedQuantizationOperator",
     "KIVIQuantizationOperator",
+    "MultiAxisRotary",
     "asymmetric_fake_quant",
     "kivi_fake_quant_key",
     "kivi_fake_quant_value",

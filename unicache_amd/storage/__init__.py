@@ -2,6 +2,7 @@
 ``unicache.storage``'s physical layouts and tensor backend)."""
 
 from .block8 import Block8KVCache
+from .paged import PagedKVCache
 from .physical import (
     GQAH2OCache,
     PackedKIVICache,
@@ -19,6 +20,7 @@ __all__ = [
     "TensorCacheStorageBackend",
     "GQAH2OCache",
     "PackedKIVICache",
+    "PagedKVCache",
     "PhysicalLayerCache",
     "PhysicalSegment",
     "gqa_probability_value",

@@ -56,26 +56,6 @@ def _check_tensor(name, t, dtype, shape, device, align) -> None:
         raise ValueError(f"Block8 cache {name} must be {align + 1}-byte aligned")
 
 
-def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
-    """A [S, T, H, D] tensor as the kernels can read it -- in place where its
-    channels are adjacent and its rows on 16 bytes, else a contiguous copy --
-    and its first three strides."""
-
-    if t.is_neg():
-        t = t.resolve_neg()
-    aligned = t.data_ptr() % 16 == 0
-    if not (aligned and t.is_contiguous()):
-        a, b, c, d = t.stride()
-        if aligned and d == 1 and not (a % 8 or b % 8 or c % 8):
-            return t, a, b, c
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-    # (a contiguous tensor's strides of dimensions of size 1 may be anything)
-    _, n, h, d = t.shape
-    return t, n * h * d, h * d, d
-
-
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(entry: str, cache: tuple, query: tuple, *args: int) -> int:
     """Workspace of an entry for the sizes of a cache and a query (the
@@ -221,7 +201,7 @@ class Block8KVCache:
             raise ValueError("Block8 cache lengths must be contiguous int32 [sequences]")
         cache = cls._allocate(s, capacity, h, d, int(block_tokens), code_dtype, key.dtype, device, t)
         if t:
-            (key, *k_strides), (value, *v_strides) = _rows16(key), _rows16(value)
+            (key, *k_strides), (value, *v_strides) = nat.rows16(key), nat.rows16(value)
             cache._call("uc_block8_pack", cache._struct(), key.data_ptr(), *k_strides, value.data_ptr(), *v_strides,
                         nat.dtype_code(key.dtype), t, nat.ptr(lengths), cache.tail.data_ptr())
         else:
@@ -235,15 +215,7 @@ class Block8KVCache:
                                *self._sizes)
 
     def _call(self, entry: str, *args) -> None:
-        """An entry point on the current stream of the cache's device, whatever
-        the current device is."""
-
-        stream = nat.stream(self.device)
-        if self.device.index == torch.cuda.current_device():
-            nat.call(entry, *args, stream)
-        else:
-            with torch.cuda.device(self.device):
-                nat.call(entry, *args, stream)
+        nat.call_on(self.device, entry, *args)
 
     def _query(self, query, query_lengths, causal):
         """The checked query as the kernels read it, its struct, and its sizes."""
@@ -262,7 +234,7 @@ class Block8KVCache:
             raise ValueError("Block8 query_lengths must be contiguous int32 [sequences]")
         if query.device != self.device or (query_lengths is not None and query_lengths.device != self.device):
             raise RuntimeError(f"Block8 attention requires GPU tensors on the cache's device {self.device}")
-        query, a, b, c = _rows16(query)
+        query, a, b, c = nat.rows16(query)
         dtype, causal = nat.dtype_code(query.dtype), 1 if causal else 0
         struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), self.max_tokens, dtype, causal)
         return query, struct, (lq, hq, self.max_tokens, dtype, causal)
@@ -307,7 +279,7 @@ class Block8KVCache:
         n = int(key.shape[1])
         if n == 0:
             return
-        (key, *k_strides), (value, *v_strides) = _rows16(key), _rows16(value)
+        (key, *k_strides), (value, *v_strides) = nat.rows16(key), nat.rows16(value)
         self._call("uc_block8_append", self._struct(), self.tail.data_ptr(), key.data_ptr(), *k_strides,
                    value.data_ptr(), *v_strides, nat.dtype_code(key.dtype), n, nat.ptr(counts))
         self.max_tokens = min(self.max_tokens + n, self.capacity)

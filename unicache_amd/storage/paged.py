@@ -1,0 +1,379 @@
+"""The paged KV cache: 16-bit keys and values of a batch of sequences over all
+layers, in pages of a common pool, the attention that reads them, and the calls that
+grow, fork, cut and thin out sequences.
+
+Beside PackedKIVICache (2/4 bits) and Block8KVCache (8 bits) this is the cache
+of full precision: sequences take pages as they grow, and those that share a
+prefix share its pages.  Tables, lengths, reference counts and free pages live on the device
+and are changed there, so a captured graph can grow and fork sequences.  No reference counterpart:
+UniCache's dense caches are contiguous tensors (storage/tensor_backend.py).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+
+import torch
+from torch.autograd import forward_ad
+
+from .. import _native as nat
+from ..operators.rotary import MultiAxisRotary, check_rows
+from .physical import tensor_bytes
+
+_PAGES = (16, 32, 64, 128, 256)
+_SIZES = "Paged cache supports pages of 16, 32, 64, 128 or 256 tokens and head_dim 64 or 128"
+
+
+def _check_tensor(name, t, dtype, shape, device) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"Paged cache {name}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)} "
+                         f"strides {tuple(t.stride())}")
+    if t.device != device:
+        raise RuntimeError("Paged cache received tensors on different devices")
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(entry: str, cache: tuple, allocator: bool, query: tuple | None) -> int:
+    """Workspace of an entry for the sizes of a cache and a query (the
+    addresses do not matter; they are stood in for by aligned numbers)."""
+
+    c = nat.PagedCache(*[16] * 4, *([16] * 3 if allocator else [None] * 3), *cache)
+    args = [] if query is None else [nat.Block8Query(16, 0, 0, 0, *query[:2], None, *query[2:])]
+    size = int(getattr(nat.lib(), entry)(c, *args))
+    if size < 0:
+        raise ValueError((nat.lib().uc_last_error() or b"").decode(errors="replace") or f"{entry}: bad arguments")
+    return size
+
+
+class PagedKVCache:
+    """16-bit keys and values of S sequences over L layers, in pages of B tokens.
+
+    The tensors, all contiguous:
+
+    - ``key``, ``value``  [L, P, Hkv, B, D] bf16 or fp16: the pool of P pages
+    - ``table``       [S, M] int32: page i of a sequence holds its tokens i * B .. i * B + B - 1; -1 for none
+    - ``lengths``     [S] int32, tokens held by each sequence
+    - ``granted``     [S] int32, tokens that the last reserve gave each sequence
+    - ``references``  [P] int32, how many sequences hold a page
+    - ``free_pages``  [ceil(P / 32)] int32, a bit for each page that none holds
+
+    D is 64 or 128, B 16, 32, 64, 128 or 256, S 4096 at most.  Whole pages may be
+    held by several sequences; a sequence's last, partly filled page (its open page) by
+    no other, which the calls here see to.  Without the last three tensors the
+    cache is another program's: write and attention work, the program keeps the table and lengths itself.
+    Table entries that are no page hide their tokens, and nothing is written there.
+
+    ``max_tokens`` is how long the caller takes the longest sequence to be
+    (default: the capacity; raised by reserve); it shapes launches, and no
+    result depends on its being right.  Only dense returns that many rows.
+
+    Tensors that track a gradient, backward or forward, are refused.  Calls
+    enqueue work on the current stream of the cache's device, allocate their
+    outputs and workspaces from torch's allocator and never wait for the GPU."""
+
+    def __init__(self, key, value, table, lengths, *, granted=None, references=None, free_pages=None,
+                 max_tokens=None) -> None:
+        if key.dim() != 5:
+            raise ValueError("Paged cache expects keys and values [layers, pages, kv_heads, page_tokens, head_dim]")
+        layers, pages, heads, b, d = map(int, key.shape)
+        if key.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("Paged cache keys and values must be bf16 or fp16, both alike")
+        if b not in _PAGES or d not in (64, 128):
+            raise ValueError(_SIZES)
+        if table.dim() != 2:
+            raise ValueError("Paged cache table must be [sequences, pages]")
+        s, m = map(int, table.shape)
+        if not (layers and pages and heads and s and m):
+            raise ValueError("Paged cache needs a layer, a page, a KV head, a sequence and a page per sequence at least")
+        device = key.device
+        for name, t, shape in (("key", key, tuple(key.shape)), ("value", value, tuple(key.shape))):
+            _check_tensor(name, t, key.dtype, shape, device)
+            check_rows(t, f"Paged cache {name}")
+            if t.data_ptr() & 15:
+                raise ValueError(f"Paged cache {name} must be 16-byte aligned")
+        _check_tensor("table", table, torch.int32, (s, m), device)
+        _check_tensor("lengths", lengths, torch.int32, (s,), device)
+        kept = (granted, references, free_pages)
+        if any(t is None for t in kept) != all(t is None for t in kept):
+            raise ValueError("Paged cache granted, references and free_pages belong together")
+        if references is not None:
+            _check_tensor("granted", granted, torch.int32, (s,), device)
+            _check_tensor("references", references, torch.int32, (pages,), device)
+            _check_tensor("free_pages", free_pages, torch.int32, (-(-pages // 32),), device)
+        if device.type != "cuda":
+            raise RuntimeError(f"Paged cache requires GPU tensors (got {device})")
+        if max_tokens is not None and int(max_tokens) < 0:
+            raise ValueError("Paged cache max_tokens must not be negative")
+        self._set(key, value, table, lengths, granted, references, free_pages, max_tokens)
+
+    def _set(self, key, value, table, lengths, granted, references, free_pages, max_tokens) -> None:
+        self.key, self.value, self.table, self.lengths = key, value, table, lengths
+        self.granted, self.references, self.free_pages = granted, references, free_pages
+        self.layers, self.pages, self.num_kv_heads, self.page_tokens, self.head_dim = map(int, key.shape)
+        self.sequences, self.sequence_pages = map(int, table.shape)
+        self.dtype, self.device = key.dtype, key.device
+        self._sizes = (self.layers, self.pages, self.sequences, self.sequence_pages, self.num_kv_heads, self.head_dim,
+                       self.page_tokens, nat.dtype_code(key.dtype))
+        self.max_tokens = self.capacity if max_tokens is None else min(int(max_tokens), self.capacity)
+        # (refuses sizes that the kernels do not take)
+        _workspace_bytes("uc_paged_attn_workspace_bytes", self._sizes, False,
+                         (0, self.num_kv_heads, 0, self._sizes[-1], 0))
+
+    @property
+    def capacity(self) -> int:
+        """Tokens that the table has room for in every sequence (the pool may have fewer)."""
+
+        return self.sequence_pages * self.page_tokens
+
+    @classmethod
+    def empty(cls, sequences: int, pages: int, num_kv_heads: int, head_dim: int, *, layers: int = 1,
+              page_tokens: int = 64, sequence_pages: int | None = None, dtype: torch.dtype = torch.bfloat16,
+              device: torch.device | str = "cuda") -> "PagedKVCache":
+        """A cache without tokens over a pool of `pages` free pages; a sequence
+        takes `sequence_pages` of them at most (default: all)."""
+
+        s, p, h, d, n, b = map(int, (sequences, pages, num_kv_heads, head_dim, layers, page_tokens))
+        m = p if sequence_pages is None else int(sequence_pages)
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"Paged cache requires a GPU (got {device})")
+        if b not in _PAGES or d not in (64, 128):
+            raise ValueError(_SIZES)
+        if min(s, p, h, n, m) <= 0:
+            raise ValueError("Paged cache needs a layer, a page, a KV head, a sequence and a page per sequence at least")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("Paged cache keys and values must be bf16 or fp16, both alike")
+        cache = cls.__new__(cls)
+        key = torch.empty((n, p, h, b, d), dtype=dtype, device=device)
+        counts = [torch.zeros(size, dtype=torch.int32, device=device) for size in (s, s, p)]
+        words = torch.full((-(-p // 32),), -1, dtype=torch.int32, device=device)
+        if p % 32:
+            words[-1:].fill_((1 << p % 32) - 1)
+        cache._set(key, torch.empty_like(key), torch.full((s, m), -1, dtype=torch.int32, device=device), counts[0],
+                   counts[1], counts[2], words, 0)
+        return cache
+
+    def layer(self, index: int) -> "PagedKVCache":
+        """One layer as a cache of its own over the same tensors: to read and write, not to grow or fork."""
+
+        index = self._layer(index)
+        view = type(self).__new__(type(self))
+        view._set(self.key[index:index + 1], self.value[index:index + 1], self.table, self.lengths, None, None, None,
+                  self.max_tokens)
+        return view
+
+    # ------------------------------------------------------------- internals --
+    def _layer(self, layer) -> int:
+        layer = int(layer)
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"Paged cache has layers 0 .. {self.layers - 1} (got {layer})")
+        return layer
+
+    def _struct(self) -> "nat.PagedCache":
+        return nat.PagedCache(self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(),
+                              self.lengths.data_ptr(), nat.ptr(self.granted), nat.ptr(self.references),
+                              nat.ptr(self.free_pages), *self._sizes)
+
+    def _numbers(self, t: torch.Tensor, what: str) -> torch.Tensor:
+        """int32 of each sequence, on the cache's device."""
+
+        if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != (self.sequences,):
+            raise ValueError(f"Paged cache {what} must be contiguous int32 [{self.sequences}]")
+        if t.device != self.device:
+            raise RuntimeError(f"Paged cache {what} must be on the cache's device {self.device}")
+        return t
+
+    def _rows(self, t: torch.Tensor, what: str, heads: int | None = None) -> torch.Tensor:
+        """Checked dense rows [S, n, H, D]."""
+
+        if t.dim() == 3 and self.sequences == 1:
+            t = t.unsqueeze(0)
+        if (t.dim() != 4 or t.shape[0] != self.sequences or t.shape[3] != self.head_dim or not t.shape[2]
+                or (heads is not None and t.shape[2] != heads)):
+            raise ValueError(f"Paged cache {what}: expected [{self.sequences}, tokens, {heads or 'heads'}, "
+                             f"{self.head_dim}], got {tuple(t.shape)}")
+        if t.dtype != self.dtype:
+            raise ValueError(f"Paged cache {what} must have the cache's dtype {self.dtype} (got {t.dtype})")
+        check_rows(t, f"Paged cache {what}")
+        if t.device != self.device:
+            raise RuntimeError(f"Paged cache {what} must be on the cache's device {self.device}")
+        return t
+
+    def _allocator(self, what: str) -> None:
+        if self.references is None:
+            raise RuntimeError(f"Paged cache {what} needs the pool's references and free pages")
+
+    # ------------------------------------------------------------------ pages --
+    def reserve(self, tokens: int, *, counts: torch.Tensor | None = None) -> torch.Tensor:
+        """Room for `tokens` more tokens of every sequence, or the first counts[s] (int32 on
+        the device) of sequence s, whose rows write then takes; all layers at once.
+
+        Free pages go out lowest first, to the sequences in order, and `lengths` advances, on
+        the device, which alone knows how far the pool goes: `granted`, which is returned, is what each
+        sequence got."""
+
+        self._allocator("reserve")
+        tokens = int(tokens)
+        if tokens < 0 or tokens >= 1 << 30:
+            raise ValueError("Paged cache reserve: tokens must not be negative, and below 2^30")
+        if counts is not None:
+            counts = self._numbers(counts, "counts")
+        nat.call_on(self.device, "uc_paged_reserve", self._struct(), tokens, nat.ptr(counts))
+        self.max_tokens = min(self.max_tokens + tokens, self.capacity)
+        return self.granted
+
+    def reorder(self, parents: torch.Tensor, *, lengths: torch.Tensor | None = None) -> None:
+        """Sequence s becomes what sequence parents[s] (int32 on the device) was before the
+        call, and empty where that is no sequence (-1): forks, the beams of a search, and freeing
+        in one call.  With `lengths` it keeps its first lengths[s] tokens at most.
+
+        Whole pages are shared.  Of the sequences with the same open page the lowest keeps it
+        (unless another holds it whole), the others get copies of its rows in free pages, taken after the
+        pages that nobody holds any more are freed; where none is left, a sequence ends with its whole pages."""
+
+        self._allocator("reorder")
+        parents = self._numbers(parents, "parents")
+        if lengths is not None:
+            lengths = self._numbers(lengths, "lengths")
+        self._reorder(parents, lengths)
+
+    def truncate(self, lengths: torch.Tensor) -> None:
+        """Each sequence keeps its first lengths[s] tokens (int32 on the device) at most, as after
+        drafted tokens were refused; pages behind are released.  (An open page that was shared is copied, as in reorder.)"""
+
+        self._allocator("truncate")
+        self._reorder(None, self._numbers(lengths, "lengths"))
+
+    def _reorder(self, parents, lengths) -> None:
+        nbytes = _workspace_bytes("uc_paged_reorder_workspace_bytes", self._sizes, True, None)
+        ws = nat.workspace(self.device, nbytes)
+        nat.call_on(self.device, "uc_paged_reorder", self._struct(), nat.ptr(parents), nat.ptr(lengths), ws.data_ptr(),
+                    nbytes)
+
+    def compact(self, keep: torch.Tensor) -> None:
+        """Each sequence keeps, in order, the tokens t with keep[s, t] (bool or uint8 [S, T], rows may
+        be strided) and those from T on: the eviction of TensorCacheStorageBackend.compact over pages, for all layers.
+
+        Pages before the first that loses a token stay, shared or not.  The kept rows behind them move into free
+        pages, the lowest first, to the sequences in order, and then the pages they leave are
+        released.  Where the free pages do not suffice, that sequence and those after it keep all their tokens."""
+
+        self._allocator("compact")
+        if keep.dtype not in (torch.bool, torch.uint8) or keep.dim() != 2 or keep.shape[0] != self.sequences:
+            raise ValueError(f"Paged cache keep must be bool or uint8 [{self.sequences}, tokens]")
+        if keep.device != self.device:
+            raise RuntimeError(f"Paged cache keep must be on the cache's device {self.device}")
+        if keep.shape[1] and keep.stride(1) != 1:
+            keep = keep.contiguous()
+        nbytes = _workspace_bytes("uc_paged_compact_workspace_bytes", self._sizes, True, None)
+        ws = nat.workspace(self.device, nbytes)
+        nat.call_on(self.device, "uc_paged_compact", self._struct(), keep.data_ptr(), keep.stride(0),
+                    int(keep.shape[1]), ws.data_ptr(), nbytes)
+
+    # ------------------------------------------------------------------ calls --
+    def write(self, key: torch.Tensor, value: torch.Tensor, *, layer: int = 0, query: torch.Tensor | None = None,
+              rotary: MultiAxisRotary | None = None, positions: torch.Tensor | None = None,
+              counts: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Write dense rows [S, n, Hkv, D] ([n, Hkv, D] for one sequence) into a layer's
+        pages, as the last granted[s] tokens of each sequence after reserve (or the last counts[s], int32
+        on the device; without granted all n): row i of counts[s] is token lengths[s] - counts[s] + i.
+
+        With `rotary` the keys are turned on the way, and so are all rows of `query` [S, n, Hq, D], which are returned;
+        `positions` [axes, S, n] (int32 or int64) default to each token's place in its sequence."""
+
+        layer = self._layer(layer)
+        key = self._rows(key, "keys", self.num_kv_heads)
+        value = self._rows(value, "values", self.num_kv_heads)
+        if key.shape != value.shape:
+            raise ValueError("Paged cache write expects keys and values of one shape")
+        n = int(key.shape[1])
+        counts = self.granted if counts is None else self._numbers(counts, "counts")
+        if rotary is None and (query is not None or positions is not None):
+            raise ValueError("Paged cache write takes queries and positions with a rotary")
+        plan = held = out = None
+        q = [None, 0, 0, 0, 0, None]
+        flat = query is not None and query.dim() == 3
+        if rotary is not None:
+            if rotary.head_dim != self.head_dim:
+                raise ValueError(f"Paged cache write: the rotary is for head_dim {rotary.head_dim}")
+            if rotary.device != self.device:
+                raise RuntimeError(f"Paged cache write: the rotary must be on the cache's device {self.device}")
+            plan, held = rotary.plan(positions, self.sequences, n)
+            if query is not None:
+                query = self._rows(query, "queries")
+                if query.shape[1] != n:
+                    raise ValueError("Paged cache write expects as many queries as keys")
+                query, *strides = nat.rows16(query)
+                out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
+                q = [query.data_ptr(), *strides, int(query.shape[2]), out.data_ptr()]
+        (key, *k_strides), (value, *v_strides) = nat.rows16(key), nat.rows16(value)
+        if n:
+            nat.call_on(self.device, "uc_paged_write", self._struct(), layer, key.data_ptr(), *k_strides,
+                        value.data_ptr(), *v_strides, n, nat.ptr(counts),
+                        None if plan is None else ctypes.byref(plan), *q)
+        return out[0] if flat else out
+
+    def attention(self, query: torch.Tensor, *, layer: int = 0, query_lengths: torch.Tensor | None = None,
+                  causal: bool = False, sm_scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """softmax(sm_scale * q K^T) V over one layer (default scale 1/sqrt(D)): query [S, Lq, Hq, D]
+        ([Lq, Hq, D] for one sequence) of the cache's dtype -> out [S, Lq, Hq, D] and the natural-log
+        LSE [S, Hq, Lq] in fp32.
+
+        Sequence s has query_lengths[s] queries (int32 on the device; default
+        Lq).  With causal=True they are its last tokens: row i sees the keys up
+        to lengths[s] - query_lengths[s] + i.  Rows that see no key, and rows
+        behind a sequence's queries, get 0 and -inf.  Keys and values that a row does not
+        see never reach it, whatever they hold."""
+
+        layer = self._layer(layer)
+        sm_scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else ctypes.c_float(float(sm_scale)).value
+        if not 0.0 < sm_scale <= 2.0 ** 127:
+            raise ValueError("Paged attention sm_scale must be positive, and 2^127 at most (as fp32)")
+        flat = query.dim() == 3
+        query = self._rows(query, "queries")
+        lq, hq = int(query.shape[1]), int(query.shape[2])
+        if hq % self.num_kv_heads:
+            raise ValueError("Query heads must be divisible by the cache's KV heads")
+        if query_lengths is not None:
+            query_lengths = self._numbers(query_lengths, "query_lengths")
+        query, a, b, c = nat.rows16(query)
+        sizes = (lq, hq, self.max_tokens, self._sizes[-1], 1 if causal else 0)
+        nbytes = _workspace_bytes("uc_paged_attn_workspace_bytes", self._sizes, False, sizes)
+        ws = nat.workspace(self.device, nbytes)
+        out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
+        lse = torch.empty((self.sequences, hq, lq), dtype=torch.float32, device=self.device)
+        struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), *sizes[2:])
+        nat.call_on(self.device, "uc_paged_attn", self._struct(), layer, struct, sm_scale, out.data_ptr(),
+                    lse.data_ptr(), ws.data_ptr(), nbytes)
+        return (out[0], lse[0]) if flat else (out, lse)
+
+    def dense(self, *, layer: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of one layer as dense [S, max_tokens, Hkv, D] rows, zeros behind each sequence's length."""
+
+        layer = self._layer(layer)
+        shape = (self.sequences, self.max_tokens, self.num_kv_heads, self.head_dim)
+        key = torch.empty(shape, dtype=self.dtype, device=self.device)
+        value = torch.empty_like(key)
+        if self.max_tokens:
+            nat.call_on(self.device, "uc_paged_dense", self._struct(), layer, key.data_ptr(), value.data_ptr(),
+                        self.max_tokens)
+        return key, value
+
+    # ------------------------------------------------------------------ bytes --
+    @property
+    def resident_bytes(self) -> int:
+        return sum(self.byte_breakdown.values())
+
+    @property
+    def byte_breakdown(self) -> dict[str, int]:
+        return {
+            "payload_bytes": tensor_bytes(self.key) + tensor_bytes(self.value),
+            "scale_bytes": 0,
+            "minimum_bytes": 0,
+            "residual_bytes": 0,
+            "indices_bytes": sum(tensor_bytes(t) for t in (self.table, self.lengths, self.granted, self.references,
+                                                           self.free_pages) if t is not None),
+            "score_bytes": 0,
+        }
