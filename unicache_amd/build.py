@@ -36,6 +36,7 @@ SOURCES = [
     "uc_block8_select.hip",
     "uc_paged.hip",
     "uc_paged_attn.hip",
+    "uc_paged_tiles.hip",
     "uc_rotary.hip",
 ]
 

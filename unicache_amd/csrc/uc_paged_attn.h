@@ -29,10 +29,19 @@ struct Query {
   }
 };
 
+constexpr int kTileRows = 128;            // rows of a unit of many (uc_paged_tiles.hip)
+
 struct Plan {
-  int32_t rows, groups;  // rows of a unit, and units of a (sequence, KV head)
-  int32_t workgroups;    // that share all steps
+  int32_t rows, groups;         // rows of a unit, and units of a (sequence, KV head)
+  int32_t workgroups;           // few rows: workgroups that share all steps; 0: many rows
+  int32_t splits, split_tiles;  // many rows: splits of a unit's keys, and the 64-key tiles of one
 };
+
+// Tiles of one split: the host's figure, or more where a sequence is longer than it expected.
+__device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) {
+  const int32_t least = (tiles + p.splits - 1) / p.splits;
+  return least > p.split_tiles ? least : p.split_tiles;
+}
 
 // The rows of a unit: row r is query token r / group of head h * group + r % group.
 struct Rows {
@@ -131,11 +140,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, V2{static_cast<T>(a), static_cast<T>(b)});
 }
 
+// Bits of the halves of w that are no finite numbers.
+template <int DT>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t e = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
+  return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == e << 16 ? 0xffff0000u : 0u);
+}
+
 // The lower or the upper halves of two dwords as one.
 template <bool UPPER>
 __device__ __forceinline__ uint32_t halves_of(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, UPPER ? 0x07060302u : 0x05040100u);
 }
+
+// uc_paged_tiles.hip: many query rows.
+int64_t tile_workgroups(int64_t lists, int64_t groups);
+int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, const Query &q, const Plan &p, uint16_t *out,
+                 float *lse, float *part, float *stat, hipStream_t stream);
 
 }  // namespace pg
 }  // namespace uc

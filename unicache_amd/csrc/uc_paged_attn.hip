@@ -81,13 +81,6 @@ __device__ __forceinline__ typename Half<DT>::V8 value_fragment(const Raw<D> &ra
   return __builtin_bit_cast(typename Half<DT>::V8, uint4{w[0], w[1], w[2], w[3]});
 }
 
-// Bits of the halves of w that are no finite numbers.
-template <int DT>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  constexpr uint32_t e = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == e << 16 ? 0xffff0000u : 0u);
-}
-
 // State of 16 query rows in one wave: the lane's row is lane % 16, its channels of o[n][i] are
 // D/4 (lane / 16) + D/16 i + n.
 template <int D>
@@ -439,6 +432,14 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
   const int32_t full = q.len * q.group, sh = index / full, s = sh / c.heads;
   x.r = index - sh * full;
   const int32_t group = p.groups == 1 ? 0 : x.r / p.rows, each = c.heads * p.groups;
+  const int32_t unit = sh * p.groups + group;
+  if (p.workgroups == 0) {
+    x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, c.length(s), q.count(s));
+    const int32_t tiles = (x.w.end_last + 63) / 64, per = split_tiles_of(p, tiles);
+    x.first = unit * p.splits;
+    x.count = tiles == 0 ? 0 : (tiles + per - 1) / per;
+    return x;
+  }
   int32_t total = 0, before = 0, mine = 0;
   for (int32_t s0 = 0; s0 < c.sequences; s0 += 64) {
     const int32_t i = s0 + (threadIdx.x & 63);
@@ -452,7 +453,7 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
     total += __builtin_amdgcn_readlane(sum, 63);
   }
   x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, c.length(s), q.count(s));
-  const int32_t unit = sh * p.groups + group, per = per_of(p, total * each);
+  const int32_t per = per_of(p, total * each);
   const int32_t start = before * each + (unit - s * each) * mine;
   x.first = mine == 0 ? 0 : start / per + unit;
   x.count = mine == 0 ? 0 : (start + mine - 1) / per + unit - x.first + 1;
@@ -516,7 +517,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(Cache c, Query q, Plan p,
                                                        const float *part, const float *stat) {
   const int32_t index = blockIdx.x * 16 + (threadIdx.x >> 4), last = rows - 1;
   const Parts x = parts_of(c, q, p, index < rows ? index : last);  // (whole waves: they sum up the lengths)
-  if (index >= rows || x.count == 1) return;
+  if (index >= rows || (x.count == 1 && p.workgroups > 0)) return;
   const Sum<D> t = sum_parts<D, 1>(p, x, 0, part, stat);
   store_row<D, DT>(q, x.w, x.r, (threadIdx.x & 15) * (D / 16), t.o, t.m, t.l, out, lse);
 }
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
   constexpr int kC = D / 16;
   __shared__ float sh_o[16][D], sh_l[16];
   const Parts x = parts_of(c, q, p, blockIdx.x);
-  if (x.count == 1) return;
+  if (x.count == 1 && p.workgroups > 0) return;
   const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
   Sum<D> t = sum_parts<D, 16>(p, x, group, part, stat);
 #pragma unroll
@@ -544,6 +545,25 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
   store_row<D, DT>(q, x.w, x.r, lane * kC, t.o, t.m, t.l, out, lse);
 }
 
+// Splits of 128-row workgroups: the least time in tiles.  Two workgroups share a CU, and up to one a CU takes 0.65
+// of the time a tile.  The launch that joins splits takes two tiles and 0.006 for each part of a workgroup.
+void split_tiles(int64_t units, int64_t tiles, Plan &p) {
+  int64_t best = 1;
+  double least = 1e300;
+  const int64_t most = ceil_div(tiles, 4) < 64 ? ceil_div(tiles, 4) : 64;
+  for (int64_t k = 1; k <= most; ++k) {
+    const double join = k > 1 ? 2.0 + 0.006 * static_cast<double>(units * k) : 0.0;
+    const double rounds = units * k <= 256 ? 0.65 : static_cast<double>(ceil_div(units * k, int64_t(512)));
+    const double time = rounds * static_cast<double>(ceil_div(tiles, k)) + join;
+    if (time < least) {
+      least = time;
+      best = k;
+    }
+  }
+  p.split_tiles = static_cast<int32_t>(ceil_div(tiles, best));
+  p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
+}
+
 constexpr int64_t kShare = 512;  // workgroups that share the steps: two a CU
 
 int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query *query, const char *what, Query &q, Plan &p) {
@@ -557,7 +577,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
             query->causal != 0, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kTileRows;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
   const int64_t capacity = c.capacity(), keys = query->max_tokens < capacity ? query->max_tokens : capacity;
   // a launch has less than 2^32 threads, and 32-bit counts of rows and steps
@@ -566,13 +586,23 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
              "%s: too many query rows", what);
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   UC_REQUIRE(units * ceil_div(capacity, int64_t(kStep)) < (1 << 30), "%s: too many keys in all", what);
+  p.workgroups = 0;
+  p.splits = 1;
+  p.split_tiles = 0;
+  if (p.rows == kTileRows) {
+    split_tiles(units, keys > 0 ? ceil_div(keys, int64_t(64)) : 1, p);
+    UC_REQUIRE(tile_workgroups(cache->sequences * cache->heads_kv * p.splits, p.groups) < (1 << 24), "%s: too many query rows",
+               what);
+    return UC_OK;
+  }
   const int64_t steps = units * ceil_div(keys, int64_t(kStep));
   p.workgroups = static_cast<int32_t>(steps < kShare ? (steps > 0 ? steps : 1) : kShare);
   return UC_OK;
 }
 
 int64_t part_rows(const uc_paged_cache *cache, const Plan &p) {
-  return (cache->sequences * cache->heads_kv * p.groups + p.workgroups) * p.rows;
+  const int64_t units = cache->sequences * cache->heads_kv * p.groups;
+  return p.workgroups > 0 ? (units + p.workgroups) * p.rows : p.splits > 1 ? units * p.splits * p.rows : 0;
 }
 
 }  // namespace
@@ -605,22 +635,25 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
              "%s: query must be 16-byte aligned with strides that are multiples of 8", what);
   UC_REQUIRE(out != nullptr && (reinterpret_cast<uintptr_t>(out) & 15) == 0, "%s: out must be 16-byte aligned", what);
   const int64_t rows = part_rows(cache, p);
-  UC_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
-                 workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float)),
+  UC_REQUIRE(rows == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
+                           workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "%s: workspace too small", what);
   q.scale = sm_scale * kLog2e;
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);
   // parts of a row, if all sequences were of the expected length
-  const bool few = ceil_div(p.workgroups, units) <= 8;
+  const bool few = (p.workgroups > 0 ? ceil_div(p.workgroups, units) : p.splits) <= 8;
   auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
     auto rows_launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(p.workgroups)), dim3(256), 0, as_stream(stream), c, q, p,
                          static_cast<uint16_t *>(out), lse, part, stat);
     };
-    if (p.rows == 16) {
+    if (p.rows == kTileRows) {
+      const int rc = launch_tiles(what, DT, D, c, q, p, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
+      if (rc != UC_OK || p.splits == 1) return rc;
+    } else if (p.rows == 16) {
       rows_launch(rows_kernel<D, DT, 1>);
     } else if (p.rows == 32) {
       rows_launch(rows_kernel<D, DT, 2>);

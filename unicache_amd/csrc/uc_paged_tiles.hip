@@ -1,0 +1,429 @@
+// Attention over the paged 16-bit cache for many query rows: a prompt's chunk, an image's queries.
+// The mathematics is that of uc_paged_attn.hip, but for the weights, which go into the products as one 16-bit number
+// (half a step, 2^-9 in bf16, 2^-12 in fp16, of each; over many keys that is as much as the output's own
+// rounding): the matrix cores, not the loads, are what such calls wait for.
+//
+// A workgroup owns 128 query rows of one KV head, 32 per wave, and walks 64-key tiles.  Its 256 threads
+// read the next tile into registers while the present one is computed, and write the other of two LDS
+// buffers: one barrier a tile.  Keys lie there as rows, values channel by channel, as the products read them: a
+// thread takes D/32 channels of eight keys and turns them round with one byte permutation per pair of keys
+// and channel.  16 keys lie in one page, so each load of a wave has its page in scalar registers.
+//
+// LDS rows (a key's channels, a channel's keys) hold 16-byte chunks in swizzled order, so that the fragments'
+// 16-byte reads meet no bank twice.  Key tile j's row r is key 32 (j / 2) + 8 (r / 4) + 4 (j % 2) + r % 4, so that a lane's
+// logits of two tiles are eight consecutive keys of its query row: the operand of O^T = V^T P^T.
+#include "uc_paged_attn.h"
+
+#include <type_traits>
+
+namespace uc {
+namespace pg {
+namespace {
+
+constexpr int kKeys = 64;  // of a tile
+
+template <int D>
+struct Tile {
+  static constexpr int kKeyRow = D * 2, kValueRow = kKeys * 2;      // bytes
+  static constexpr int kKeyBytes = kKeys * kKeyRow, kValueBytes = D * kValueRow;
+  static constexpr int kBytes = kKeyBytes + kValueBytes;            // of one buffer
+  static constexpr int kLoads = kKeys * D / 8 / 256;                // 16-byte loads of keys per thread
+  static constexpr int kChannels = D / 32;                          // of a thread's values
+};
+
+// A tile on its way to LDS.
+template <int D>
+struct Staged {
+  uint4 k[Tile<D>::kLoads];
+  uint32_t v[8][D / 64];
+  int32_t t;           // its first key
+  int64_t quarter[4];  // where 16 keys each begin, in elements from the head's first in page 0; -1: no page
+};
+
+// What a thread loads: a chunk of keys (16 lanes, at D = 64 eight, a key), and channels of eight keys.
+template <int D>
+struct Loader {
+  int key, chunk, group, channel, wave;
+  uint32_t koff, voff;
+
+  __device__ __forceinline__ Loader() {
+    const int tid = threadIdx.x;
+    wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    chunk = tid & (D / 8 - 1);
+    key = tid / (D / 8);
+    group = tid >> 5;
+    channel = (tid & 31) * Tile<D>::kChannels;
+    koff = (key & 15) * D + chunk * 8;
+    voff = (group & 1) * 8 * D + channel;
+  }
+  // The quarter of key load i: the same for a wave.
+  __device__ __forceinline__ int quarter(int i) const { return D == 128 ? i : 2 * i + (wave >> 1); }
+};
+
+__device__ __forceinline__ int64_t pick(const int64_t (&q)[4], int i) {
+  return i == 0 ? q[0] : i == 1 ? q[1] : i == 2 ? q[2] : q[3];
+}
+
+template <int D>
+__device__ __forceinline__ void fetch(Staged<D> &st, const Cache &c, Pages &pages, const uint16_t *key, const uint16_t *value,
+                                      const Loader<D> &ld, int32_t t) {
+  st.t = t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int32_t at = t + 16 * i, p = pages.entry(at >> c.shift);
+    st.quarter[i] = p < 0 ? -1 : int64_t(p) * c.page_elems + (at & (c.page - 1)) * D;
+  }
+#pragma unroll
+  for (int i = 0; i < Tile<D>::kLoads; ++i) {
+    const int64_t at = D == 128 ? st.quarter[i] : pick(st.quarter, ld.quarter(i));
+    st.k[i] = *reinterpret_cast<const uint4 *>(key + (at < 0 ? 0 : at) + ld.koff);
+  }
+  const int64_t at = pick(st.quarter, ld.wave);
+  const uint16_t *v = value + (at < 0 ? 0 : at) + ld.voff;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (D == 128) {
+      const uint2 x = *reinterpret_cast<const uint2 *>(v + j * D);
+      st.v[j][0] = x.x;
+      st.v[j][1] = x.y;
+    } else {
+      st.v[j][0] = *reinterpret_cast<const uint32_t *>(v + j * D);
+    }
+  }
+}
+
+// The orders of a key's and of a channel's chunks in LDS.
+template <int D>
+__device__ __forceinline__ int key_swizzle(int key) {
+  return ((key & 3) | ((key >> 3) & 3) << 2) & (D / 8 - 1);
+}
+template <int D>
+__device__ __forceinline__ int value_swizzle(int channel) {
+  return D == 128 ? ((channel >> 2) & 7) ^ ((channel & 3) << 1) : ((channel >> 1) & 7) ^ ((channel & 1) << 2);
+}
+
+template <int D>
+__device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const Loader<D> &ld) {
+#pragma unroll
+  for (int i = 0; i < Tile<D>::kLoads; ++i) {
+    const int key = ld.key + i * (2048 / D);
+    *reinterpret_cast<uint4 *>(buf + key * Tile<D>::kKeyRow + 16 * (ld.chunk ^ key_swizzle<D>(key))) = st.k[i];
+  }
+}
+
+// Values behind the length are zeroed, and what is not finite in a tile that not every row sees whole; whether there
+// was any such goes to `odd`.
+template <int D, int DT>
+__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t length, int32_t *odd) {
+  const bool there = pick(st.quarter, ld.wave) >= 0;
+  uint32_t any = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      if (!there || st.t + 8 * ld.group + j >= length) st.v[j][i] = 0;
+      const uint32_t bad = not_finite<DT>(st.v[j][i]);
+      any |= bad;
+      st.v[j][i] &= ~bad;
+    }
+  }
+  if (__any(any != 0) && (threadIdx.x & 63) == 0) *odd = 1;
+}
+
+template <int D>
+__device__ __forceinline__ void store_values(const Staged<D> &st, char *buf, const Loader<D> &ld) {
+#pragma unroll
+  for (int c = 0; c < Tile<D>::kChannels; ++c) {
+    const int channel = ld.channel + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      w[p] = c % 2 ? halves_of<true>(st.v[2 * p][c / 2], st.v[2 * p + 1][c / 2])
+                   : halves_of<false>(st.v[2 * p][c / 2], st.v[2 * p + 1][c / 2]);
+    }
+    *reinterpret_cast<uint4 *>(buf + Tile<D>::kKeyBytes + channel * Tile<D>::kValueRow +
+                               16 * (ld.group ^ value_swizzle<D>(channel))) = uint4{w[0], w[1], w[2], w[3]};
+  }
+}
+
+// Sixteen query rows of a wave: the lane's row is lane % 16, its channels 16 n + 4 (lane / 16) + i.
+template <int D>
+struct Acc16 {
+  f4 o[D / 16];
+  float m, l;
+};
+
+// The reference of 16 rows' weights, raised where one of the tile's logits asks for it.  seen[h]: keys of half h that the
+// lane's row sees, from the lane's own first on.
+template <int D, bool MASK>
+__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], float factor, const int32_t (&seen)[2]) {
+  float top = mf::kNegInf;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float x = s[j / 4][j % 4];
+    top = fmaxf(top, MASK && j % 8 >= seen[j / 8] ? mf::kNegInf : x);
+  }
+  top = mf::max_over_slices(top * factor);
+  if (__any(top > acc.m + kRaise)) {
+    const float m = fmaxf(acc.m, top - kHead);
+    const float alpha = acc.m == mf::kNegInf ? 0.0f : mf::fast_exp2(acc.m - m);
+    acc.m = m;
+    acc.l *= alpha;
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) acc.o[n] *= alpha;
+  }
+  return acc.m == mf::kNegInf ? 0.0f : acc.m;
+}
+
+// The weights of half a tile, and the sum of all.
+template <int DT, bool MASK>
+__device__ __forceinline__ float weights(const f4 (&s)[4], int half, float factor, float m, int32_t seen, float l,
+                                         typename Half<DT>::V8 &p) {
+  typedef typename Half<DT>::T T;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float e = mf::fast_exp2(__builtin_fmaf(s[2 * half + j / 4][j % 4], factor, -m));
+    if (MASK && j >= seen) e = 0.0f;
+    l += e;
+    p[j] = static_cast<T>(e);
+  }
+  return l;
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse, float *part,
+                                                      float *stat) {
+  typedef Tile<D> T;
+  typedef Half<DT> H;
+  typedef typename H::V8 V8;
+  __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
+  __shared__ int32_t odd[2];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
+  // Two waves share a SIMD, in slots that differ in their last bit (HW_ID's first four bits).
+  // One goes before the other in its vector phases, so that they do not reach the matrix cores together.
+  const bool before = (__builtin_amdgcn_s_getreg((3 << 11) | 4) & 1) != 0;
+  auto vector_phase = [&] {
+    if (before) {
+      __builtin_amdgcn_s_setprio(1);
+    } else {
+      __builtin_amdgcn_s_setprio(0);
+    }
+  };
+  // Workgroups go to the 8 XCDs in turn.  A list is one split of the keys of one (sequence, head); its row
+  // groups are dealt into `deal` hands so that 8 divides the number of hands, and an XCD plays whole hands: its
+  // L2 then holds the keys of few lists.
+  const int32_t lists = c.sequences * c.heads * p.splits, deal = 8 / (lists & 7 ? lists & -lists : 8);
+  const int32_t slots = (p.groups + deal - 1) / deal, x = blockIdx.x & 7, at = blockIdx.x >> 3, turn = at / slots;
+  const int32_t hand = x + 8 * turn, list = hand % lists, group = (at - turn * slots) * deal + hand / lists;
+  if (group >= p.groups || hand >= lists * deal) return;
+  const int32_t split = list % p.splits, sh = list / p.splits, s_index = sh / c.heads;
+  // the later rows of a causal call see more keys: the longest first
+  const int32_t row_group = q.causal ? p.groups - 1 - group : group, unit = sh * p.groups + row_group;
+  const Rows w = rows_at(q, s_index, sh - s_index * c.heads, row_group, kTileRows, c.length(s_index), q.count(s_index));
+  const int32_t tiles = (w.end_last + kKeys - 1) / kKeys, per = split_tiles_of(p, tiles);
+  const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
+  if (begin >= end && split > 0) return;
+  Pages pages(c, w.s);
+  const int64_t head = int64_t(w.h << c.shift) * D;
+  const uint16_t *key = c.key + head, *value = c.value + head;
+
+  V8 frag[2][D / 32];
+  int32_t row_end[2];
+  Acc16<D> acc[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int32_t r = w.r0 + wave * 32 + n * 16 + col, token = token_of(q, r);
+    const bool there = r < w.rows && token < w.count;
+    row_end[n] = there ? visible(q, w.length, w.count, token) : 0;
+    const uint16_t *row = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r - token * q.group) * q.sh + quad * 8;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      uint4 v = {0, 0, 0, 0};
+      if (there) v = *reinterpret_cast<const uint4 *>(row + k * 32);
+      frag[n][k] = __builtin_bit_cast(V8, v);
+    }
+    acc[n].m = mf::kNegInf;
+    acc[n].l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
+  }
+  // LDS offsets of the fragments: key tile j adds (32 (j / 2) + 4 (j % 2)) rows, channel tile n 16 rows
+  const int krow = (col >> 2) * 8 + (col & 3);
+  int ka[D / 32], va[2];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) ka[k] = krow * T::kKeyRow + 16 * ((4 * k + quad) ^ key_swizzle<D>(krow));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ value_swizzle<D>(col));
+
+  Staged<D> st;
+  const Loader<D> ld;
+  // whether every row sees all keys of the staged tile
+  auto whole = [&] {
+    return st.t + kKeys <= w.end_first && (st.quarter[0] | st.quarter[1] | st.quarter[2] | st.quarter[3]) >= 0;
+  };
+  int32_t t = begin;
+  int present = 0;  // the tile's buffer
+  auto step = [&](auto mask_tag) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    const char *buf = lds + present * T::kBytes;
+    const int32_t t0 = st.t;
+    int64_t quarter[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) quarter[i] = st.quarter[i];
+    const bool more = t + 1 < end;
+    if (more) fetch<D>(st, c, pages, key, value, ld, (t + 1) * kKeys);
+
+    __builtin_amdgcn_s_setprio(3);
+    f4 s[2][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[0][j] = s[1][j] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const V8 a = *reinterpret_cast<const V8 *>(buf + ka[k] + (32 * (j / 2) + 4 * (j % 2)) * T::kKeyRow);
+        s[0][j] = H::mfma(a, frag[0][k], s[0][j]);
+        s[1][j] = H::mfma(a, frag[1][k], s[1][j]);
+      }
+    }
+    vector_phase();
+    V8 pr[2][2];
+    float m[2];
+    int32_t seen[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        seen[n][h] = row_end[n] - t0 - 32 * h - 8 * quad;
+        if (MASK && ((quad & 2) ? quarter[2 * h + 1] : quarter[2 * h]) < 0) seen[n][h] = 0;
+      }
+      m[n] = reference<D, MASK>(acc[n], s[n], q.scale, seen[n]);
+    }
+    auto weigh = [&](int h) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) acc[n].l = weights<DT, MASK>(s[n], h, q.scale, m[n], seen[n][h], acc[n].l, pr[n][h]);
+    };
+    weigh(0);
+    weigh(1);
+    if constexpr (MASK) {
+      if (odd[present] != 0) {
+        // values that are not finite: added key by key to the rows that see them
+#pragma unroll 1
+        for (int k = 0; k < kKeys; ++k) {
+          const int64_t place = pick(quarter, k >> 4);
+          if (place < 0 || t0 + k >= w.length) continue;
+          const uint16_t *v = value + place + (k & 15) * D + 4 * quad;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            float weight = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float e = static_cast<float>(k < 32 ? pr[n][0][j] : pr[n][1][j]);
+              if (j == (k & 7)) weight = e;
+            }
+            weight = __shfl(weight, ((k & 31) >> 3) * 16 + col, kWave);
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t u = v[16 * d + i];
+                if (t0 + k < row_end[n] && not_finite<DT>(u) != 0) acc[n].o[d][i] += weight * half_bits_to_f32<DT>(u);
+              }
+            }
+          }
+        }
+      }
+    }
+    present ^= 1;
+    const bool all = whole();
+    if (more && threadIdx.x == 0) odd[present] = 0;
+    if (more && !all) __syncthreads();
+    if (more && !all) clear_values<D, DT>(st, ld, w.length, odd + present);
+    __builtin_amdgcn_s_setprio(3);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      V8 a[D / 16];
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        // (at 128 channels the chunks' order of channels 16 on is the first's with 4 changed)
+        a[d] = *reinterpret_cast<const V8 *>(buf + va[D == 128 ? h ^ (d & 1) : h] + d * 16 * T::kValueRow);
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
+        acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
+      }
+      // (after the last tile the present one's again, into the buffer that nobody reads)
+      if (h == 0) store_keys<D>(st, lds + present * T::kBytes, ld);
+      if (h == 1) store_values<D>(st, lds + present * T::kBytes, ld);
+    }
+    vector_phase();
+    __syncthreads();
+    ++t;
+  };
+  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+  __syncthreads();
+  st.t = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st.quarter[i] = -1;
+  if (begin < end) {
+    fetch<D>(st, c, pages, key, value, ld, begin * kKeys);
+    if (!whole()) clear_values<D, DT>(st, ld, w.length, odd);
+    store_keys<D>(st, lds, ld);
+    store_values<D>(st, lds, ld);
+  }
+  __syncthreads();
+  // tiles that every row sees come first; from the first other one on, every tile is masked
+  while (t < end && whole()) step(std::false_type());
+  while (t < end) step(std::true_type());
+
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
+    const float total = mf::sum_over_slices(acc[n].l);
+    if (r >= w.rows) continue;
+    if (p.splits > 1) {
+      const int64_t slot = (int64_t(unit) * p.splits + split) * kTileRows + rr;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(part + slot * D + 16 * d + 4 * quad) = acc[n].o[d];
+      if (quad == 0) {
+        stat[2 * slot] = acc[n].m;
+        stat[2 * slot + 1] = total;
+      }
+    } else {
+      const int32_t token = token_of(q, r), h = w.h * q.group + r - token * q.group;
+      const bool none = token >= w.count || total == 0.0f;
+      const float f = none ? 0.0f : 1.0f / total;
+      uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + h) * D + 4 * quad;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        const f4 y = none ? f4{0, 0, 0, 0} : acc[n].o[d] * f;
+        *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+      }
+      if (quad == 0 && lse != nullptr) {
+        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : kLn2 * (acc[n].m + __builtin_amdgcn_logf(total));
+      }
+    }
+  }
+}
+
+}  // namespace
+
+int64_t tile_workgroups(int64_t lists, int64_t groups) {
+  const int64_t deal = 8 / (lists & 7 ? lists & -lists : 8);  // (the hands may be one row group longer than they need to be)
+  return ceil_div(lists * deal, int64_t(8)) * 8 * ceil_div(groups, deal);
+}
+
+int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, const Query &q, const Plan &p, uint16_t *out,
+                 float *lse, float *part, float *stat, hipStream_t stream) {
+  const dim3 grid(static_cast<uint32_t>(tile_workgroups(int64_t(c.sequences) * c.heads * p.splits, p.groups)));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, c, q, p, out, lse, part, stat); };
+  if (head_dim == 128) {
+    dtype == UC_FP16 ? go(tile_kernel<128, UC_FP16>) : go(tile_kernel<128, UC_BF16>);
+  } else {
+    dtype == UC_FP16 ? go(tile_kernel<64, UC_FP16>) : go(tile_kernel<64, UC_BF16>);
+  }
+  return check_launch(what);
+}
+
+}  // namespace pg
+}  // namespace uc
