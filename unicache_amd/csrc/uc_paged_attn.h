@@ -8,6 +8,9 @@ namespace pg {
 
 using mf::f4;
 
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
 constexpr int kTile = 32;                 // keys of a wave's tile
 constexpr int kStep = 4 * kTile;          // keys of a workgroup's step
 constexpr float kHead = 6.0f;             // a raised reference lies 2^6 below the largest weight
@@ -77,44 +80,26 @@ __device__ __forceinline__ Rows rows_at(const Query &q, int32_t s, int32_t h, in
   return w;
 }
 
-// A sequence's pages, 64 entries at a time in a wave's lanes, so that a tile's page is no load that its
-// rows' loads would wait for.  What is no page reads as -1.
+// A sequence's row of the table, read by scalar loads: an entry that is asked for a tile ahead of its use
+// costs no wave a wait, and what follows from it stays in scalar registers.
 struct Pages {
-  const int32_t *row;
-  int32_t width, pages, chunk, held;
+  typedef const __attribute__((address_space(4))) int32_t *Scalars;
+  Scalars row;
+  int32_t last, shift;
 
   __device__ __forceinline__ Pages(const Cache &c, int32_t s)
-      : row(c.table + int64_t(s) * c.width), width(c.width), pages(c.pages), chunk(-1), held(-1) {}
+      : row((Scalars)(c.table + int64_t(s) * c.width)), last(c.width - 1), shift(c.shift) {}
 
-  __device__ __forceinline__ int32_t entry(int32_t e) {
-    if (e >= width) return -1;
-    if ((e >> 6) != chunk) {
-      chunk = e >> 6;
-      const int32_t i = chunk * 64 + (threadIdx.x & 63), p = i < width ? row[i] : -1;
-      held = static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : -1;
-    }
-    return __builtin_amdgcn_readlane(held, e & 63);
+  // The entry of token t, which is the same in the whole wave; past the table the last one (no row sees such tokens).
+  __device__ __forceinline__ int32_t of(int32_t t) const {
+    const int32_t e = __builtin_amdgcn_readfirstlane(t >> shift);
+    return row[e < last ? e : last];
   }
 };
 
-// Where 32 keys lie: each half's first row, in elements from a head's first in page 0; -1 where there is no page.
-struct Place {
-  int32_t t;
-  int64_t a, b;
-};
-
-__device__ __forceinline__ Place place_of(const Cache &c, Pages &pages, int32_t t, int32_t d) {
-  Place x;
-  x.t = t;
-  const int32_t p = pages.entry(t >> c.shift);
-  x.a = p < 0 ? -1 : int64_t(p) * c.page_elems + (t & (c.page - 1)) * d;
-  if (c.shift >= 5) {
-    x.b = p < 0 ? -1 : x.a + 16 * d;
-  } else {
-    const int32_t n = pages.entry((t >> c.shift) + 1);
-    x.b = n < 0 ? -1 : int64_t(n) * c.page_elems;
-  }
-  return x;
+// The first row of a head's tokens t .. in their page, in elements from its first in page 0; -1 where there is no page.
+__device__ __forceinline__ int64_t place_of(const Cache &c, int32_t entry, int32_t t, int32_t d) {
+  return c.is_page(entry) ? int64_t(entry) * c.page_elems + (t & (c.page - 1)) * d : -1;
 }
 
 // 16-bit operands.
@@ -140,11 +125,50 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, V2{static_cast<T>(a), static_cast<T>(b)});
 }
 
-// Bits of the halves of w that are no finite numbers.
+// Values that are not finite, in tiles that not every row sees whole: a hidden key's weight is 0, and 0 times them is
+// NaN.  So the products take 0 in their place, and a second product counts, for each row, the keys that it
+// does see of each kind; one is enough to make the sum what it is.
 template <int DT>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  constexpr uint32_t e = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
-  return ((w & e) == e ? 0xffffu : 0u) | ((w & (e << 16)) == e << 16 ? 0xffff0000u : 0u);
+constexpr uint32_t kInfinity = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
+
+// A fragment with zeros in their place; whether there was any in the wave.
+template <int DT>
+__device__ __forceinline__ bool take_finite(typename Half<DT>::V8 &v) {
+  constexpr uint32_t e = kInfinity<DT>;
+  u4 w = __builtin_bit_cast(u4, v);
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bad = ((w[i] & e) == e ? 0xffffu : 0u) | ((w[i] & (e << 16)) == e << 16 ? 0xffff0000u : 0u);
+    any |= bad;
+    w[i] &= ~bad;
+  }
+  v = __builtin_bit_cast(typename Half<DT>::V8, w);
+  return __any(any != 0);
+}
+
+// What the others of fragment v do to rows that see the first `seen` of a lane's eight keys.
+template <int DT>
+__device__ __forceinline__ void add_infinite(typename Half<DT>::V8 v, int32_t seen, f4 &o) {
+  typedef typename Half<DT>::T T;
+  constexpr uint32_t e = kInfinity<DT>;
+  typename Half<DT>::V8 sees;
+  const u4 u = __builtin_bit_cast(u4, v);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sees[j] = static_cast<T>(j < seen ? 1.0f : 0.0f);
+#pragma unroll
+  for (int kind = 0; kind < 3; ++kind) {  // infinity, its negative, NaN
+    typename Half<DT>::V8 is;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t x = j % 2 ? u[j / 2] >> 16 : u[j / 2] & 0xffffu;
+      is[j] = static_cast<T>((kind == 0 ? x == e : kind == 1 ? x == (e | 0x8000u) : (x & 0x7fffu) > e) ? 1.0f : 0.0f);
+    }
+    const f4 count = Half<DT>::mfma(is, sees, f4{0, 0, 0, 0});
+    const float add = kind == 0 ? __builtin_huge_valf() : kind == 1 ? -__builtin_huge_valf() : __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += count[i] > 0.0f ? add : 0.0f;
+  }
 }
 
 // The lower or the upper halves of two dwords as one.

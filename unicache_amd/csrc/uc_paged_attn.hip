@@ -15,9 +15,6 @@
 // byte permutation per pair of keys and channel turns them round.  Fragment n then holds
 // channels D/16 r + n, and a lane ends with consecutive channels of its query row.
 //
-// What a row does not see must not reach it: rows behind the length are zeroed before the products, and
-// where a hidden key's value is not finite (0 times it would be NaN) the finite part goes
-// through the products and the rest is added key by key to the rows that see it.
 #include "uc_paged_attn.h"
 
 #include <type_traits>
@@ -29,7 +26,7 @@ namespace {
 // Rows of one tile as they come from memory.
 template <int D>
 struct Raw {
-  uint4 k[2][D / 32];
+  u4 k[2][D / 32];
   uint32_t v[8][D / 32];
 };
 
@@ -39,32 +36,30 @@ struct Lane {
 };
 
 template <int D>
-__device__ __forceinline__ void load_keys(Raw<D> &raw, const Lane<D> &l, const Place &x) {
-  const int64_t at = (threadIdx.x & 8) ? x.b : x.a;
+__device__ __forceinline__ void load_keys(Raw<D> &raw, const Lane<D> &l, int64_t a, int64_t b) {
+  const int64_t at = (threadIdx.x & 8) ? b : a;
   const uint16_t *p = l.key + (at < 0 ? 0 : at);
 #pragma unroll
-  for (int a = 0; a < 2; ++a) {
+  for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) raw.k[a][k] = *reinterpret_cast<const uint4 *>(p + a * 4 * D + k * 32);
+    for (int k = 0; k < D / 32; ++k) raw.k[t][k] = *reinterpret_cast<const u4 *>(p + t * 4 * D + k * 32);
   }
 }
 
 template <int D>
-__device__ __forceinline__ void load_values(Raw<D> &raw, const Lane<D> &l, const Place &x) {
-  const int64_t at = (threadIdx.x & 32) ? x.b : x.a;
+__device__ __forceinline__ void load_values(Raw<D> &raw, const Lane<D> &l, int64_t a, int64_t b) {
+  const int64_t at = (threadIdx.x & 32) ? b : a;
   const uint16_t *p = l.value + (at < 0 ? 0 : at);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if constexpr (D == 128) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(p + j * D);
-      raw.v[j][0] = v.x;
-      raw.v[j][1] = v.y;
-      raw.v[j][2] = v.z;
-      raw.v[j][3] = v.w;
+      const u4 v = *reinterpret_cast<const u4 *>(p + j * D);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw.v[j][i] = v[i];
     } else {
-      const uint2 v = *reinterpret_cast<const uint2 *>(p + j * D);
-      raw.v[j][0] = v.x;
-      raw.v[j][1] = v.y;
+      const u2 v = *reinterpret_cast<const u2 *>(p + j * D);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) raw.v[j][i] = v[i];
     }
   }
 }
@@ -78,7 +73,7 @@ __device__ __forceinline__ typename Half<DT>::V8 value_fragment(const Raw<D> &ra
     w[t] = n % 2 ? halves_of<true>(raw.v[2 * t][n / 2], raw.v[2 * t + 1][n / 2])
                  : halves_of<false>(raw.v[2 * t][n / 2], raw.v[2 * t + 1][n / 2]);
   }
-  return __builtin_bit_cast(typename Half<DT>::V8, uint4{w[0], w[1], w[2], w[3]});
+  return __builtin_bit_cast(typename Half<DT>::V8, u4{w[0], w[1], w[2], w[3]});
 }
 
 // State of 16 query rows in one wave: the lane's row is lane % 16, its channels of o[n][i] are
@@ -167,11 +162,16 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
   const int32_t stop = end * kStep < w.end_last ? end * kStep : w.end_last;
   int32_t t = begin * kStep + wave * kTile;
   Raw<D> raw;
-  Place x = {t, -1, -1};
+  // where a tile's halves begin (16 keys lie in one page), and the entries of the next one
+  int64_t first_a = -1, first_b = -1;
+  int32_t entry_a = 0, entry_b = 0;
   if (t < stop) {
-    x = place_of(c, pages, t, D);
-    load_keys(raw, l, x);
-    load_values(raw, l, x);
+    first_a = place_of(c, pages.of(t), t, D);
+    first_b = place_of(c, pages.of(t + 16), t + 16, D);
+    load_keys(raw, l, first_a, first_b);
+    load_values(raw, l, first_a, first_b);
+    entry_a = pages.of(t + kStep);
+    entry_b = pages.of(t + kStep + 16);
   }
   V8 frag[NR][D / 32];
   int32_t row_end[NR];
@@ -211,9 +211,10 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     int at = lane;  // opaque, so that the fragments are read in every tile and not kept
     if constexpr (J::kHeld) asm volatile("" : "+v"(at));
     auto query = [&](int n, int k) { return J::kHeld ? joined.frag[n * (D / 32) + k][at] : frag[n][k]; };
-    Place next = {t + kStep, -1, -1};
     const bool more = t + kStep < stop;
-    if (more) next = place_of(c, pages, t + kStep, D);
+    const int64_t next_a = place_of(c, entry_a, t + kStep, D), next_b = place_of(c, entry_b, t + kStep + 16, D);
+    entry_a = pages.of(t + 2 * kStep);
+    entry_b = pages.of(t + 2 * kStep + 16);
     f4 s[NR][2];
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
@@ -226,71 +227,37 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
         for (int n = 0; n < NR; ++n) s[n][a] = H::mfma(rows, query(n, k), s[n][a]);
       }
     }
-    if (more) load_keys(raw, l, next);
+    if (more) load_keys(raw, l, next_a, next_b);
     const int32_t mine = t + 8 * quad;                              // the lane's first key
-    const bool there = ((quad & 2) ? x.b : x.a) >= 0;                // and its page
+    const bool there = ((quad & 2) ? first_b : first_a) >= 0;              // and its page
     V8 high[NR], low[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
     }
-    if constexpr (MASK) {
-      uint32_t odd = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          if (!there || mine + j >= w.length) raw.v[j][i] = 0;
-          odd |= not_finite<DT>(raw.v[j][i]);
-        }
-      }
-      if (__any(odd != 0)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t bad[D / 32], any = 0;
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            bad[i] = raw.v[j][i] & not_finite<DT>(raw.v[j][i]);
-            any |= bad[i];
-            raw.v[j][i] &= ~not_finite<DT>(raw.v[j][i]);
-          }
-          const uint64_t lanes = __ballot(any != 0);
-#pragma unroll 1
-          for (int g = 0; g < 4; ++g) {
-            if (((lanes >> (16 * g)) & 0xffff) == 0) continue;
-#pragma unroll
-            for (int n = 0; n < NR; ++n) {
-              const float weight = __shfl(static_cast<float>(high[n][j]) + static_cast<float>(low[n][j]), 16 * g + col, kWave);
-              const bool sees = t + 8 * g + j < row_end[n];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                  const uint32_t b = __shfl(bad[d / 2], 16 * g + 4 * quad + i, kWave);
-                  const uint32_t u = d % 2 ? b >> 16 : b & 0xffff;
-                  if (sees && u != 0) acc[n].o[d][i] += weight * half_bits_to_f32<DT>(u);
-                }
-              }
-            }
-          }
-        }
-      }
-    }
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) {
-      const V8 v = value_fragment<D, DT>(raw, d);
+      V8 v = value_fragment<D, DT>(raw, d);
+      if constexpr (MASK) {
+        const V8 all = v;
+        if (take_finite<DT>(v)) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n) add_infinite<DT>(all, there ? row_end[n] - mine : 0, acc[n].o[d]);
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         acc[n].o[d] = H::mfma(v, high[n], acc[n].o[d]);
         acc[n].o[d] = H::mfma(v, low[n], acc[n].o[d]);
       }
     }
-    if (more) load_values(raw, l, next);
-    x = next;
+    if (more) load_values(raw, l, next_a, next_b);
+    first_a = next_a;
+    first_b = next_b;
     t += kStep;
   };
   // tiles that every row sees come first; from the first other one on, every tile is masked
-  while (t < stop && t + kTile <= w.end_first && x.a >= 0 && x.b >= 0) step(std::false_type());
+  while (t < stop && t + kTile <= w.end_first && first_a >= 0 && first_b >= 0) step(std::false_type());
   while (t < stop) step(std::true_type());
 
   // join the waves: 16 threads a row, D / 16 channels each

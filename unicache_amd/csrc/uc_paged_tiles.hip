@@ -34,10 +34,17 @@ struct Tile {
 // A tile on its way to LDS.
 template <int D>
 struct Staged {
-  uint4 k[Tile<D>::kLoads];
+  u4 k[Tile<D>::kLoads];
   uint32_t v[8][D / 64];
-  int32_t t;           // its first key
-  int64_t quarter[4];  // where 16 keys each begin, in elements from the head's first in page 0; -1: no page
+  int32_t t;        // its first key
+  uint32_t absent;  // bit i: its keys 16 i .. 16 i + 15 have no page
+};
+
+// Table entries of a tile to come.  WHOLE: pages of 64 tokens or more, one entry a tile; else those of each 16 keys, and
+// of a wave's loads.
+template <int D, bool WHOLE>
+struct Entries {
+  int32_t quarter[WHOLE ? 1 : 4], key[WHOLE ? 1 : Tile<D>::kLoads], value;
 };
 
 // What a thread loads: a chunk of keys (16 lanes, at D = 64 eight, a key), and channels of eight keys.
@@ -57,35 +64,43 @@ struct Loader {
     voff = (group & 1) * 8 * D + channel;
   }
   // The quarter of key load i: the same for a wave.
-  __device__ __forceinline__ int quarter(int i) const { return D == 128 ? i : 2 * i + (wave >> 1); }
+  __device__ __forceinline__ int32_t quarter(int i) const { return D == 128 ? i : 2 * i + (wave >> 1); }
 };
 
-__device__ __forceinline__ int64_t pick(const int64_t (&q)[4], int i) {
-  return i == 0 ? q[0] : i == 1 ? q[1] : i == 2 ? q[2] : q[3];
+template <int D, bool WHOLE>
+__device__ __forceinline__ void ask(Entries<D, WHOLE> &e, const Pages &pages, const Loader<D> &ld, int32_t t) {
+#pragma unroll
+  for (int i = 0; i < (WHOLE ? 1 : 4); ++i) e.quarter[i] = pages.of(t + 16 * i);
+  if constexpr (!WHOLE) {
+#pragma unroll
+    for (int i = 0; i < Tile<D>::kLoads; ++i) e.key[i] = D == 128 ? e.quarter[i] : pages.of(t + 16 * ld.quarter(i));
+    e.value = pages.of(t + 16 * ld.wave);
+  }
 }
 
-template <int D>
-__device__ __forceinline__ void fetch(Staged<D> &st, const Cache &c, Pages &pages, const uint16_t *key, const uint16_t *value,
-                                      const Loader<D> &ld, int32_t t) {
+template <int D, bool WHOLE>
+__device__ __forceinline__ void fetch(Staged<D> &st, const Cache &c, const Entries<D, WHOLE> &e, const uint16_t *key,
+                                      const uint16_t *value, const Loader<D> &ld, int32_t t) {
   st.t = t;
+  st.absent = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t at = t + 16 * i, p = pages.entry(at >> c.shift);
-    st.quarter[i] = p < 0 ? -1 : int64_t(p) * c.page_elems + (at & (c.page - 1)) * D;
-  }
+  for (int i = 0; i < (WHOLE ? 1 : 4); ++i) st.absent |= c.is_page(e.quarter[i]) ? 0u : WHOLE ? 15u : 1u << i;
+  // (what has no page is read from the first)
+  auto place = [&](int32_t entry, int32_t at) {
+    return (c.is_page(entry) ? int64_t(entry) * c.page_elems : 0) + (at & (c.page - 1)) * D;
+  };
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
-    const int64_t at = D == 128 ? st.quarter[i] : pick(st.quarter, ld.quarter(i));
-    st.k[i] = *reinterpret_cast<const uint4 *>(key + (at < 0 ? 0 : at) + ld.koff);
+    const uint16_t *k = key + place(WHOLE ? e.quarter[0] : e.key[i], t + 16 * ld.quarter(i));
+    st.k[i] = *reinterpret_cast<const u4 *>(k + ld.koff);
   }
-  const int64_t at = pick(st.quarter, ld.wave);
-  const uint16_t *v = value + (at < 0 ? 0 : at) + ld.voff;
+  const uint16_t *v = value + place(WHOLE ? e.quarter[0] : e.value, t + 16 * ld.wave) + ld.voff;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if constexpr (D == 128) {
-      const uint2 x = *reinterpret_cast<const uint2 *>(v + j * D);
-      st.v[j][0] = x.x;
-      st.v[j][1] = x.y;
+      const u2 x = *reinterpret_cast<const u2 *>(v + j * D);
+      st.v[j][0] = x[0];
+      st.v[j][D / 64 - 1] = x[1];
     } else {
       st.v[j][0] = *reinterpret_cast<const uint32_t *>(v + j * D);
     }
@@ -107,27 +122,8 @@ __device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const
 #pragma unroll
   for (int i = 0; i < Tile<D>::kLoads; ++i) {
     const int key = ld.key + i * (2048 / D);
-    *reinterpret_cast<uint4 *>(buf + key * Tile<D>::kKeyRow + 16 * (ld.chunk ^ key_swizzle<D>(key))) = st.k[i];
+    *reinterpret_cast<u4 *>(buf + key * Tile<D>::kKeyRow + 16 * (ld.chunk ^ key_swizzle<D>(key))) = st.k[i];
   }
-}
-
-// Values behind the length are zeroed, and what is not finite in a tile that not every row sees whole; whether there
-// was any such goes to `odd`.
-template <int D, int DT>
-__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t length, int32_t *odd) {
-  const bool there = pick(st.quarter, ld.wave) >= 0;
-  uint32_t any = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-#pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
-      if (!there || st.t + 8 * ld.group + j >= length) st.v[j][i] = 0;
-      const uint32_t bad = not_finite<DT>(st.v[j][i]);
-      any |= bad;
-      st.v[j][i] &= ~bad;
-    }
-  }
-  if (__any(any != 0) && (threadIdx.x & 63) == 0) *odd = 1;
 }
 
 template <int D>
@@ -141,8 +137,8 @@ __device__ __forceinline__ void store_values(const Staged<D> &st, char *buf, con
       w[p] = c % 2 ? halves_of<true>(st.v[2 * p][c / 2], st.v[2 * p + 1][c / 2])
                    : halves_of<false>(st.v[2 * p][c / 2], st.v[2 * p + 1][c / 2]);
     }
-    *reinterpret_cast<uint4 *>(buf + Tile<D>::kKeyBytes + channel * Tile<D>::kValueRow +
-                               16 * (ld.group ^ value_swizzle<D>(channel))) = uint4{w[0], w[1], w[2], w[3]};
+    *reinterpret_cast<u4 *>(buf + Tile<D>::kKeyBytes + channel * Tile<D>::kValueRow +
+                               16 * (ld.group ^ value_swizzle<D>(channel))) = u4{w[0], w[1], w[2], w[3]};
   }
 }
 
@@ -190,14 +186,13 @@ __device__ __forceinline__ float weights(const f4 (&s)[4], int half, float facto
   return l;
 }
 
-template <int D, int DT>
+template <int D, int DT, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse, float *part,
                                                       float *stat) {
   typedef Tile<D> T;
   typedef Half<DT> H;
   typedef typename H::V8 V8;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
-  __shared__ int32_t odd[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   // Two waves share a SIMD, in slots that differ in their last bit (HW_ID's first four bits).
   // One goes before the other in its vector phases, so that they do not reach the matrix cores together.
@@ -256,10 +251,11 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   for (int h = 0; h < 2; ++h) va[h] = T::kKeyBytes + col * T::kValueRow + 16 * ((4 * h + quad) ^ value_swizzle<D>(col));
 
   Staged<D> st;
+  Entries<D, WHOLE> entries;  // of the tile after the staged one
   const Loader<D> ld;
   // whether every row sees all keys of the staged tile
   auto whole = [&] {
-    return st.t + kKeys <= w.end_first && (st.quarter[0] | st.quarter[1] | st.quarter[2] | st.quarter[3]) >= 0;
+    return st.t + kKeys <= w.end_first && st.absent == 0;
   };
   int32_t t = begin;
   int present = 0;  // the tile's buffer
@@ -267,11 +263,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     constexpr bool MASK = decltype(mask_tag)::value;
     const char *buf = lds + present * T::kBytes;
     const int32_t t0 = st.t;
-    int64_t quarter[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) quarter[i] = st.quarter[i];
+    const uint32_t absent = st.absent;
     const bool more = t + 1 < end;
-    if (more) fetch<D>(st, c, pages, key, value, ld, (t + 1) * kKeys);
+    if (more) fetch<D, WHOLE>(st, c, entries, key, value, ld, (t + 1) * kKeys);
+    ask(entries, pages, ld, (t + 2) * kKeys);
 
     __builtin_amdgcn_s_setprio(3);
     f4 s[2][4];
@@ -294,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         seen[n][h] = row_end[n] - t0 - 32 * h - 8 * quad;
-        if (MASK && ((quad & 2) ? quarter[2 * h + 1] : quarter[2 * h]) < 0) seen[n][h] = 0;
+        if (MASK && ((absent >> (2 * h + (quad >> 1))) & 1) != 0) seen[n][h] = 0;
       }
       m[n] = reference<D, MASK>(acc[n], s[n], q.scale, seen[n]);
     }
@@ -304,53 +299,35 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     };
     weigh(0);
     weigh(1);
-    if constexpr (MASK) {
-      if (odd[present] != 0) {
-        // values that are not finite: added key by key to the rows that see them
-#pragma unroll 1
-        for (int k = 0; k < kKeys; ++k) {
-          const int64_t place = pick(quarter, k >> 4);
-          if (place < 0 || t0 + k >= w.length) continue;
-          const uint16_t *v = value + place + (k & 15) * D + 4 * quad;
-#pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            float weight = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float e = static_cast<float>(k < 32 ? pr[n][0][j] : pr[n][1][j]);
-              if (j == (k & 7)) weight = e;
-            }
-            weight = __shfl(weight, ((k & 31) >> 3) * 16 + col, kWave);
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t u = v[16 * d + i];
-                if (t0 + k < row_end[n] && not_finite<DT>(u) != 0) acc[n].o[d][i] += weight * half_bits_to_f32<DT>(u);
-              }
-            }
-          }
-        }
-      }
-    }
     present ^= 1;
-    const bool all = whole();
-    if (more && threadIdx.x == 0) odd[present] = 0;
-    if (more && !all) __syncthreads();
-    if (more && !all) clear_values<D, DT>(st, ld, w.length, odd + present);
     __builtin_amdgcn_s_setprio(3);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      V8 a[D / 16];
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
+      auto load = [&](int d) {
         // (at 128 channels the chunks' order of channels 16 on is the first's with 4 changed)
-        a[d] = *reinterpret_cast<const V8 *>(buf + va[D == 128 ? h ^ (d & 1) : h] + d * 16 * T::kValueRow);
-      }
+        return *reinterpret_cast<const V8 *>(buf + va[D == 128 ? h ^ (d & 1) : h] + d * 16 * T::kValueRow);
+      };
+      if constexpr (MASK) {
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
-        acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
+        for (int d = 0; d < D / 16; ++d) {
+          V8 a = load(d);
+          const V8 all = a;
+          if (take_finite<DT>(a)) {
+            add_infinite<DT>(all, seen[0][h], acc[0].o[d]);
+            add_infinite<DT>(all, seen[1][h], acc[1].o[d]);
+          }
+          acc[0].o[d] = H::mfma(a, pr[0][h], acc[0].o[d]);
+          acc[1].o[d] = H::mfma(a, pr[1][h], acc[1].o[d]);
+        }
+      } else {
+        V8 a[D / 16];
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) a[d] = load(d);
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
+          acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
+        }
       }
       // (after the last tile the present one's again, into the buffer that nobody reads)
       if (h == 0) store_keys<D>(st, lds + present * T::kBytes, ld);
@@ -360,14 +337,12 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     __syncthreads();
     ++t;
   };
-  if (threadIdx.x < 2) odd[threadIdx.x] = 0;
-  __syncthreads();
   st.t = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) st.quarter[i] = -1;
+  st.absent = 0;
   if (begin < end) {
-    fetch<D>(st, c, pages, key, value, ld, begin * kKeys);
-    if (!whole()) clear_values<D, DT>(st, ld, w.length, odd);
+    ask(entries, pages, ld, begin * kKeys);
+    fetch<D, WHOLE>(st, c, entries, key, value, ld, begin * kKeys);
+    ask(entries, pages, ld, (begin + 1) * kKeys);
     store_keys<D>(st, lds, ld);
     store_values<D>(st, lds, ld);
   }
@@ -417,11 +392,14 @@ int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, 
                  float *lse, float *part, float *stat, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>(tile_workgroups(int64_t(c.sequences) * c.heads * p.splits, p.groups)));
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, c, q, p, out, lse, part, stat); };
-  if (head_dim == 128) {
-    dtype == UC_FP16 ? go(tile_kernel<128, UC_FP16>) : go(tile_kernel<128, UC_BF16>);
-  } else {
-    dtype == UC_FP16 ? go(tile_kernel<64, UC_FP16>) : go(tile_kernel<64, UC_BF16>);
-  }
+  auto by_page = [&](auto d_tag, auto dt_tag) {
+    constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
+    c.page >= kKeys ? go(tile_kernel<D, DT, true>) : go(tile_kernel<D, DT, false>);
+  };
+  auto by_type = [&](auto d_tag) {
+    dtype == UC_FP16 ? by_page(d_tag, std::integral_constant<int, UC_FP16>()) : by_page(d_tag, std::integral_constant<int, UC_BF16>());
+  };
+  head_dim == 128 ? by_type(std::integral_constant<int, 128>()) : by_type(std::integral_constant<int, 64>());
   return check_launch(what);
 }
 
