@@ -276,6 +276,19 @@ def test_few_rows_over_many_keys_in_tiles(device):
     check_attention(cache, k, v, lengths, q, None, True)
 
 
+def test_many_row_groups_of_many_sequences(device):
+    # more row groups than the workgroups share out: one workgroup each
+    s, lq = 2100, 130
+    lengths = [(37 * i) % 190 for i in range(s)]
+    cache, k, v = filled(lengths, hkv=1, d=64, b=16)
+    q = randn(s, lq, 1, 64, seed=3)
+    counts = [n % (lq + 1) for n in lengths]
+    out, lse = cache.attention(q, query_lengths=i32(counts), causal=True)
+    some = [0, 1, 5, 700, 2099]
+    few = [lengths[i] for i in some]
+    check_attention(cache, k[some], v[some], few, q[some], [counts[i] for i in some], True, result=(out[some], lse[some]))
+
+
 def test_many_sequences_share_the_workgroups(device):
     # more sequences than a wave has lanes, empty ones among them; max_tokens far from the truth
     lengths = [(37 * i) % 260 if i % 3 else 0 for i in range(131)]

@@ -35,16 +35,9 @@ struct Query {
 constexpr int kTileRows = 128;            // rows of a unit of many (uc_paged_tiles.hip)
 
 struct Plan {
-  int32_t rows, groups;         // rows of a unit, and units of a (sequence, KV head)
-  int32_t workgroups;           // few rows: workgroups that share all steps; 0: many rows
-  int32_t splits, split_tiles;  // many rows: splits of a unit's keys, and the 64-key tiles of one
+  int32_t rows, groups;  // rows of a unit, and units of a (sequence, KV head)
+  int32_t workgroups;    // that share all steps; 0 (many rows): one a unit
 };
-
-// Tiles of one split: the host's figure, or more where a sequence is longer than it expected.
-__device__ __forceinline__ int32_t split_tiles_of(const Plan &p, int32_t tiles) {
-  const int32_t least = (tiles + p.splits - 1) / p.splits;
-  return least > p.split_tiles ? least : p.split_tiles;
-}
 
 // The rows of a unit: row r is query token r / group of head h * group + r % group.
 struct Rows {
@@ -177,8 +170,31 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, UPPER ? 0x07060302u : 0x05040100u);
 }
 
+// D / 16 channels of a finished row.
+template <int D, int DT>
+__device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t r, int32_t c0, const float *o, float m,
+                                          float l, uint16_t *out, float *lse) {
+  constexpr int kC = D / 16;
+  const int32_t t = token_of(q, r), head = w.h * q.group + r - t * q.group;
+  const bool none = t >= w.count || l == 0.0f;
+  const float f = none ? 0.0f : 1.0f / l;
+  uint32_t v[kC / 2];
+#pragma unroll
+  for (int j = 0; j < kC / 2; ++j) v[j] = none ? 0u : pack2<DT>(o[2 * j] * f, o[2 * j + 1] * f);
+  uint16_t *dst = out + ((int64_t(w.s) * q.len + t) * q.heads + head) * D + c0;
+  if constexpr (kC == 8) {
+    *reinterpret_cast<uint4 *>(dst) = uint4{v[0], v[1], v[2], v[3]};
+  } else {
+    *reinterpret_cast<uint2 *>(dst) = uint2{v[0], v[1]};
+  }
+  if (c0 == 0 && lse != nullptr) {
+    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(l));
+  }
+}
+
 // uc_paged_tiles.hip: many query rows.
-int64_t tile_workgroups(int64_t lists, int64_t groups);
+constexpr int kKeys = 64;                 // keys of a tile
+constexpr int64_t kMostShared = 4096;     // row groups of all sequences that a wave adds up
 int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, const Query &q, const Plan &p, uint16_t *out,
                  float *lse, float *part, float *stat, hipStream_t stream);
 

@@ -123,27 +123,6 @@ struct Joined {
   typename Half<DT>::V8 frag[kHeld ? NR * D / 32 : 1][64];
 };
 
-template <int D, int DT>
-__device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t r, int32_t c0, const float *o, float m,
-                                          float l, uint16_t *out, float *lse) {
-  constexpr int kC = D / 16;
-  const int32_t t = token_of(q, r), head = w.h * q.group + r - t * q.group;
-  const bool none = t >= w.count || l == 0.0f;
-  const float f = none ? 0.0f : 1.0f / l;
-  uint32_t v[kC / 2];
-#pragma unroll
-  for (int j = 0; j < kC / 2; ++j) v[j] = none ? 0u : pack2<DT>(o[2 * j] * f, o[2 * j + 1] * f);
-  uint16_t *dst = out + ((int64_t(w.s) * q.len + t) * q.heads + head) * D + c0;
-  if constexpr (kC == 8) {
-    *reinterpret_cast<uint4 *>(dst) = uint4{v[0], v[1], v[2], v[3]};
-  } else {
-    *reinterpret_cast<uint2 *>(dst) = uint2{v[0], v[1]};
-  }
-  if (c0 == 0 && lse != nullptr) {
-    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(l));
-  }
-}
-
 // Steps begin .. end - 1 of the rows w, by a whole workgroup.  slot >= 0: the part goes there; else it
 // is all there is, and the rows are finished.
 template <int D, int DT, int NR>
@@ -400,13 +379,6 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
   x.r = index - sh * full;
   const int32_t group = p.groups == 1 ? 0 : x.r / p.rows, each = c.heads * p.groups;
   const int32_t unit = sh * p.groups + group;
-  if (p.workgroups == 0) {
-    x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, c.length(s), q.count(s));
-    const int32_t tiles = (x.w.end_last + 63) / 64, per = split_tiles_of(p, tiles);
-    x.first = unit * p.splits;
-    x.count = tiles == 0 ? 0 : (tiles + per - 1) / per;
-    return x;
-  }
   int32_t total = 0, before = 0, mine = 0;
   for (int32_t s0 = 0; s0 < c.sequences; s0 += 64) {
     const int32_t i = s0 + (threadIdx.x & 63);
@@ -496,7 +468,7 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
   constexpr int kC = D / 16;
   __shared__ float sh_o[16][D], sh_l[16];
   const Parts x = parts_of(c, q, p, blockIdx.x);
-  if (x.count == 1 && p.workgroups > 0) return;
+  if (x.count == 1) return;
   const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
   Sum<D> t = sum_parts<D, 16>(p, x, group, part, stat);
 #pragma unroll
@@ -510,25 +482,6 @@ __global__ __launch_bounds__(256) void join_many_kernel(Cache c, Query q, Plan p
     for (int j = 0; j < kC; ++j) t.o[j] += sh_o[g][lane * kC + j];
   }
   store_row<D, DT>(q, x.w, x.r, lane * kC, t.o, t.m, t.l, out, lse);
-}
-
-// Splits of 128-row workgroups: the least time in tiles.  Two workgroups share a CU, and up to one a CU takes 0.65
-// of the time a tile.  The launch that joins splits takes two tiles and 0.006 for each part of a workgroup.
-void split_tiles(int64_t units, int64_t tiles, Plan &p) {
-  int64_t best = 1;
-  double least = 1e300;
-  const int64_t most = ceil_div(tiles, 4) < 64 ? ceil_div(tiles, 4) : 64;
-  for (int64_t k = 1; k <= most; ++k) {
-    const double join = k > 1 ? 2.0 + 0.006 * static_cast<double>(units * k) : 0.0;
-    const double rounds = units * k <= 256 ? 0.65 : static_cast<double>(ceil_div(units * k, int64_t(512)));
-    const double time = rounds * static_cast<double>(ceil_div(tiles, k)) + join;
-    if (time < least) {
-      least = time;
-      best = k;
-    }
-  }
-  p.split_tiles = static_cast<int32_t>(ceil_div(tiles, best));
-  p.splits = static_cast<int32_t>(ceil_div(tiles, p.split_tiles));
 }
 
 constexpr int64_t kShare = 512;  // workgroups that share the steps: two a CU
@@ -553,13 +506,14 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
              "%s: too many query rows", what);
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   UC_REQUIRE(units * ceil_div(capacity, int64_t(kStep)) < (1 << 30), "%s: too many keys in all", what);
-  p.workgroups = 0;
-  p.splits = 1;
-  p.split_tiles = 0;
   if (p.rows == kTileRows) {
-    split_tiles(units, keys > 0 ? ceil_div(keys, int64_t(64)) : 1, p);
-    UC_REQUIRE(tile_workgroups(cache->sequences * cache->heads_kv * p.splits, p.groups) < (1 << 24), "%s: too many query rows",
-               what);
+    // four tiles a workgroup at least, and two workgroups a CU at most; each XCD takes as many
+    const int64_t tiles = units * (keys > 0 ? ceil_div(keys, int64_t(kKeys)) : 1);
+    p.workgroups = 0;
+    if (cache->sequences * p.groups <= kMostShared && units * ceil_div(capacity, int64_t(kKeys)) < (1 << 30)) {
+      p.workgroups = static_cast<int32_t>(tiles < 4 * kShare ? ceil_div(tiles, int64_t(32)) * 8 : kShare);
+    }
+    UC_REQUIRE(units < (1 << 24), "%s: too many query rows", what);
     return UC_OK;
   }
   const int64_t steps = units * ceil_div(keys, int64_t(kStep));
@@ -568,8 +522,9 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
 }
 
 int64_t part_rows(const uc_paged_cache *cache, const Plan &p) {
-  const int64_t units = cache->sequences * cache->heads_kv * p.groups;
-  return p.workgroups > 0 ? (units + p.workgroups) * p.rows : p.splits > 1 ? units * p.splits * p.rows : 0;
+  // (of many rows, a workgroup's first and last unit may be parts)
+  if (p.rows == kTileRows) return int64_t(2) * p.workgroups * p.rows;
+  return (cache->sequences * cache->heads_kv * p.groups + p.workgroups) * p.rows;
 }
 
 }  // namespace
@@ -610,7 +565,7 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);
   // parts of a row, if all sequences were of the expected length
-  const bool few = (p.workgroups > 0 ? ceil_div(p.workgroups, units) : p.splits) <= 8;
+  const bool few = ceil_div(p.workgroups, units) <= 8;
   auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
     auto rows_launch = [&](auto kernel) {
@@ -618,8 +573,7 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
                          static_cast<uint16_t *>(out), lse, part, stat);
     };
     if (p.rows == kTileRows) {
-      const int rc = launch_tiles(what, DT, D, c, q, p, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
-      if (rc != UC_OK || p.splits == 1) return rc;
+      return launch_tiles(what, DT, D, c, q, p, static_cast<uint16_t *>(out), lse, part, stat, as_stream(stream));
     } else if (p.rows == 16) {
       rows_launch(rows_kernel<D, DT, 1>);
     } else if (p.rows == 32) {

@@ -20,8 +20,6 @@ namespace uc {
 namespace pg {
 namespace {
 
-constexpr int kKeys = 64;  // of a tile
-
 template <int D>
 struct Tile {
   static constexpr int kKeyRow = D * 2, kValueRow = kKeys * 2;      // bytes
@@ -186,6 +184,98 @@ __device__ __forceinline__ float weights(const f4 (&s)[4], int half, float facto
   return l;
 }
 
+// The tiles of all units, ordered by KV head, sequence and row group, are cut into runs of equal length for the
+// workgroups: calls of any lengths and any number of units load them alike, and only a run's first and last
+// unit may be parts, joined by a second launch.  (Causal rows see fewer keys the earlier they are, so units differ.)
+// `flat` counts the row groups of all sequences.
+__device__ __forceinline__ int32_t tiles_of(const Cache &c, const Query &q, const Plan &p, int32_t flat) {
+  if (flat >= c.sequences * p.groups) return 0;
+  const int32_t s = flat / p.groups;
+  return (rows_at(q, s, 0, flat - s * p.groups, kTileRows, c.length(s), q.count(s)).end_last + kKeys - 1) / kKeys;
+}
+
+// For a whole wave: tiles of a head, of its units before `flat`, and of that.
+struct Sums {
+  int32_t total, before, mine;
+
+  __device__ __forceinline__ Sums(const Cache &c, const Query &q, const Plan &p, int32_t flat) : total(0), before(0), mine(0) {
+    for (int32_t f0 = 0; f0 < c.sequences * p.groups; f0 += 64) {
+      const int32_t n = tiles_of(c, q, p, f0 + (threadIdx.x & 63)), sum = wave_prefix(n);
+      if (flat >= f0 && flat < f0 + 64) {
+        mine = __builtin_amdgcn_readlane(n, flat - f0);
+        before = total + __builtin_amdgcn_readlane(sum, flat - f0) - mine;
+      }
+      total += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  __device__ __forceinline__ int32_t per(const Cache &c, const Plan &p) const {
+    const int32_t n = (total * c.heads + p.workgroups - 1) / p.workgroups;
+    return n > 0 ? n : 1;
+  }
+};
+
+// Where a workgroup leaves a part: that of its first unit, or that of its last.
+__device__ __forceinline__ int32_t slot_of(int32_t run, bool first) { return 2 * run + (first ? 0 : 1); }
+
+// A workgroup's way through its run.
+struct Walk {
+  int32_t h, flat, tiles;       // the unit, and its tiles
+  int32_t begin, end;           // those of them that are the workgroup's
+  int32_t left;                 // tiles of the run from `begin` on
+  bool first;
+
+  __device__ __forceinline__ Walk(const Cache &c, const Query &q, const Plan &p, int32_t run) : begin(0), first(true) {
+    if (p.workgroups == 0) {  // a unit
+      const int32_t flats = c.sequences * p.groups;
+      h = run / flats;
+      flat = run - h * flats;
+      tiles = end = left = __builtin_amdgcn_readfirstlane(tiles_of(c, q, p, flat));
+      if (left == 0) left = 1;  // (rows without keys are finished too)
+      return;
+    }
+    const Sums sums(c, q, p, 0);
+    const int32_t per = sums.per(c, p), all = sums.total * c.heads, at = run * per;
+    left = at + per < all ? per : all - at;
+    if (left <= 0) return;
+    h = at / sums.total;
+    int32_t rest = at - h * sums.total;
+    for (flat = 0;; flat += 64) {
+      const int32_t n = tiles_of(c, q, p, flat + (threadIdx.x & 63)), sum = wave_prefix(n);
+      const uint64_t past = __ballot(sum > rest);
+      if (past != 0) {
+        const int32_t i = __builtin_ctzll(past);
+        tiles = __builtin_amdgcn_readlane(n, i);
+        begin = rest - (__builtin_amdgcn_readlane(sum, i) - tiles);
+        flat += i;
+        break;
+      }
+      rest -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    end = tiles - begin < left ? tiles : begin + left;
+  }
+  __device__ __forceinline__ bool more() const { return left > 0; }
+  __device__ __forceinline__ void next(const Cache &c, const Query &q, const Plan &p) {
+    left -= p.workgroups == 0 ? left : end - begin;
+    if (left <= 0) return;
+    do {
+      if (++flat == c.sequences * p.groups) {
+        flat = 0;
+        ++h;
+      }
+      tiles = __builtin_amdgcn_readfirstlane(tiles_of(c, q, p, flat));
+    } while (tiles == 0);  // (there are `left` more)
+    begin = 0;
+    end = tiles < left ? tiles : left;
+    first = false;
+  }
+  __device__ __forceinline__ Rows rows(const Cache &c, const Query &q, const Plan &p) const {
+    const int32_t s = flat / p.groups;
+    return rows_at(q, s, h, flat - s * p.groups, kTileRows, c.length(s), q.count(s));
+  }
+  __device__ __forceinline__ bool part() const { return end - begin != tiles; }
+  __device__ __forceinline__ int32_t slot(int32_t run) const { return slot_of(run, first); }
+};
+
 template <int D, int DT, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse, float *part,
                                                       float *stat) {
@@ -204,20 +294,14 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       __builtin_amdgcn_s_setprio(0);
     }
   };
-  // Workgroups go to the 8 XCDs in turn.  A list is one split of the keys of one (sequence, head); its row
-  // groups are dealt into `deal` hands so that 8 divides the number of hands, and an XCD plays whole hands: its
-  // L2 then holds the keys of few lists.
-  const int32_t lists = c.sequences * c.heads * p.splits, deal = 8 / (lists & 7 ? lists & -lists : 8);
-  const int32_t slots = (p.groups + deal - 1) / deal, x = blockIdx.x & 7, at = blockIdx.x >> 3, turn = at / slots;
-  const int32_t hand = x + 8 * turn, list = hand % lists, group = (at - turn * slots) * deal + hand / lists;
-  if (group >= p.groups || hand >= lists * deal) return;
-  const int32_t split = list % p.splits, sh = list / p.splits, s_index = sh / c.heads;
-  // the later rows of a causal call see more keys: the longest first
-  const int32_t row_group = q.causal ? p.groups - 1 - group : group, unit = sh * p.groups + row_group;
-  const Rows w = rows_at(q, s_index, sh - s_index * c.heads, row_group, kTileRows, c.length(s_index), q.count(s_index));
-  const int32_t tiles = (w.end_last + kKeys - 1) / kKeys, per = split_tiles_of(p, tiles);
-  const int32_t begin = split * per, end = begin + per < tiles ? begin + per : tiles;
-  if (begin >= end && split > 0) return;
+  // Workgroups go to the 8 XCDs in turn; an XCD takes runs that follow each other, so that its L2 holds the keys of few heads.
+  const int32_t run = p.workgroups == 0 ? blockIdx.x : (blockIdx.x & 7) * (p.workgroups / 8) + (blockIdx.x >> 3);
+  Walk walk(c, q, p, run);
+  const Loader<D> ld;
+  const int krow = (col >> 2) * 8 + (col & 3);
+  for (; walk.more(); walk.next(c, q, p)) {
+  const Rows w = walk.rows(c, q, p);
+  const int32_t begin = walk.begin, end = walk.end;
   Pages pages(c, w.s);
   const int64_t head = int64_t(w.h << c.shift) * D;
   const uint16_t *key = c.key + head, *value = c.value + head;
@@ -243,7 +327,6 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
   }
   // LDS offsets of the fragments: key tile j adds (32 (j / 2) + 4 (j % 2)) rows, channel tile n 16 rows
-  const int krow = (col >> 2) * 8 + (col & 3);
   int ka[D / 32], va[2];
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) ka[k] = krow * T::kKeyRow + 16 * ((4 * k + quad) ^ key_swizzle<D>(krow));
@@ -252,7 +335,6 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 
   Staged<D> st;
   Entries<D, WHOLE> entries;  // of the tile after the staged one
-  const Loader<D> ld;
   // whether every row sees all keys of the staged tile
   auto whole = [&] {
     return st.t + kKeys <= w.end_first && st.absent == 0;
@@ -356,8 +438,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
     const float total = mf::sum_over_slices(acc[n].l);
     if (r >= w.rows) continue;
-    if (p.splits > 1) {
-      const int64_t slot = (int64_t(unit) * p.splits + split) * kTileRows + rr;
+    if (walk.part()) {
+      const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(part + slot * D + 16 * d + 4 * quad) = acc[n].o[d];
       if (quad == 0) {
@@ -379,28 +461,62 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       }
     }
   }
+  }
+}
+
+// Units in parts are joined by a workgroup each, and those without keys finished: 16 lanes a row, 16 rows at a time.
+template <int D, int DT>
+__global__ __launch_bounds__(256) void tile_join_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
+                                                        const float *part, const float *stat) {
+  constexpr int kC = D / 16;
+  const int32_t unit = blockIdx.x, flats = c.sequences * p.groups, h = unit / flats, flat = unit - h * flats;
+  const Sums sums(c, q, p, flat);
+  const int32_t per = sums.per(c, p), start = h * sums.total + sums.before, stop = start + sums.mine;
+  const int32_t w0 = start / per, w1 = sums.mine == 0 ? w0 - 1 : (stop - 1) / per;
+  if (w1 == w0) return;
+  const int32_t s = flat / p.groups, lane = threadIdx.x & 15;
+  const Rows w = rows_at(q, s, h, flat - s * p.groups, kTileRows, c.length(s), q.count(s));
+  for (int32_t rr = threadIdx.x >> 4; rr < kTileRows && w.r0 + rr < w.rows; rr += 16) {
+    float m = mf::kNegInf, l = 0.0f, o[kC];
+#pragma unroll
+    for (int j = 0; j < kC; ++j) o[j] = 0.0f;
+    for (int32_t i = w0; i <= w1; ++i) {
+      const int64_t at = int64_t(slot_of(i, i > w0 || start == w0 * per)) * kTileRows + rr;
+      const float mi = stat[2 * at], li = stat[2 * at + 1];
+      if (mi == mf::kNegInf && li == 0.0f) continue;
+      const float top = fmaxf(m, mi), f = m == mf::kNegInf ? 0.0f : mf::fast_exp2(m - top), fi = mf::fast_exp2(mi - top);
+      m = top;
+      l = l * f + li * fi;
+#pragma unroll
+      for (int j = 0; j < kC / 4; ++j) {
+        const f4 x = *reinterpret_cast<const f4 *>(part + at * D + lane * kC + 4 * j);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[4 * j + u] = o[4 * j + u] * f + x[u] * fi;
+      }
+    }
+    store_row<D, DT>(q, w, w.r0 + rr, lane * kC, o, m, l, out, lse);
+  }
 }
 
 }  // namespace
 
-int64_t tile_workgroups(int64_t lists, int64_t groups) {
-  const int64_t deal = 8 / (lists & 7 ? lists & -lists : 8);  // (the hands may be one row group longer than they need to be)
-  return ceil_div(lists * deal, int64_t(8)) * 8 * ceil_div(groups, deal);
-}
-
 int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, const Query &q, const Plan &p, uint16_t *out,
                  float *lse, float *part, float *stat, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>(tile_workgroups(int64_t(c.sequences) * c.heads * p.splits, p.groups)));
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, c, q, p, out, lse, part, stat); };
-  auto by_page = [&](auto d_tag, auto dt_tag) {
+  const int32_t units = c.sequences * c.heads * p.groups;
+  const dim3 grid(static_cast<uint32_t>(p.workgroups > 0 ? p.workgroups : units));
+  auto go = [&](auto kernel, dim3 workgroups) {
+    hipLaunchKernelGGL(kernel, workgroups, dim3(256), 0, stream, c, q, p, out, lse, part, stat);
+    return check_launch(what);
+  };
+  auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
-    c.page >= kKeys ? go(tile_kernel<D, DT, true>) : go(tile_kernel<D, DT, false>);
+    const int rc = c.page >= kKeys ? go(tile_kernel<D, DT, true>, grid) : go(tile_kernel<D, DT, false>, grid);
+    return rc != UC_OK || p.workgroups == 0 ? rc : go(tile_join_kernel<D, DT>, dim3(units));
   };
   auto by_type = [&](auto d_tag) {
-    dtype == UC_FP16 ? by_page(d_tag, std::integral_constant<int, UC_FP16>()) : by_page(d_tag, std::integral_constant<int, UC_BF16>());
+    return dtype == UC_FP16 ? run(d_tag, std::integral_constant<int, UC_FP16>()) : run(d_tag, std::integral_constant<int, UC_BF16>());
   };
-  head_dim == 128 ? by_type(std::integral_constant<int, 128>()) : by_type(std::integral_constant<int, 64>());
-  return check_launch(what);
+  return head_dim == 128 ? by_type(std::integral_constant<int, 128>()) : by_type(std::integral_constant<int, 64>());
 }
 
 }  // namespace pg
