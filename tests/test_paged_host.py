@@ -164,6 +164,7 @@ def _rotary():
     rotary = MultiAxisRotary.__new__(MultiAxisRotary)
     rotary.head_dim, rotary.pairs, rotary.num_axes, rotary.pairing = 64, 32, 2, "halves"
     rotary._turns, rotary._axis = torch.zeros(32, dtype=torch.float64), torch.zeros(32, dtype=torch.int32)
+    rotary._tables, rotary._adjacent = (16, 16), 0
     rotary.device = rotary._turns.device
     return rotary
 

@@ -391,6 +391,7 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def stream(device: torch.device) -> int:
@@ -404,8 +405,11 @@ def stream(device: torch.device) -> int:
 def call_on(device: torch.device, name: str, *args) -> None:
     """An entry point on the current stream of `device`, whatever the current device is."""
 
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream(device))
+    index = device.index
+    if index == _current_device():
+        rc = getattr(_lib or load_library(), name)(*args, _raw_stream(index) if _raw_stream else stream(device))
+        if rc != UC_OK:
+            check(rc, name)
     else:
         with torch.cuda.device(device):
             call(name, *args, stream(device))

@@ -331,13 +331,25 @@ __global__ __launch_bounds__(kThreads) void thin_scan_kernel(Cache c, Thin t) {
   const uint8_t *keep = t.keep + s * t.stride;
   if (threadIdx.x == 0) lost = length;
   int32_t kept = 0;
-  for (int32_t t0 = 0; t0 < length; t0 += kThreads) {
-    const int32_t token = t0 + threadIdx.x;
-    const bool there = token < length, stays = there && (token >= t.tokens || keep[token] != 0);
+  // eight tokens a thread and round
+  for (int32_t t0 = 0; t0 < length; t0 += 8 * kThreads) {
+    const int32_t token = t0 + 8 * threadIdx.x;
+    uint32_t stays = 0;  // a bit each
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int32_t at = token + i;
+      if (at < length && (at >= t.tokens || keep[at] != 0)) stays |= 1u << i;
+    }
     int32_t total;
-    const int32_t sum = block_prefix(stays, total, waves);
-    if (stays) source[kept + sum - 1] = token;
-    if (there && !stays) atomicMin(&lost, token);
+    const int32_t count = __popc(stays), sum = block_prefix(count, total, waves);
+    int32_t to = kept + sum - count;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (stays & (1u << i)) source[to++] = token + i;
+    }
+    const int32_t there = length - token >= 8 ? 8 : length > token ? length - token : 0;
+    const uint32_t gone = ~stays & ((1u << there) - 1u);
+    if (gone != 0) atomicMin(&lost, token + __ffs(gone) - 1);
     kept += total;
   }
   __syncthreads();

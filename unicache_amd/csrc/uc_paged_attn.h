@@ -119,48 +119,65 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // Values that are not finite, in tiles that not every row sees whole: a hidden key's weight is 0, and 0 times them is
-// NaN.  So the products take 0 in their place, and a second product counts, for each row, the keys that it
-// does see of each kind; one is enough to make the sum what it is.
+// NaN.  So where there are any the products take 0 in their place, and others count, for each row,
+// the keys that it does see of each kind; one is enough to make the sum what it is.
 template <int DT>
 constexpr uint32_t kInfinity = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
 
-// A fragment with zeros in their place; whether there was any in the wave.
+// Not 0 where a half of w is not finite: its exponent and 1 overflow into the sign.
 template <int DT>
-__device__ __forceinline__ bool take_finite(typename Half<DT>::V8 &v) {
-  constexpr uint32_t e = kInfinity<DT>;
-  u4 w = __builtin_bit_cast(u4, v);
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t bad = ((w[i] & e) == e ? 0xffffu : 0u) | ((w[i] & (e << 16)) == e << 16 ? 0xffff0000u : 0u);
-    any |= bad;
-    w[i] &= ~bad;
-  }
-  v = __builtin_bit_cast(typename Half<DT>::V8, w);
-  return __any(any != 0);
+__device__ __forceinline__ uint32_t infinite_bits(uint32_t w) {
+  constexpr uint32_t e = kInfinity<DT>, one = DT == UC_FP16 ? 0x0400u : 0x0080u;
+  return ((w & (e | e << 16)) + (one | one << 16)) & 0x80008000u;
 }
 
-// What the others of fragment v do to rows that see the first `seen` of a lane's eight keys.
+// w with zeros in the place of halves that are not finite.
 template <int DT>
-__device__ __forceinline__ void add_infinite(typename Half<DT>::V8 v, int32_t seen, f4 &o) {
+__device__ __forceinline__ uint32_t finite_half(uint32_t w) {
+  const uint32_t b = infinite_bits<DT>(w);
+  return w & ~((b >> 15) * 0xffffu);
+}
+
+// A bit for each of a lane's outputs, 4 d + i: the row sees an infinity (or a negative one) there; both for NaN.
+struct Infinite {
+  uint32_t up, down;
+};
+
+// What fragment v, of the outputs' fragment d, holds of them for rows that see the first `seen` of a lane's eight keys.
+template <int DT>
+__device__ __forceinline__ void note_infinite(typename Half<DT>::V8 v, int32_t seen, int d, Infinite &x) {
   typedef typename Half<DT>::T T;
+  typedef typename Half<DT>::V8 V8;
   constexpr uint32_t e = kInfinity<DT>;
-  typename Half<DT>::V8 sees;
   const u4 u = __builtin_bit_cast(u4, v);
+  V8 sees, up, down;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sees[j] = static_cast<T>(j < seen ? 1.0f : 0.0f);
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t h = j % 2 ? u[j / 2] >> 16 : u[j / 2] & 0xffffu, size = h & 0x7fffu;
+    sees[j] = static_cast<T>(j < seen ? 1.0f : 0.0f);
+    up[j] = static_cast<T>(size > e || h == e ? 1.0f : 0.0f);
+    down[j] = static_cast<T>(size > e || h == (e | 0x8000u) ? 1.0f : 0.0f);
+  }
+  const f4 a = Half<DT>::mfma(up, sees, f4{0, 0, 0, 0}), b = Half<DT>::mfma(down, sees, f4{0, 0, 0, 0});
 #pragma unroll
-  for (int kind = 0; kind < 3; ++kind) {  // infinity, its negative, NaN
-    typename Half<DT>::V8 is;
+  for (int i = 0; i < 4; ++i) {
+    x.up |= (a[i] > 0.0f ? 1u : 0u) << (4 * d + i);
+    x.down |= (b[i] > 0.0f ? 1u : 0u) << (4 * d + i);
+  }
+}
+
+// And to the sums of finite values.
+template <int N>
+__device__ __forceinline__ void add_infinite(f4 (&o)[N], const Infinite &x) {
+  if (__builtin_expect(!__any((x.up | x.down) != 0), true)) return;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t x = j % 2 ? u[j / 2] >> 16 : u[j / 2] & 0xffffu;
-      is[j] = static_cast<T>((kind == 0 ? x == e : kind == 1 ? x == (e | 0x8000u) : (x & 0x7fffu) > e) ? 1.0f : 0.0f);
+  for (int d = 0; d < N; ++d) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t bit = 1u << (4 * d + i);
+      o[d][i] += (x.up & bit) != 0 ? __builtin_huge_valf() : 0.0f;
+      o[d][i] -= (x.down & bit) != 0 ? __builtin_huge_valf() : 0.0f;
     }
-    const f4 count = Half<DT>::mfma(is, sees, f4{0, 0, 0, 0});
-    const float add = kind == 0 ? __builtin_huge_valf() : kind == 1 ? -__builtin_huge_valf() : __builtin_nanf("");
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += count[i] > 0.0f ? add : 0.0f;
   }
 }
 

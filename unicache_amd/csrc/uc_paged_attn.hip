@@ -118,7 +118,7 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], floa
 template <int D, int DT, int NR>
 struct Joined {
   static constexpr bool kHeld = NR * D >= 192;
-  float o[4][16][D + 4];
+  float o[4][16][D + 4];  // (a wave's part holds a tile's values, 8 D / 32 dwords a lane)
   float m[4][16], l[4][16];
   typename Half<DT>::V8 frag[kHeld ? NR * D / 32 : 1][64];
 };
@@ -155,8 +155,10 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
   V8 frag[NR][D / 32];
   int32_t row_end[NR];
   Acc<D> acc[NR];
+  Infinite infinite[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
+    infinite[n] = Infinite{0, 0};
     const int32_t r = w.r0 + 16 * n + col;
     const int32_t token = token_of(q, r);
     const bool there = r < w.rows && token < w.count;
@@ -175,7 +177,6 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
   }
   typedef Joined<D, DT, NR> J;
   if constexpr (J::kHeld) {
-    __syncthreads();  // the fragments of the piece before have been read
     if (wave == 0) {
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
@@ -214,16 +215,54 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     for (int n = 0; n < NR; ++n) {
       softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
     }
+    if constexpr (MASK) {
+      // what lies behind the length is no value
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) {
-      V8 v = value_fragment<D, DT>(raw, d);
-      if constexpr (MASK) {
-        const V8 all = v;
-        if (take_finite<DT>(v)) {
+      for (int j = 0; j < 8; ++j) {
+        const bool held = there && mine + j < w.length;
 #pragma unroll
-          for (int n = 0; n < NR; ++n) add_infinite<DT>(all, there ? row_end[n] - mine : 0, acc[n].o[d]);
+        for (int i = 0; i < D / 32; ++i) raw.v[j][i] = held ? raw.v[j][i] : 0u;
+      }
+      if (w.end_first != w.end_last) {  // some rows see more than others
+        uint32_t bad = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) bad |= infinite_bits<DT>(raw.v[j][i]);
+        }
+        if (__builtin_expect(__any(bad != 0), false)) {
+// (a loop over the fragments, through the wave's part of the LDS that the join takes: it is rare, and written
+          // out it takes the registers that the other tiles need)
+          uint32_t *held = reinterpret_cast<uint32_t *>(joined.o[wave]) + lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) held[(j * (D / 32) + i) * 64] = raw.v[j][i];
+          }
+#pragma unroll 1
+          for (int d = 0; d < D / 16; ++d) {
+            u4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t a = held[(2 * j * (D / 32) + d / 2) * 64], b = held[((2 * j + 1) * (D / 32) + d / 2) * 64];
+              v[j] = d % 2 ? halves_of<true>(a, b) : halves_of<false>(a, b);
+            }
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+              note_infinite<DT>(__builtin_bit_cast(V8, v), there ? row_end[n] - mine : 0, d, infinite[n]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) raw.v[j][i] = finite_half<DT>(raw.v[j][i]);
+          }
         }
       }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const V8 v = value_fragment<D, DT>(raw, d);
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
         acc[n].o[d] = H::mfma(v, high[n], acc[n].o[d]);
@@ -245,6 +284,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const float l_row = mf::sum_over_slices(acc[n].l);
+    add_infinite(acc[n].o, infinite[n]);
     __syncthreads();  // what was joined before has been read
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -290,6 +330,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
       store_row<D, DT>(q, w, r, c0, o, m, total, out, lse);
     }
   }
+  __syncthreads();  // the next piece may write what has been read here
 }
 
 // The steps of all units ((sequence, head, group) in order) are cut into runs of equal length for the
@@ -497,7 +538,8 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
             query->causal != 0, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kTileRows;
+  p.rows = rows <= 64 ? static_cast<int32_t>(ceil_div(rows, int64_t(16))) * 16 : kTileRows;
+  if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
   const int64_t capacity = c.capacity(), keys = query->max_tokens < capacity ? query->max_tokens : capacity;
   // a launch has less than 2^32 threads, and 32-bit counts of rows and steps
@@ -578,6 +620,8 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
       rows_launch(rows_kernel<D, DT, 1>);
     } else if (p.rows == 32) {
       rows_launch(rows_kernel<D, DT, 2>);
+    } else if (p.rows == 48) {
+      rows_launch(rows_kernel<D, DT, 3>);
     } else {
       rows_launch(rows_kernel<D, DT, 4>);
     }

@@ -124,6 +124,18 @@ __device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const
   }
 }
 
+// What lies behind the length is no value.
+template <int D>
+__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t length) {
+  const bool there = ((st.absent >> ld.wave) & 1) == 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const bool held = there && st.t + 8 * ld.group + j < length;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) st.v[j][i] = held ? st.v[j][i] : 0u;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ void store_values(const Staged<D> &st, char *buf, const Loader<D> &ld) {
 #pragma unroll
@@ -304,13 +316,15 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   const int32_t begin = walk.begin, end = walk.end;
   Pages pages(c, w.s);
   const int64_t head = int64_t(w.h << c.shift) * D;
-  const uint16_t *key = c.key + head, *value = c.value + head;
+  const uint16_t *keys = c.key + head, *values = c.value + head;
 
   V8 frag[2][D / 32];
   int32_t row_end[2];
   Acc16<D> acc[2];
+  Infinite infinite[2];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
+    infinite[n] = Infinite{0, 0};
     const int32_t r = w.r0 + wave * 32 + n * 16 + col, token = token_of(q, r);
     const bool there = r < w.rows && token < w.count;
     row_end[n] = there ? visible(q, w.length, w.count, token) : 0;
@@ -345,9 +359,13 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     constexpr bool MASK = decltype(mask_tag)::value;
     const char *buf = lds + present * T::kBytes;
     const int32_t t0 = st.t;
+    auto value = [&](int h, int d) {
+      // (at 128 channels the chunks' order of channels 16 on is the first's with 4 changed)
+      return *reinterpret_cast<const V8 *>(buf + ((D == 128 ? h ^ (d & 1) : h) ? va[1] : va[0]) + d * 16 * T::kValueRow);
+    };
     const uint32_t absent = st.absent;
     const bool more = t + 1 < end;
-    if (more) fetch<D, WHOLE>(st, c, entries, key, value, ld, (t + 1) * kKeys);
+    if (more) fetch<D, WHOLE>(st, c, entries, keys, values, ld, (t + 1) * kKeys);
     ask(entries, pages, ld, (t + 2) * kKeys);
 
     __builtin_amdgcn_s_setprio(3);
@@ -382,34 +400,42 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     weigh(0);
     weigh(1);
     present ^= 1;
+    if (MASK && w.end_first != w.end_last) {  // some rows see more keys than others
+      u4 *held = reinterpret_cast<u4 *>(lds + (present ^ 1) * T::kBytes + T::kKeyBytes);
+      uint32_t bad = 0;
+      for (int i = lane; i < T::kValueBytes / 16; i += 64) {
+        const u4 v = held[i];
+        bad |= infinite_bits<DT>(v[0]) | infinite_bits<DT>(v[1]) | infinite_bits<DT>(v[2]) | infinite_bits<DT>(v[3]);
+      }
+      if (__builtin_expect(__any(bad != 0), false)) {  // (the same in every wave)
+#pragma unroll 1
+        for (int i = 0; i < D / 8; ++i) {
+          const int d = i >> 1, h = i & 1;
+          const V8 v = value(h, d);
+          note_infinite<DT>(v, h ? seen[0][1] : seen[0][0], d, infinite[0]);
+          note_infinite<DT>(v, h ? seen[1][1] : seen[1][0], d, infinite[1]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < T::kValueBytes / 16; i += 256) {
+          u4 v = held[i];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = finite_half<DT>(v[k]);
+          held[i] = v;
+        }
+        __syncthreads();
+      }
+    }
+    if (more && !whole()) clear_values<D>(st, ld, w.length);
     __builtin_amdgcn_s_setprio(3);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      auto load = [&](int d) {
-        // (at 128 channels the chunks' order of channels 16 on is the first's with 4 changed)
-        return *reinterpret_cast<const V8 *>(buf + va[D == 128 ? h ^ (d & 1) : h] + d * 16 * T::kValueRow);
-      };
-      if constexpr (MASK) {
+      V8 a[D / 16];
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          V8 a = load(d);
-          const V8 all = a;
-          if (take_finite<DT>(a)) {
-            add_infinite<DT>(all, seen[0][h], acc[0].o[d]);
-            add_infinite<DT>(all, seen[1][h], acc[1].o[d]);
-          }
-          acc[0].o[d] = H::mfma(a, pr[0][h], acc[0].o[d]);
-          acc[1].o[d] = H::mfma(a, pr[1][h], acc[1].o[d]);
-        }
-      } else {
-        V8 a[D / 16];
+      for (int d = 0; d < D / 16; ++d) a[d] = value(h, d);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) a[d] = load(d);
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d) {
-          acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
-          acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
-        }
+      for (int d = 0; d < D / 16; ++d) {
+        acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
+        acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
       }
       // (after the last tile the present one's again, into the buffer that nobody reads)
       if (h == 0) store_keys<D>(st, lds + present * T::kBytes, ld);
@@ -423,7 +449,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   st.absent = 0;
   if (begin < end) {
     ask(entries, pages, ld, begin * kKeys);
-    fetch<D, WHOLE>(st, c, entries, key, value, ld, begin * kKeys);
+    fetch<D, WHOLE>(st, c, entries, keys, values, ld, begin * kKeys);
+    if (!whole()) clear_values<D>(st, ld, w.length);
     ask(entries, pages, ld, (begin + 1) * kKeys);
     store_keys<D>(st, lds, ld);
     store_values<D>(st, lds, ld);
@@ -437,6 +464,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   for (int n = 0; n < 2; ++n) {
     const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
     const float total = mf::sum_over_slices(acc[n].l);
+    add_infinite(acc[n].o, infinite[n]);
     if (r >= w.rows) continue;
     if (walk.part()) {
       const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;

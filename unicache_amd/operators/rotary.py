@@ -13,6 +13,7 @@ from torch.autograd import forward_ad
 from .. import _native as nat
 
 _HALVES = (torch.bfloat16, torch.float16)
+_POSITION_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
 def check_rows(t: torch.Tensor, what: str) -> None:
@@ -78,27 +79,30 @@ class MultiAxisRotary:
         turns = [f / (2.0 * math.pi) for f in frequencies]
         self._turns = torch.tensor(turns, dtype=torch.float64, device=device)
         self._axis = torch.tensor(axes, dtype=torch.int32, device=device)
+        self._tables = self._turns.data_ptr(), self._axis.data_ptr()
+        self._adjacent = 1 if pairing == "adjacent" else 0
         self.device = self._turns.device
 
     def plan(self, positions: torch.Tensor | None, sequences: int, tokens: int, *, inverse: bool = False):
         """The C plan for [axes, sequences, tokens] positions (None: a cache's own), and the tensor it points to."""
 
-        size = 0
+        size, at = 0, None
         if positions is not None:
-            if positions.dtype not in (torch.int32, torch.int64):
+            size = _POSITION_BYTES.get(positions.dtype, 0)
+            if not size:
                 raise ValueError(f"Rotary positions must be int32 or int64 (got {positions.dtype})")
             if positions.dim() == 2 and sequences == 1:
                 positions = positions.unsqueeze(1)
-            if tuple(positions.shape) != (self.num_axes, sequences, tokens):
+            if positions.shape != (self.num_axes, sequences, tokens):
                 raise ValueError(f"Rotary positions must be [{self.num_axes}, {sequences}, {tokens}] (axes, sequences, "
                                  f"tokens), got {tuple(positions.shape)}")
             if positions.device != self.device:
                 raise RuntimeError(f"Rotary positions must be on the plan's device {self.device}")
-            positions = positions.contiguous()
-            size = positions.element_size()
-        struct = nat.RotaryPlan(self._turns.data_ptr(), self._axis.data_ptr(), nat.ptr(positions), self.num_axes,
-                                self.pairs, size, 1 if self.pairing == "adjacent" else 0, 1 if inverse else 0, 0)
-        return struct, positions
+            if not positions.is_contiguous():
+                positions = positions.contiguous()
+            at = positions.data_ptr()
+        return nat.RotaryPlan(*self._tables, at, self.num_axes, self.pairs, size, self._adjacent,
+                              1 if inverse else 0, 0), positions
 
     def rotate(self, query: torch.Tensor, key: torch.Tensor | None = None, *, positions: torch.Tensor,
                inverse: bool = False):

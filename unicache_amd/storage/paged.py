@@ -23,6 +23,7 @@ from ..operators.rotary import MultiAxisRotary, check_rows
 from .physical import tensor_bytes
 
 _PAGES = (16, 32, 64, 128, 256)
+_TENSORS = frozenset(("key", "value", "table", "lengths", "granted", "references", "free_pages"))
 _SIZES = "Paged cache supports pages of 16, 32, 64, 128 or 256 tokens and head_dim 64 or 128"
 
 
@@ -116,10 +117,16 @@ class PagedKVCache:
         self.dtype, self.device = key.dtype, key.device
         self._sizes = (self.layers, self.pages, self.sequences, self.sequence_pages, self.num_kv_heads, self.head_dim,
                        self.page_tokens, nat.dtype_code(key.dtype))
+        self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._workspaces = {}
         self.max_tokens = self.capacity if max_tokens is None else min(int(max_tokens), self.capacity)
         # (refuses sizes that the kernels do not take)
-        _workspace_bytes("uc_paged_attn_workspace_bytes", self._sizes, False,
-                         (0, self.num_kv_heads, 0, self._sizes[-1], 0))
+        self._attention_workspace((0, self.num_kv_heads, 0, self._sizes[-1], 0))
+
+    def __setattr__(self, name, value) -> None:
+        object.__setattr__(self, name, value)
+        if name in _TENSORS:  # the C struct of the tensors is made again
+            object.__setattr__(self, "_built", None)
 
     @property
     def capacity(self) -> int:
@@ -166,15 +173,26 @@ class PagedKVCache:
 
     # ------------------------------------------------------------- internals --
     def _layer(self, layer) -> int:
-        layer = int(layer)
+        if layer.__class__ is not int:
+            layer = int(layer)
         if not 0 <= layer < self.layers:
             raise ValueError(f"Paged cache has layers 0 .. {self.layers - 1} (got {layer})")
         return layer
 
     def _struct(self) -> "nat.PagedCache":
-        return nat.PagedCache(self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(),
-                              self.lengths.data_ptr(), nat.ptr(self.granted), nat.ptr(self.references),
-                              nat.ptr(self.free_pages), *self._sizes)
+        if self._built is None:
+            self._built = nat.PagedCache(self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(),
+                                         self.lengths.data_ptr(), nat.ptr(self.granted), nat.ptr(self.references),
+                                         nat.ptr(self.free_pages), *self._sizes)
+        return self._built
+
+    def _attention_workspace(self, sizes: tuple) -> int:
+        nbytes = self._workspaces.get(sizes)
+        if nbytes is None:
+            if len(self._workspaces) >= 256:
+                self._workspaces.clear()
+            nbytes = self._workspaces[sizes] = _workspace_bytes("uc_paged_attn_workspace_bytes", self._sizes, False, sizes)
+        return nbytes
 
     def _numbers(self, t: torch.Tensor, what: str) -> torch.Tensor:
         """int32 of each sequence, on the cache's device."""
@@ -185,21 +203,24 @@ class PagedKVCache:
             raise RuntimeError(f"Paged cache {what} must be on the cache's device {self.device}")
         return t
 
-    def _rows(self, t: torch.Tensor, what: str, heads: int | None = None) -> torch.Tensor:
-        """Checked dense rows [S, n, H, D]."""
+    def _rows(self, t: torch.Tensor, what: str, heads: int | None = None):
+        """Checked dense rows [S, n, H, D] as the kernels read them, and their strides."""
 
-        if t.dim() == 3 and self.sequences == 1:
+        shape = t.shape
+        if len(shape) == 3 and self.sequences == 1:
             t = t.unsqueeze(0)
-        if (t.dim() != 4 or t.shape[0] != self.sequences or t.shape[3] != self.head_dim or not t.shape[2]
-                or (heads is not None and t.shape[2] != heads)):
+            shape = t.shape
+        if (len(shape) != 4 or shape[0] != self.sequences or shape[3] != self.head_dim or not shape[2]
+                or (heads is not None and shape[2] != heads)):
             raise ValueError(f"Paged cache {what}: expected [{self.sequences}, tokens, {heads or 'heads'}, "
-                             f"{self.head_dim}], got {tuple(t.shape)}")
+                             f"{self.head_dim}], got {tuple(shape)}")
         if t.dtype != self.dtype:
             raise ValueError(f"Paged cache {what} must have the cache's dtype {self.dtype} (got {t.dtype})")
-        check_rows(t, f"Paged cache {what}")
+        if t.requires_grad or forward_ad._current_level >= 0:
+            check_rows(t, f"Paged cache {what}")
         if t.device != self.device:
             raise RuntimeError(f"Paged cache {what} must be on the cache's device {self.device}")
-        return t
+        return nat.rows16(t)
 
     def _allocator(self, what: str) -> None:
         if self.references is None:
@@ -284,17 +305,15 @@ class PagedKVCache:
         `positions` [axes, S, n] (int32 or int64) default to each token's place in its sequence."""
 
         layer = self._layer(layer)
-        key = self._rows(key, "keys", self.num_kv_heads)
-        value = self._rows(value, "values", self.num_kv_heads)
         if key.shape != value.shape:
             raise ValueError("Paged cache write expects keys and values of one shape")
-        n = int(key.shape[1])
+        key, k_s, k_t, k_h = self._rows(key, "keys", self.num_kv_heads)
+        value, v_s, v_t, v_h = self._rows(value, "values", self.num_kv_heads)
+        n = key.shape[1]
         counts = self.granted if counts is None else self._numbers(counts, "counts")
-        if rotary is None and (query is not None or positions is not None):
-            raise ValueError("Paged cache write takes queries and positions with a rotary")
-        plan = held = out = None
-        q = [None, 0, 0, 0, 0, None]
-        flat = query is not None and query.dim() == 3
+        plan = held = out = at = None
+        q_s = q_t = q_h = heads = 0
+        flat = False
         if rotary is not None:
             if rotary.head_dim != self.head_dim:
                 raise ValueError(f"Paged cache write: the rotary is for head_dim {rotary.head_dim}")
@@ -302,17 +321,19 @@ class PagedKVCache:
                 raise RuntimeError(f"Paged cache write: the rotary must be on the cache's device {self.device}")
             plan, held = rotary.plan(positions, self.sequences, n)
             if query is not None:
-                query = self._rows(query, "queries")
+                flat = query.dim() == 3
+                query, q_s, q_t, q_h = self._rows(query, "queries")
+                heads = query.shape[2]
                 if query.shape[1] != n:
                     raise ValueError("Paged cache write expects as many queries as keys")
-                query, *strides = nat.rows16(query)
                 out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
-                q = [query.data_ptr(), *strides, int(query.shape[2]), out.data_ptr()]
-        (key, *k_strides), (value, *v_strides) = nat.rows16(key), nat.rows16(value)
+                at = out.data_ptr()
+        elif query is not None or positions is not None:
+            raise ValueError("Paged cache write takes queries and positions with a rotary")
         if n:
-            nat.call_on(self.device, "uc_paged_write", self._struct(), layer, key.data_ptr(), *k_strides,
-                        value.data_ptr(), *v_strides, n, nat.ptr(counts),
-                        None if plan is None else ctypes.byref(plan), *q)
+            nat.call_on(self.device, "uc_paged_write", self._struct(), layer, key.data_ptr(), k_s, k_t, k_h,
+                        value.data_ptr(), v_s, v_t, v_h, n, nat.ptr(counts), plan, nat.ptr(query), q_s, q_t, q_h, heads,
+                        at)
         return out[0] if flat else out
 
     def attention(self, query: torch.Tensor, *, layer: int = 0, query_lengths: torch.Tensor | None = None,
@@ -328,25 +349,28 @@ class PagedKVCache:
         see never reach it, whatever they hold."""
 
         layer = self._layer(layer)
-        sm_scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else ctypes.c_float(float(sm_scale)).value
-        if not 0.0 < sm_scale <= 2.0 ** 127:
-            raise ValueError("Paged attention sm_scale must be positive, and 2^127 at most (as fp32)")
+        if sm_scale is None:
+            sm_scale = self._scale
+        else:
+            sm_scale = ctypes.c_float(float(sm_scale)).value
+            if not 0.0 < sm_scale <= 2.0 ** 127:
+                raise ValueError("Paged attention sm_scale must be positive, and 2^127 at most (as fp32)")
         flat = query.dim() == 3
-        query = self._rows(query, "queries")
-        lq, hq = int(query.shape[1]), int(query.shape[2])
+        query, a, b, c = self._rows(query, "queries")
+        shape = query.shape
+        lq, hq = shape[1], shape[2]
         if hq % self.num_kv_heads:
             raise ValueError("Query heads must be divisible by the cache's KV heads")
         if query_lengths is not None:
             query_lengths = self._numbers(query_lengths, "query_lengths")
-        query, a, b, c = nat.rows16(query)
         sizes = (lq, hq, self.max_tokens, self._sizes[-1], 1 if causal else 0)
-        nbytes = _workspace_bytes("uc_paged_attn_workspace_bytes", self._sizes, False, sizes)
-        ws = nat.workspace(self.device, nbytes)
-        out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
+        nbytes = self._attention_workspace(sizes)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        out = torch.empty(shape, dtype=self.dtype, device=self.device)
         lse = torch.empty((self.sequences, hq, lq), dtype=torch.float32, device=self.device)
         struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), *sizes[2:])
         nat.call_on(self.device, "uc_paged_attn", self._struct(), layer, struct, sm_scale, out.data_ptr(),
-                    lse.data_ptr(), ws.data_ptr(), nbytes)
+                    lse.data_ptr(), nat.ptr(ws), nbytes)
         return (out[0], lse[0]) if flat else (out, lse)
 
     def dense(self, *, layer: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
