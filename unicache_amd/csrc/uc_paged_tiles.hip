@@ -492,38 +492,47 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   }
 }
 
-// Units in parts are joined by a workgroup each, and those without keys finished: 16 lanes a row, 16 rows at a time.
+// Units in parts are joined, and those without keys finished: a workgroup takes 16 rows of a unit, 16 lanes each.
 template <int D, int DT>
 __global__ __launch_bounds__(256) void tile_join_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse,
                                                         const float *part, const float *stat) {
-  constexpr int kC = D / 16;
+  constexpr int kC = D / 16, kAhead = 4;  // parts on their way
   const int32_t unit = blockIdx.x, flats = c.sequences * p.groups, h = unit / flats, flat = unit - h * flats;
   const Sums sums(c, q, p, flat);
   const int32_t per = sums.per(c, p), start = h * sums.total + sums.before, stop = start + sums.mine;
   const int32_t w0 = start / per, w1 = sums.mine == 0 ? w0 - 1 : (stop - 1) / per;
   if (w1 == w0) return;
-  const int32_t s = flat / p.groups, lane = threadIdx.x & 15;
+  const int32_t s = flat / p.groups, lane = threadIdx.x & 15, rr = blockIdx.y * 16 + (threadIdx.x >> 4);
   const Rows w = rows_at(q, s, h, flat - s * p.groups, kTileRows, c.length(s), q.count(s));
-  for (int32_t rr = threadIdx.x >> 4; rr < kTileRows && w.r0 + rr < w.rows; rr += 16) {
-    float m = mf::kNegInf, l = 0.0f, o[kC];
+  if (w.r0 + rr >= w.rows) return;
+  auto slot = [&](int32_t i) { return int64_t(slot_of(i, i > w0 || start == w0 * per)) * kTileRows + rr; };
+  float m = mf::kNegInf, l = 0.0f, o[kC];
 #pragma unroll
-    for (int j = 0; j < kC; ++j) o[j] = 0.0f;
-    for (int32_t i = w0; i <= w1; ++i) {
-      const int64_t at = int64_t(slot_of(i, i > w0 || start == w0 * per)) * kTileRows + rr;
-      const float mi = stat[2 * at], li = stat[2 * at + 1];
-      if (mi == mf::kNegInf && li == 0.0f) continue;
-      const float top = fmaxf(m, mi), f = m == mf::kNegInf ? 0.0f : mf::fast_exp2(m - top), fi = mf::fast_exp2(mi - top);
-      m = top;
-      l = l * f + li * fi;
+  for (int j = 0; j < kC; ++j) o[j] = 0.0f;
+  for (int32_t i = w0 + lane; i <= w1; i += 16) m = fmaxf(m, stat[2 * slot(i)]);
 #pragma unroll
-      for (int j = 0; j < kC / 4; ++j) {
-        const f4 x = *reinterpret_cast<const f4 *>(part + at * D + lane * kC + 4 * j);
+  for (int x = 1; x < 16; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, kWave));
+  for (int32_t i0 = w0; i0 <= w1; i0 += kAhead) {
+    float mi[kAhead], li[kAhead];
+    f4 x[kAhead][kC / 4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) o[4 * j + u] = o[4 * j + u] * f + x[u] * fi;
-      }
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t at = slot(i0 + u <= w1 ? i0 + u : w1);
+      mi[u] = stat[2 * at];
+      li[u] = stat[2 * at + 1];
+#pragma unroll
+      for (int j = 0; j < kC / 4; ++j) x[u][j] = *reinterpret_cast<const f4 *>(part + at * D + lane * kC + 4 * j);
     }
-    store_row<D, DT>(q, w, w.r0 + rr, lane * kC, o, m, l, out, lse);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u > w1 || (mi[u] == mf::kNegInf && li[u] == 0.0f)) continue;
+      const float f = mf::fast_exp2(mi[u] - m);
+      l += li[u] * f;
+#pragma unroll
+      for (int j = 0; j < kC; ++j) o[j] += x[u][j / 4][j % 4] * f;
+    }
   }
+  store_row<D, DT>(q, w, w.r0 + rr, lane * kC, o, m, l, out, lse);
 }
 
 }  // namespace
@@ -539,7 +548,7 @@ int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, 
   auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
     const int rc = c.page >= kKeys ? go(tile_kernel<D, DT, true>, grid) : go(tile_kernel<D, DT, false>, grid);
-    return rc != UC_OK || p.workgroups == 0 ? rc : go(tile_join_kernel<D, DT>, dim3(units));
+    return rc != UC_OK || p.workgroups == 0 ? rc : go(tile_join_kernel<D, DT>, dim3(units, kTileRows / 16));
   };
   auto by_type = [&](auto d_tag) {
     return dtype == UC_FP16 ? run(d_tag, std::integral_constant<int, UC_FP16>()) : run(d_tag, std::integral_constant<int, UC_BF16>());
