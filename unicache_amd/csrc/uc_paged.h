@@ -18,8 +18,9 @@ struct Cache {
   __host__ __device__ __forceinline__ int32_t capacity() const { return width << shift; }
 
   // Tokens of sequence s; a length outside [0, capacity] reads as the nearer end.
-  __device__ __forceinline__ int32_t length(int32_t s) const {
-    const int32_t n = lengths[s], most = capacity();
+  __device__ __forceinline__ int32_t length(int32_t s) const { return clamped(lengths[s]); }
+  __device__ __forceinline__ int32_t clamped(int32_t n) const {
+    const int32_t most = capacity();
     return n < 0 ? 0 : n > most ? most : n;
   }
   // Pages that n tokens take.

@@ -25,12 +25,16 @@ struct Query {
   float scale;  // sm_scale * log2(e)
   FastDiv by_group;
 
-  __device__ __forceinline__ int32_t count(int32_t s) const {
-    if (lens == nullptr) return len;
-    const int32_t n = lens[s];
-    return n < 0 ? 0 : n > len ? len : n;
-  }
+  __device__ __forceinline__ int32_t count(int32_t s) const { return lens == nullptr ? len : clamped(lens[s]); }
+  __device__ __forceinline__ int32_t clamped(int32_t n) const { return n < 0 ? 0 : n > len ? len : n; }
 };
+
+// A sequence's length and number of queries, both on their way at once.
+__device__ __forceinline__ void sizes_of(const Cache &c, const Query &q, int32_t s, int32_t &length, int32_t &count) {
+  const int32_t n = c.lengths[s], m = (q.lens != nullptr ? q.lens : c.lengths)[s];
+  length = c.clamped(n);
+  count = q.lens != nullptr ? q.clamped(m) : q.len;
+}
 
 constexpr int kTileRows = 128;            // rows of a unit of many (uc_paged_tiles.hip)
 
@@ -92,7 +96,9 @@ struct Pages {
 
 // The first row of a head's tokens t .. in their page, in elements from its first in page 0; -1 where there is no page.
 __device__ __forceinline__ int64_t place_of(const Cache &c, int32_t entry, int32_t t, int32_t d) {
-  return c.is_page(entry) ? int64_t(entry) * c.page_elems + (t & (c.page - 1)) * d : -1;
+  const bool is = c.is_page(entry);
+  const int64_t at = int64_t(is ? entry : 0) * c.page_elems + (t & (c.page - 1)) * d;
+  return is ? at : -1;
 }
 
 // 16-bit operands.

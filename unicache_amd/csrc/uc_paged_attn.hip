@@ -138,6 +138,26 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
   l.key = c.key + head + (8 * ((col >> 2) & 1) + (col & 3)) * D + quad * 8;
   l.value = c.value + head + 8 * (quad & 1) * D + col * (D / 16);
 
+  V8 frag[NR][D / 32];
+  int32_t row_end[NR];
+  Acc<D> acc[NR];
+  Infinite infinite[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int32_t r = w.r0 + 16 * n + col;
+    const bool there = r < w.rows;
+    // (rows past the last are the first's again, and nobody's)
+    const int32_t at = there ? r : w.r0, token = token_of(q, at);
+    row_end[n] = there ? visible(q, w.length, w.count, token) : 0;
+    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + at - token * q.group) * q.sh + quad * 8;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) frag[n][k] = *reinterpret_cast<const V8 *>(p + k * 32);
+    acc[n].m = mf::kNegInf;
+    acc[n].l = 0.0f;
+    infinite[n] = Infinite{0, 0};
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
+  }
   const int32_t stop = end * kStep < w.end_last ? end * kStep : w.end_last;
   int32_t t = begin * kStep + wave * kTile;
   Raw<D> raw;
@@ -145,35 +165,14 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
   int64_t first_a = -1, first_b = -1;
   int32_t entry_a = 0, entry_b = 0;
   if (t < stop) {
-    first_a = place_of(c, pages.of(t), t, D);
-    first_b = place_of(c, pages.of(t + 16), t + 16, D);
+    entry_a = pages.of(t);
+    entry_b = pages.of(t + 16);
+    first_a = place_of(c, entry_a, t, D);
+    first_b = place_of(c, entry_b, t + 16, D);
     load_keys(raw, l, first_a, first_b);
     load_values(raw, l, first_a, first_b);
     entry_a = pages.of(t + kStep);
     entry_b = pages.of(t + kStep + 16);
-  }
-  V8 frag[NR][D / 32];
-  int32_t row_end[NR];
-  Acc<D> acc[NR];
-  Infinite infinite[NR];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    infinite[n] = Infinite{0, 0};
-    const int32_t r = w.r0 + 16 * n + col;
-    const int32_t token = token_of(q, r);
-    const bool there = r < w.rows && token < w.count;
-    row_end[n] = there ? visible(q, w.length, w.count, token) : 0;
-    const uint16_t *p = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r - token * q.group) * q.sh + quad * 8;
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      uint4 v = {0, 0, 0, 0};
-      if (there) v = *reinterpret_cast<const uint4 *>(p + k * 32);
-      frag[n][k] = __builtin_bit_cast(V8, v);
-    }
-    acc[n].m = mf::kNegInf;
-    acc[n].l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D / 16; ++d) acc[n].o[d] = f4{0, 0, 0, 0};
   }
   typedef Joined<D, DT, NR> J;
   if constexpr (J::kHeld) {
@@ -193,8 +192,6 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     auto query = [&](int n, int k) { return J::kHeld ? joined.frag[n * (D / 32) + k][at] : frag[n][k]; };
     const bool more = t + kStep < stop;
     const int64_t next_a = place_of(c, entry_a, t + kStep, D), next_b = place_of(c, entry_b, t + kStep + 16, D);
-    entry_a = pages.of(t + 2 * kStep);
-    entry_b = pages.of(t + 2 * kStep + 16);
     f4 s[NR][2];
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
@@ -208,6 +205,11 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
       }
     }
     if (more) load_keys(raw, l, next_a, next_b);
+    // (asked for here: LDS reads and scalar loads are waited for together, and none of the former follows for a while)
+    __builtin_amdgcn_sched_barrier(0);
+    entry_a = pages.of(t + 2 * kStep);
+    entry_b = pages.of(t + 2 * kStep + 16);
+    __builtin_amdgcn_sched_barrier(0);
     const int32_t mine = t + 8 * quad;                              // the lane's first key
     const bool there = ((quad & 2) ? first_b : first_a) >= 0;              // and its page
     V8 high[NR], low[NR];
@@ -352,8 +354,8 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   int32_t length = 0, count = 0, steps = 0, sum = 0, total = 0;
   auto fill = [&] {
     const int32_t i = s0 + lane;
-    length = i < c.sequences ? c.length(i) : 0;
-    count = i < c.sequences ? q.count(i) : 0;
+    length = count = 0;
+    if (i < c.sequences) sizes_of(c, q, i, length, count);
     steps = steps_of(length, count);
     sum = wave_prefix(steps);
   };
@@ -420,19 +422,24 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
   x.r = index - sh * full;
   const int32_t group = p.groups == 1 ? 0 : x.r / p.rows, each = c.heads * p.groups;
   const int32_t unit = sh * p.groups + group;
-  int32_t total = 0, before = 0, mine = 0;
+  int32_t total = 0, before = 0, mine = 0, my_length = 0, my_count = 0;
   for (int32_t s0 = 0; s0 < c.sequences; s0 += 64) {
     const int32_t i = s0 + (threadIdx.x & 63);
-    const int32_t n = i < c.sequences ? steps_of(c.length(i), q.count(i)) : 0;
+    int32_t length = 0, count = 0;
+    if (i < c.sequences) sizes_of(c, q, i, length, count);
+    const int32_t n = steps_of(length, count);
     const int32_t sum = wave_prefix(n);
     const int32_t m = __shfl(n, s - s0, kWave), b = __shfl(sum, s - s0, kWave);
+    const int32_t ml = __shfl(length, s - s0, kWave), mc = __shfl(count, s - s0, kWave);
     if (s >= s0 && s < s0 + 64) {
       mine = m;
       before = total + b - m;
+      my_length = ml;
+      my_count = mc;
     }
     total += __builtin_amdgcn_readlane(sum, 63);
   }
-  x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, c.length(s), q.count(s));
+  x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, my_length, my_count);
   const int32_t per = per_of(p, total * each);
   const int32_t start = before * each + (unit - s * each) * mine;
   x.first = mine == 0 ? 0 : start / per + unit;
@@ -549,11 +556,12 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   UC_REQUIRE(units * ceil_div(capacity, int64_t(kStep)) < (1 << 30), "%s: too many keys in all", what);
   if (p.rows == kTileRows) {
-    // four tiles a workgroup at least, and two workgroups a CU at most; each XCD takes as many
-    const int64_t tiles = units * (keys > 0 ? ceil_div(keys, int64_t(kKeys)) : 1);
+    // Two workgroups a CU at most, as many on each XCD, of four tiles at least; two where that leaves a unit in 16 parts at
+    // most (50 queries of 500 tokens 20.5 -> 16.4 us; 20 of 10,000 33 with four, 39 with two).
+    const int64_t each = keys > 0 ? ceil_div(keys, int64_t(kKeys)) : 1, least = each <= 32 ? 2 : 4, tiles = units * each;
     p.workgroups = 0;
     if (cache->sequences * p.groups <= kMostShared && units * ceil_div(capacity, int64_t(kKeys)) < (1 << 30)) {
-      p.workgroups = static_cast<int32_t>(tiles < 4 * kShare ? ceil_div(tiles, int64_t(32)) * 8 : kShare);
+      p.workgroups = static_cast<int32_t>(tiles < least * kShare ? ceil_div(tiles, 8 * least) * 8 : kShare);
     }
     UC_REQUIRE(units < (1 << 24), "%s: too many query rows", what);
     return UC_OK;

@@ -203,7 +203,9 @@ __device__ __forceinline__ float weights(const f4 (&s)[4], int half, float facto
 __device__ __forceinline__ int32_t tiles_of(const Cache &c, const Query &q, const Plan &p, int32_t flat) {
   if (flat >= c.sequences * p.groups) return 0;
   const int32_t s = flat / p.groups;
-  return (rows_at(q, s, 0, flat - s * p.groups, kTileRows, c.length(s), q.count(s)).end_last + kKeys - 1) / kKeys;
+  int32_t length, count;
+  sizes_of(c, q, s, length, count);
+  return (rows_at(q, s, 0, flat - s * p.groups, kTileRows, length, count).end_last + kKeys - 1) / kKeys;
 }
 
 // For a whole wave: tiles of a head, of its units before `flat`, and of that.
@@ -282,7 +284,9 @@ struct Walk {
   }
   __device__ __forceinline__ Rows rows(const Cache &c, const Query &q, const Plan &p) const {
     const int32_t s = flat / p.groups;
-    return rows_at(q, s, h, flat - s * p.groups, kTileRows, c.length(s), q.count(s));
+    int32_t length, count;
+    sizes_of(c, q, s, length, count);
+    return rows_at(q, s, h, flat - s * p.groups, kTileRows, length, count);
   }
   __device__ __forceinline__ bool part() const { return end - begin != tiles; }
   __device__ __forceinline__ int32_t slot(int32_t run) const { return slot_of(run, first); }
@@ -325,16 +329,14 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     infinite[n] = Infinite{0, 0};
-    const int32_t r = w.r0 + wave * 32 + n * 16 + col, token = token_of(q, r);
-    const bool there = r < w.rows && token < w.count;
+    const int32_t r = w.r0 + wave * 32 + n * 16 + col;
+    const bool there = r < w.rows;
+    // (rows past the last are the first's again, and nobody's)
+    const int32_t at = there ? r : w.r0, token = token_of(q, at);
     row_end[n] = there ? visible(q, w.length, w.count, token) : 0;
-    const uint16_t *row = q.p + w.s * q.ss + token * q.st + (w.h * q.group + r - token * q.group) * q.sh + quad * 8;
+    const uint16_t *row = q.p + w.s * q.ss + token * q.st + (w.h * q.group + at - token * q.group) * q.sh + quad * 8;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      uint4 v = {0, 0, 0, 0};
-      if (there) v = *reinterpret_cast<const uint4 *>(row + k * 32);
-      frag[n][k] = __builtin_bit_cast(V8, v);
-    }
+    for (int k = 0; k < D / 32; ++k) frag[n][k] = *reinterpret_cast<const V8 *>(row + k * 32);
     acc[n].m = mf::kNegInf;
     acc[n].l = 0.0f;
 #pragma unroll
@@ -366,7 +368,6 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     const uint32_t absent = st.absent;
     const bool more = t + 1 < end;
     if (more) fetch<D, WHOLE>(st, c, entries, keys, values, ld, (t + 1) * kKeys);
-    ask(entries, pages, ld, (t + 2) * kKeys);
 
     __builtin_amdgcn_s_setprio(3);
     f4 s[2][4];
@@ -381,6 +382,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       }
     }
     vector_phase();
+    // (asked for here: LDS reads and scalar loads are waited for together, and none of the former follows for a while)
+    __builtin_amdgcn_sched_barrier(0);
+    ask(entries, pages, ld, (t + 2) * kKeys);
+    __builtin_amdgcn_sched_barrier(0);
     V8 pr[2][2];
     float m[2];
     int32_t seen[2][2];
