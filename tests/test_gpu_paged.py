@@ -565,12 +565,14 @@ def test_reserve_write_and_the_end_of_the_pool(device):
     agrees(cache, model, None)
 
 
-@pytest.mark.parametrize("seed,b,pages", [(0, 16, 40), (1, 16, 9), (2, 32, 16), (3, 16, 70), (4, 64, 12)])
-def test_any_order_of_calls_keeps_the_books(device, seed, b, pages):
+@pytest.mark.parametrize("seed,b,pages,room", [(0, 16, 40, 0), (1, 16, 9, 0), (2, 32, 16, 0), (3, 16, 70, 0), (4, 64, 12, 0),
+                                               (5, 16, 40, 900), (6, 32, 20, 900)])
+def test_any_order_of_calls_keeps_the_books(device, seed, b, pages, room):
+    # (with room the table is more than one workgroup takes in reorder)
     import random
 
     rng = random.Random(seed)
-    s, width = 5, 6
+    s, width = 5, 6 + room
     cache = PagedKVCache.empty(s, pages, 1, 64, layers=2, page_tokens=b, sequence_pages=width, dtype=torch.float16)
     model, store = Model(s, pages, width, b), {}
     for step in range(30):
@@ -589,7 +591,7 @@ def test_any_order_of_calls_keeps_the_books(device, seed, b, pages):
             model.write(granted, [[(step, i, j) for j in range(n)] for i in range(s)])
         elif call in ("reorder", "cut"):
             parents = [rng.choice([i, i, rng.randrange(s), rng.randrange(s), -1, s]) for i in range(s)]
-            cut = [rng.choice([-1, 0, rng.randrange(width * b), width * b]) for _ in range(s)] if call == "cut" else None
+            cut = [rng.choice([-1, 0, rng.randrange(6 * b), width * b]) for _ in range(s)] if call == "cut" else None
             cache.reorder(i32(parents), lengths=None if cut is None else i32(cut))
             model.reorder(parents, cut)
         elif call == "truncate":
@@ -597,7 +599,7 @@ def test_any_order_of_calls_keeps_the_books(device, seed, b, pages):
             cache.truncate(i32(cut))
             model.reorder(list(range(s)), cut)
         else:
-            t = rng.choice([0, b, 3 * b, width * b])
+            t = rng.choice([0, b, 3 * b, 6 * b])
             p = rng.choice([0.0, 0.5, 0.95, 1.0])
             keep = [[rng.random() < p if i != 2 else True for _ in range(t)] for i in range(s)]
             cache.compact(torch.tensor(keep, dtype=torch.bool, device=device).view(s, t))
@@ -778,3 +780,42 @@ def test_empty_calls(device):
     cache.truncate(i32([0, 0]))
     cache.reorder(i32([1, 0]))
     assert cache.lengths.tolist() == [0, 0] and (cache.table == -1).all()
+
+
+@pytest.mark.parametrize("lq", [1, 3, 60])
+def test_mixed_attention_over_paged_segments(device, lq):
+    # the adapter's mixed call: dense rows, a packed KIVI segment and two sequences' pages as one softmax
+    from unicache_amd.adapters.bagel import run_batched_physical_attention, run_fused_mixed_attention
+    from unicache_amd.storage import PackedKIVICache
+
+    dk, dv = randn(90, 4, 128, seed=1, scale=0.3), randn(90, 4, 128, seed=2)
+    pk, pv = randn(300, 4, 128, seed=3, scale=0.3), randn(300, 4, 128, seed=4)
+    packed = PackedKIVICache.from_dense(pk, pv, logical_token_ids=torch.arange(300, device=device), token_type_id=0,
+                                        k_bits=4, v_bits=4, group_size=32, residual_length=10, backend="cuda")
+    cache = PagedKVCache.empty(2, 20, 4, 128, layers=2, page_tokens=32)
+    cache.reserve(150, counts=i32([150, 33]))
+    rows = randn(2, 2, 150, 4, 128, seed=5, scale=0.3)
+    values = randn(2, 2, 150, 4, 128, seed=6)
+    for layer in range(2):
+        cache.write(rows[layer], values[layer], layer=layer)
+    first, second = cache.layer(1, sequence=0), cache.layer(1, sequence=1)
+    rk, rv = packed.dequantize()
+    q = randn(lq, 28, 128, seed=7)
+    for segments, keys, vals in (([packed, first, second], [dk, rk, rows[1, 0], rows[1, 1, :33]],
+                                  [dv, rv, values[1, 0], values[1, 1, :33]]), ([second], [dk, rows[1, 1, :33]], [dv, values[1, 1, :33]])):
+        out, lse = run_fused_mixed_attention(q, dk, dv, segments, return_lse=True)
+        k, v = (torch.cat([t.double().cpu() for t in ts]).repeat_interleave(7, dim=1) for ts in (keys, vals))
+        x = torch.einsum("rhd,thd->hrt", q.double().cpu(), k) / math.sqrt(128)
+        want = torch.einsum("hrt,thd->rhd", torch.softmax(x, dim=-1), v)
+        # the tolerances of the other mixed-attention tests: summaries are rounded to bf16 before they are merged
+        assert float((out.double().cpu() - want).abs().max()) < 2e-2
+        assert float((lse.double().cpu() - torch.logsumexp(x, dim=-1)).abs().max()) < 5e-3
+        batched = run_batched_physical_attention(q, dk, dv, [0, lq], [0, 90], [segments])
+        assert torch.equal(batched, out)
+    none = dk[:0]
+    cache.truncate(i32([0, 5]))
+    out, lse = run_fused_mixed_attention(q, none, none, [cache.layer(0, sequence=0)], return_lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+    for bad in (cache, cache.layer(0)):
+        with pytest.raises(ValueError, match="one layer of one sequence"):
+            run_fused_mixed_attention(q, dk, dv, [bad])

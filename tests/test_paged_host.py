@@ -101,7 +101,8 @@ def test_call_checks():
             (lambda: cache.attention(q, sm_scale=math.inf), "sm_scale"),
             (lambda: cache.attention(q, query_lengths=torch.zeros(3)), "query_lengths"),
             (lambda: cache.attention(q.clone().requires_grad_()), "gradient"), (lambda: cache.dense(layer=2), "layers 0"),
-            (lambda: cache.layer(2), "layers 0")):
+            (lambda: cache.layer(2), "layers 0"), (lambda: cache.layer(0, sequence=3), "sequences 0"),
+            (lambda: cache.layer(0, sequence=-1), "sequences 0")):
         with pytest.raises(ValueError, match=match):
             call()
     view = cache.layer(1)

@@ -57,6 +57,12 @@ struct Pool {
   uint32_t *free;
 };
 
+// What atomics of this launch may have changed, past the CU's own cache.
+template <class T>
+__device__ __forceinline__ T fresh(const T *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Inclusive prefix sum over a workgroup of 1024, and its total.
 __device__ __forceinline__ int32_t block_prefix(int32_t v, int32_t &total, int32_t *waves) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -85,7 +91,7 @@ struct Giver {
 __device__ __forceinline__ uint32_t free_word(const Pool &pool, int32_t pages, int32_t w) {
   if (w >= (pages + 31) / 32) return 0;
   const int32_t tail = pages - 32 * w;  // pages of this word
-  return pool.free[w] & (tail >= 32 ? ~0u : (1u << tail) - 1u);
+  return fresh(pool.free + w) & (tail >= 32 ? ~0u : (1u << tail) - 1u);
 }
 
 // Free pages, up to `want`, counted by a whole workgroup.
@@ -201,10 +207,8 @@ __device__ __forceinline__ int32_t parent_of(const Cache &c, const Order &o, int
   return p < 0 || p >= c.sequences ? -1 : p;
 }
 
-// Release what sequences hold no more.  A thread an entry of the table.
-__global__ __launch_bounds__(256) void reorder_release_kernel(Cache c, Pool pool, Order o) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= int64_t(c.sequences) * c.width) return;
+// An entry of the table that its sequence may hold no more is released.
+__device__ __forceinline__ void release_entry(const Cache &c, const Pool &pool, const Order &o, int64_t at) {
   const int32_t s = static_cast<int32_t>(at / c.width), i = static_cast<int32_t>(at - int64_t(s) * c.width);
   const int32_t p = parent_of(c, o, s), length = c.length(s);
   int32_t now = p < 0 ? 0 : c.length(p);
@@ -230,10 +234,8 @@ __global__ __launch_bounds__(256) void reorder_release_kernel(Cache c, Pool pool
   }
 }
 
-// Take hold of what they hold now.
-__global__ __launch_bounds__(256) void reorder_hold_kernel(Cache c, Pool pool, Order o) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= int64_t(c.sequences) * c.width) return;
+// And what its sequence holds now, held.
+__device__ __forceinline__ void hold_entry(const Cache &c, const Pool &pool, const Order &o, int64_t at) {
   const int32_t s = static_cast<int32_t>(at / c.width), i = static_cast<int32_t>(at - int64_t(s) * c.width);
   const int32_t p = parent_of(c, o, s), now = o.length[s], pages = c.pages_of(now);
   if (i >= pages) {
@@ -253,10 +255,8 @@ __global__ __launch_bounds__(256) void reorder_hold_kernel(Cache c, Pool pool, O
   }
 }
 
-// Pages for the copies of open pages, and the new lengths.  One workgroup.
-__global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool pool, Order o) {
-  __shared__ Giver g;
-  extern __shared__ int32_t first[];  // [S]
+// Pages for the copies of open pages, and the new lengths.  One workgroup; first: [S] in LDS.
+__device__ __forceinline__ void open_pages(const Cache &c, const Pool &pool, const Order &o, Giver &g, int32_t *first) {
   int32_t want = 0;
   for (int32_t s0 = 0; s0 < c.sequences; s0 += kThreads) {
     const int32_t s = s0 + threadIdx.x;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool po
       if ((now & (c.page - 1)) != 0) {
         const int32_t open = c.table[int64_t(s) * c.width + c.pages_of(now) - 1];
         // another sequence's, or held whole by one
-        need = c.is_page(open) && (o.owner[open] != s || pool.references[open] != o.opens[open]);
+        need = c.is_page(open) && (fresh(o.owner + open) != s || fresh(pool.references + open) != fresh(o.opens + open));
         o.source[s] = open;
       }
     }
@@ -293,6 +293,37 @@ __global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool po
     c.lengths[s] = now;
   }
 }
+
+// A thread an entry of the table.
+__global__ __launch_bounds__(256) void reorder_release_kernel(Cache c, Pool pool, Order o) {
+  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at < int64_t(c.sequences) * c.width) release_entry(c, pool, o, at);
+}
+
+__global__ __launch_bounds__(256) void reorder_hold_kernel(Cache c, Pool pool, Order o) {
+  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (at < int64_t(c.sequences) * c.width) hold_entry(c, pool, o, at);
+}
+
+__global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool pool, Order o) {
+  __shared__ Giver g;
+  extern __shared__ int32_t first[];
+  open_pages(c, pool, o, g, first);
+}
+
+// All of it by one workgroup, for tables of a few entries a thread (8 sequences forked three times: 24.2 -> KK us a call).
+__global__ __launch_bounds__(kThreads) void reorder_small_kernel(Cache c, Pool pool, Order o) {
+  __shared__ Giver g;
+  extern __shared__ int32_t first[];
+  const int64_t entries = int64_t(c.sequences) * c.width;
+  for (int64_t at = threadIdx.x; at < entries; at += kThreads) release_entry(c, pool, o, at);
+  __syncthreads();  // (one workgroup's accesses, and its atomics' in L2: no fence of a wider scope is needed)
+  for (int64_t at = threadIdx.x; at < entries; at += kThreads) hold_entry(c, pool, o, at);
+  __syncthreads();  // (one workgroup's accesses, and its atomics' in L2: no fence of a wider scope is needed)
+  open_pages(c, pool, o, g, first);
+}
+
+constexpr int64_t kSmallTable = 4 * kThreads;
 
 // The rows of open pages into their copies: a workgroup a (sequence, layer and head).
 __global__ __launch_bounds__(256) void reorder_copy_kernel(Cache c, Order o, int32_t row_bytes) {
@@ -568,13 +599,19 @@ extern "C" int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *pare
   UC_REQUIRE(cache->layers * c.heads * c.sequences < (1 << 24), "%s: too many layers, heads and sequences", what);
   o.parents = parents;
   o.cut = lengths;
-  const uint32_t groups = static_cast<uint32_t>(ceil_div(int64_t(c.sequences) * c.width, int64_t(256)));
-  hipLaunchKernelGGL(reorder_release_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
-  if (int rc = check_launch(what)) return rc;
-  hipLaunchKernelGGL(reorder_hold_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
-  if (int rc = check_launch(what)) return rc;
-  hipLaunchKernelGGL(reorder_open_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, o);
-  if (int rc = check_launch(what)) return rc;
+  const int64_t entries = int64_t(c.sequences) * c.width;
+  if (entries <= kSmallTable) {
+    hipLaunchKernelGGL(reorder_small_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, o);
+    if (int rc = check_launch(what)) return rc;
+  } else {
+    const uint32_t groups = static_cast<uint32_t>(ceil_div(entries, int64_t(256)));
+    hipLaunchKernelGGL(reorder_release_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
+    if (int rc = check_launch(what)) return rc;
+    hipLaunchKernelGGL(reorder_hold_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
+    if (int rc = check_launch(what)) return rc;
+    hipLaunchKernelGGL(reorder_open_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, o);
+    if (int rc = check_launch(what)) return rc;
+  }
   hipLaunchKernelGGL(reorder_copy_kernel, dim3(static_cast<uint32_t>(cache->layers * c.heads), c.sequences), dim3(256), 0,
                      as_stream(stream), c, o, static_cast<int32_t>(cache->head_dim * 2));
   return check_launch(what);

@@ -162,12 +162,19 @@ class PagedKVCache:
                    counts[1], counts[2], words, 0)
         return cache
 
-    def layer(self, index: int) -> "PagedKVCache":
-        """One layer as a cache of its own over the same tensors: to read and write, not to grow or fork."""
+    def layer(self, index: int, *, sequence: int | None = None) -> "PagedKVCache":
+        """One layer (of one sequence) as a cache of its own over the same tensors: to read and write, not to grow or
+        fork.  A segment of run_fused_mixed_attention and run_batched_physical_attention is such a view."""
 
         index = self._layer(index)
+        table, lengths = self.table, self.lengths
+        if sequence is not None:
+            sequence = int(sequence)
+            if not 0 <= sequence < self.sequences:
+                raise ValueError(f"Paged cache has sequences 0 .. {self.sequences - 1} (got {sequence})")
+            table, lengths = table[sequence:sequence + 1], lengths[sequence:sequence + 1]
         view = type(self).__new__(type(self))
-        view._set(self.key[index:index + 1], self.value[index:index + 1], self.table, self.lengths, None, None, None,
+        view._set(self.key[index:index + 1], self.value[index:index + 1], table, lengths, None, None, None,
                   self.max_tokens)
         return view
 
