@@ -489,6 +489,12 @@ def mq_workspace_bytes(heads_kv, head_dim, quantized_tokens, residual_tokens) ->
     return size
 
 
+def empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and dtype, the cheaper way where t is contiguous itself."""
+
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """A caller-owned uint8 workspace from torch's caching allocator."""
 

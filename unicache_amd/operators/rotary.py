@@ -4,7 +4,6 @@ a PagedKVCache.  No reference counterpart: UniCache receives rotated keys."""
 
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -112,32 +111,34 @@ class MultiAxisRotary:
         ``inverse`` turns back, which is also what a gradient of the rotated rows takes."""
 
         flat = query.dim() == 3
-        rows = [t.unsqueeze(0) if t is not None and flat else t for t in (query, key)]
-        for t, what in zip(rows, ("Rotary queries", "Rotary keys")):
-            if t is None:
-                continue
-            if t.dim() != 4 or t.shape[3] != self.head_dim or t.shape[:2] != rows[0].shape[:2] or not t.shape[2]:
-                raise ValueError(f"{what}: expected [sequences, tokens, heads, {self.head_dim}], got {tuple(t.shape)}")
-            check_rows(t, what)
-        if key is not None and key.dtype != query.dtype:
-            raise ValueError("Rotary queries and keys must have one dtype")
+        if flat:
+            query, key = query.unsqueeze(0), None if key is None else key.unsqueeze(0)
         if positions is None:
             raise ValueError("Rotary rows need positions")
-        if nat.require_device(query, key, what="Rotary positions") != self.device:
-            raise RuntimeError(f"Rotary positions: rows must be on the plan's device {self.device}")
-        s, n = int(rows[0].shape[0]), int(rows[0].shape[1])
-        struct, held = self.plan(positions, s, n, inverse=inverse)
-        outs, args = [], []
-        for t in rows:
+        shape, outs, args = query.shape, [], []
+        for t, what in ((query, "Rotary queries"), (key, "Rotary keys")):
             if t is None:
-                args += [None, 0, 0, 0, 0, None]
                 continue
-            t, *strides = nat.rows16(t)
-            out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            if t.dim() != 4 or t.shape[3] != self.head_dim or t.shape[:2] != shape[:2] or not t.shape[2]:
+                raise ValueError(f"{what}: expected [sequences, tokens, heads, {self.head_dim}], got {tuple(t.shape)}")
+            check_rows(t, what)
+            if t.dtype != query.dtype:
+                raise ValueError("Rotary queries and keys must have one dtype")
+        for t in (query, key):
+            if t is None:
+                args += (None, 0, 0, 0, 0, None)
+                continue
+            if t.device.type != "cuda":
+                raise RuntimeError(f"Rotary positions requires GPU tensors (got {t.device})")
+            if t.device != self.device:
+                raise RuntimeError(f"Rotary positions: rows must be on the plan's device {self.device}")
+            t, a, b, c = nat.rows16(t)
+            out = nat.empty_like(t)
             outs.append((t, out))  # (the inputs stay alive until the launch)
-            args += [t.data_ptr(), *strides, int(t.shape[2]), out.data_ptr()]
-        if s and n:
-            nat.call_on(self.device, "uc_rotary", ctypes.byref(struct), s, n, self.head_dim, nat.dtype_code(query.dtype),
-                        *args)
+            args += (t.data_ptr(), a, b, c, t.shape[2], out.data_ptr())
+        struct, held = self.plan(positions, shape[0], shape[1], inverse=inverse)
+        if shape[0] and shape[1]:
+            nat.call_on(self.device, "uc_rotary", struct, shape[0], shape[1], self.head_dim,
+                        nat.dtype_code(query.dtype), *args)
         outs = [out[0] if flat else out for _, out in outs]
         return outs[0] if key is None else tuple(outs)

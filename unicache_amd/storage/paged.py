@@ -333,7 +333,7 @@ class PagedKVCache:
                 heads = query.shape[2]
                 if query.shape[1] != n:
                     raise ValueError("Paged cache write expects as many queries as keys")
-                out = torch.empty(query.shape, dtype=query.dtype, device=self.device)
+                out = nat.empty_like(query)
                 at = out.data_ptr()
         elif query is not None or positions is not None:
             raise ValueError("Paged cache write takes queries and positions with a rotary")
@@ -373,8 +373,8 @@ class PagedKVCache:
         sizes = (lq, hq, self.max_tokens, self._sizes[-1], 1 if causal else 0)
         nbytes = self._attention_workspace(sizes)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-        out = torch.empty(shape, dtype=self.dtype, device=self.device)
-        lse = torch.empty((self.sequences, hq, lq), dtype=torch.float32, device=self.device)
+        out = nat.empty_like(query)
+        lse = query.new_empty((self.sequences, hq, lq), dtype=torch.float32)
         struct = nat.Block8Query(query.data_ptr(), a, b, c, lq, hq, nat.ptr(query_lengths), *sizes[2:])
         nat.call_on(self.device, "uc_paged_attn", self._struct(), layer, struct, sm_scale, out.data_ptr(),
                     lse.data_ptr(), nat.ptr(ws), nbytes)
