@@ -942,10 +942,11 @@ int uc_paged_reserve(const uc_paged_cache *cache, int64_t tokens, const int32_t 
  * lengths[s] tokens where that is less (NULL: uncut).  Pages are shared, not copied, but for open pages: of the
  * sequences that hold one as their open page the lowest keeps it, unless another holds it whole, and the
  * others get copies of its rows in free pages, the lowest first, in order.  Pages held no more are freed before that.
- * A sequence for which no free page is left ends with its whole pages.
+ * A sequence for which no free page is left ends with its whole pages.  max_tokens: how long the caller
+ * expects the longest sequence to be; it shapes the launches only.
  */
-int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *parents, const int32_t *lengths, void *workspace,
-                     int64_t workspace_bytes, uc_stream_t stream);
+int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *parents, const int32_t *lengths, int64_t max_tokens,
+                     void *workspace, int64_t workspace_bytes, uc_stream_t stream);
 
 /* Workspace of uc_paged_reorder; -1 for bad arguments. */
 int64_t uc_paged_reorder_workspace_bytes(const uc_paged_cache *cache);
@@ -954,10 +955,10 @@ int64_t uc_paged_reorder_workspace_bytes(const uc_paged_cache *cache);
  * Each sequence keeps the tokens t with keep[s * keep_stride + t] != 0 (bytes) and those from `tokens` on, in order.
  * Pages before the first that loses a token stay; the kept rows behind them move into free pages, the
  * lowest first, by the sequences in order, and the pages they leave are released after that.  Where the free pages
- * do not suffice, that sequence and those after it keep all their tokens.
+ * do not suffice, that sequence and those after it keep all their tokens.  max_tokens as in uc_paged_reorder.
  */
 int uc_paged_compact(const uc_paged_cache *cache, const uint8_t *keep, int64_t keep_stride, int64_t tokens,
-                     void *workspace, int64_t workspace_bytes, uc_stream_t stream);
+                     int64_t max_tokens, void *workspace, int64_t workspace_bytes, uc_stream_t stream);
 
 /* Workspace of uc_paged_compact; -1 for bad arguments. */
 int64_t uc_paged_compact_workspace_bytes(const uc_paged_cache *cache);

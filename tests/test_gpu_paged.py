@@ -365,6 +365,10 @@ def test_large_logits_and_scales(device):
     check_attention(cache, k, v, lengths, q, None, False, sm_scale=0.5)
     check_attention(cache, k, v, lengths, q * 0, None, False, sm_scale=1e-3)
     check_attention(cache, k, v, lengths, q, None, False, sm_scale=1e-30)
+    # logits past fp32's range are no numbers, and no zeros
+    for lq in (2, 40):
+        out, lse = cache.attention(randn(1, lq, 3, 128, seed=7, dtype=torch.float16, scale=40.0), sm_scale=2.0 ** 127)
+        assert out.isnan().all() and lse.isnan().all()
 
 
 def test_strides_offsets_and_views(device):
@@ -574,8 +578,10 @@ def test_any_order_of_calls_keeps_the_books(device, seed, b, pages, room):
     rng = random.Random(seed)
     s, width = 5, 6 + room
     cache = PagedKVCache.empty(s, pages, 1, 64, layers=2, page_tokens=b, sequence_pages=width, dtype=torch.float16)
+    hints = (1, 4096, cache.capacity)
     model, store = Model(s, pages, width, b), {}
     for step in range(30):
+        cache.max_tokens = hints[step % 3] if room else cache.max_tokens
         call = rng.choice(["reserve", "reserve", "reserve", "reorder", "truncate", "compact", "cut"])
         if call == "reserve":
             counts = [rng.choice([0, 1, b // 2, b, 2 * b + 3]) for _ in range(s)]

@@ -200,8 +200,8 @@ def _calls(c, layer=0):
         lambda: nat.call("uc_paged_write", c, layer, 16, 0, 0, 0, 16, 0, 0, 0, 1, None, None, None, 0, 0, 0, 0, None, None),
         lambda: nat.call("uc_paged_dense", c, layer, 16, 16, 1, None),
         lambda: nat.call("uc_paged_reserve", c, 1, None, None),
-        lambda: nat.call("uc_paged_reorder", c, None, None, 16, BIG, None),
-        lambda: nat.call("uc_paged_compact", c, 16, 0, 1, 16, BIG, None),
+        lambda: nat.call("uc_paged_reorder", c, None, None, 640, 16, BIG, None),
+        lambda: nat.call("uc_paged_compact", c, 16, 0, 1, 640, 16, BIG, None),
     ]
 
 
@@ -242,7 +242,7 @@ def test_layers_and_pools():
 @pytest.mark.parametrize("fields,match", [
     (dict(dtype=nat.UC_FP16), "the cache's dtype"), (dict(heads_q=30), "multiple of KV heads"), (dict(heads_q=0), "multiple"),
     (dict(query_len=-1), "query_len"), (dict(query_len=1 << 24), "query_len"), (dict(max_tokens=-1), "max_tokens"),
-    (dict(query_len=1 << 20), "too many query rows"), (dict(query=None), "16-byte aligned"), (dict(query=8), "16-byte aligned"),
+    (dict(query_len=(1 << 24) - 1), "too many query rows"), (dict(query=None), "16-byte aligned"), (dict(query=8), "16-byte aligned"),
     (dict(q_ss=4), "multiples of 8"), (dict(q_st=7), "multiples of 8"), (dict(q_sh=1), "multiples of 8"),
 ])
 def test_query_validation(fields, match):
@@ -311,9 +311,11 @@ def test_rotary_and_write_validation():
 def test_page_call_validation():
     c = _cache()
     lib = nat.lib()
-    for entry, args in (("uc_paged_reorder", (None, None)), ("uc_paged_compact", (16, 0, 1))):
+    for entry, args in (("uc_paged_reorder", (None, None, 640)), ("uc_paged_compact", (16, 0, 1, 640))):
         need = getattr(lib, entry + "_workspace_bytes")(c)
         assert need > 0 and need % 16 == 0
+        with pytest.raises(ValueError, match="max_tokens"):
+            nat.call(entry, c, *args[:-1], -1, 16, need, None)
         for ws, size in ((16, need - 1), (None, need), (8, need)):
             with pytest.raises(ValueError, match="workspace"):
                 nat.call(entry, c, *args, ws, size, None)
@@ -321,9 +323,9 @@ def test_page_call_validation():
         with pytest.raises(ValueError, match="number of tokens"):
             nat.call("uc_paged_reserve", c, tokens, None, None)
         with pytest.raises(ValueError, match="number of tokens"):
-            nat.call("uc_paged_compact", c, 16, 0, tokens, 16, BIG, None)
+            nat.call("uc_paged_compact", c, 16, 0, tokens, 640, 16, BIG, None)
     with pytest.raises(ValueError, match="keep is NULL"):
-        nat.call("uc_paged_compact", c, None, 0, 5, 16, BIG, None)
+        nat.call("uc_paged_compact", c, None, 0, 5, 640, 16, BIG, None)
     with pytest.raises(ValueError, match="number of tokens"):
         nat.call("uc_paged_dense", c, 0, 16, 16, 641, None)
     with pytest.raises(ValueError, match="aligned"):

@@ -306,9 +306,9 @@ _SIGNATURES = {
     ),
     "uc_paged_dense": (_I, [ctypes.POINTER(PagedCache), _L, _P, _P, _L, _P]),
     "uc_paged_reserve": (_I, [ctypes.POINTER(PagedCache), _L, _P, _P]),
-    "uc_paged_reorder": (_I, [ctypes.POINTER(PagedCache), _P, _P, _P, _L, _P]),
+    "uc_paged_reorder": (_I, [ctypes.POINTER(PagedCache), _P, _P, _L, _P, _L, _P]),
     "uc_paged_reorder_workspace_bytes": (_L, [ctypes.POINTER(PagedCache)]),
-    "uc_paged_compact": (_I, [ctypes.POINTER(PagedCache), _P, _L, _L, _P, _L, _P]),
+    "uc_paged_compact": (_I, [ctypes.POINTER(PagedCache), _P, _L, _L, _L, _P, _L, _P]),
     "uc_paged_compact_workspace_bytes": (_L, [ctypes.POINTER(PagedCache)]),
     "uc_workspace_bytes": (_L, [_I, _L, _L, _L, _L, _L]),
     "uc_kivi_decode_workspace_bytes": (_L, [_L, _I, _I, _L, _L, _L, _L, _L, _L]),

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void reserve_kernel(Cache c, Pool pool, i
 struct Order {
   const int32_t *parents, *cut;
   int32_t *old_table;            // [S, M]
-  int32_t *old_length, *length;  // [S]
+  int32_t *before, *length;      // [S] pages held before; tokens held now
   int32_t *source, *target;      // [S] the open page's copy; target -1: none
   int32_t *owner, *opens;        // [P] of pages that are some sequence's open page: the lowest such sequence, their number
 };
@@ -207,26 +207,41 @@ __device__ __forceinline__ int32_t parent_of(const Cache &c, const Order &o, int
   return p < 0 || p >= c.sequences ? -1 : p;
 }
 
-// An entry of the table that its sequence may hold no more is released.
-__device__ __forceinline__ void release_entry(const Cache &c, const Pool &pool, const Order &o, int64_t at) {
-  const int32_t s = static_cast<int32_t>(at / c.width), i = static_cast<int32_t>(at - int64_t(s) * c.width);
-  const int32_t p = parent_of(c, o, s), length = c.length(s);
-  int32_t now = p < 0 ? 0 : c.length(p);
+// A sequence before and after.
+struct Change {
+  int32_t parent, before, after;  // pages
+  int32_t now;                    // tokens
+};
+
+__device__ __forceinline__ Change change_of(const Cache &c, const Order &o, int32_t s) {
+  Change x;
+  x.parent = parent_of(c, o, s);
+  x.before = c.pages_of(c.length(s));
+  x.now = x.parent < 0 ? 0 : c.length(x.parent);
   if (o.cut != nullptr) {
     const int32_t cut = o.cut[s] < 0 ? 0 : o.cut[s];
-    now = now < cut ? now : cut;
+    x.now = x.now < cut ? x.now : cut;
   }
-  const int32_t entry = c.table[at];
-  o.old_table[at] = entry;
+  x.after = c.pages_of(x.now);
+  return x;
+}
+
+// Entry i of a sequence, which it may hold no more, is released (i from 0 on, one at least).
+__device__ __forceinline__ void release_entry(const Cache &c, const Pool &pool, const Order &o, int32_t s, int32_t i,
+                                              const Change &x) {
+  const int64_t at = int64_t(s) * c.width + i;
   if (i == 0) {
-    o.old_length[s] = length;
-    o.length[s] = now;
+    o.before[s] = x.before;
+    o.length[s] = x.now;
     o.target[s] = -1;
   }
-  const int32_t pages = c.pages_of(now);
-  if (i < c.pages_of(length) && c.is_page(entry) && !(p == s && i < pages)) release(pool, entry);
-  if (i == pages - 1 && (now & (c.page - 1)) != 0) {
-    const int32_t open = c.table[int64_t(p) * c.width + i];
+  if (i < x.before) {
+    const int32_t entry = c.table[at];
+    o.old_table[at] = entry;
+    if (c.is_page(entry) && !(x.parent == s && i < x.after)) release(pool, entry);
+  }
+  if (i == x.after - 1 && (x.now & (c.page - 1)) != 0) {
+    const int32_t open = c.table[int64_t(x.parent) * c.width + i];
     if (c.is_page(open)) {
       o.owner[open] = c.sequences;
       o.opens[open] = 0;
@@ -234,12 +249,13 @@ __device__ __forceinline__ void release_entry(const Cache &c, const Pool &pool, 
   }
 }
 
-// And what its sequence holds now, held.
-__device__ __forceinline__ void hold_entry(const Cache &c, const Pool &pool, const Order &o, int64_t at) {
-  const int32_t s = static_cast<int32_t>(at / c.width), i = static_cast<int32_t>(at - int64_t(s) * c.width);
-  const int32_t p = parent_of(c, o, s), now = o.length[s], pages = c.pages_of(now);
-  if (i >= pages) {
-    if (p != s || i < c.pages_of(o.old_length[s])) c.table[at] = -1;
+// And what it holds now, held.
+__device__ __forceinline__ void hold_entry(const Cache &c, const Pool &pool, const Order &o, int32_t s, int32_t i, int32_t p,
+                                           int32_t before, int32_t now) {
+  const int64_t at = int64_t(s) * c.width + i;
+  const int32_t after = c.pages_of(now);
+  if (i >= after) {
+    if (i < before) c.table[at] = -1;
     return;
   }
   const int32_t entry = o.old_table[int64_t(p) * c.width + i];
@@ -249,7 +265,7 @@ __device__ __forceinline__ void hold_entry(const Cache &c, const Pool &pool, con
       atomicAnd(pool.free + entry / 32, ~(1u << (entry % 32)));
     }
   }
-  if (i == pages - 1 && (now & (c.page - 1)) != 0 && c.is_page(entry)) {
+  if (i == after - 1 && (now & (c.page - 1)) != 0 && c.is_page(entry)) {
     atomicMin(o.owner + entry, s);
     atomicAdd(o.opens + entry, 1);
   }
@@ -294,15 +310,18 @@ __device__ __forceinline__ void open_pages(const Cache &c, const Pool &pool, con
   }
 }
 
-// A thread an entry of the table.
+// A row of workgroups a sequence, a thread an entry.
 __global__ __launch_bounds__(256) void reorder_release_kernel(Cache c, Pool pool, Order o) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at < int64_t(c.sequences) * c.width) release_entry(c, pool, o, at);
+  const int32_t s = blockIdx.y;
+  const Change x = change_of(c, o, s);
+  const int32_t end = x.before > x.after ? x.before : x.after;
+  for (int32_t i = blockIdx.x * 256 + threadIdx.x; i < end || i == 0; i += gridDim.x * 256) release_entry(c, pool, o, s, i, x);
 }
 
 __global__ __launch_bounds__(256) void reorder_hold_kernel(Cache c, Pool pool, Order o) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at < int64_t(c.sequences) * c.width) hold_entry(c, pool, o, at);
+  const int32_t s = blockIdx.y, p = parent_of(c, o, s), before = o.before[s], now = o.length[s], after = c.pages_of(now);
+  const int32_t end = before > after ? before : after;
+  for (int32_t i = blockIdx.x * 256 + threadIdx.x; i < end; i += gridDim.x * 256) hold_entry(c, pool, o, s, i, p, before, now);
 }
 
 __global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool pool, Order o) {
@@ -311,15 +330,29 @@ __global__ __launch_bounds__(kThreads) void reorder_open_kernel(Cache c, Pool po
   open_pages(c, pool, o, g, first);
 }
 
-// All of it by one workgroup, for tables of a few entries a thread (8 sequences forked three times: 24.2 -> KK us a call).
+// All of it by one workgroup, for few entries a thread (8 sequences forked three times: 23.0 -> 20.5 us a call).
 __global__ __launch_bounds__(kThreads) void reorder_small_kernel(Cache c, Pool pool, Order o) {
   __shared__ Giver g;
+  __shared__ int32_t widest;
   extern __shared__ int32_t first[];
-  const int64_t entries = int64_t(c.sequences) * c.width;
-  for (int64_t at = threadIdx.x; at < entries; at += kThreads) release_entry(c, pool, o, at);
+  if (threadIdx.x == 0) widest = 1;
+  __syncthreads();
+  for (int32_t s = threadIdx.x; s < c.sequences; s += kThreads) {
+    const Change x = change_of(c, o, s);
+    atomicMax(&widest, x.before > x.after ? x.before : x.after);
+  }
+  __syncthreads();
+  const int64_t entries = int64_t(c.sequences) * widest;
+  for (int64_t at = threadIdx.x; at < entries; at += kThreads) {
+    const int32_t s = static_cast<int32_t>(at / widest);
+    release_entry(c, pool, o, s, static_cast<int32_t>(at - int64_t(s) * widest), change_of(c, o, s));
+  }
   __syncthreads();  // (one workgroup's accesses, and its atomics' in L2: no fence of a wider scope is needed)
-  for (int64_t at = threadIdx.x; at < entries; at += kThreads) hold_entry(c, pool, o, at);
-  __syncthreads();  // (one workgroup's accesses, and its atomics' in L2: no fence of a wider scope is needed)
+  for (int64_t at = threadIdx.x; at < entries; at += kThreads) {
+    const int32_t s = static_cast<int32_t>(at / widest);
+    hold_entry(c, pool, o, s, static_cast<int32_t>(at - int64_t(s) * widest), parent_of(c, o, s), o.before[s], o.length[s]);
+  }
+  __syncthreads();
   open_pages(c, pool, o, g, first);
 }
 
@@ -345,49 +378,79 @@ struct Thin {
   const uint8_t *keep;
   int64_t stride;
   int32_t tokens;
-  int32_t *source;           // [S, capacity] token that becomes token j
-  int32_t *table;            // [S, M] pages to come
-  int32_t *moves;            // [S M] sequence and page of each page to come, in order
+  int32_t *source;           // [P, page] of each page to come, in order: the tokens that move there
+  int32_t *page;             // [P] the page
+  int32_t *moves;            // [P] its sequence and place in that
+  int32_t *first;            // [S] the first of a sequence's
   int32_t *length;           // [S] tokens before
   int32_t *kept, *whole;     // [S] tokens that stay; leading pages that do
   int32_t *count;            // [1] pages to come
 };
 
-// A sequence's kept tokens, and how many of its pages lose none before the first that does.
-__global__ __launch_bounds__(kThreads) void thin_scan_kernel(Cache c, Thin t) {
-  __shared__ int32_t waves[kThreads / 64];
-  __shared__ int32_t lost;
-  const int32_t s = blockIdx.x, length = c.length(s);
-  int32_t *source = t.source + int64_t(s) * c.capacity();
-  const uint8_t *keep = t.keep + s * t.stride;
-  if (threadIdx.x == 0) lost = length;
-  int32_t kept = 0;
-  // eight tokens a thread and round
-  for (int32_t t0 = 0; t0 < length; t0 += 8 * kThreads) {
-    const int32_t token = t0 + 8 * threadIdx.x;
-    uint32_t stays = 0;  // a bit each
+// Eight tokens of a mask that starts at keep: a bit for each that stays.
+__device__ __forceinline__ uint32_t stays_of(const Thin &t, const uint8_t *keep, int32_t token, int32_t length) {
+  uint32_t stays = 0;
+  if (token + 8 <= length && token + 8 <= t.tokens && (reinterpret_cast<uintptr_t>(keep + token) & 7) == 0) {
+    const uint2 w = *reinterpret_cast<const uint2 *>(keep + token);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int32_t at = token + i;
-      if (at < length && (at >= t.tokens || keep[at] != 0)) stays |= 1u << i;
-    }
-    int32_t total;
-    const int32_t count = __popc(stays), sum = block_prefix(count, total, waves);
-    int32_t to = kept + sum - count;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (stays & (1u << i)) source[to++] = token + i;
-    }
-    const int32_t there = length - token >= 8 ? 8 : length > token ? length - token : 0;
-    const uint32_t gone = ~stays & ((1u << there) - 1u);
-    if (gone != 0) atomicMin(&lost, token + __ffs(gone) - 1);
-    kept += total;
+    for (int i = 0; i < 8; ++i) stays |= (((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu) != 0 ? 1u << i : 0u;
+    return stays;
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int32_t at = token + i;
+    if (at < length && (at >= t.tokens || keep[at] != 0)) stays |= 1u << i;
+  }
+  return stays;
+}
+
+// How many tokens a sequence keeps, and how many of its pages come before the first that loses one.
+__global__ __launch_bounds__(kThreads) void thin_count_kernel(Cache c, Thin t) {
+  __shared__ int32_t lost, kept;
+  const int32_t s = blockIdx.x, length = c.length(s);
+  const uint8_t *keep = t.keep + s * t.stride;
+  if (threadIdx.x == 0) {
+    lost = length;
+    kept = 0;
+  }
+  __syncthreads();
+  int32_t mine = 0, first = length;
+  for (int32_t token = 8 * threadIdx.x; token < length; token += 8 * kThreads) {
+    const uint32_t stays = stays_of(t, keep, token, length);
+    const int32_t there = length - token >= 8 ? 8 : length - token;
+    const uint32_t gone = ~stays & ((1u << there) - 1u);
+    mine += __popc(stays);
+    if (gone != 0 && first == length) first = token + __ffs(gone) - 1;
+  }
+  if (mine != 0) atomicAdd(&kept, mine);
+  if (first != length) atomicMin(&lost, first);
   __syncthreads();
   if (threadIdx.x == 0) {
     t.length[s] = length;
     t.kept[s] = kept;
     t.whole[s] = lost < length ? lost >> c.shift : c.pages_of(length);
+  }
+}
+
+// The tokens that move, page by page.
+__global__ __launch_bounds__(kThreads) void thin_list_kernel(Cache c, Thin t) {
+  __shared__ int32_t waves[kThreads / 64];
+  const int32_t s = blockIdx.x, length = t.length[s], stay = t.whole[s] << c.shift;
+  if (t.kept[s] <= stay) return;  // (also where nothing is lost)
+  const uint8_t *keep = t.keep + s * t.stride;
+  int32_t *source = t.source + (int64_t(t.first[s]) << c.shift) - stay;
+  // (every token of the pages that stay is kept, so the count begins behind them)
+  for (int32_t t0 = stay, kept = stay; t0 < length; t0 += 8 * kThreads) {
+    const int32_t token = t0 + 8 * threadIdx.x;
+    const uint32_t stays = token < length ? stays_of(t, keep, token, length) : 0;
+    int32_t total;
+    const int32_t count = __popc(stays);
+    int32_t to = kept + block_prefix(count, total, waves) - count;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (stays & (1u << i)) source[to++] = token + i;
+    }
+    kept += total;
   }
 }
 
@@ -427,12 +490,12 @@ __global__ __launch_bounds__(kThreads) void thin_give_kernel(Cache c, Pool pool,
     want = most;
   }
   give_pages(pool, c.pages, want, g, [&](int32_t rank, int32_t page) {
-    const int32_t s = taker(first, c.sequences, rank), i = t.whole[s] + rank - first[s];
-    const int64_t at = int64_t(s) * c.width + i;
-    t.table[at] = page;
-    t.moves[rank] = static_cast<int32_t>(at);
+    const int32_t s = taker(first, c.sequences, rank);
+    t.page[rank] = page;
+    t.moves[rank] = s * c.width + t.whole[s] + rank - first[s];
     pool.references[page] = 1;
   });
+  for (int32_t s = threadIdx.x; s < c.sequences; s += kThreads) t.first[s] = first[s];
   if (threadIdx.x == 0) *t.count = want;
 }
 
@@ -441,12 +504,12 @@ __global__ __launch_bounds__(256) void thin_copy_kernel(Cache c, Thin t, int32_t
   const int64_t parts = int64_t(layers) * c.heads, jobs = *t.count * parts;
   const int32_t elems = chunks * 8;
   for (int64_t job = blockIdx.x; job < jobs; job += gridDim.x) {
-    const int32_t at = t.moves[job / parts], part = static_cast<int32_t>(job % parts);
+    const int32_t rank = static_cast<int32_t>(job / parts), at = t.moves[rank], part = static_cast<int32_t>(job % parts);
     const int32_t s = at / c.width, i = at - s * c.width, layer = part / c.heads, head = part - layer * c.heads;
     const int32_t first = i << c.shift, left = t.kept[s] - first, rows = left < c.page ? left : c.page;
-    const int32_t *source = t.source + int64_t(s) * c.capacity() + first;
+    const int32_t *source = t.source + (int64_t(rank) << c.shift);
     const int64_t base = layer * c.layer_elems + int64_t(head) * c.page * elems;
-    const int64_t to = base + int64_t(t.table[at]) * c.page_elems;
+    const int64_t to = base + int64_t(t.page[rank]) * c.page_elems;
     for (int32_t u = threadIdx.x; u < rows * chunks; u += 256) {
       const int32_t row = u / chunks, x = (u - row * chunks) * 8, token = source[row];
       const int32_t page = c.table[int64_t(s) * c.width + (token >> c.shift)];
@@ -459,17 +522,16 @@ __global__ __launch_bounds__(256) void thin_copy_kernel(Cache c, Thin t, int32_t
   }
 }
 
-// The pages left behind are released, and the new ones take their place.  A thread an entry of the table.
+// The pages left behind are released, and the new ones take their place.  A row of workgroups a sequence.
 __global__ __launch_bounds__(256) void thin_commit_kernel(Cache c, Pool pool, Thin t) {
-  const int64_t at = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (at >= int64_t(c.sequences) * c.width) return;
-  const int32_t s = static_cast<int32_t>(at / c.width), i = static_cast<int32_t>(at - int64_t(s) * c.width);
-  const int32_t kept = t.kept[s], held = c.pages_of(t.length[s]);
-  if (i == 0) c.lengths[s] = kept;
-  if (i < t.whole[s] || i >= held) return;
-  const int32_t entry = c.table[at];
-  if (c.is_page(entry)) release(pool, entry);
-  c.table[at] = i < c.pages_of(kept) ? t.table[at] : -1;
+  const int32_t s = blockIdx.y, kept = t.kept[s], held = c.pages_of(t.length[s]), whole = t.whole[s], first = t.first[s];
+  if (blockIdx.x == 0 && threadIdx.x == 0) c.lengths[s] = kept;
+  for (int32_t i = whole + blockIdx.x * 256 + threadIdx.x; i < held; i += gridDim.x * 256) {
+    const int64_t at = int64_t(s) * c.width + i;
+    const int32_t entry = c.table[at];
+    if (c.is_page(entry)) release(pool, entry);
+    c.table[at] = i < c.pages_of(kept) ? t.page[first + i - whole] : -1;
+  }
 }
 
 // ------------------------------------------------------------------ dense --
@@ -500,6 +562,17 @@ int check_pool(const uc_paged_cache *cache, const char *what, Cache &c, Pool &po
   return UC_OK;
 }
 
+int64_t pages_expected(const Cache &c, int64_t max_tokens) {
+  const int64_t n = ceil_div(max_tokens < c.capacity() ? max_tokens : int64_t(c.capacity()), int64_t(c.page));
+  return n > 0 ? n : 1;
+}
+
+// Workgroups for the entries of each sequence: 16 of them at most, which then take more than one entry a thread.
+dim3 entry_groups(const Cache &c, int64_t widest) {
+  const int64_t n = ceil_div(widest, int64_t(256));
+  return dim3(static_cast<uint32_t>(n < 16 ? n : 16), c.sequences);
+}
+
 size_t first_bytes(const Cache &c) { return static_cast<size_t>(c.sequences) * sizeof(int32_t); }
 
 // Workspaces in int32 words, every part on 16 bytes.
@@ -516,7 +589,7 @@ int64_t lay_out(const Cache &c, int32_t *base, Order &o) {
   Parts p;
   const int64_t s = c.sequences;
   o.old_table = base + p.take(s * c.width);
-  o.old_length = base + p.take(s);
+  o.before = base + p.take(s);
   o.length = base + p.take(s);
   o.source = base + p.take(s);
   o.target = base + p.take(s);
@@ -528,9 +601,10 @@ int64_t lay_out(const Cache &c, int32_t *base, Order &o) {
 int64_t lay_out(const Cache &c, int32_t *base, Thin &t) {
   Parts p;
   const int64_t s = c.sequences;
-  t.source = base + p.take(s * c.capacity());
-  t.table = base + p.take(s * c.width);
-  t.moves = base + p.take(s * c.width);
+  t.source = base + p.take(int64_t(c.pages) * c.page);
+  t.page = base + p.take(c.pages);
+  t.moves = base + p.take(c.pages);
+  t.first = base + p.take(s);
   t.kept = base + p.take(s);
   t.whole = base + p.take(s);
   t.count = base + p.take(1);
@@ -585,7 +659,7 @@ extern "C" int64_t uc_paged_reorder_workspace_bytes(const uc_paged_cache *cache)
 }
 
 extern "C" int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *parents, const int32_t *lengths,
-                                void *workspace, int64_t workspace_bytes, uc_stream_t stream) {
+                                int64_t max_tokens, void *workspace, int64_t workspace_bytes, uc_stream_t stream) {
   using namespace uc;
   using namespace uc::pg;
   const char *what = "uc_paged_reorder";
@@ -597,17 +671,19 @@ extern "C" int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *pare
                  workspace_bytes >= lay_out(c, static_cast<int32_t *>(workspace), o),
              "%s: workspace too small", what);
   UC_REQUIRE(cache->layers * c.heads * c.sequences < (1 << 24), "%s: too many layers, heads and sequences", what);
+  UC_REQUIRE(max_tokens >= 0, "%s: negative max_tokens", what);
   o.parents = parents;
   o.cut = lengths;
-  const int64_t entries = int64_t(c.sequences) * c.width;
-  if (entries <= kSmallTable) {
+  // what the launches are shaped for; they do with any lengths
+  const int64_t widest = pages_expected(c, max_tokens);
+  if (c.sequences * widest <= kSmallTable) {
     hipLaunchKernelGGL(reorder_small_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, o);
     if (int rc = check_launch(what)) return rc;
   } else {
-    const uint32_t groups = static_cast<uint32_t>(ceil_div(entries, int64_t(256)));
-    hipLaunchKernelGGL(reorder_release_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
+    const dim3 groups = entry_groups(c, widest);
+    hipLaunchKernelGGL(reorder_release_kernel, groups, dim3(256), 0, as_stream(stream), c, pool, o);
     if (int rc = check_launch(what)) return rc;
-    hipLaunchKernelGGL(reorder_hold_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, o);
+    hipLaunchKernelGGL(reorder_hold_kernel, groups, dim3(256), 0, as_stream(stream), c, pool, o);
     if (int rc = check_launch(what)) return rc;
     hipLaunchKernelGGL(reorder_open_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, o);
     if (int rc = check_launch(what)) return rc;
@@ -627,7 +703,7 @@ extern "C" int64_t uc_paged_compact_workspace_bytes(const uc_paged_cache *cache)
 }
 
 extern "C" int uc_paged_compact(const uc_paged_cache *cache, const uint8_t *keep, int64_t keep_stride, int64_t tokens,
-                                void *workspace, int64_t workspace_bytes, uc_stream_t stream) {
+                                int64_t max_tokens, void *workspace, int64_t workspace_bytes, uc_stream_t stream) {
   using namespace uc;
   using namespace uc::pg;
   const char *what = "uc_paged_compact";
@@ -640,17 +716,20 @@ extern "C" int uc_paged_compact(const uc_paged_cache *cache, const uint8_t *keep
   UC_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 &&
                  workspace_bytes >= lay_out(c, static_cast<int32_t *>(workspace), t),
              "%s: workspace too small", what);
+  UC_REQUIRE(max_tokens >= 0, "%s: negative max_tokens", what);
   t.keep = keep;
   t.stride = keep_stride;
   t.tokens = static_cast<int32_t>(tokens);
-  const uint32_t groups = static_cast<uint32_t>(ceil_div(int64_t(c.sequences) * c.width, int64_t(256)));
-  hipLaunchKernelGGL(thin_scan_kernel, dim3(c.sequences), dim3(kThreads), 0, as_stream(stream), c, t);
+  hipLaunchKernelGGL(thin_count_kernel, dim3(c.sequences), dim3(kThreads), 0, as_stream(stream), c, t);
   if (int rc = check_launch(what)) return rc;
   hipLaunchKernelGGL(thin_give_kernel, dim3(1), dim3(kThreads), first_bytes(c), as_stream(stream), c, pool, t);
+  if (int rc = check_launch(what)) return rc;
+  hipLaunchKernelGGL(thin_list_kernel, dim3(c.sequences), dim3(kThreads), 0, as_stream(stream), c, t);
   if (int rc = check_launch(what)) return rc;
   hipLaunchKernelGGL(thin_copy_kernel, dim3(4096), dim3(256), 0, as_stream(stream), c, t, static_cast<int32_t>(cache->layers),
                      static_cast<int32_t>(cache->head_dim / 8));
   if (int rc = check_launch(what)) return rc;
-  hipLaunchKernelGGL(thin_commit_kernel, dim3(groups), dim3(256), 0, as_stream(stream), c, pool, t);
+  hipLaunchKernelGGL(thin_commit_kernel, entry_groups(c, pages_expected(c, max_tokens)), dim3(256), 0, as_stream(stream), c,
+                     pool, t);
   return check_launch(what);
 }

@@ -199,7 +199,7 @@ __device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t
                                           float l, uint16_t *out, float *lse) {
   constexpr int kC = D / 16;
   const int32_t t = token_of(q, r), head = w.h * q.group + r - t * q.group;
-  const bool none = t >= w.count || l == 0.0f;
+  const bool none = t >= w.count || (l == 0.0f && m == mf::kNegInf);  // (logits past fp32's range are no sum: NaN)
   const float f = none ? 0.0f : 1.0f / l;
   uint32_t v[kC / 2];
 #pragma unroll

@@ -549,9 +549,9 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
   const int64_t capacity = c.capacity(), keys = query->max_tokens < capacity ? query->max_tokens : capacity;
-  // a launch has less than 2^32 threads, and 32-bit counts of rows and steps
+  // a launch has less than 2^32 threads, and 32-bit counts of rows and steps (few rows are joined by up to a workgroup each)
   UC_REQUIRE(cache->sequences * cache->heads_kv < (1 << 28) && rows < (1 << 28) &&
-                 cache->sequences * cache->heads_kv * rows < (1 << 24),
+                 cache->sequences * cache->heads_kv * rows < (p.rows >= kTileRows ? 1 << 27 : 1 << 24),
              "%s: too many query rows", what);
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   UC_REQUIRE(units * ceil_div(capacity, int64_t(kStep)) < (1 << 30), "%s: too many keys in all", what);
@@ -563,7 +563,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
     if (cache->sequences * p.groups <= kMostShared && units * ceil_div(capacity, int64_t(kKeys)) < (1 << 30)) {
       p.workgroups = static_cast<int32_t>(tiles < least * kShare ? ceil_div(tiles, 8 * least) * 8 : kShare);
     }
-    UC_REQUIRE(units < (1 << 24), "%s: too many query rows", what);
+    UC_REQUIRE(units < (1 << 21), "%s: too many query rows", what);
     return UC_OK;
   }
   const int64_t steps = units * ceil_div(keys, int64_t(kStep));

@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       }
     } else {
       const int32_t token = token_of(q, r), h = w.h * q.group + r - token * q.group;
-      const bool none = token >= w.count || total == 0.0f;
+      const bool none = token >= w.count || (total == 0.0f && acc[n].m == mf::kNegInf);
       const float f = none ? 0.0f : 1.0f / total;
       uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + h) * D + 4 * quad;
 #pragma unroll

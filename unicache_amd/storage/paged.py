@@ -277,8 +277,8 @@ class PagedKVCache:
     def _reorder(self, parents, lengths) -> None:
         nbytes = _workspace_bytes("uc_paged_reorder_workspace_bytes", self._sizes, True, None)
         ws = nat.workspace(self.device, nbytes)
-        nat.call_on(self.device, "uc_paged_reorder", self._struct(), nat.ptr(parents), nat.ptr(lengths), ws.data_ptr(),
-                    nbytes)
+        nat.call_on(self.device, "uc_paged_reorder", self._struct(), nat.ptr(parents), nat.ptr(lengths),
+                    self.max_tokens, ws.data_ptr(), nbytes)
 
     def compact(self, keep: torch.Tensor) -> None:
         """Each sequence keeps, in order, the tokens t with keep[s, t] (bool or uint8 [S, T], rows may
@@ -298,7 +298,7 @@ class PagedKVCache:
         nbytes = _workspace_bytes("uc_paged_compact_workspace_bytes", self._sizes, True, None)
         ws = nat.workspace(self.device, nbytes)
         nat.call_on(self.device, "uc_paged_compact", self._struct(), keep.data_ptr(), keep.stride(0),
-                    int(keep.shape[1]), ws.data_ptr(), nbytes)
+                    int(keep.shape[1]), self.max_tokens, ws.data_ptr(), nbytes)
 
     # ------------------------------------------------------------------ calls --
     def write(self, key: torch.Tensor, value: torch.Tensor, *, layer: int = 0, query: torch.Tensor | None = None,
