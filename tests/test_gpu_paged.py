@@ -768,6 +768,28 @@ def test_layer_views_and_rows_behind_the_end(device):
         cache.layer(0).reserve(1)
 
 
+def test_tensors_may_be_replaced_by_their_like(device):
+    cache, k, v = filled([100, 37], d=64, b=16)
+    q = randn(2, 1, 4, 64, seed=1)
+    want = cache.attention(q)
+    cache.key, cache.value = cache.key.clone(), cache.value.clone()
+    cache.table = cache.table.clone()
+    again = cache.attention(q)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    lengths, cache.lengths = cache.lengths, i32([50, 37])
+    check_attention(cache, k, v, [50, 37], q, None, False)
+    cache.lengths, table = lengths, cache.table
+    for name, bad, match in (("table", table[:, :2].contiguous(), "same sizes"), ("table", table.long(), "table"),
+                             ("lengths", i32([1]), "lengths"), ("key", cache.key.half(), "value"),
+                             ("key", cache.key[:, :2].contiguous(), "value")):
+        good = getattr(cache, name)
+        setattr(cache, name, bad)
+        with pytest.raises(ValueError, match=match):
+            cache.attention(q)
+        setattr(cache, name, good)
+    assert torch.equal(cache.attention(q)[0], want[0])
+
+
 def test_empty_calls(device):
     cache = PagedKVCache.empty(2, 4, 1, 64, page_tokens=16)
     out, lse = cache.attention(randn(2, 0, 3, 64, seed=0))

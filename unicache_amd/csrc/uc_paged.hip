@@ -5,8 +5,9 @@
 // sequences in order, found by prefix sums over a bit for each page; reference counts and bits move by
 // atomics whose order does not matter (a count's zero is seen by the one that makes it).
 //
-// Copies (the rows of open pages; the kept rows of thinned sequences) are bound by HBM, the rest by
-// latency: chains of short launches over a few kilobytes.
+// Copies (the rows of open pages; the kept rows of thinned sequences) are bound by HBM (the latter 5.4 TB/s over 244 MB of
+// reads and writes), the rest by latency: chains of short launches over a few kilobytes (reserve 2.3 us, a small
+// reorder 10, count, give, list and commit of thinning 3 to 8 each).
 #include "uc_paged.h"
 
 namespace uc {

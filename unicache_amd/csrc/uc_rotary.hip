@@ -10,6 +10,9 @@
 // A workgroup takes one or a few tokens: it works out each pair's sine and cosine once, into LDS, and
 // turns all heads of the token by them, 16 channels (two 16-byte vectors, both sides of eight pairs) a
 // thread.  The values on their way into a cache ride along as rows without pairs.
+//
+// Bound by HBM: 7k tokens of 32 + 8 heads 29.3 us (4.9 TB/s over reads and writes), 16k tokens into a cache 66.6 (4.5).  Four
+// tokens a workgroup from 2048 tokens on, where their pairs fill its threads; below that one, for more workgroups.
 #include "uc_paged.h"
 
 namespace uc {

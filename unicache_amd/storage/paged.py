@@ -23,7 +23,8 @@ from ..operators.rotary import MultiAxisRotary, check_rows
 from .physical import tensor_bytes
 
 _PAGES = (16, 32, 64, 128, 256)
-_TENSORS = frozenset(("key", "value", "table", "lengths", "granted", "references", "free_pages"))
+_ORDER = ("key", "value", "table", "lengths", "granted", "references", "free_pages")
+_TENSORS = frozenset(_ORDER)
 _SIZES = "Paged cache supports pages of 16, 32, 64, 128 or 256 tokens and head_dim 64 or 128"
 
 
@@ -76,6 +77,13 @@ class PagedKVCache:
 
     def __init__(self, key, value, table, lengths, *, granted=None, references=None, free_pages=None,
                  max_tokens=None) -> None:
+        self._check(key, value, table, lengths, granted, references, free_pages)
+        if max_tokens is not None and int(max_tokens) < 0:
+            raise ValueError("Paged cache max_tokens must not be negative")
+        self._set(key, value, table, lengths, granted, references, free_pages, max_tokens)
+
+    @staticmethod
+    def _check(key, value, table, lengths, granted, references, free_pages) -> None:
         if key.dim() != 5:
             raise ValueError("Paged cache expects keys and values [layers, pages, kv_heads, page_tokens, head_dim]")
         layers, pages, heads, b, d = map(int, key.shape)
@@ -105,9 +113,6 @@ class PagedKVCache:
             _check_tensor("free_pages", free_pages, torch.int32, (-(-pages // 32),), device)
         if device.type != "cuda":
             raise RuntimeError(f"Paged cache requires GPU tensors (got {device})")
-        if max_tokens is not None and int(max_tokens) < 0:
-            raise ValueError("Paged cache max_tokens must not be negative")
-        self._set(key, value, table, lengths, granted, references, free_pages, max_tokens)
 
     def _set(self, key, value, table, lengths, granted, references, free_pages, max_tokens) -> None:
         self.key, self.value, self.table, self.lengths = key, value, table, lengths
@@ -188,6 +193,10 @@ class PagedKVCache:
 
     def _struct(self) -> "nat.PagedCache":
         if self._built is None:
+            self._check(*(getattr(self, name) for name in _ORDER))
+            if (*self.key.shape[:2], *self.table.shape, *self.key.shape[2:]) != (
+                    *self._sizes[:5], self.page_tokens, self.head_dim) or self.key.dtype != self.dtype:
+                raise ValueError("Paged cache tensors may be replaced by ones of the same sizes only")
             self._built = nat.PagedCache(self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(),
                                          self.lengths.data_ptr(), nat.ptr(self.granted), nat.ptr(self.references),
                                          nat.ptr(self.free_pages), *self._sizes)
@@ -370,7 +379,8 @@ class PagedKVCache:
             raise ValueError("Query heads must be divisible by the cache's KV heads")
         if query_lengths is not None:
             query_lengths = self._numbers(query_lengths, "query_lengths")
-        sizes = (lq, hq, self.max_tokens, self._sizes[-1], 1 if causal else 0)
+        # (in whole steps of 128 keys, so that a decode loop's sizes repeat)
+        sizes = (lq, hq, (self.max_tokens + 127) & -128, self._sizes[-1], 1 if causal else 0)
         nbytes = self._attention_workspace(sizes)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         out = nat.empty_like(query)
