@@ -201,6 +201,25 @@ __device__ __forceinline__ float weights(const f4 (&s)[4], int half, float facto
   return l;
 }
 
+// Products of N fragments read from LDS, with the reads kAhead fragments ahead of their use, in just this order.  (Left to itself
+// the compiler, short of registers, reads each one right before its use and waits for it: 2 x 2k of 13k 803 us, 755 so; two more
+// ahead 760.)
+template <int N, class Load, class Use>
+__device__ __forceinline__ void products(Load load, Use use) {
+  constexpr int kAhead = 4;
+  decltype(load(0)) a[N];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) a[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + kAhead < N) a[i + kAhead] = load(i + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+    use(i, a[i]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // The tiles of all units, ordered by KV head, sequence and row group, are cut into runs of equal length for the
 // workgroups: calls of any lengths and any number of units load them alike, and only a run's first and last
 // unit may be parts, joined by a second launch.  (Causal rows see fewer keys the earlier they are, so units differ.)
@@ -377,15 +396,17 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     __builtin_amdgcn_s_setprio(3);
     f4 s[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[0][j] = s[1][j] = f4{0, 0, 0, 0};
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const V8 a = *reinterpret_cast<const V8 *>(buf + ka[k] + (32 * (j / 2) + 4 * (j % 2)) * T::kKeyRow);
-        s[0][j] = H::mfma(a, frag[0][k], s[0][j]);
-        s[1][j] = H::mfma(a, frag[1][k], s[1][j]);
-      }
-    }
+    for (int j = 0; j < 4; ++j) s[0][j] = s[1][j] = f4{0, 0, 0, 0};
+    products<D / 8>(
+        [&](int i) {
+          const int j = i / (D / 32), k = i % (D / 32);
+          return *reinterpret_cast<const V8 *>(buf + ka[k] + (32 * (j / 2) + 4 * (j % 2)) * T::kKeyRow);
+        },
+        [&](int i, V8 a) {
+          const int j = i / (D / 32), k = i % (D / 32);
+          s[0][j] = H::mfma(a, frag[0][k], s[0][j]);
+          s[1][j] = H::mfma(a, frag[1][k], s[1][j]);
+        });
     vector_phase();
     // (asked for here: LDS reads and scalar loads are waited for together, and none of the former follows for a while)
     __builtin_amdgcn_sched_barrier(0);
@@ -437,20 +458,15 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     }
     if (more && !whole()) clear_values<D>(st, ld, w.length);
     __builtin_amdgcn_s_setprio(3);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      V8 a[D / 16];
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) a[d] = value(h, d);
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        acc[0].o[d] = H::mfma(a[d], pr[0][h], acc[0].o[d]);
-        acc[1].o[d] = H::mfma(a[d], pr[1][h], acc[1].o[d]);
-      }
-      // (after the last tile the present one's again, into the buffer that nobody reads)
-      if (h == 0) store_keys<D>(st, lds + present * T::kBytes, ld);
-      if (h == 1) store_values<D>(st, lds + present * T::kBytes, ld);
-    }
+    products<D / 8>([&](int i) { return value(i / (D / 16), i % (D / 16)); },
+                    [&](int i, V8 a) {
+                      const int h = i / (D / 16), d = i % (D / 16);
+                      acc[0].o[d] = H::mfma(a, pr[0][h], acc[0].o[d]);
+                      acc[1].o[d] = H::mfma(a, pr[1][h], acc[1].o[d]);
+                    });
+    // (after the last tile the present one's again, into the buffer that nobody reads)
+    store_keys<D>(st, lds + present * T::kBytes, ld);
+    store_values<D>(st, lds + present * T::kBytes, ld);
     vector_phase();
     __syncthreads();
     ++t;
@@ -464,6 +480,15 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     ask(entries, pages, ld, (begin + 1) * kKeys);
     store_keys<D>(st, lds, ld);
     store_values<D>(st, lds, ld);
+  }
+  // (The queries are here now: else the first products of every tile would wait for whatever was asked for last, which
+  // is the next tile: 2 x 2k of 13k 755 us, 733 so.  At 64 channels that wait does no harm: 104 us, 109 so.)
+  if constexpr (D == 128) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(frag[n][k]));
+    }
   }
   __syncthreads();
   // tiles that every row sees come first; from the first other one on, every tile is masked
