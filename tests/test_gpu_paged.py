@@ -766,6 +766,17 @@ def test_layer_views_and_rows_behind_the_end(device):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     with pytest.raises(RuntimeError, match="references"):
         cache.layer(0).reserve(1)
+    # rows of one sequence without their first dimension
+    one, want = cache.layer(2, sequence=0), cache.attention(q, layer=2)
+    out, lse = one.attention(q[0])
+    assert out.shape == (1, 4, 64) and lse.shape == (4, 1)
+    assert torch.equal(out, want[0][0]) and torch.equal(lse, want[1][0])
+    rotary = MultiAxisRotary(64, (32,))
+    new = randn(2, 2, 64, seed=3)
+    turned = one.write(new, -new, query=new, rotary=rotary)
+    where = torch.tensor([[31, 32]], device=device)
+    assert torch.equal(turned, rotary.rotate(new, positions=where))
+    assert torch.equal(cache.dense(layer=2)[0][0, 31:33], turned) and torch.equal(cache.dense(layer=2)[1][0, 31:33], -new)
 
 
 def test_tensors_may_be_replaced_by_their_like(device):

@@ -98,7 +98,7 @@ def test_call_checks():
             (lambda: cache.attention(q.float()), "dtype"), (lambda: cache.attention(q[:, :, :0]), "queries"),
             (lambda: cache.attention(q, layer=5), "layers 0"), (lambda: cache.attention(q, sm_scale=0.0), "sm_scale"),
             (lambda: cache.attention(q, sm_scale=-1.0), "sm_scale"), (lambda: cache.attention(q, sm_scale=math.nan), "sm_scale"),
-            (lambda: cache.attention(q, sm_scale=math.inf), "sm_scale"),
+            (lambda: cache.attention(q, sm_scale=math.inf), "sm_scale"), (lambda: cache.attention(q, sm_scale=1e-39), "sm_scale"),
             (lambda: cache.attention(q, query_lengths=torch.zeros(3)), "query_lengths"),
             (lambda: cache.attention(q.clone().requires_grad_()), "gradient"), (lambda: cache.dense(layer=2), "layers 0"),
             (lambda: cache.layer(2), "layers 0"), (lambda: cache.layer(0, sequence=3), "sequences 0"),

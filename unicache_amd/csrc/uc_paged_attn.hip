@@ -15,7 +15,6 @@
 // byte permutation per pair of keys and channel turns them round.  Fragment n then holds
 // channels D/16 r + n, and a lane ends with consecutive channels of its query row.
 //
-//
 // Bound by HBM: each row is read once, straight into registers, a wave's next 32 keys (16 KB at 128
 // channels) on their way while it computes on the present ones.  Of 8 sequences of 32k tokens (28/4 heads, 537 MB) both
 // launches take 98.7 us (5.4 TB/s; a large copy 5.0), of 64 ragged ones up to 8k in pages of 16 193 (5.6).
@@ -606,8 +605,8 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
   Plan p;
   if (int rc = check_cache(cache, layer, what, c)) return rc;
   if (int rc = make_plan(cache, c, query, what, q, p)) return rc;
-  // (times log2(e) it stays in fp32's range)
-  UC_REQUIRE(sm_scale > 0.0f && sm_scale <= 0x1p127f, "%s: sm_scale must be positive, and 2^127 at most", what);
+  // (times log2(e) it stays in fp32's range, and a normal number: the kernels flush others to 0)
+  UC_REQUIRE(sm_scale >= 0x1p-126f && sm_scale <= 0x1p127f, "%s: sm_scale must be 2^-126 at least, and 2^127 at most", what);
   if (q.len == 0) return UC_OK;
   UC_REQUIRE(q.p != nullptr && (reinterpret_cast<uintptr_t>(q.p) & 15) == 0 && ((q.ss | q.st | q.sh) & 7) == 0,
              "%s: query must be 16-byte aligned with strides that are multiples of 8", what);

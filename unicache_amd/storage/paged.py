@@ -369,8 +369,8 @@ class PagedKVCache:
             sm_scale = self._scale
         else:
             sm_scale = ctypes.c_float(float(sm_scale)).value
-            if not 0.0 < sm_scale <= 2.0 ** 127:
-                raise ValueError("Paged attention sm_scale must be positive, and 2^127 at most (as fp32)")
+            if not 2.0 ** -126 <= sm_scale <= 2.0 ** 127:
+                raise ValueError("Paged attention sm_scale must be 2^-126 at least, and 2^127 at most (as fp32)")
         flat = query.dim() == 3
         query, a, b, c = self._rows(query, "queries")
         shape = query.shape
