@@ -952,10 +952,11 @@ int uc_paged_reorder(const uc_paged_cache *cache, const int32_t *parents, const 
 int64_t uc_paged_reorder_workspace_bytes(const uc_paged_cache *cache);
 
 /*
- * Each sequence keeps the tokens t with keep[s * keep_stride + t] != 0 (bytes) and those from `tokens` on, in order.
- * Pages before the first that loses a token stay; the kept rows behind them move into free pages, the
- * lowest first, by the sequences in order, and the pages they leave are released after that.  Where the free pages
- * do not suffice, that sequence and those after it keep all their tokens.  max_tokens as in uc_paged_reorder.
+ * Each sequence keeps the tokens t with keep[s * keep_stride + t] != 0 (bytes) and those from `tokens` on, in order; tokens
+ * whose table entry is no page are dropped, whatever the mask says.  Pages before the first that loses a token stay; the kept
+ * rows behind them move into free pages, the lowest first, by the sequences in order, and the pages they leave are
+ * released after that.  Where the free pages do not suffice, that sequence and those after it keep all their tokens.
+ * max_tokens as in uc_paged_reorder.
  */
 int uc_paged_compact(const uc_paged_cache *cache, const uint8_t *keep, int64_t keep_stride, int64_t tokens,
                      int64_t max_tokens, void *workspace, int64_t workspace_bytes, uc_stream_t stream);

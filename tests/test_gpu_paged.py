@@ -858,3 +858,72 @@ def test_mixed_attention_over_paged_segments(device, lq):
     for bad in (cache, cache.layer(0)):
         with pytest.raises(ValueError, match="one layer of one sequence"):
             run_fused_mixed_attention(q, dk, dv, [bad])
+
+
+# ----------------------------------------------------------- what lies hidden --
+def booked(lengths, *, spare=6, b=16, d=64, layers=2, seed=0):
+    """filled() over a pool with its books, `spare` pages free, and what free pages hold finite and large."""
+
+    need = sum(-(-n // b) for n in lengths)
+    bare, _, _ = filled(lengths, hkv=2, d=d, b=b, layers=layers, pages=need + spare, seed=seed)
+    held = bare.table[bare.table >= 0].long()
+    references = torch.zeros(bare.pages, dtype=torch.int32, device="cuda").scatter_add_(0, held, torch.ones_like(held, dtype=torch.int32))
+    bits = [sum((int(references[w * 32 + i]) == 0) << i for i in range(min(32, bare.pages - w * 32)))
+            for w in range(-(-bare.pages // 32))]
+    words = i32([x - (1 << 32) if x >> 31 else x for x in bits])
+    key, value = torch.nan_to_num(bare.key, nan=500.0), torch.nan_to_num(bare.value, nan=500.0)
+    return PagedKVCache(key, value, bare.table, bare.lengths, granted=i32([0] * len(lengths)), references=references,
+                        free_pages=words, max_tokens=max(lengths))
+
+
+@pytest.mark.parametrize("b", [16, 64])
+def test_compact_drops_tokens_without_a_page(device, b):
+    """Tokens whose table entries are no page have no rows: they do not come back as those of whoever had the page before."""
+
+    n = 5 * b
+    lengths = [n + 3, n, n + 7, 2 * b, n]
+    cache = booked(lengths, b=b, spare=40)
+    hidden = [{1}, {0, 4}, {5}, {0, 1}, set()]  # a page between, at both ends, the open one, all, none
+    odd = [-1, cache.pages, -2 ** 31]
+    for s, entries in enumerate(hidden):
+        for i in entries:
+            page = int(cache.table[s, i])
+            cache.references[page] -= 1  # (it went to somebody else, and is free again)
+            word = int(cache.free_pages[page // 32]) | (1 << page % 32) - (1 << 32 if page % 32 == 31 else 0)
+            cache.free_pages[page // 32] = word
+            cache.table[s, i] = odd[(s + i) % 3]
+    key, value = cache.dense(layer=1)
+    g = torch.Generator().manual_seed(b)
+    keep = torch.rand(5, n, generator=g) < 0.7
+    keep[2] = True  # (loses nothing but the page that is not there)
+    keep[4] = True
+    want = [[t for t in range(length) if t // b not in hidden[s] and (t >= n or bool(keep[s, t]))]
+            for s, length in enumerate(lengths)]
+    q = randn(5, 1, 4, 64, seed=1)
+    before = cache.attention(q, layer=1)
+    cache.compact(keep.cuda())
+    assert cache.lengths.tolist() == [len(w) for w in want]
+    after_k, after_v = cache.dense(layer=1)
+    for s, w in enumerate(want):
+        assert torch.equal(after_k[s, :len(w)], key[s, w]) and torch.equal(after_v[s, :len(w)], value[s, w])
+        assert not after_k[s, len(w):].any()
+        pages = -(-len(w) // b)
+        row = cache.table[s].tolist()
+        assert all(0 <= p < cache.pages for p in row[:pages]) and row[pages:] == [-1] * (cache.sequence_pages - pages)
+    held = [p for row in cache.table.tolist() for p in row if p >= 0]
+    assert cache.references.tolist() == [held.count(p) for p in range(cache.pages)]
+    bits = [(w >> i) & 1 for w in cache.free_pages.tolist() for i in range(32)][:cache.pages]
+    assert bits == [int(p not in held) for p in range(cache.pages)]
+    # a mask that keeps all drops what was hidden, and what attention sees stays
+    again = booked(lengths, b=b, spare=40)
+    for s, entries in enumerate(hidden):
+        for i in entries:
+            again.table[s, i] = -1
+    again.compact(torch.ones(5, 1, dtype=torch.bool, device=device))
+    assert again.lengths.tolist() == [sum(t // b not in hidden[s] for t in range(x)) for s, x in enumerate(lengths)]
+    out, lse = again.attention(q, layer=1)
+    # (sums of the same weights over tiles cut otherwise: two roundings of the output, 64 steps of a sum of 5 b terms)
+    assert ((out.float() - before[0].float()).abs() <= 2 * EPS[q.dtype] * before[0].float().abs() + 2.0 ** -10).all()
+    seen = lse != -math.inf
+    assert torch.equal(seen, before[1] != -math.inf)
+    assert ((lse - before[1])[seen].abs() <= 2.0 ** -16 * (1 + lse[seen].abs())).all()

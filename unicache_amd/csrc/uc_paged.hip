@@ -388,21 +388,24 @@ struct Thin {
   int32_t *count;            // [1] pages to come
 };
 
-// Eight tokens of a mask that starts at keep: a bit for each that stays.
-__device__ __forceinline__ uint32_t stays_of(const Thin &t, const uint8_t *keep, int32_t token, int32_t length) {
+// Eight tokens of sequence s, whose mask starts at keep: a bit for each that stays.  Tokens without a page (one holds all eight)
+// do not: they have no rows to move, and a new page would show what it held before in their place.
+__device__ __forceinline__ uint32_t stays_of(const Cache &c, const Thin &t, const uint8_t *keep, int32_t s, int32_t token,
+                                             int32_t length) {
   uint32_t stays = 0;
+  const bool held = c.is_page(c.table[int64_t(s) * c.width + (token >> c.shift)]);
   if (token + 8 <= length && token + 8 <= t.tokens && (reinterpret_cast<uintptr_t>(keep + token) & 7) == 0) {
     const uint2 w = *reinterpret_cast<const uint2 *>(keep + token);
 #pragma unroll
     for (int i = 0; i < 8; ++i) stays |= (((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xffu) != 0 ? 1u << i : 0u;
-    return stays;
+    return held ? stays : 0;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int32_t at = token + i;
     if (at < length && (at >= t.tokens || keep[at] != 0)) stays |= 1u << i;
   }
-  return stays;
+  return held ? stays : 0;
 }
 
 // How many tokens a sequence keeps, and how many of its pages come before the first that loses one.
@@ -417,7 +420,7 @@ __global__ __launch_bounds__(kThreads) void thin_count_kernel(Cache c, Thin t) {
   __syncthreads();
   int32_t mine = 0, first = length;
   for (int32_t token = 8 * threadIdx.x; token < length; token += 8 * kThreads) {
-    const uint32_t stays = stays_of(t, keep, token, length);
+    const uint32_t stays = stays_of(c, t, keep, s, token, length);
     const int32_t there = length - token >= 8 ? 8 : length - token;
     const uint32_t gone = ~stays & ((1u << there) - 1u);
     mine += __popc(stays);
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(kThreads) void thin_list_kernel(Cache c, Thin t) {
   // (every token of the pages that stay is kept, so the count begins behind them)
   for (int32_t t0 = stay, kept = stay; t0 < length; t0 += 8 * kThreads) {
     const int32_t token = t0 + 8 * threadIdx.x;
-    const uint32_t stays = token < length ? stays_of(t, keep, token, length) : 0;
+    const uint32_t stays = token < length ? stays_of(c, t, keep, s, token, length) : 0;
     int32_t total;
     const int32_t count = __popc(stays);
     int32_t to = kept + block_prefix(count, total, waves) - count;

@@ -292,6 +292,7 @@ class PagedKVCache:
     def compact(self, keep: torch.Tensor) -> None:
         """Each sequence keeps, in order, the tokens t with keep[s, t] (bool or uint8 [S, T], rows may
         be strided) and those from T on: the eviction of TensorCacheStorageBackend.compact over pages, for all layers.
+        Tokens whose table entries are no page are dropped, whatever the mask says.
 
         Pages before the first that loses a token stay, shared or not.  The kept rows behind them move into free
         pages, the lowest first, to the sequences in order, and then the pages they leave are
