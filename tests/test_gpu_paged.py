@@ -927,3 +927,23 @@ def test_compact_drops_tokens_without_a_page(device, b):
     seen = lse != -math.inf
     assert torch.equal(seen, before[1] != -math.inf)
     assert ((lse - before[1])[seen].abs() <= 2.0 ** -16 * (1 + lse[seen].abs())).all()
+
+
+@pytest.mark.parametrize("dtype,d,b", [(torch.bfloat16, 64, 16), (torch.float16, 128, 64)])
+@pytest.mark.parametrize("hq,lq", [(128, 3), (200, 4), (400, 2)])
+def test_a_tile_of_one_token_hides_what_follows_it(device, dtype, d, b, hq, lq):
+    # all rows of a workgroup's unit are of one query token: they all see less than the sequence holds
+    lengths = [100, 70]
+    cache, _, _ = filled(lengths, hkv=1, d=d, b=b, dtype=dtype)
+    key, value = cache.key.clone(), cache.value.clone()
+    table = cache.table.cpu()
+    for s, n in enumerate(lengths):
+        page, t = table[s, (n - 1) // b], (n - 1) % b
+        key[0, page, :, t, 3], value[0, page, :, t] = math.nan, math.inf
+        value[0, page, :, t, 5] = math.nan
+    dirty = PagedKVCache(key, value, cache.table, cache.lengths, max_tokens=100)
+    q = randn(2, lq, hq, d, seed=6, dtype=dtype)
+    out, lse = dirty.attention(q, causal=True)
+    clean, clean_lse = cache.attention(q, causal=True)
+    assert torch.equal(out[:, :lq - 1], clean[:, :lq - 1]) and torch.equal(lse[:, :, :lq - 1], clean_lse[:, :, :lq - 1])
+    assert out[:, lq - 1].isnan().all() and lse[:, :, lq - 1].isnan().all()

@@ -223,10 +223,10 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
       softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
     }
     if constexpr (MASK) {
-      // what lies behind the length is no value
+      // what no row sees is no value
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const bool held = there && mine + j < w.length;
+        const bool held = there && mine + j < w.end_last;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) raw.v[j][i] = held ? raw.v[j][i] : 0u;
       }

@@ -129,13 +129,14 @@ __device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const
   }
 }
 
-// What lies behind the length is no value.
+// What no row of the unit sees is no value: from `end` on, which for the rows of one causal token (128 query heads or more of a KV
+// head) lies before the sequence's length.
 template <int D>
-__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t length) {
+__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t end) {
   const bool there = ((st.absent >> ld.wave) & 1) == 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const bool held = there && st.t + 8 * ld.group + j < length;
+    const bool held = there && st.t + 8 * ld.group + j < end;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) st.v[j][i] = held ? st.v[j][i] : 0u;
   }
@@ -456,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         __syncthreads();
       }
     }
-    if (more && !whole()) clear_values<D>(st, ld, w.length);
+    if (more && !whole()) clear_values<D>(st, ld, w.end_last);
     __builtin_amdgcn_s_setprio(3);
     products<D / 8>([&](int i) { return value(i / (D / 16), i % (D / 16)); },
                     [&](int i, V8 a) {
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   if (begin < end) {
     ask(entries, pages, ld, begin * kKeys);
     fetch<D, WHOLE>(st, c, entries, keys, values, ld, begin * kKeys);
-    if (!whole()) clear_values<D>(st, ld, w.length);
+    if (!whole()) clear_values<D>(st, ld, w.end_last);
     ask(entries, pages, ld, (begin + 1) * kKeys);
     store_keys<D>(st, lds, ld);
     store_values<D>(st, lds, ld);
