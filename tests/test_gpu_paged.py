@@ -947,3 +947,24 @@ def test_a_tile_of_one_token_hides_what_follows_it(device, dtype, d, b, hq, lq):
     clean, clean_lse = cache.attention(q, causal=True)
     assert torch.equal(out[:, :lq - 1], clean[:, :lq - 1]) and torch.equal(lse[:, :, :lq - 1], clean_lse[:, :, :lq - 1])
     assert out[:, lq - 1].isnan().all() and lse[:, :, lq - 1].isnan().all()
+
+
+def test_storage_that_was_swapped_is_read_where_it_is(device):
+    import copy
+
+    cache, _, _ = filled([100, 37], d=64, b=16)
+    q = randn(2, 1, 4, 64, seed=1)
+    want = cache.attention(q)
+    kept = cache.key.clone(), cache.value.clone(), cache.table.clone(), cache.lengths.clone()
+    old = [t.detach() for t in (cache.key, cache.value, cache.table, cache.lengths)]
+    cache.key.data, cache.value.data = kept[0], kept[1]
+    cache.table.set_(kept[2])
+    cache.lengths.data = kept[3]
+    for t in old:
+        t.zero_()
+    got = cache.attention(q)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    other = copy.deepcopy(cache)
+    cache.key.zero_(), cache.lengths.zero_()
+    got = other.attention(q)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

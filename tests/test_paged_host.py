@@ -331,3 +331,54 @@ def test_page_call_validation():
     with pytest.raises(ValueError, match="aligned"):
         nat.call("uc_paged_dense", c, 0, 16, 24, 640, None)
     nat.call("uc_paged_dense", c, 0, None, None, 0, None)
+
+
+# -------------------------------------------------------- tensors that change --
+_NAMES = ("key", "value", "table", "lengths", "granted", "references", "free_pages")
+
+
+def _built(monkeypatch):
+    """A cache of CPU tensors whose C struct stands."""
+
+    cache = _on_host()
+    with monkeypatch.context() as m:
+        m.setattr(PagedKVCache, "_check", staticmethod(lambda *tensors: None))
+        cache._struct()
+    return cache
+
+
+@pytest.mark.parametrize("name", _NAMES)
+@pytest.mark.parametrize("how", ["data", "set"])
+def test_the_struct_follows_storage_that_was_swapped(monkeypatch, name, how):
+    cache = _built(monkeypatch)
+    t = getattr(cache, name)
+    old = t.detach()  # (keeps the first memory, so that the addresses differ)
+    if how == "data":
+        t.data = t.clone()
+    else:
+        t.set_(t.clone())
+    monkeypatch.setattr(PagedKVCache, "_check", staticmethod(lambda *tensors: None))
+    assert {n: getattr(cache._struct(), n) for n in _NAMES} == {n: getattr(cache, n).data_ptr() for n in _NAMES}
+    del old
+
+
+def test_swapped_storage_is_checked(monkeypatch):
+    for name, bad in (("key", lambda t: t.half()), ("value", lambda t: t[:, :2].contiguous()), ("table", lambda t: t.long()),
+                      ("lengths", lambda t: torch.zeros(9, dtype=torch.int32)), ("references", lambda t: t[:2].clone())):
+        cache = _built(monkeypatch)
+        t = getattr(cache, name)
+        old, t.data = t.detach(), bad(t)
+        with pytest.raises(ValueError, match="Paged cache"):
+            cache._struct()
+        del old
+
+
+def test_a_used_cache_is_copied_with_its_addresses_made_anew(monkeypatch):
+    import copy
+    import pickle
+
+    cache = _built(monkeypatch)
+    monkeypatch.setattr(PagedKVCache, "_check", staticmethod(lambda *tensors: None))
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert other.key.data_ptr() != cache.key.data_ptr() and torch.equal(other.table, cache.table)
+        assert {n: getattr(other._struct(), n) for n in _NAMES} == {n: getattr(other, n).data_ptr() for n in _NAMES}

@@ -66,6 +66,7 @@ class PagedKVCache:
     no other, which the calls here see to.  Without the last three tensors the
     cache is another program's: write and attention work, the program keeps the table and lengths itself.
     Table entries that are no page hide their tokens, and nothing is written there.
+    Tensors may be replaced by others of their dtype and sizes, or get other storage; calls read them where they are.
 
     ``max_tokens`` is how long the caller takes the longest sequence to be
     (default: the capacity; raised by reserve); it shapes launches, and no
@@ -130,7 +131,7 @@ class PagedKVCache:
 
     def __setattr__(self, name, value) -> None:
         object.__setattr__(self, name, value)
-        if name in _TENSORS:  # the C struct of the tensors is made again
+        if name in _TENSORS:  # they are checked, and their C struct is made, again
             object.__setattr__(self, "_built", None)
 
     @property
@@ -191,15 +192,22 @@ class PagedKVCache:
             raise ValueError(f"Paged cache has layers 0 .. {self.layers - 1} (got {layer})")
         return layer
 
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "_built": None}  # (a copy's tensors lie elsewhere)
+
+    def _addresses(self) -> tuple:
+        return (self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(), self.lengths.data_ptr(),
+                *((None, None, None) if self.references is None else
+                  (self.granted.data_ptr(), self.references.data_ptr(), self.free_pages.data_ptr())))
+
     def _struct(self) -> "nat.PagedCache":
-        if self._built is None:
+        if self._built is None or self._at != self._addresses():  # (storage can be swapped under a tensor)
             self._check(*(getattr(self, name) for name in _ORDER))
             if (*self.key.shape[:2], *self.table.shape, *self.key.shape[2:]) != (
                     *self._sizes[:5], self.page_tokens, self.head_dim) or self.key.dtype != self.dtype:
                 raise ValueError("Paged cache tensors may be replaced by ones of the same sizes only")
-            self._built = nat.PagedCache(self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(),
-                                         self.lengths.data_ptr(), nat.ptr(self.granted), nat.ptr(self.references),
-                                         nat.ptr(self.free_pages), *self._sizes)
+            self._at = self._addresses()
+            self._built = nat.PagedCache(*self._at, *self._sizes)
         return self._built
 
     def _attention_workspace(self, sizes: tuple) -> int:
