@@ -968,3 +968,15 @@ def test_storage_that_was_swapped_is_read_where_it_is(device):
     cache.key.zero_(), cache.lengths.zero_()
     got = other.attention(q)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_copied_rotary_reads_its_own_tables(device):
+    import copy
+
+    q = randn(2, 1, 4, 64, seed=1)
+    rotary = MultiAxisRotary(64, (16, 16))
+    positions = torch.arange(4, device=device).view(2, 2, 1)
+    want = rotary.rotate(q, positions=positions)
+    other = copy.deepcopy(rotary)
+    rotary._turns.zero_()
+    assert torch.equal(other.rotate(q, positions=positions), want)

@@ -382,3 +382,14 @@ def test_a_used_cache_is_copied_with_its_addresses_made_anew(monkeypatch):
     for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
         assert other.key.data_ptr() != cache.key.data_ptr() and torch.equal(other.table, cache.table)
         assert {n: getattr(other._struct(), n) for n in _NAMES} == {n: getattr(other, n).data_ptr() for n in _NAMES}
+
+
+def test_a_plan_follows_its_tables():
+    import copy
+    import pickle
+
+    rotary = _rotary()
+    positions = torch.zeros(2, 1, 3, dtype=torch.int64)
+    for other in (rotary, copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
+        struct, _ = other.plan(positions, 1, 3)
+        assert struct.turns == other._turns.data_ptr() and struct.axis == other._axis.data_ptr()

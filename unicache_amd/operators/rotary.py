@@ -78,7 +78,6 @@ class MultiAxisRotary:
         turns = [f / (2.0 * math.pi) for f in frequencies]
         self._turns = torch.tensor(turns, dtype=torch.float64, device=device)
         self._axis = torch.tensor(axes, dtype=torch.int32, device=device)
-        self._tables = self._turns.data_ptr(), self._axis.data_ptr()
         self._adjacent = 1 if pairing == "adjacent" else 0
         self.device = self._turns.device
 
@@ -100,8 +99,8 @@ class MultiAxisRotary:
             if not positions.is_contiguous():
                 positions = positions.contiguous()
             at = positions.data_ptr()
-        return nat.RotaryPlan(*self._tables, at, self.num_axes, self.pairs, size, self._adjacent,
-                              1 if inverse else 0, 0), positions
+        return nat.RotaryPlan(self._turns.data_ptr(), self._axis.data_ptr(), at, self.num_axes, self.pairs, size,
+                              self._adjacent, 1 if inverse else 0, 0), positions
 
     def rotate(self, query: torch.Tensor, key: torch.Tensor | None = None, *, positions: torch.Tensor,
                inverse: bool = False):
