@@ -393,3 +393,14 @@ def test_a_plan_follows_its_tables():
     for other in (rotary, copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
         struct, _ = other.plan(positions, 1, 3)
         assert struct.turns == other._turns.data_ptr() and struct.axis == other._axis.data_ptr()
+
+
+def test_tensors_that_came_to_track_a_gradient(monkeypatch):
+    # under no_grad, or after the cache was made
+    for name in ("key", "value"):
+        cache = _built(monkeypatch)
+        getattr(cache, name).requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            cache._struct()
+        with torch.no_grad():
+            cache._struct()

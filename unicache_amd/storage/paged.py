@@ -208,6 +208,9 @@ class PagedKVCache:
                 raise ValueError("Paged cache tensors may be replaced by ones of the same sizes only")
             self._at = self._addresses()
             self._built = nat.PagedCache(*self._at, *self._sizes)
+        elif self.key.requires_grad or self.value.requires_grad:  # (since the cache was made, or under no_grad till now)
+            check_rows(self.key, "Paged cache key")
+            check_rows(self.value, "Paged cache value")
         return self._built
 
     def _attention_workspace(self, sizes: tuple) -> int:
