@@ -980,3 +980,40 @@ def test_a_copied_rotary_reads_its_own_tables(device):
     other = copy.deepcopy(rotary)
     rotary._turns.zero_()
     assert torch.equal(other.rotate(q, positions=positions), want)
+
+
+# ------------------------------------------------------------ ends of the range --
+@pytest.mark.parametrize("hq,lq", [(3, 1), (3, 9), (2, 17), (2, 40), (130, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_logits_that_all_overflow_downwards_give_nan(device, hq, lq, d):
+    """A row that sees keys, all of whose logits are below fp32's range, is no row without keys; a logit within the range beside
+    them takes all the weight, as exp(-inf) = 0 says."""
+
+    far, b = 700, 16
+    lengths = [lq, far, far, far, 2 * b]
+    key = torch.full((5, far, 1, d), -1.0, dtype=torch.float16)
+    key[2, 650] = 0.0    # the only logit in range, in the last steps
+    key[3, :300] = 0.0   # and many, in the first
+    value = randn(5, far, 1, d, seed=3, dtype=torch.float16).cpu()
+    cache, _, _ = filled(lengths, hkv=1, d=d, b=b, dtype=torch.float16)
+    table = cache.table.cpu()
+    for s, n in enumerate(lengths):
+        for i in range(-(-n // b)):
+            r = min(b, n - i * b)
+            cache.key[0, table[s, i], :, :r] = key[s, i * b:i * b + r].transpose(0, 1).cuda()
+            cache.value[0, table[s, i], :, :r] = value[s, i * b:i * b + r].transpose(0, 1).cuda()
+    cache.table[4] = -1  # no page: these rows see no key, and get 0 and -inf
+    q = torch.ones(5, lq, hq, d, dtype=torch.float16, device=device)
+    for hint in (1, far):
+        cache.max_tokens = hint
+        for causal in (False, True):
+            out, lse = cache.attention(q, causal=causal, sm_scale=2.0 ** 127 if causal else 1.1e38)
+            assert out[:2].isnan().all() and lse[:2].isnan().all()
+            assert not out[4].any() and (lse[4] == -math.inf).all()
+            want = value[2, 650, 0].double()
+            assert ((out[2].double().cpu() - want).abs() <= 2 * EPS[q.dtype] * want.abs()).all()
+            assert (lse[2].abs() <= 2.0 ** -20).all()
+            # equal weights of 300 values: their roundings to 16 bits and the sum's
+            want, size = value[3, :300, 0].double().mean(0), value[3, :300, 0].double().abs().mean(0)
+            assert ((out[3].double().cpu() - want).abs() <= EPS[q.dtype] * (want.abs() + size) + 2.0 ** -14 * size).all()
+            assert ((lse[3] - math.log(300)).abs() <= 2.0 ** -18).all()

@@ -23,11 +23,16 @@ struct Query {
   int32_t len, heads, group;
   int32_t causal;
   float scale;  // sm_scale * log2(e)
+  float floor;  // the lowest product q . k that the scale keeps in fp32's range
   FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const { return lens == nullptr ? len : clamped(lens[s]); }
   __device__ __forceinline__ int32_t clamped(int32_t n) const { return n < 0 ? 0 : n > len ? len : n; }
 };
+
+// The largest logit of a row starts here, before the scale: rows whose logits all lie below fp32's range have a reference, and so
+// end as 0 / 0 = NaN; -inf remains for those that see no key.
+__device__ __forceinline__ float lowest(const Query &q, bool sees) { return sees ? q.floor : mf::kNegInf; }
 
 // A sequence's length and number of queries, both on their way at once.
 __device__ __forceinline__ void sizes_of(const Cache &c, const Query &q, int32_t s, int32_t &length, int32_t &count) {
@@ -193,13 +198,18 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, UPPER ? 0x07060302u : 0x05040100u);
 }
 
+// The log-sum-exp of a row that sees keys (a sum of 0 is of logits below fp32's range).
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.0f ? __builtin_nanf("") : kLn2 * (m + __builtin_amdgcn_logf(l));
+}
+
 // D / 16 channels of a finished row.
 template <int D, int DT>
 __device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t r, int32_t c0, const float *o, float m,
                                           float l, uint16_t *out, float *lse) {
   constexpr int kC = D / 16;
   const int32_t t = token_of(q, r), head = w.h * q.group + r - t * q.group;
-  const bool none = t >= w.count || (l == 0.0f && m == mf::kNegInf);  // (logits past fp32's range are no sum: NaN)
+  const bool none = t >= w.count || (l == 0.0f && m == mf::kNegInf);
   const float f = none ? 0.0f : 1.0f / l;
   uint32_t v[kC / 2];
 #pragma unroll
@@ -211,7 +221,7 @@ __device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t
     *reinterpret_cast<uint2 *>(dst) = uint2{v[0], v[1]};
   }
   if (c0 == 0 && lse != nullptr) {
-    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : kLn2 * (m + __builtin_amdgcn_logf(l));
+    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : lse_of(m, l);
   }
 }
 

@@ -90,10 +90,11 @@ struct Acc {
 };
 
 template <int D, int DT, bool MASK>
-__device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], float factor, int32_t seen,
+__device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], const Query &q, int32_t seen,
                                              typename Half<DT>::V8 &high, typename Half<DT>::V8 &low) {
   typedef typename Half<DT>::T T;
-  float top = mf::kNegInf;
+  const float factor = q.scale;
+  float top = lowest(q, !MASK || seen > 0);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = s[j / 4][j % 4];
@@ -220,7 +221,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     V8 high[NR], low[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
+      softmax_step<D, DT, MASK>(acc[n], s[n], q, there ? row_end[n] - mine : 0, high[n], low[n]);
     }
     if constexpr (MASK) {
       // what no row sees is no value
@@ -549,7 +550,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   const int64_t group = query->heads_q / cache->heads_kv, rows = group * query->query_len;
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
-            query->causal != 0, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
+            query->causal != 0, 0.0f, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
   p.rows = rows <= 64 ? static_cast<int32_t>(ceil_div(rows, int64_t(16))) * 16 : kTileRows;
   if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
@@ -616,6 +617,7 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
                            workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "%s: workspace too small", what);
   q.scale = sm_scale * kLog2e;
+  q.floor = -0x1.fffffp127f / (q.scale > 1.0f ? q.scale : 1.0f);  // (times the scale it is finite, however it is rounded)
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);

@@ -168,14 +168,14 @@ struct Acc16 {
 // The reference of 16 rows' weights, raised where one of the tile's logits asks for it.  seen[h]: keys of half h that the
 // lane's row sees, from the lane's own first on.
 template <int D, bool MASK>
-__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], float factor, const int32_t (&seen)[2]) {
-  float top = mf::kNegInf;
+__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], const Query &q, const int32_t (&seen)[2]) {
+  float top = lowest(q, !MASK || seen[0] > 0 || seen[1] > 0);
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float x = s[j / 4][j % 4];
     top = fmaxf(top, MASK && j % 8 >= seen[j / 8] ? mf::kNegInf : x);
   }
-  top = mf::max_over_slices(top * factor);
+  top = mf::max_over_slices(top * q.scale);
   if (__any(top > acc.m + kRaise)) {
     const float m = fmaxf(acc.m, top - kHead);
     const float alpha = acc.m == mf::kNegInf ? 0.0f : mf::fast_exp2(acc.m - m);
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         seen[n][h] = row_end[n] - t0 - 32 * h - 8 * quad;
         if (MASK && ((absent >> (2 * h + (quad >> 1))) & 1) != 0) seen[n][h] = 0;
       }
-      m[n] = reference<D, MASK>(acc[n], s[n], q.scale, seen[n]);
+      m[n] = reference<D, MASK>(acc[n], s[n], q, seen[n]);
     }
     auto weigh = [&](int h) {
 #pragma unroll
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
       }
       if (quad == 0 && lse != nullptr) {
-        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : kLn2 * (acc[n].m + __builtin_amdgcn_logf(total));
+        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
       }
     }
   }

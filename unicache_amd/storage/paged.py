@@ -374,7 +374,8 @@ class PagedKVCache:
         Lq).  With causal=True they are its last tokens: row i sees the keys up
         to lengths[s] - query_lengths[s] + i.  Rows that see no key, and rows
         behind a sequence's queries, get 0 and -inf.  Keys and values that a row does not
-        see never reach it, whatever they hold."""
+        see never reach it, whatever they hold.  Rows with a logit above fp32's range, or
+        with none but below it, are NaN."""
 
         layer = self._layer(layer)
         if sm_scale is None:
