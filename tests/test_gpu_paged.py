@@ -1017,3 +1017,21 @@ def test_logits_that_all_overflow_downwards_give_nan(device, hq, lq, d):
             want, size = value[3, :300, 0].double().mean(0), value[3, :300, 0].double().abs().mean(0)
             assert ((out[3].double().cpu() - want).abs() <= EPS[q.dtype] * (want.abs() + size) + 2.0 ** -14 * size).all()
             assert ((lse[3] - math.log(300)).abs() <= 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,lq", [(7, 6), (4, 16), (4, 70), (16, 40)])
+def test_a_hidden_key_changes_no_bit_of_a_row(device, dtype, hq, lq):
+    # the newest key is finite and far larger than all others: only the last row sees it
+    lengths = [1000, 517]
+    for seed in range(3):
+        cache, _, _ = filled(lengths, hkv=1, d=64, b=32, dtype=dtype, seed=seed)
+        key, table = cache.key.clone(), cache.table.cpu()
+        q = randn(2, lq, hq, 64, seed=seed, dtype=dtype)
+        for s, n in enumerate(lengths):
+            key[0, table[s, (n - 1) // 32], :, (n - 1) % 32] = 30 * q[s, lq - 1, 0]
+        other = PagedKVCache(key, cache.value, cache.table, cache.lengths, max_tokens=1000)
+        out, lse = other.attention(q, causal=True)
+        want, want_lse = cache.attention(q, causal=True)
+        assert torch.equal(out[:, :lq - 1], want[:, :lq - 1]) and torch.equal(lse[:, :, :lq - 1], want_lse[:, :, :lq - 1])
+        assert not torch.equal(lse[:, :, lq - 1], want_lse[:, :, lq - 1])

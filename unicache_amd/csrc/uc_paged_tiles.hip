@@ -177,7 +177,8 @@ __device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], cons
   }
   top = mf::max_over_slices(top * q.scale);
   if (__any(top > acc.m + kRaise)) {
-    const float m = fmaxf(acc.m, top - kHead);
+    // (of the rows that ask for it: no row's last bits hang on what only another one sees)
+    const float m = top > acc.m + kRaise ? top - kHead : acc.m;
     const float alpha = acc.m == mf::kNegInf ? 0.0f : mf::fast_exp2(acc.m - m);
     acc.m = m;
     acc.l *= alpha;
