@@ -1035,3 +1035,47 @@ def test_a_hidden_key_changes_no_bit_of_a_row(device, dtype, hq, lq):
         want, want_lse = cache.attention(q, causal=True)
         assert torch.equal(out[:, :lq - 1], want[:, :lq - 1]) and torch.equal(lse[:, :, :lq - 1], want_lse[:, :, :lq - 1])
         assert not torch.equal(lse[:, :, lq - 1], want_lse[:, :, lq - 1])
+
+
+# ------------------------------------------------------------ rows that are held --
+def test_dense_after_replays_of_a_captured_reserve(device):
+    cache = PagedKVCache.empty(2, 12, 1, 64, page_tokens=16, sequence_pages=6)
+    view, one = cache.layer(0), cache.layer(0, sequence=1)
+    cache.reserve(5)
+    rows = randn(2, 90, 1, 64, seed=1)
+    cache.write(rows[:, :5], -rows[:, :5])
+    for v, s in ((view, slice(0, 2)), (one, slice(1, 2))):  # views know of what was reserved after they were made
+        key, value = v.dense()
+        assert torch.equal(key, rows[s, :5]) and torch.equal(value, -rows[s, :5])
+    new = torch.empty(2, 10, 1, 64, dtype=torch.bfloat16, device=device)
+
+    def step():
+        cache.reserve(10)
+        cache.write(new, -new)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        new.copy_(rows[:, 5:15])
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        new.copy_(rows[:, 15 + 10 * i:25 + 10 * i])
+        graph.replay()
+        torch.cuda.synchronize()
+        n = 25 + 10 * i
+        assert cache.lengths.tolist() == [n, n]
+        key, value = cache.dense()
+        assert key.shape[1] >= n and torch.equal(key[:, :n], rows[:, :n]) and torch.equal(value[:, :n], -rows[:, :n])
+        assert not key[:, n:].any() and not value[:, n:].any()
+        key, _ = one.dense()
+        assert torch.equal(key[:, :n], rows[1:, :n]) and not key[:, n:].any()
+        key, value = cache.dense(tokens=n - 3)
+        assert torch.equal(key, rows[:, :n - 3]) and torch.equal(value, -rows[:, :n - 3])
+    key, _ = cache.dense(tokens=0)
+    assert key.shape == (2, 0, 1, 64)
+    for tokens in (-1, cache.capacity + 1):
+        with pytest.raises(ValueError, match="tokens"):
+            cache.dense(tokens=tokens)

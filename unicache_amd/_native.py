@@ -415,6 +415,15 @@ def call_on(device: torch.device, name: str, *args) -> None:
             call(name, *args, stream(device))
 
 
+def capturing(device: torch.device) -> bool:
+    """Whether the current stream of `device` is being captured into a graph."""
+
+    if device.index == _current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def require_device(*tensors: torch.Tensor | None, what: str) -> torch.device:
     """All given tensors must live on one GPU; returns that device."""
 

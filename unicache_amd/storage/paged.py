@@ -69,8 +69,11 @@ class PagedKVCache:
     Tensors may be replaced by others of their dtype and sizes, or get other storage; calls read them where they are.
 
     ``max_tokens`` is how long the caller takes the longest sequence to be
-    (default: the capacity; raised by reserve); it shapes launches, and no
-    result depends on its being right.  Only dense returns that many rows.
+    (default: the capacity; raised by reserve).  It shapes launches, and no
+    result depends on its being right; only dense returns that many rows.
+    The lengths are on the device, so neither replays of a captured reserve raise it
+    nor do truncate, reorder and compact lower it: set it before a capture to
+    what the loop will reach, and after a cut to what is left, where the caller knows.
 
     Tensors that track a gradient, backward or forward, are refused.  Calls
     enqueue work on the current stream of the cache's device, allocate their
@@ -115,7 +118,7 @@ class PagedKVCache:
         if device.type != "cuda":
             raise RuntimeError(f"Paged cache requires GPU tensors (got {device})")
 
-    def _set(self, key, value, table, lengths, granted, references, free_pages, max_tokens) -> None:
+    def _set(self, key, value, table, lengths, granted, references, free_pages, max_tokens, grown=None) -> None:
         self.key, self.value, self.table, self.lengths = key, value, table, lengths
         self.granted, self.references, self.free_pages = granted, references, free_pages
         self.layers, self.pages, self.num_kv_heads, self.page_tokens, self.head_dim = map(int, key.shape)
@@ -126,6 +129,9 @@ class PagedKVCache:
         self._scale = 1.0 / math.sqrt(self.head_dim)
         self._workspaces = {}
         self.max_tokens = self.capacity if max_tokens is None else min(int(max_tokens), self.capacity)
+        # tokens that were reserved in all, which a cache and its views share, and those of them that max_tokens counts
+        self._grown = [0] if grown is None else grown
+        self._counted = self._grown[0]
         # (refuses sizes that the kernels do not take)
         self._attention_workspace((0, self.num_kv_heads, 0, self._sizes[-1], 0))
 
@@ -181,7 +187,8 @@ class PagedKVCache:
             table, lengths = table[sequence:sequence + 1], lengths[sequence:sequence + 1]
         view = type(self).__new__(type(self))
         view._set(self.key[index:index + 1], self.value[index:index + 1], table, lengths, None, None, None,
-                  self.max_tokens)
+                  self.max_tokens, self._grown)
+        view._counted = self._counted
         return view
 
     # ------------------------------------------------------------- internals --
@@ -260,7 +267,7 @@ class PagedKVCache:
 
         Free pages go out lowest first, to the sequences in order, and `lengths` advances, on
         the device, which alone knows how far the pool goes: `granted`, which is returned, is what each
-        sequence got."""
+        sequence got.  `max_tokens` is raised by `tokens`; replays of a captured call do not raise it."""
 
         self._allocator("reserve")
         tokens = int(tokens)
@@ -269,6 +276,10 @@ class PagedKVCache:
         if counts is not None:
             counts = self._numbers(counts, "counts")
         nat.call_on(self.device, "uc_paged_reserve", self._struct(), tokens, nat.ptr(counts))
+        if nat.capturing(self.device):  # (replays are not seen from here)
+            self._grown[0] += 1 << 40
+        self._grown[0] += tokens
+        self._counted += tokens
         self.max_tokens = min(self.max_tokens + tokens, self.capacity)
         return self.granted
 
@@ -403,16 +414,24 @@ class PagedKVCache:
                     lse.data_ptr(), nat.ptr(ws), nbytes)
         return (out[0], lse[0]) if flat else (out, lse)
 
-    def dense(self, *, layer: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values of one layer as dense [S, max_tokens, Hkv, D] rows, zeros behind each sequence's length."""
+    def dense(self, *, layer: int = 0, tokens: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of one layer as dense [S, tokens, Hkv, D] rows, zeros behind each sequence's length.
+
+        `tokens` defaults to max_tokens; to the capacity after a reserve was
+        captured into a graph, whose replays may have passed max_tokens."""
 
         layer = self._layer(layer)
-        shape = (self.sequences, self.max_tokens, self.num_kv_heads, self.head_dim)
+        if tokens is None:
+            tokens = min(self.max_tokens + self._grown[0] - self._counted, self.capacity)
+        else:
+            tokens = int(tokens)
+            if not 0 <= tokens <= self.capacity:
+                raise ValueError(f"Paged cache dense: tokens must be 0 .. {self.capacity} (got {tokens})")
+        shape = (self.sequences, tokens, self.num_kv_heads, self.head_dim)
         key = torch.empty(shape, dtype=self.dtype, device=self.device)
         value = torch.empty_like(key)
-        if self.max_tokens:
-            nat.call_on(self.device, "uc_paged_dense", self._struct(), layer, key.data_ptr(), value.data_ptr(),
-                        self.max_tokens)
+        if tokens:
+            nat.call_on(self.device, "uc_paged_dense", self._struct(), layer, key.data_ptr(), value.data_ptr(), tokens)
         return key, value
 
     # ------------------------------------------------------------------ bytes --
