@@ -358,18 +358,19 @@ def test_the_struct_follows_storage_that_was_swapped(monkeypatch, name, how):
     else:
         t.set_(t.clone())
     monkeypatch.setattr(PagedKVCache, "_check", staticmethod(lambda *tensors: None))
-    assert {n: getattr(cache._struct(), n) for n in _NAMES} == {n: getattr(cache, n).data_ptr() for n in _NAMES}
+    assert {n: getattr(cache._struct(True), n) for n in _NAMES} == {n: getattr(cache, n).data_ptr() for n in _NAMES}
     del old
 
 
 def test_swapped_storage_is_checked(monkeypatch):
+    # (attention and writes do without the last three)
     for name, bad in (("key", lambda t: t.half()), ("value", lambda t: t[:, :2].contiguous()), ("table", lambda t: t.long()),
                       ("lengths", lambda t: torch.zeros(9, dtype=torch.int32)), ("references", lambda t: t[:2].clone())):
         cache = _built(monkeypatch)
         t = getattr(cache, name)
         old, t.data = t.detach(), bad(t)
         with pytest.raises(ValueError, match="Paged cache"):
-            cache._struct()
+            cache._struct(True)
         del old
 
 
@@ -381,7 +382,7 @@ def test_a_used_cache_is_copied_with_its_addresses_made_anew(monkeypatch):
     monkeypatch.setattr(PagedKVCache, "_check", staticmethod(lambda *tensors: None))
     for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
         assert other.key.data_ptr() != cache.key.data_ptr() and torch.equal(other.table, cache.table)
-        assert {n: getattr(other._struct(), n) for n in _NAMES} == {n: getattr(other, n).data_ptr() for n in _NAMES}
+        assert {n: getattr(other._struct(True), n) for n in _NAMES} == {n: getattr(other, n).data_ptr() for n in _NAMES}
 
 
 def test_a_plan_follows_its_tables():

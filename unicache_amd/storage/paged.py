@@ -200,24 +200,29 @@ class PagedKVCache:
         return layer
 
     def __getstate__(self) -> dict:
-        return {**self.__dict__, "_built": None}  # (a copy's tensors lie elsewhere)
+        return {**self.__dict__, "_built": None, "_reads": None, "_at": None}  # (a copy's tensors lie elsewhere)
 
-    def _addresses(self) -> tuple:
-        return (self.key.data_ptr(), self.value.data_ptr(), self.table.data_ptr(), self.lengths.data_ptr(),
-                *((None, None, None) if self.references is None else
-                  (self.granted.data_ptr(), self.references.data_ptr(), self.free_pages.data_ptr())))
+    def _struct(self, books: bool = False) -> "nat.PagedCache":
+        """The C struct of the tensors where they lie now (storage can be swapped under a tensor); calls that read
+        granted, references and free_pages through it ask for those with `books`."""
 
-    def _struct(self) -> "nat.PagedCache":
-        if self._built is None or self._at != self._addresses():  # (storage can be swapped under a tensor)
-            self._check(*(getattr(self, name) for name in _ORDER))
-            if (*self.key.shape[:2], *self.table.shape, *self.key.shape[2:]) != (
-                    *self._sizes[:5], self.page_tokens, self.head_dim) or self.key.dtype != self.dtype:
-                raise ValueError("Paged cache tensors may be replaced by ones of the same sizes only")
-            self._at = self._addresses()
-            self._built = nat.PagedCache(*self._at, *self._sizes)
-        elif self.key.requires_grad or self.value.requires_grad:  # (since the cache was made, or under no_grad till now)
-            check_rows(self.key, "Paged cache key")
-            check_rows(self.value, "Paged cache value")
+        if self._built is not None:
+            key, value, table, lengths = self._reads[0]
+            if (key(), value(), table(), lengths()) == self._at[0] and (
+                    not books or tuple(read() for read in self._reads[1]) == self._at[1]):
+                if self.key.requires_grad or self.value.requires_grad:  # (since then, or under no_grad till now)
+                    check_rows(self.key, "Paged cache key")
+                    check_rows(self.value, "Paged cache value")
+                return self._built
+        tensors = [getattr(self, name) for name in _ORDER]
+        self._check(*tensors)
+        if (*self.key.shape[:2], *self.table.shape, *self.key.shape[2:]) != (
+                *self._sizes[:5], self.page_tokens, self.head_dim) or self.key.dtype != self.dtype:
+            raise ValueError("Paged cache tensors may be replaced by ones of the same sizes only")
+        reads = [t.data_ptr for t in tensors if t is not None]
+        at = [read() for read in reads]
+        self._reads, self._at = (tuple(reads[:4]), tuple(reads[4:])), (tuple(at[:4]), tuple(at[4:]))
+        self._built = nat.PagedCache(*at, *[None] * (7 - len(at)), *self._sizes)
         return self._built
 
     def _attention_workspace(self, sizes: tuple) -> int:
@@ -275,7 +280,7 @@ class PagedKVCache:
             raise ValueError("Paged cache reserve: tokens must not be negative, and below 2^30")
         if counts is not None:
             counts = self._numbers(counts, "counts")
-        nat.call_on(self.device, "uc_paged_reserve", self._struct(), tokens, nat.ptr(counts))
+        nat.call_on(self.device, "uc_paged_reserve", self._struct(True), tokens, nat.ptr(counts))
         if nat.capturing(self.device):  # (replays are not seen from here)
             self._grown[0] += 1 << 40
         self._grown[0] += tokens
@@ -308,7 +313,7 @@ class PagedKVCache:
     def _reorder(self, parents, lengths) -> None:
         nbytes = _workspace_bytes("uc_paged_reorder_workspace_bytes", self._sizes, True, None)
         ws = nat.workspace(self.device, nbytes)
-        nat.call_on(self.device, "uc_paged_reorder", self._struct(), nat.ptr(parents), nat.ptr(lengths),
+        nat.call_on(self.device, "uc_paged_reorder", self._struct(True), nat.ptr(parents), nat.ptr(lengths),
                     self.max_tokens, ws.data_ptr(), nbytes)
 
     def compact(self, keep: torch.Tensor) -> None:
@@ -329,7 +334,7 @@ class PagedKVCache:
             keep = keep.contiguous()
         nbytes = _workspace_bytes("uc_paged_compact_workspace_bytes", self._sizes, True, None)
         ws = nat.workspace(self.device, nbytes)
-        nat.call_on(self.device, "uc_paged_compact", self._struct(), keep.data_ptr(), keep.stride(0),
+        nat.call_on(self.device, "uc_paged_compact", self._struct(True), keep.data_ptr(), keep.stride(0),
                     int(keep.shape[1]), self.max_tokens, ws.data_ptr(), nbytes)
 
     # ------------------------------------------------------------------ calls --
