@@ -875,8 +875,9 @@ typedef struct uc_paged_cache {
  * out = softmax(sm_scale * q K^T) V of one layer over each row's visible keys, contiguous [S, Lq, Hq, D], and lse
  * [S, Hq, Lq] (natural log, may be NULL).  query as in uc_block8_attn, its dtype the cache's.  Rows that
  * see no key, and rows behind a sequence's queries, get 0 and -inf.  What a row does not see never
- * reaches it, whatever it holds.  2^-126 <= sm_scale <= 2^127; a row with a logit above fp32's range, or with
- * none but below it, is NaN.
+ * reaches it, whatever it holds; an infinity among the values that it sees is its output in that channel (NaN for two
+ * of both signs), however small the weight.  2^-126 <= sm_scale <= 2^127; a row with a logit above fp32's range, or
+ * with none but below it, is NaN.
  * workspace: uc_paged_attn_workspace_bytes(cache, query).
  */
 int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const uc_block8_query *query, float sm_scale, void *out,

@@ -1079,3 +1079,45 @@ def test_dense_after_replays_of_a_captured_reserve(device):
     for tokens in (-1, cache.capacity + 1):
         with pytest.raises(ValueError, match="tokens"):
             cache.dense(tokens=tokens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,lq,causal", [(1, 1, False), (7, 1, True), (8, 5, True), (4, 60, False), (4, 60, True)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, dtype, hq, lq, causal, d):
+    """Weights are positive: a visible infinity makes its channel that infinity, two of both signs or a NaN make it NaN, however
+    small the weight, in whole tiles and in parts that are joined; the other channels are as without it."""
+
+    b, lengths = 16, [40, 700, 9000]
+    for hint in (1, 9000):
+        cache, _, _ = filled(lengths, hkv=1, d=d, b=b, dtype=dtype)
+        cache.max_tokens = hint
+        table, rows = cache.table.cpu(), {}
+        q = randn(3, lq, hq, d, seed=1, dtype=dtype)
+        q[..., 0] = 4.0
+        far = math.sqrt(d) * 40.0  # a logit 160 below the others': fp32 holds no e^-160
+        for s, n in enumerate(lengths):
+            for t, channel, x, small in ((2, 7, math.inf, False), (n // 2, 8, -math.inf, False), (3, 9, math.inf, False),
+                                         (n // 3, 9, -math.inf, False), (1, 10, math.nan, False), (0, 11, math.inf, True),
+                                         (n // 4, 12, -math.inf, True)):
+                at = 0, table[s, t // b], 0, t % b
+                if small:
+                    cache.key[at][0] = -far
+                rows[s, t, channel] = at, x
+        clean = cache.attention(q, causal=causal)
+        for (s, t, channel), (at, x) in rows.items():
+            cache.value[at][channel] = x
+        zeros = PagedKVCache(cache.key, torch.nan_to_num(cache.value, nan=0.0, posinf=0.0, neginf=0.0), cache.table, cache.lengths,
+                             max_tokens=hint)
+        out, lse = cache.attention(q, causal=causal)
+        want, want_lse = zeros.attention(q, causal=causal)
+        assert torch.equal(lse, want_lse) and torch.equal(lse, clean[1])
+        for s, n in enumerate(lengths):
+            if causal and lq > n:
+                continue  # (rows that see few keys or none)
+            got = out[s].float()
+            assert (got[..., 7] == math.inf).all() and (got[..., 8] == -math.inf).all()
+            assert got[..., 9].isnan().all() and got[..., 10].isnan().all()
+            assert (got[..., 11] == math.inf).all() and (got[..., 12] == -math.inf).all()
+            others = [c for c in range(d) if not 7 <= c <= 12]
+            assert torch.equal(out[s][..., others], want[s][..., others])

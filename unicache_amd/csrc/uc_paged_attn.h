@@ -129,9 +129,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, V2{static_cast<T>(a), static_cast<T>(b)});
 }
 
-// Values that are not finite, in tiles that not every row sees whole: a hidden key's weight is 0, and 0 times them is
-// NaN.  So where there are any the products take 0 in their place, and others count, for each row,
-// the keys that it does see of each kind; one is enough to make the sum what it is.
+// Values that are not finite.  In tiles that not every row sees whole a hidden key's weight is 0, and 0 times them is NaN; where a
+// row sees them its weight may have been rounded to 0, or be two numbers of which one is 0 or negative.  So where there are
+// any the products take 0 in their place, and others count, for each row, the keys that it does see of each kind; one is
+// enough to make the sum what it is.  Tiles that some rows see in part are searched for them; the others only when a sum is no number
+// at the end, in a second pass over all tiles.
 template <int DT>
 constexpr uint32_t kInfinity = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
 
@@ -190,6 +192,21 @@ __device__ __forceinline__ void add_infinite(f4 (&o)[N], const Infinite &x) {
       o[d][i] -= (x.down & bit) != 0 ? __builtin_huge_valf() : 0.0f;
     }
   }
+}
+
+// Whether a row's N sums, and that of its weights, show that such values went into them.
+template <int N, class At>
+__device__ __forceinline__ bool spoiled(At at, float l) {
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = __builtin_elementwise_maximum(top, __builtin_fabsf(at(j)));  // (passes NaN on)
+  return !(top < __builtin_huge_valf()) && l < __builtin_huge_valf();
+}
+
+// A part's sum as it joins others: where it is not finite it stays so, however small the factor.
+__device__ __forceinline__ float joining(float f, float o) {
+  const float x = f * o;
+  return x == x ? x : o;  // (a factor that is no number makes the sum of the weights NaN, and so the row)
 }
 
 // The lower or the upper halves of two dwords as one.

@@ -127,14 +127,16 @@ struct Joined {
   static constexpr bool kHeld = NR * D >= 192;
   float o[4][16][D + 4];  // (a wave's part holds a tile's values, 8 D / 32 dwords a lane)
   float m[4][16], l[4][16];
+  uint32_t bad;  // whether sums are not finite, though their weights are
   typename Half<DT>::V8 frag[kHeld ? NR * D / 32 : 1][64];
 };
 
 // Steps begin .. end - 1 of the rows w, by a whole workgroup.  slot >= 0: the part goes there; else it
-// is all there is, and the rows are finished.
+// is all there is, and the rows are finished.  Returns whether values that are not finite went into sums: then once more with `search`.
 template <int D, int DT, int NR>
-__device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows &w, int32_t begin, int32_t end, int32_t slot,
-                                      Joined<D, DT, NR> &joined, uint16_t *out, float *lse, float *part, float *stat) {
+__device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows &w, int32_t begin, int32_t end, int32_t slot,
+                                      bool search, Joined<D, DT, NR> &joined, uint16_t *out, float *lse, float *part,
+                                      float *stat) {
   typedef Half<DT> H;
   typedef typename H::V8 V8;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15,
@@ -232,7 +234,7 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) raw.v[j][i] = held ? raw.v[j][i] : 0u;
       }
-      if (w.end_first != w.end_last) {  // some rows see more than others
+      if (search || w.end_first != w.end_last) {  // some rows see more than others
         uint32_t bad = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -284,17 +286,20 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     t += kStep;
   };
   // tiles that every row sees come first; from the first other one on, every tile is masked
-  while (t < stop && t + kTile <= w.end_first && first_a >= 0 && first_b >= 0) step(std::false_type());
+  while (!search && t < stop && t + kTile <= w.end_first && first_a >= 0 && first_b >= 0) step(std::false_type());
   while (t < stop) step(std::true_type());
 
   // join the waves: 16 threads a row, D / 16 channels each
   constexpr int kC = D / 16;
   const int row = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * kC;
+  const float least = search ? 0x1p-126f : 0.0f;  // (infinities stay, however small the factor)
+  bool bad = false;
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const float l_row = mf::sum_over_slices(acc[n].l);
     add_infinite(acc[n].o, infinite[n]);
-    __syncthreads();  // what was joined before has been read
+    __syncthreads();  // what was joined before, and its flag, have been read
+    if (n == 0 && threadIdx.x == 0) joined.bad = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -318,13 +323,14 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
     for (int v = 0; v < 4; ++v) {
       // a wave without keys of this row has nothing to add, unless what it has is not a number
       if (joined.m[v][row] == mf::kNegInf && joined.l[v][row] == 0.0f) continue;
-      const float f = mf::fast_exp2(joined.m[v][row] - m);
+      const float f = fmaxf(mf::fast_exp2(joined.m[v][row] - m), least);
       total += f * joined.l[v][row];
 #pragma unroll
       for (int j = 0; j < kC; ++j) o[j] += f * joined.o[v][row][c0 + j];
     }
     const int32_t r = w.r0 + 16 * n + row;
     if (r >= w.rows) continue;
+    bad |= spoiled<kC>([&](int j) { return o[j]; }, total);
     if (slot >= 0) {
       const int64_t at = int64_t(slot) * (16 * NR) + 16 * n + row;
 #pragma unroll
@@ -339,7 +345,9 @@ __device__ __forceinline__ void piece(const Cache &c, const Query &q, const Rows
       store_row<D, DT>(q, w, r, c0, o, m, total, out, lse);
     }
   }
+  if (__any(bad)) joined.bad = 1;  // (barriers lie between this, the first write and the read)
   __syncthreads();  // the next piece may write what has been read here
+  return __builtin_expect(__builtin_amdgcn_readfirstlane(joined.bad) != 0, false);
 }
 
 // The steps of all units ((sequence, head, group) in order) are cut into runs of equal length for the
@@ -394,12 +402,15 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   int32_t now = __builtin_amdgcn_readlane(steps, first);  // steps of each of the sequence's units
   rest -= (__builtin_amdgcn_readlane(sum, first) - now) * each;
   int32_t n = rest / now, t = rest - n * now;  // the unit within the sequence, and its step
+  bool search = false;
   while (at < stop) {
     const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
     const int32_t h = p.groups == 1 ? n : n / p.groups, group = n - h * p.groups;
     const Rows w = rows_at(q, s, h, group, 16 * NR, __builtin_amdgcn_readlane(length, first),
                            __builtin_amdgcn_readlane(count, first));
-    piece<D, DT, NR>(c, q, w, t, end, end - t == now ? -1 : g + s * each + n, joined, out, lse, part, stat);
+    const int32_t slot = end - t == now ? -1 : g + s * each + n;
+    search = piece<D, DT, NR>(c, q, w, t, end, slot, search, joined, out, lse, part, stat) && !search;
+    if (search) continue;
     at += end - t;
     t = 0;
     if (++n == each && at < stop) {
@@ -497,7 +508,7 @@ __device__ __forceinline__ Sum<D> sum_parts(const Plan &p, const Parts &x, int32
       const float f = mf::fast_exp2(mi[u] - t.m);
       t.l += f * li[u];
 #pragma unroll
-      for (int j = 0; j < kC; ++j) t.o[j] += f * oi[u][j / 4][j % 4];
+      for (int j = 0; j < kC; ++j) t.o[j] += joining(f, oi[u][j / 4][j % 4]);
     }
     i0 += 2 * STRIDE;
     if (i0 < x.count) load(i0);

@@ -325,6 +325,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   typedef Half<DT> H;
   typedef typename H::V8 V8;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
+  __shared__ uint32_t bad;  // whether sums are not finite, though their weights are: the unit's tiles once more, each searched
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   // Two waves share a SIMD, in slots that differ in their last bit (HW_ID's first four bits).
   // One goes before the other in its vector phases, so that they do not reach the matrix cores together.
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   Walk walk(c, q, p, run);
   const Loader<D> ld;
   const int krow = (col >> 2) * 8 + (col & 3);
-  for (; walk.more(); walk.next(c, q, p)) {
+  bool search = false;
+  while (walk.more()) {
   const Rows w = walk.rows(c, q, p);
   const int32_t begin = walk.begin, end = walk.end;
   Pages pages(c, w.s);
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     weigh(0);
     weigh(1);
     present ^= 1;
-    if (MASK && w.end_first != w.end_last) {  // some rows see more keys than others
+    if (MASK && (search || w.end_first != w.end_last)) {  // some rows see more keys than others
       u4 *held = reinterpret_cast<u4 *>(lds + (present ^ 1) * T::kBytes + T::kKeyBytes);
       uint32_t bad = 0;
       for (int i = lane; i < T::kValueBytes / 16; i += 64) {
@@ -493,8 +495,9 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0) bad = 0;  // (the last unit's has been read; a barrier a tile lies before this one's is written)
   // tiles that every row sees come first; from the first other one on, every tile is masked
-  while (t < end && whole()) step(std::false_type());
+  while (!search && t < end && whole()) step(std::false_type());
   while (t < end) step(std::true_type());
 
 #pragma unroll
@@ -503,6 +506,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     const float total = mf::sum_over_slices(acc[n].l);
     add_infinite(acc[n].o, infinite[n]);
     if (r >= w.rows) continue;
+    if (spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total)) bad = 1;
     if (walk.part()) {
       const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;
 #pragma unroll
@@ -526,6 +530,9 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
       }
     }
   }
+  __syncthreads();
+  search = __builtin_amdgcn_readfirstlane(bad) != 0 && !search;
+  if (!search) walk.next(c, q, p);
   }
 }
 
@@ -566,7 +573,7 @@ __global__ __launch_bounds__(256) void tile_join_kernel(Cache c, Query q, Plan p
       const float f = mf::fast_exp2(mi[u] - m);
       l += li[u] * f;
 #pragma unroll
-      for (int j = 0; j < kC; ++j) o[j] += x[u][j / 4][j % 4] * f;
+      for (int j = 0; j < kC; ++j) o[j] += joining(f, x[u][j / 4][j % 4]);
     }
   }
   store_row<D, DT>(q, w, w.r0 + rr, lane * kC, o, m, l, out, lse);

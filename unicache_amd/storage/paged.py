@@ -390,8 +390,9 @@ class PagedKVCache:
         Lq).  With causal=True they are its last tokens: row i sees the keys up
         to lengths[s] - query_lengths[s] + i.  Rows that see no key, and rows
         behind a sequence's queries, get 0 and -inf.  Keys and values that a row does not
-        see never reach it, whatever they hold.  Rows with a logit above fp32's range, or
-        with none but below it, are NaN."""
+        see never reach it, whatever they hold; an infinity among the values that it does
+        see is its output in that channel (NaN for two of both signs), however small the weight.
+        Rows with a logit above fp32's range, or with none but below it, are NaN."""
 
         layer = self._layer(layer)
         if sm_scale is None:
