@@ -44,7 +44,7 @@ __device__ __forceinline__ void sizes_of(const Cache &c, const Query &q, int32_t
 constexpr int kTileRows = 128;            // rows of a unit of many (uc_paged_tiles.hip)
 
 struct Plan {
-  int32_t rows, groups;  // rows of a unit, and units of a (sequence, KV head)
+  int32_t rows, groups;  // rows of a unit, and units of a (sequence, KV head): one, of all its rows, up to 64
   int32_t workgroups;    // that share all steps; 0 (many rows): one a unit
 };
 

@@ -5,7 +5,7 @@
 // m is a running reference of the row, 2^6 below its largest weight when it was last raised; it is raised
 // when a weight passes 2^14, so that most tiles leave O alone, and fp16 weights keep their bits
 // down to 2^-24.  Sums, m and O are fp32.  A weight goes into the matrix products as two 16-bit numbers,
-// its rounding and what that leaves, so that the products lose 2^-17 of it and not 2^-9: the
+// its rounding and what that leaves, so that the products lose 2^-16 of it and not 2^-8 (fp16: 2^-22 and not 2^-11): the
 // cores have the time beside the loads.
 //
 // Layout: S^T = K Q^T on 16x16x32 MFMAs.  Row r of key tile a is key 8 (r / 4) + 4 a + r % 4 of a wave's 32,
@@ -350,7 +350,7 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
   return __builtin_expect(__builtin_amdgcn_readfirstlane(joined.bad) != 0, false);
 }
 
-// The steps of all units ((sequence, head, group) in order) are cut into runs of equal length for the
+// The steps of all units ((sequence, head) in order) are cut into runs of equal length for the
 // workgroups, so that sequences of any lengths load them alike.  A unit's part in workgroup g is in slot
 // g + unit: of two parts in order one of the two is larger.
 __device__ __forceinline__ int32_t steps_of(int32_t length, int32_t count) {
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
                                                                              float *lse, float *part, float *stat) {
   __shared__ Joined<D, DT, NR> joined;
   const int lane = threadIdx.x & 63;
-  const int32_t g = blockIdx.x, each = c.heads * p.groups;
+  const int32_t g = blockIdx.x, each = c.heads;  // (a unit holds all rows of a head)
   int32_t s0 = 0, first = 0;  // sequences s0 .. s0 + 63 are in the lanes, `first` of them is the present one
   int32_t length = 0, count = 0, steps = 0, sum = 0, total = 0;
   auto fill = [&] {
@@ -405,8 +405,7 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   bool search = false;
   while (at < stop) {
     const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
-    const int32_t h = p.groups == 1 ? n : n / p.groups, group = n - h * p.groups;
-    const Rows w = rows_at(q, s, h, group, 16 * NR, __builtin_amdgcn_readlane(length, first),
+    const Rows w = rows_at(q, s, n, 0, 16 * NR, __builtin_amdgcn_readlane(length, first),
                            __builtin_amdgcn_readlane(count, first));
     const int32_t slot = end - t == now ? -1 : g + s * each + n;
     search = piece<D, DT, NR>(c, q, w, t, end, slot, search, joined, out, lse, part, stat) && !search;
@@ -438,8 +437,7 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
   Parts x;
   const int32_t full = q.len * q.group, sh = index / full, s = sh / c.heads;
   x.r = index - sh * full;
-  const int32_t group = p.groups == 1 ? 0 : x.r / p.rows, each = c.heads * p.groups;
-  const int32_t unit = sh * p.groups + group;
+  const int32_t each = c.heads;
   int32_t total = 0, before = 0, mine = 0, my_length = 0, my_count = 0;
   for (int32_t s0 = 0; s0 < c.sequences; s0 += 64) {
     const int32_t i = s0 + (threadIdx.x & 63);
@@ -457,11 +455,11 @@ __device__ __forceinline__ Parts parts_of(const Cache &c, const Query &q, const 
     }
     total += __builtin_amdgcn_readlane(sum, 63);
   }
-  x.w = rows_at(q, s, sh - s * c.heads, group, p.rows, my_length, my_count);
+  x.w = rows_at(q, s, sh - s * c.heads, 0, p.rows, my_length, my_count);
   const int32_t per = per_of(p, total * each);
-  const int32_t start = before * each + (unit - s * each) * mine;
-  x.first = mine == 0 ? 0 : start / per + unit;
-  x.count = mine == 0 ? 0 : (start + mine - 1) / per + unit - x.first + 1;
+  const int32_t start = before * each + (sh - s * each) * mine;
+  x.first = mine == 0 ? 0 : start / per + sh;
+  x.count = mine == 0 ? 0 : (start + mine - 1) / per + sh - x.first + 1;
   return x;
 }
 
@@ -522,7 +520,7 @@ __global__ __launch_bounds__(256) void join_few_kernel(Cache c, Query q, Plan p,
                                                        const float *part, const float *stat) {
   const int32_t index = blockIdx.x * 16 + (threadIdx.x >> 4), last = rows - 1;
   const Parts x = parts_of(c, q, p, index < rows ? index : last);  // (whole waves: they sum up the lengths)
-  if (index >= rows || (x.count == 1 && p.workgroups > 0)) return;
+  if (index >= rows || x.count == 1) return;
   const Sum<D> t = sum_parts<D, 1>(p, x, 0, part, stat);
   store_row<D, DT>(q, x.w, x.r, (threadIdx.x & 15) * (D / 16), t.o, t.m, t.l, out, lse);
 }

@@ -1,7 +1,7 @@
 // Attention over the paged 16-bit cache for many query rows: a prompt's chunk, an image's queries.
 // The mathematics is that of uc_paged_attn.hip, but for the weights, which go into the products as one 16-bit number
-// (half a step, 2^-9 in bf16, 2^-12 in fp16, of each; over many keys that is as much as the output's own
-// rounding): the matrix cores, not the loads, are what such calls wait for.
+// (half a step, 2^-8 in bf16, 2^-11 in fp16, of each at most; over 13k keys outputs lie 2.3e-3 from 64-bit arithmetic,
+// 1.7e-3 of it their own rounding): the matrix cores, not the loads, are what such calls wait for.
 //
 // A workgroup owns 128 query rows of one KV head, 32 per wave, and walks 64-key tiles.  Its 256 threads
 // read the next tile into registers while the present one is computed, and write the other of two LDS
