@@ -23,16 +23,11 @@ struct Query {
   int32_t len, heads, group;
   int32_t causal;
   float scale;  // sm_scale * log2(e)
-  float floor;  // the lowest product q . k that the scale keeps in fp32's range
   FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const { return lens == nullptr ? len : clamped(lens[s]); }
   __device__ __forceinline__ int32_t clamped(int32_t n) const { return n < 0 ? 0 : n > len ? len : n; }
 };
-
-// The largest logit of a row starts here, before the scale: rows whose logits all lie below fp32's range have a reference, and so
-// end as 0 / 0 = NaN; -inf remains for those that see no key.
-__device__ __forceinline__ float lowest(const Query &q, bool sees) { return sees ? q.floor : mf::kNegInf; }
 
 // A sequence's length and number of queries, both on their way at once.
 __device__ __forceinline__ void sizes_of(const Cache &c, const Query &q, int32_t s, int32_t &length, int32_t &count) {
@@ -194,7 +189,7 @@ __device__ __forceinline__ void add_infinite(f4 (&o)[N], const Infinite &x) {
   }
 }
 
-// Whether a row's N sums, and that of its weights, show that such values went into them.
+// Whether a row's N sums, beside that of its weights, show that such values went into them.
 template <int N, class At>
 __device__ __forceinline__ bool spoiled(At at, float l) {
   float top = 0.0f;
@@ -213,6 +208,15 @@ __device__ __forceinline__ float joining(float f, float o) {
 template <bool UPPER>
 __device__ __forceinline__ uint32_t halves_of(uint32_t first, uint32_t second) {
   return __builtin_amdgcn_perm(second, first, UPPER ? 0x07060302u : 0x05040100u);
+}
+
+// The reference of a row that has none after tokens first .. end - 1: -inf where there is no key among them, else its logits all lie
+// below fp32's range, and with the lowest finite one it ends as 0 / 0 = NaN, unless another part has weights.
+__device__ __forceinline__ float no_reference(const Cache &c, int32_t s, int32_t first, int32_t end) {
+  for (int32_t t = first; t < end; t = (t | (c.page - 1)) + 1) {
+    if (c.is_page(c.table[int64_t(s) * c.width + (t >> c.shift)])) return -0x1.fffffep127f;
+  }
+  return mf::kNegInf;
 }
 
 // The log-sum-exp of a row that sees keys (a sum of 0 is of logits below fp32's range).

@@ -90,11 +90,10 @@ struct Acc {
 };
 
 template <int D, int DT, bool MASK>
-__device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], const Query &q, int32_t seen,
+__device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], float factor, int32_t seen,
                                              typename Half<DT>::V8 &high, typename Half<DT>::V8 &low) {
   typedef typename Half<DT>::T T;
-  const float factor = q.scale;
-  float top = lowest(q, !MASK || seen > 0);
+  float top = mf::kNegInf;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = s[j / 4][j % 4];
@@ -224,7 +223,7 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
     V8 high[NR], low[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      softmax_step<D, DT, MASK>(acc[n], s[n], q, there ? row_end[n] - mine : 0, high[n], low[n]);
+      softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
     }
     if constexpr (MASK) {
       // what no row sees is no value
@@ -292,7 +291,7 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
   // join the waves: 16 threads a row, D / 16 channels each
   constexpr int kC = D / 16;
   const int row = threadIdx.x >> 4, c0 = (threadIdx.x & 15) * kC;
-  const float least = search ? 0x1p-126f : 0.0f;  // (infinities stay, however small the factor)
+  const float least = search ? 0x1p-149f : 0.0f;  // (infinities stay, however small the factor)
   bool bad = false;
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
@@ -330,6 +329,10 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
     }
     const int32_t r = w.r0 + 16 * n + row;
     if (r >= w.rows) continue;
+    if (total == 0.0f && m == mf::kNegInf) {
+      const int32_t mine = visible(q, w.length, w.count, token_of(q, r));
+      m = no_reference(c, w.s, begin * kStep, mine < stop ? mine : stop);
+    }
     bad |= spoiled<kC>([&](int j) { return o[j]; }, total);
     if (slot >= 0) {
       const int64_t at = int64_t(slot) * (16 * NR) + 16 * n + row;
@@ -405,7 +408,11 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   bool search = false;
   while (at < stop) {
     const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
-    const Rows w = rows_at(q, s, n, 0, 16 * NR, __builtin_amdgcn_readlane(length, first),
+    // Of 64 rows it is opaque, so that what their numbers give is worked out for each piece: held across pieces it takes registers
+    // that the tiles spill (16 x 8 tokens of 4k at 64 channels 27.1 us, 26.4 so; of 48 rows 21.2 held, 21.7 so).
+    int32_t only = 0;
+    if constexpr (NR == 4) asm volatile("" : "+s"(only));
+    const Rows w = rows_at(q, s, n, only, 16 * NR, __builtin_amdgcn_readlane(length, first),
                            __builtin_amdgcn_readlane(count, first));
     const int32_t slot = end - t == now ? -1 : g + s * each + n;
     search = piece<D, DT, NR>(c, q, w, t, end, slot, search, joined, out, lse, part, stat) && !search;
@@ -560,7 +567,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   const int64_t group = query->heads_q / cache->heads_kv, rows = group * query->query_len;
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
-            query->causal != 0, 0.0f, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
+            query->causal != 0, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
   p.rows = rows <= 64 ? static_cast<int32_t>(ceil_div(rows, int64_t(16))) * 16 : kTileRows;
   if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
@@ -627,7 +634,6 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
                            workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "%s: workspace too small", what);
   q.scale = sm_scale * kLog2e;
-  q.floor = -0x1.fffffp127f / (q.scale > 1.0f ? q.scale : 1.0f);  // (times the scale it is finite, however it is rounded)
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);

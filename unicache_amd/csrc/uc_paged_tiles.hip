@@ -129,14 +129,13 @@ __device__ __forceinline__ void store_keys(const Staged<D> &st, char *buf, const
   }
 }
 
-// What no row of the unit sees is no value: from `end` on, which for the rows of one causal token (128 query heads or more of a KV
-// head) lies before the sequence's length.
+// What lies behind the length is no value.
 template <int D>
-__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t end) {
+__device__ __forceinline__ void clear_values(Staged<D> &st, const Loader<D> &ld, int32_t length) {
   const bool there = ((st.absent >> ld.wave) & 1) == 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const bool held = there && st.t + 8 * ld.group + j < end;
+    const bool held = there && st.t + 8 * ld.group + j < length;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) st.v[j][i] = held ? st.v[j][i] : 0u;
   }
@@ -168,14 +167,14 @@ struct Acc16 {
 // The reference of 16 rows' weights, raised where one of the tile's logits asks for it.  seen[h]: keys of half h that the
 // lane's row sees, from the lane's own first on.
 template <int D, bool MASK>
-__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], const Query &q, const int32_t (&seen)[2]) {
-  float top = lowest(q, !MASK || seen[0] > 0 || seen[1] > 0);
+__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], float factor, const int32_t (&seen)[2]) {
+  float top = mf::kNegInf;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     const float x = s[j / 4][j % 4];
     top = fmaxf(top, MASK && j % 8 >= seen[j / 8] ? mf::kNegInf : x);
   }
-  top = mf::max_over_slices(top * q.scale);
+  top = mf::max_over_slices(top * factor);
   if (__any(top > acc.m + kRaise)) {
     // (of the rows that ask for it: no row's last bits hang on what only another one sees)
     const float m = top > acc.m + kRaise ? top - kHead : acc.m;
@@ -318,9 +317,47 @@ struct Walk {
   __device__ __forceinline__ int32_t slot(int32_t run) const { return slot_of(run, first); }
 };
 
+struct Args {
+  Cache c;
+  Query q;
+  Plan p;
+  uint16_t *out;
+  float *lse, *part, *stat;
+};
+
+// The kernel's arguments, read anew: what only a unit's beginning or end asks for takes no scalar registers from the tiles between.
+// (Held throughout they pass the 102 that there are, and the tiles read some back from vector registers one at a time: 2 x 2k of
+// 13k 730 us, 720 so; of 9k at 64 channels 219, 208 so.)  What is loaded from stays as given: the compiler knows it for global
+// memory only so, and flat loads count as LDS reads too (790 us).
+__device__ __forceinline__ Args arguments(const Args &given) {
+  struct Words {
+    uint32_t w[sizeof(Args) / 4];
+  } words;
+  typedef const __attribute__((address_space(4))) uint32_t *Scalars;
+  Scalars p = (Scalars)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+#pragma unroll
+  for (size_t i = 0; i < sizeof(Args) / 4; ++i) words.w[i] = p[i];
+  Args a = __builtin_bit_cast(Args, words);
+  a.c.key = given.c.key;
+  a.c.value = given.c.value;
+  a.c.table = given.c.table;
+  a.c.lengths = given.c.lengths;
+  a.q.p = given.q.p;
+  a.q.lens = given.q.lens;
+  return a;
+}
+
+// A pointer to global memory, for stores through what was read anew.
+template <class T>
+using Global = __attribute__((address_space(1))) T;
+template <class T>
+__device__ __forceinline__ Global<T> *global(T *p) {
+  return (Global<T> *)p;
+}
+
 template <int D, int DT, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse, float *part,
-                                                      float *stat) {
+__global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
   typedef Tile<D> T;
   typedef Half<DT> H;
   typedef typename H::V8 V8;
@@ -338,13 +375,21 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     }
   };
   // Workgroups go to the 8 XCDs in turn; an XCD takes runs that follow each other, so that its L2 holds the keys of few heads.
-  const int32_t run = p.workgroups == 0 ? blockIdx.x : (blockIdx.x & 7) * (p.workgroups / 8) + (blockIdx.x >> 3);
-  Walk walk(c, q, p, run);
+  auto own_run = [&](const Plan &p) -> int32_t {
+    return p.workgroups == 0 ? blockIdx.x : (blockIdx.x & 7) * (p.workgroups / 8) + (blockIdx.x >> 3);
+  };
+  Walk walk = [&] {
+    const Args x = arguments(given);
+    return Walk(x.c, x.q, x.p, own_run(x.p));
+  }();
   const Loader<D> ld;
   const int krow = (col >> 2) * 8 + (col & 3);
   bool search = false;
   while (walk.more()) {
-  const Rows w = walk.rows(c, q, p);
+  const Args unit = arguments(given);
+  const Cache &c = unit.c;
+  const Query &q = unit.q;
+  const Rows w = walk.rows(c, q, unit.p);
   const int32_t begin = walk.begin, end = walk.end;
   Pages pages(c, w.s);
   const int64_t head = int64_t(w.h << c.shift) * D;
@@ -426,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         seen[n][h] = row_end[n] - t0 - 32 * h - 8 * quad;
         if (MASK && ((absent >> (2 * h + (quad >> 1))) & 1) != 0) seen[n][h] = 0;
       }
-      m[n] = reference<D, MASK>(acc[n], s[n], q, seen[n]);
+      m[n] = reference<D, MASK>(acc[n], s[n], q.scale, seen[n]);
     }
     auto weigh = [&](int h) {
 #pragma unroll
@@ -435,7 +480,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     weigh(0);
     weigh(1);
     present ^= 1;
-    if (MASK && (search || w.end_first != w.end_last)) {  // some rows see more keys than others
+    // (some rows see less than there is; those of one causal token, 128 query heads or more of a KV head, all do)
+    if (MASK && (search || w.end_first < w.length)) {
       u4 *held = reinterpret_cast<u4 *>(lds + (present ^ 1) * T::kBytes + T::kKeyBytes);
       uint32_t bad = 0;
       for (int i = lane; i < T::kValueBytes / 16; i += 64) {
@@ -460,7 +506,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         __syncthreads();
       }
     }
-    if (more && !whole()) clear_values<D>(st, ld, w.end_last);
+    if (more && !whole()) clear_values<D>(st, ld, w.length);
     __builtin_amdgcn_s_setprio(3);
     products<D / 8>([&](int i) { return value(i / (D / 16), i % (D / 16)); },
                     [&](int i, V8 a) {
@@ -480,19 +526,17 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   if (begin < end) {
     ask(entries, pages, ld, begin * kKeys);
     fetch<D, WHOLE>(st, c, entries, keys, values, ld, begin * kKeys);
-    if (!whole()) clear_values<D>(st, ld, w.end_last);
+    if (!whole()) clear_values<D>(st, ld, w.length);
     ask(entries, pages, ld, (begin + 1) * kKeys);
     store_keys<D>(st, lds, ld);
     store_values<D>(st, lds, ld);
   }
   // (The queries are here now: else the first products of every tile would wait for whatever was asked for last, which
-  // is the next tile: 2 x 2k of 13k 755 us, 733 so.  At 64 channels that wait does no harm: 104 us, 109 so.)
-  if constexpr (D == 128) {
+  // is the next tile: 2 x 2k of 13k 755 us, 733 so; 4 x 1k of 4k at 64 channels 66.9, 64.0 so.)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(frag[n][k]));
-    }
+    for (int k = 0; k < D / 32; ++k) asm volatile("" : "+v"(frag[n][k]));
   }
   __syncthreads();
   if (threadIdx.x == 0) bad = 0;  // (the last unit's has been read; a barrier a tile lies before this one's is written)
@@ -500,39 +544,43 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
   while (!search && t < end && whole()) step(std::false_type());
   while (t < end) step(std::true_type());
 
+  const Args x = arguments(given);
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
     const float total = mf::sum_over_slices(acc[n].l);
     add_infinite(acc[n].o, infinite[n]);
     if (r >= w.rows) continue;
+    if (total == 0.0f && acc[n].m == mf::kNegInf) {
+      acc[n].m = no_reference(x.c, w.s, begin * kKeys, row_end[n] < end * kKeys ? row_end[n] : end * kKeys);
+    }
     if (spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total)) bad = 1;
     if (walk.part()) {
-      const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;
+      const int64_t slot = int64_t(walk.slot(own_run(x.p))) * kTileRows + rr;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(part + slot * D + 16 * d + 4 * quad) = acc[n].o[d];
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<Global<f4> *>(global(x.part + slot * D + 16 * d + 4 * quad)) = acc[n].o[d];
       if (quad == 0) {
-        stat[2 * slot] = acc[n].m;
-        stat[2 * slot + 1] = total;
+        global(x.stat)[2 * slot] = acc[n].m;
+        global(x.stat)[2 * slot + 1] = total;
       }
     } else {
-      const int32_t token = token_of(q, r), h = w.h * q.group + r - token * q.group;
+      const int32_t token = token_of(x.q, r), h = w.h * x.q.group + r - token * x.q.group;
       const bool none = token >= w.count || (total == 0.0f && acc[n].m == mf::kNegInf);
       const float f = none ? 0.0f : 1.0f / total;
-      uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + h) * D + 4 * quad;
+      uint16_t *dst = x.out + ((int64_t(w.s) * x.q.len + token) * x.q.heads + h) * D + 4 * quad;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         const f4 y = none ? f4{0, 0, 0, 0} : acc[n].o[d] * f;
-        *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+        *reinterpret_cast<Global<u2> *>(global(dst + 16 * d)) = u2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
       }
-      if (quad == 0 && lse != nullptr) {
-        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
+      if (quad == 0 && x.lse != nullptr) {
+        global(x.lse)[(int64_t(w.s) * x.q.heads + h) * x.q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
       }
     }
   }
   __syncthreads();
   search = __builtin_amdgcn_readfirstlane(bad) != 0 && !search;
-  if (!search) walk.next(c, q, p);
+  if (!search) walk.next(x.c, x.q, x.p);
   }
 }
 
@@ -585,14 +633,18 @@ int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, 
                  float *lse, float *part, float *stat, hipStream_t stream) {
   const int32_t units = c.sequences * c.heads * p.groups;
   const dim3 grid(static_cast<uint32_t>(p.workgroups > 0 ? p.workgroups : units));
-  auto go = [&](auto kernel, dim3 workgroups) {
+  auto tiles = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, Args{c, q, p, out, lse, part, stat});
+    return check_launch(what);
+  };
+  auto join = [&](auto kernel, dim3 workgroups) {
     hipLaunchKernelGGL(kernel, workgroups, dim3(256), 0, stream, c, q, p, out, lse, part, stat);
     return check_launch(what);
   };
   auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
-    const int rc = c.page >= kKeys ? go(tile_kernel<D, DT, true>, grid) : go(tile_kernel<D, DT, false>, grid);
-    return rc != UC_OK || p.workgroups == 0 ? rc : go(tile_join_kernel<D, DT>, dim3(units, kTileRows / 16));
+    const int rc = c.page >= kKeys ? tiles(tile_kernel<D, DT, true>) : tiles(tile_kernel<D, DT, false>);
+    return rc != UC_OK || p.workgroups == 0 ? rc : join(tile_join_kernel<D, DT>, dim3(units, kTileRows / 16));
   };
   auto by_type = [&](auto d_tag) {
     return dtype == UC_FP16 ? run(d_tag, std::integral_constant<int, UC_FP16>()) : run(d_tag, std::integral_constant<int, UC_BF16>());
