@@ -1017,6 +1017,13 @@ def test_logits_that_all_overflow_downwards_give_nan(device, hq, lq, d):
             want, size = value[3, :300, 0].double().mean(0), value[3, :300, 0].double().abs().mean(0)
             assert ((out[3].double().cpu() - want).abs() <= EPS[q.dtype] * (want.abs() + size) + 2.0 ** -14 * size).all()
             assert ((lse[3] - math.log(300)).abs() <= 2.0 ** -18).all()
+    # the one in range may lie as low as fp32 goes
+    cache.key.mul_(4)
+    cache.key[0, table[2, 650 // b], :, 650 % b] = -1.125
+    out, lse = cache.attention(q, sm_scale=2.9e38 / (1.125 * d * math.log2(math.e)))
+    want = value[2, 650, 0].double()
+    assert ((out[2].double().cpu() - want).abs() <= 2 * EPS[q.dtype] * want.abs()).all()
+    assert ((lse[2] / (-2.9e38 * math.log(2)) - 1).abs() <= 2.0 ** -18).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -1121,3 +1128,37 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(device, dtype, 
             assert (got[..., 11] == math.inf).all() and (got[..., 12] == -math.inf).all()
             others = [c for c in range(d) if not 7 <= c <= 12]
             assert torch.equal(out[s][..., others], want[s][..., others])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,lq", [(1, 1), (3, 9), (4, 40)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_logits_whose_steps_pass_one_take_the_largest(device, dtype, hq, lq, d):
+    """Logits so large that fp32 holds them in steps above 1: those that are the largest share the weight, whichever way they, the
+    scale and the reference were rounded."""
+
+    lengths, b = [40, 700], 16
+    cache, k, v = filled(lengths, hkv=1, d=d, b=b, dtype=dtype)
+    table = cache.table.cpu()
+    q = torch.full((2, lq, hq, d), 64.0, dtype=dtype, device=device)
+    for sign in (1.0, -1.0):
+        for s, n in enumerate(lengths):
+            # a key's channels are all alike, so that products and sums are exact: d * 64 * size
+            sizes = sign * (torch.arange(n) * 7 % 31 + 32.0)
+            for i in range(-(-n // b)):
+                r = min(b, n - i * b)
+                cache.key[0, table[s, i], :, :r] = sizes[i * b:i * b + r].to(dtype)[:, None].cuda()
+        for scale in (300.0, 4000.0, 4321.0, 33333.0, 5e5, 7.7e5, 3.3e9, 1.7e17, 2.9e30):
+            for hint in (1, 700):
+                cache.max_tokens = hint
+                out, lse = cache.attention(q, sm_scale=scale)
+                for s, n in enumerate(lengths):
+                    sizes = sign * (torch.arange(n) * 7 % 31 + 32.0)
+                    at = sizes == sizes.max()
+                    top = v[s, :n, 0][at].double()
+                    want, size = top.mean(0), top.abs().mean(0)
+                    # equal weights, each rounded the same way, the sum's terms and the output's rounding
+                    tol = EPS[dtype] * (want.abs() + size) + 2.0 ** -14 * size
+                    assert ((out[s].double().cpu() - want).abs() <= tol).all(), (sign, scale)
+                    x = d * 64.0 * float(sizes.max()) * float(torch.tensor(scale, dtype=torch.float32))
+                    assert ((lse[s].double() - x - math.log(int(at.sum()))).abs() <= 2.0 ** -21 * abs(x)).all()

@@ -128,7 +128,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // row sees them its weight may have been rounded to 0, or be two numbers of which one is 0 or negative.  So where there are
 // any the products take 0 in their place, and others count, for each row, the keys that it does see of each kind; one is
 // enough to make the sum what it is.  Tiles that some rows see in part are searched for them; the others only when a sum is no number
-// at the end, in a second pass over all tiles.
+// at the end, in a second pass over all tiles, each searched.
 template <int DT>
 constexpr uint32_t kInfinity = DT == UC_FP16 ? 0x7c00u : 0x7f80u;
 
@@ -196,6 +196,27 @@ __device__ __forceinline__ bool spoiled(At at, float l) {
 #pragma unroll
   for (int j = 0; j < N; ++j) top = __builtin_elementwise_maximum(top, __builtin_fabsf(at(j)));  // (passes NaN on)
   return !(top < __builtin_huge_valf()) && l < __builtin_huge_valf();
+}
+
+// Logits in base 2 are products s factor, fused with the reference m taken off: s factor is not rounded, while m was made of the
+// largest one rounded.  So x of the largest is off by half a step of either, one at most up to kFar; beyond, weights
+// would leave what 16 bits hold.  Where a reference lies there, all is done in a second pass too, in which
+// such rows' products are rounded first: they are replaced by x.
+constexpr float kFar = 0x1p24f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && fabsf(m) < __builtin_huge_valf(); }
+template <int N>
+__device__ __forceinline__ void round_far(f4 (&s)[N], float &factor, float &m) {
+  const bool far = is_far(m);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float product = s[j][i] * factor;
+      s[j][i] = far ? product - m : s[j][i];
+    }
+  }
+  factor = far ? 1.0f : factor;
+  m = far ? 0.0f : m;
 }
 
 // A part's sum as it joins others: where it is not finite it stays so, however small the factor.

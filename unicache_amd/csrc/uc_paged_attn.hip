@@ -90,7 +90,7 @@ struct Acc {
 };
 
 template <int D, int DT, bool MASK>
-__device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], float factor, int32_t seen,
+__device__ __forceinline__ void softmax_step(Acc<D> &acc, f4 (&s)[2], float factor, int32_t seen, bool again,
                                              typename Half<DT>::V8 &high, typename Half<DT>::V8 &low) {
   typedef typename Half<DT>::T T;
   float top = mf::kNegInf;
@@ -100,16 +100,17 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, const f4 (&s)[2], floa
     top = fmaxf(top, MASK && j >= seen ? mf::kNegInf : x);
   }
   top = mf::max_over_slices(top * factor);
-  if (__any(top > acc.m + kRaise)) {
+  if (__any(top - acc.m > kRaise)) {
     // (of the rows that ask for it: no row's last bits hang on what only another one sees)
-    const float m = top > acc.m + kRaise ? top - kHead : acc.m;
+    const float m = top - acc.m > kRaise ? top - kHead : acc.m;
     const float alpha = acc.m == mf::kNegInf ? 0.0f : mf::fast_exp2(acc.m - m);
     acc.m = m;
     acc.l *= alpha;
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) acc.o[n] *= alpha;
   }
-  const float m = acc.m == mf::kNegInf ? 0.0f : acc.m;
+  float m = acc.m == mf::kNegInf ? 0.0f : acc.m;
+  if (MASK && __builtin_expect(again, false)) round_far(s, factor, m);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = __builtin_fmaf(s[j / 4][j % 4], factor, -m);
@@ -126,12 +127,13 @@ struct Joined {
   static constexpr bool kHeld = NR * D >= 192;
   float o[4][16][D + 4];  // (a wave's part holds a tile's values, 8 D / 32 dwords a lane)
   float m[4][16], l[4][16];
-  uint32_t bad;  // whether sums are not finite, though their weights are
+  uint32_t bad;  // whether a second pass is asked for
   typename Half<DT>::V8 frag[kHeld ? NR * D / 32 : 1][64];
 };
 
 // Steps begin .. end - 1 of the rows w, by a whole workgroup.  slot >= 0: the part goes there; else it
-// is all there is, and the rows are finished.  Returns whether values that are not finite went into sums: then once more with `search`.
+// is all there is, and the rows are finished.  Returns whether values that are not finite went into sums, or a reference lies far off:
+// then once more with `search`.
 template <int D, int DT, int NR>
 __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows &w, int32_t begin, int32_t end, int32_t slot,
                                       bool search, Joined<D, DT, NR> &joined, uint16_t *out, float *lse, float *part,
@@ -223,7 +225,7 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
     V8 high[NR], low[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, high[n], low[n]);
+      softmax_step<D, DT, MASK>(acc[n], s[n], q.scale, there ? row_end[n] - mine : 0, search, high[n], low[n]);
     }
     if constexpr (MASK) {
       // what no row sees is no value
@@ -296,6 +298,7 @@ __device__ __forceinline__ bool piece(const Cache &c, const Query &q, const Rows
 #pragma unroll
   for (int n = 0; n < NR; ++n) {
     const float l_row = mf::sum_over_slices(acc[n].l);
+    bad |= is_far(acc[n].m);
     add_infinite(acc[n].o, infinite[n]);
     __syncthreads();  // what was joined before, and its flag, have been read
     if (n == 0 && threadIdx.x == 0) joined.bad = 0;
@@ -408,10 +411,11 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   bool search = false;
   while (at < stop) {
     const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
-    // Of 64 rows it is opaque, so that what their numbers give is worked out for each piece: held across pieces it takes registers
-    // that the tiles spill (16 x 8 tokens of 4k at 64 channels 27.1 us, 26.4 so; of 48 rows 21.2 held, 21.7 so).
+    // Where registers are short the row's number is opaque, so that what it gives is worked out for each piece: held across
+    // pieces the tiles spill for it (8 x 4 tokens of 16k at 128 channels 51.9 us, 49.9 so; 16 x 8 of 4k at 64 27.1, 26.4
+    // so; but 16 x 5, 48 rows, 21.2 held, 21.7 so).
     int32_t only = 0;
-    if constexpr (NR == 4) asm volatile("" : "+s"(only));
+    if constexpr (NR * D >= 256) asm volatile("" : "+s"(only));
     const Rows w = rows_at(q, s, n, only, 16 * NR, __builtin_amdgcn_readlane(length, first),
                            __builtin_amdgcn_readlane(count, first));
     const int32_t slot = end - t == now ? -1 : g + s * each + n;

@@ -175,9 +175,9 @@ __device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], floa
     top = fmaxf(top, MASK && j % 8 >= seen[j / 8] ? mf::kNegInf : x);
   }
   top = mf::max_over_slices(top * factor);
-  if (__any(top > acc.m + kRaise)) {
+  if (__any(top - acc.m > kRaise)) {
     // (of the rows that ask for it: no row's last bits hang on what only another one sees)
-    const float m = top > acc.m + kRaise ? top - kHead : acc.m;
+    const float m = top - acc.m > kRaise ? top - kHead : acc.m;
     const float alpha = acc.m == mf::kNegInf ? 0.0f : mf::fast_exp2(acc.m - m);
     acc.m = m;
     acc.l *= alpha;
@@ -317,52 +317,14 @@ struct Walk {
   __device__ __forceinline__ int32_t slot(int32_t run) const { return slot_of(run, first); }
 };
 
-struct Args {
-  Cache c;
-  Query q;
-  Plan p;
-  uint16_t *out;
-  float *lse, *part, *stat;
-};
-
-// The kernel's arguments, read anew: what only a unit's beginning or end asks for takes no scalar registers from the tiles between.
-// (Held throughout they pass the 102 that there are, and the tiles read some back from vector registers one at a time: 2 x 2k of
-// 13k 730 us, 720 so; of 9k at 64 channels 219, 208 so.)  What is loaded from stays as given: the compiler knows it for global
-// memory only so, and flat loads count as LDS reads too (790 us).
-__device__ __forceinline__ Args arguments(const Args &given) {
-  struct Words {
-    uint32_t w[sizeof(Args) / 4];
-  } words;
-  typedef const __attribute__((address_space(4))) uint32_t *Scalars;
-  Scalars p = (Scalars)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(p));
-#pragma unroll
-  for (size_t i = 0; i < sizeof(Args) / 4; ++i) words.w[i] = p[i];
-  Args a = __builtin_bit_cast(Args, words);
-  a.c.key = given.c.key;
-  a.c.value = given.c.value;
-  a.c.table = given.c.table;
-  a.c.lengths = given.c.lengths;
-  a.q.p = given.q.p;
-  a.q.lens = given.q.lens;
-  return a;
-}
-
-// A pointer to global memory, for stores through what was read anew.
-template <class T>
-using Global = __attribute__((address_space(1))) T;
-template <class T>
-__device__ __forceinline__ Global<T> *global(T *p) {
-  return (Global<T> *)p;
-}
-
 template <int D, int DT, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
+__global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, uint16_t *out, float *lse, float *part,
+                                                      float *stat) {
   typedef Tile<D> T;
   typedef Half<DT> H;
   typedef typename H::V8 V8;
   __shared__ __attribute__((aligned(16))) char lds[2 * T::kBytes];
-  __shared__ uint32_t bad;  // whether sums are not finite, though their weights are: the unit's tiles once more, each searched
+  __shared__ uint32_t bad;  // whether a second pass over the unit's tiles is asked for
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, quad = lane >> 4;
   // Two waves share a SIMD, in slots that differ in their last bit (HW_ID's first four bits).
   // One goes before the other in its vector phases, so that they do not reach the matrix cores together.
@@ -375,21 +337,13 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
     }
   };
   // Workgroups go to the 8 XCDs in turn; an XCD takes runs that follow each other, so that its L2 holds the keys of few heads.
-  auto own_run = [&](const Plan &p) -> int32_t {
-    return p.workgroups == 0 ? blockIdx.x : (blockIdx.x & 7) * (p.workgroups / 8) + (blockIdx.x >> 3);
-  };
-  Walk walk = [&] {
-    const Args x = arguments(given);
-    return Walk(x.c, x.q, x.p, own_run(x.p));
-  }();
+  const int32_t run = p.workgroups == 0 ? blockIdx.x : (blockIdx.x & 7) * (p.workgroups / 8) + (blockIdx.x >> 3);
+  Walk walk(c, q, p, run);
   const Loader<D> ld;
   const int krow = (col >> 2) * 8 + (col & 3);
   bool search = false;
   while (walk.more()) {
-  const Args unit = arguments(given);
-  const Cache &c = unit.c;
-  const Query &q = unit.q;
-  const Rows w = walk.rows(c, q, unit.p);
+  const Rows w = walk.rows(c, q, p);
   const int32_t begin = walk.begin, end = walk.end;
   Pages pages(c, w.s);
   const int64_t head = int64_t(w.h << c.shift) * D;
@@ -462,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
     ask(entries, pages, ld, (t + 2) * kKeys);
     __builtin_amdgcn_sched_barrier(0);
     V8 pr[2][2];
-    float m[2];
+    float m[2], factor[2] = {q.scale, q.scale};
     int32_t seen[2][2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -472,10 +426,17 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
         if (MASK && ((absent >> (2 * h + (quad >> 1))) & 1) != 0) seen[n][h] = 0;
       }
       m[n] = reference<D, MASK>(acc[n], s[n], q.scale, seen[n]);
+      if (MASK && __builtin_expect(search, false)) round_far(s[n], factor[n], m[n]);
     }
     auto weigh = [&](int h) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) acc[n].l = weights<DT, MASK>(s[n], h, q.scale, m[n], seen[n][h], acc[n].l, pr[n][h]);
+      for (int n = 0; n < 2; ++n) {
+        // (opaque, so that the comparisons are made again: held since the maximum was found they take 64 scalar registers, for which
+        // the whole tiles' addresses were read back from vector registers every time: 2 x 2k of 13k 719 us, 704 so,
+        // of 9k at 64 channels 217, 188 so)
+        if (MASK) asm volatile("" : "+v"(seen[n][h]));
+        acc[n].l = weights<DT, MASK>(s[n], h, factor[n], m[n], seen[n][h], acc[n].l, pr[n][h]);
+      }
     };
     weigh(0);
     weigh(1);
@@ -532,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
     store_values<D>(st, lds, ld);
   }
   // (The queries are here now: else the first products of every tile would wait for whatever was asked for last, which
-  // is the next tile: 2 x 2k of 13k 755 us, 733 so; 4 x 1k of 4k at 64 channels 66.9, 64.0 so.)
+  // is the next tile: 2 x 2k of 13k 755 us, 733 so; 4 x 1k of 4k at 64 channels 64.5, 61.0 so.)
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
 #pragma unroll
@@ -544,7 +505,6 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
   while (!search && t < end && whole()) step(std::false_type());
   while (t < end) step(std::true_type());
 
-  const Args x = arguments(given);
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
     const int32_t rr = wave * 32 + n * 16 + col, r = w.r0 + rr;
@@ -552,35 +512,35 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Args given) {
     add_infinite(acc[n].o, infinite[n]);
     if (r >= w.rows) continue;
     if (total == 0.0f && acc[n].m == mf::kNegInf) {
-      acc[n].m = no_reference(x.c, w.s, begin * kKeys, row_end[n] < end * kKeys ? row_end[n] : end * kKeys);
+      acc[n].m = no_reference(c, w.s, begin * kKeys, row_end[n] < end * kKeys ? row_end[n] : end * kKeys);
     }
-    if (spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total)) bad = 1;
+    if (is_far(acc[n].m) || spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total)) bad = 1;
     if (walk.part()) {
-      const int64_t slot = int64_t(walk.slot(own_run(x.p))) * kTileRows + rr;
+      const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<Global<f4> *>(global(x.part + slot * D + 16 * d + 4 * quad)) = acc[n].o[d];
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f4 *>(part + slot * D + 16 * d + 4 * quad) = acc[n].o[d];
       if (quad == 0) {
-        global(x.stat)[2 * slot] = acc[n].m;
-        global(x.stat)[2 * slot + 1] = total;
+        stat[2 * slot] = acc[n].m;
+        stat[2 * slot + 1] = total;
       }
     } else {
-      const int32_t token = token_of(x.q, r), h = w.h * x.q.group + r - token * x.q.group;
+      const int32_t token = token_of(q, r), h = w.h * q.group + r - token * q.group;
       const bool none = token >= w.count || (total == 0.0f && acc[n].m == mf::kNegInf);
       const float f = none ? 0.0f : 1.0f / total;
-      uint16_t *dst = x.out + ((int64_t(w.s) * x.q.len + token) * x.q.heads + h) * D + 4 * quad;
+      uint16_t *dst = out + ((int64_t(w.s) * q.len + token) * q.heads + h) * D + 4 * quad;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         const f4 y = none ? f4{0, 0, 0, 0} : acc[n].o[d] * f;
-        *reinterpret_cast<Global<u2> *>(global(dst + 16 * d)) = u2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+        *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
       }
-      if (quad == 0 && x.lse != nullptr) {
-        global(x.lse)[(int64_t(w.s) * x.q.heads + h) * x.q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
+      if (quad == 0 && lse != nullptr) {
+        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
       }
     }
   }
   __syncthreads();
   search = __builtin_amdgcn_readfirstlane(bad) != 0 && !search;
-  if (!search) walk.next(x.c, x.q, x.p);
+  if (!search) walk.next(c, q, p);
   }
 }
 
@@ -633,18 +593,14 @@ int launch_tiles(const char *what, int dtype, int64_t head_dim, const Cache &c, 
                  float *lse, float *part, float *stat, hipStream_t stream) {
   const int32_t units = c.sequences * c.heads * p.groups;
   const dim3 grid(static_cast<uint32_t>(p.workgroups > 0 ? p.workgroups : units));
-  auto tiles = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, Args{c, q, p, out, lse, part, stat});
-    return check_launch(what);
-  };
-  auto join = [&](auto kernel, dim3 workgroups) {
+  auto go = [&](auto kernel, dim3 workgroups) {
     hipLaunchKernelGGL(kernel, workgroups, dim3(256), 0, stream, c, q, p, out, lse, part, stat);
     return check_launch(what);
   };
   auto run = [&](auto d_tag, auto dt_tag) {
     constexpr int D = decltype(d_tag)::value, DT = decltype(dt_tag)::value;
-    const int rc = c.page >= kKeys ? tiles(tile_kernel<D, DT, true>) : tiles(tile_kernel<D, DT, false>);
-    return rc != UC_OK || p.workgroups == 0 ? rc : join(tile_join_kernel<D, DT>, dim3(units, kTileRows / 16));
+    const int rc = c.page >= kKeys ? go(tile_kernel<D, DT, true>, grid) : go(tile_kernel<D, DT, false>, grid);
+    return rc != UC_OK || p.workgroups == 0 ? rc : go(tile_join_kernel<D, DT>, dim3(units, kTileRows / 16));
   };
   auto by_type = [&](auto d_tag) {
     return dtype == UC_FP16 ? run(d_tag, std::integral_constant<int, UC_FP16>()) : run(d_tag, std::integral_constant<int, UC_BF16>());
