@@ -514,7 +514,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     if (total == 0.0f && acc[n].m == mf::kNegInf) {
       acc[n].m = no_reference(c, w.s, begin * kKeys, row_end[n] < end * kKeys ? row_end[n] : end * kKeys);
     }
-    if (is_far(acc[n].m) || spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total)) bad = 1;
+    if (row_end[n] > 0 && (is_far(acc[n].m) || spoiled<D / 4>([&](int j) { return acc[n].o[j / 4][j % 4]; }, total))) bad = 1;
     if (walk.part()) {
       const int64_t slot = int64_t(walk.slot(run)) * kTileRows + rr;
 #pragma unroll
