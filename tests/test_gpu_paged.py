@@ -1162,3 +1162,22 @@ def test_logits_whose_steps_pass_one_take_the_largest(device, dtype, hq, lq, d):
                     assert ((out[s].double().cpu() - want).abs() <= tol).all(), (sign, scale)
                     x = d * 64.0 * float(sizes.max()) * float(torch.tensor(scale, dtype=torch.float32))
                     assert ((lse[s].double() - x - math.log(int(at.sum()))).abs() <= 2.0 ** -21 * abs(x)).all()
+
+
+@pytest.mark.parametrize("hq,lq", [(3, 5), (4, 40)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_log_sum_exp_is_rounded_once(device, hq, lq, d):
+    """One key a row, whose product with the query fp32 holds exactly: what is left are the logarithm's last rounding and, of the
+    weight, a few units of numbers below 16."""
+
+    cache, _, _ = filled([1] * 8, hkv=1, d=d, b=16)
+    g = torch.Generator().manual_seed(d)
+    k = torch.randint(-8, 9, (8, d), generator=g)
+    q = torch.randint(-8, 9, (8, lq, hq, d), generator=g) * 64
+    for s in range(8):
+        cache.key[0, int(cache.table[s, 0]), 0, 0] = k[s].to(torch.bfloat16).cuda()
+    product = torch.einsum("slhd,sd->shl", q.double(), k.double())
+    for scale in (0.07, 0.1, 1 / math.sqrt(128), 0.77):
+        _, lse = cache.attention(q.to(torch.bfloat16).cuda(), sm_scale=scale)
+        want = product * float(torch.tensor(scale, dtype=torch.float32))
+        assert ((lse.double().cpu() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -19).all()

@@ -23,6 +23,7 @@ struct Query {
   int32_t len, heads, group;
   int32_t causal;
   float scale;  // sm_scale * log2(e)
+  float unit, unit_rest;  // what a unit of the scaled products is in natural logarithms, sm_scale / scale, and what rounding left of it
   FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const { return lens == nullptr ? len : clamped(lens[s]); }
@@ -240,9 +241,11 @@ __device__ __forceinline__ float no_reference(const Cache &c, int32_t s, int32_t
   return mf::kNegInf;
 }
 
-// The log-sum-exp of a row that sees keys (a sum of 0 is of logits below fp32's range).
-__device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.0f ? __builtin_nanf("") : kLn2 * (m + __builtin_amdgcn_logf(l));
+// The log-sum-exp of a row that sees keys (a sum of 0 is of logits below fp32's range), rounded once: the scale's own rounding and
+// that of a sum with m would each be as much again.
+__device__ __forceinline__ float lse_of(const Query &q, float m, float l) {
+  const float rest = __builtin_fmaf(m, q.unit_rest, kLn2 * __builtin_amdgcn_logf(l));
+  return l == 0.0f ? __builtin_nanf("") : __builtin_fmaf(m, q.unit, rest);
 }
 
 // D / 16 channels of a finished row.
@@ -263,7 +266,7 @@ __device__ __forceinline__ void store_row(const Query &q, const Rows &w, int32_t
     *reinterpret_cast<uint2 *>(dst) = uint2{v[0], v[1]};
   }
   if (c0 == 0 && lse != nullptr) {
-    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : lse_of(m, l);
+    lse[(int64_t(w.s) * q.heads + head) * q.len + t] = none ? mf::kNegInf : lse_of(q, m, l);
   }
 }
 

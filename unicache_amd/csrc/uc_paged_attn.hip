@@ -571,7 +571,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   const int64_t group = query->heads_q / cache->heads_kv, rows = group * query->query_len;
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
-            query->causal != 0, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
+            query->causal != 0, 0.0f, 0.0f, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
   p.rows = rows <= 64 ? static_cast<int32_t>(ceil_div(rows, int64_t(16))) * 16 : kTileRows;
   if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
@@ -638,6 +638,9 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
                            workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "%s: workspace too small", what);
   q.scale = sm_scale * kLog2e;
+  const double unit = static_cast<double>(sm_scale) / static_cast<double>(q.scale);
+  q.unit = static_cast<float>(unit);
+  q.unit_rest = static_cast<float>(unit - static_cast<double>(q.unit));
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);

@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
         *reinterpret_cast<uint2 *>(dst + 16 * d) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
       }
       if (quad == 0 && lse != nullptr) {
-        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : lse_of(acc[n].m, total);
+        lse[(int64_t(w.s) * q.heads + h) * q.len + token] = none ? mf::kNegInf : lse_of(q, acc[n].m, total);
       }
     }
   }
