@@ -23,7 +23,7 @@ struct Query {
   int32_t len, heads, group;
   int32_t causal;
   float scale;  // sm_scale * log2(e)
-  float unit, unit_rest;  // what a unit of the scaled products is in natural logarithms, sm_scale / scale, and what rounding left of it
+  float unit;   // sm_scale / scale - ln2: what rounding made of a unit of the scaled products in natural logarithms
   FastDiv by_group;
 
   __device__ __forceinline__ int32_t count(int32_t s) const { return lens == nullptr ? len : clamped(lens[s]); }
@@ -244,8 +244,8 @@ __device__ __forceinline__ float no_reference(const Cache &c, int32_t s, int32_t
 // The log-sum-exp of a row that sees keys (a sum of 0 is of logits below fp32's range), rounded once: the scale's own rounding and
 // that of a sum with m would each be as much again.
 __device__ __forceinline__ float lse_of(const Query &q, float m, float l) {
-  const float rest = __builtin_fmaf(m, q.unit_rest, kLn2 * __builtin_amdgcn_logf(l));
-  return l == 0.0f ? __builtin_nanf("") : __builtin_fmaf(m, q.unit, rest);
+  const float rest = __builtin_fmaf(m, q.unit, kLn2 * __builtin_amdgcn_logf(l));
+  return l == 0.0f ? __builtin_nanf("") : __builtin_fmaf(m, kLn2, rest);
 }
 
 // D / 16 channels of a finished row.

@@ -96,8 +96,8 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, f4 (&s)[2], float fact
   float top = mf::kNegInf;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float x = s[j / 4][j % 4];
-    top = fmaxf(top, MASK && j >= seen ? mf::kNegInf : x);
+    if (MASK) s[j / 4][j % 4] = j >= seen ? mf::kNegInf : s[j / 4][j % 4];  // (its weight is 0 then)
+    top = fmaxf(top, s[j / 4][j % 4]);
   }
   top = mf::max_over_slices(top * factor);
   if (__any(top - acc.m > kRaise)) {
@@ -114,7 +114,7 @@ __device__ __forceinline__ void softmax_step(Acc<D> &acc, f4 (&s)[2], float fact
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float x = __builtin_fmaf(s[j / 4][j % 4], factor, -m);
-    const float e = MASK && j >= seen ? 0.0f : mf::fast_exp2(x);
+    const float e = mf::fast_exp2(x);
     acc.l += e;
     high[j] = static_cast<T>(e);
     low[j] = static_cast<T>(e - static_cast<float>(high[j]));
@@ -412,10 +412,10 @@ __global__ __launch_bounds__(256, D == 128 && NR > 2 ? 1 : 2) void rows_kernel(C
   while (at < stop) {
     const int32_t end = now - t < stop - at ? now : t + (stop - at), s = s0 + first;
     // Where registers are short the row's number is opaque, so that what it gives is worked out for each piece: held across
-    // pieces the tiles spill for it (8 x 4 tokens of 16k at 128 channels 51.9 us, 49.9 so; 16 x 8 of 4k at 64 27.1, 26.4
-    // so; but 16 x 5, 48 rows, 21.2 held, 21.7 so).
+    // pieces the tiles spill for it (8 x 4 tokens of 16k at 128 channels 52.6 us, 51.2 so; at 64, 16 x 8 of 4k 28.7 and 26.7,
+    // 16 x 5 21.9 and 21.7).
     int32_t only = 0;
-    if constexpr (NR * D >= 256) asm volatile("" : "+s"(only));
+    if constexpr (Joined<D, DT, NR>::kHeld) asm volatile("" : "+s"(only));
     const Rows w = rows_at(q, s, n, only, 16 * NR, __builtin_amdgcn_readlane(length, first),
                            __builtin_amdgcn_readlane(count, first));
     const int32_t slot = end - t == now ? -1 : g + s * each + n;
@@ -571,7 +571,7 @@ int make_plan(const uc_paged_cache *cache, const Cache &c, const uc_block8_query
   const int64_t group = query->heads_q / cache->heads_kv, rows = group * query->query_len;
   q = Query{static_cast<const uint16_t *>(query->query), query->q_ss, query->q_st, query->q_sh, query->query_lengths,
             static_cast<int32_t>(query->query_len), static_cast<int32_t>(query->heads_q), static_cast<int32_t>(group),
-            query->causal != 0, 0.0f, 0.0f, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
+            query->causal != 0, 0.0f, 0.0f, make_fastdiv(static_cast<uint32_t>(group))};
   p.rows = rows <= 64 ? static_cast<int32_t>(ceil_div(rows, int64_t(16))) * 16 : kTileRows;
   if (p.rows == 0) p.rows = 16;
   p.groups = static_cast<int32_t>(ceil_div(rows, int64_t(p.rows)));
@@ -638,9 +638,7 @@ extern "C" int uc_paged_attn(const uc_paged_cache *cache, int64_t layer, const u
                            workspace_bytes >= rows * (cache->head_dim + 2) * int64_t(sizeof(float))),
              "%s: workspace too small", what);
   q.scale = sm_scale * kLog2e;
-  const double unit = static_cast<double>(sm_scale) / static_cast<double>(q.scale);
-  q.unit = static_cast<float>(unit);
-  q.unit_rest = static_cast<float>(unit - static_cast<double>(q.unit));
+  q.unit = static_cast<float>(static_cast<double>(sm_scale) / static_cast<double>(q.scale) - static_cast<double>(kLn2));
   float *part = static_cast<float *>(workspace), *stat = part + rows * cache->head_dim;
   const int64_t units = cache->sequences * cache->heads_kv * p.groups;
   const int32_t q_rows = static_cast<int32_t>(cache->sequences * cache->heads_kv * q.len * q.group);

@@ -167,12 +167,12 @@ struct Acc16 {
 // The reference of 16 rows' weights, raised where one of the tile's logits asks for it.  seen[h]: keys of half h that the
 // lane's row sees, from the lane's own first on.
 template <int D, bool MASK>
-__device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], float factor, const int32_t (&seen)[2]) {
+__device__ __forceinline__ float reference(Acc16<D> &acc, f4 (&s)[4], float factor, const int32_t (&seen)[2]) {
   float top = mf::kNegInf;
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
-    const float x = s[j / 4][j % 4];
-    top = fmaxf(top, MASK && j % 8 >= seen[j / 8] ? mf::kNegInf : x);
+    if (MASK) s[j / 4][j % 4] = j % 8 >= seen[j / 8] ? mf::kNegInf : s[j / 4][j % 4];  // (its weight is 0 then)
+    top = fmaxf(top, s[j / 4][j % 4]);
   }
   top = mf::max_over_slices(top * factor);
   if (__any(top - acc.m > kRaise)) {
@@ -188,14 +188,13 @@ __device__ __forceinline__ float reference(Acc16<D> &acc, const f4 (&s)[4], floa
 }
 
 // The weights of half a tile, and the sum of all.
-template <int DT, bool MASK>
-__device__ __forceinline__ float weights(const f4 (&s)[4], int half, float factor, float m, int32_t seen, float l,
+template <int DT>
+__device__ __forceinline__ float weights(const f4 (&s)[4], int half, float factor, float m, float l,
                                          typename Half<DT>::V8 &p) {
   typedef typename Half<DT>::T T;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    float e = mf::fast_exp2(__builtin_fmaf(s[2 * half + j / 4][j % 4], factor, -m));
-    if (MASK && j >= seen) e = 0.0f;
+    const float e = mf::fast_exp2(__builtin_fmaf(s[2 * half + j / 4][j % 4], factor, -m));
     l += e;
     p[j] = static_cast<T>(e);
   }
@@ -430,13 +429,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Cache c, Query q, Plan p, 
     }
     auto weigh = [&](int h) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        // (opaque, so that the comparisons are made again: held since the maximum was found they take 64 scalar registers, for which
-        // the whole tiles' addresses were read back from vector registers every time: 2 x 2k of 13k 719 us, 704 so,
-        // of 9k at 64 channels 217, 188 so)
-        if (MASK) asm volatile("" : "+v"(seen[n][h]));
-        acc[n].l = weights<DT, MASK>(s[n], h, factor[n], m[n], seen[n][h], acc[n].l, pr[n][h]);
-      }
+      for (int n = 0; n < 2; ++n) acc[n].l = weights<DT>(s[n], h, factor[n], m[n], acc[n].l, pr[n][h]);
     };
     weigh(0);
     weigh(1);
