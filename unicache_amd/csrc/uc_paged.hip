@@ -7,7 +7,7 @@
 //
 // Copies (the rows of open pages; the kept rows of thinned sequences) are bound by HBM (the latter 5.4 TB/s over 244 MB of
 // reads and writes), the rest by latency: chains of short launches over a few kilobytes (reserve 2.3 us, a small
-// reorder 10, count, give, list and commit of thinning 3 to 8 each).
+// reorder 11, count, give, list and commit of thinning 5 to 9 each).
 #include "uc_paged.h"
 
 namespace uc {

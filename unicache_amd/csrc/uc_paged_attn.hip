@@ -17,8 +17,8 @@
 //
 // Bound by HBM: each row is read once, straight into registers, a wave's next 32 keys (16 KB at 128
 // channels) on their way while it computes on the present ones.  Of 8 sequences of 32k tokens (28/4 heads, 537 MB) both
-// launches take 98.7 us (5.4 TB/s; a large copy 5.0), of 64 ragged ones up to 8k in pages of 16 193 (5.6).
-// Small calls are two launches: 2k tokens 5.9 + 4.4 us, 16 x 5 tokens (40 rows) 15.3 + 4.6.  What they wait for
+// launches take 98.6 us (5.4 TB/s; a large copy 5.0), of 64 ragged ones up to 8k in pages of 16 194 (5.5).
+// Small calls are two launches: 2k tokens 6.0 + 4.5 us, 16 x 5 tokens (40 rows) 16.3 + 4.7.  What they wait for
 // first are the lengths, then the table, then the rows; queries ride along.
 #include "uc_paged_attn.h"
 

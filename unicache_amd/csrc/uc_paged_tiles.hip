@@ -15,8 +15,8 @@
 //
 // Bound by phases that overlap in part: at D = 128 a wave's tile is 64 MFMAs (1,024 cycles), about 190 other vector
 // instructions (32 exponentials among them) and 32 KB of LDS reads, each about 40 % of what two waves a SIMD could
-// have.  2 x 2k causal queries (32/8 heads) behind 11k tokens: 730 us, 900 TFLOP/s; 4096 of 16k not
-// causal 1,105 us, 995; a large library product reaches 1,413.
+// have.  2 x 2k causal queries (32/8 heads) behind 11k tokens: 705 to 760 us by box, up to 930
+// TFLOP/s; 4096 of 16k not causal 1,058 to 1,105 us, 995 to 1,039; a large library product reaches 1,413.
 #include "uc_paged_attn.h"
 
 #include <type_traits>

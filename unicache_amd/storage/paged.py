@@ -392,7 +392,8 @@ class PagedKVCache:
         behind a sequence's queries, get 0 and -inf.  Keys and values that a row does not
         see never reach it, whatever they hold; an infinity among the values that it does
         see is its output in that channel (NaN for two of both signs), however small the weight.
-        Rows with a logit above fp32's range, or with none but below it, are NaN."""
+        Rows with a logit above fp32's range, or with none but below it, are NaN.  bf16
+        values above 2^90 in magnitude may overflow sums."""
 
         layer = self._layer(layer)
         if sm_scale is None:
