@@ -1181,3 +1181,24 @@ def test_log_sum_exp_is_rounded_once(device, hq, lq, d):
         _, lse = cache.attention(q.to(torch.bfloat16).cuda(), sm_scale=scale)
         want = product * float(torch.tensor(scale, dtype=torch.float32))
         assert ((lse.double().cpu() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -19).all()
+
+
+@pytest.mark.parametrize("hq,lq", [(7, 6), (4, 70)])
+def test_a_far_hidden_key_changes_no_bit_of_a_row(device, hq, lq):
+    # the newest key's logits pass 2^24: its row's unit is gone over again, and the other rows come out as they were
+    lengths = [1000, 517]
+    cache, _, _ = filled(lengths, hkv=1, d=64, b=32)
+    key, table = cache.key.clone(), cache.table.cpu()
+    q = randn(2, lq, hq, 64, seed=1)
+    for s, n in enumerate(lengths):
+        key[0, table[s, (n - 1) // 32], :, (n - 1) % 32] = 1e12 * q[s, lq - 1, 0]
+    other = PagedKVCache(key, cache.value, cache.table, cache.lengths, max_tokens=1000)
+    out, lse = other.attention(q, causal=True)
+    want, want_lse = cache.attention(q, causal=True)
+    assert torch.equal(out[:, :lq - 1], want[:, :lq - 1]) and torch.equal(lse[:, :, :lq - 1], want_lse[:, :, :lq - 1])
+    # the last row's first head has all its weight there, and all of its logits' size
+    for s, n in enumerate(lengths):
+        value = cache.value[0, table[s, (n - 1) // 32], 0, (n - 1) % 32]
+        assert torch.equal(out[s, lq - 1, 0], value)
+        x = float((key[0, table[s, (n - 1) // 32], 0, (n - 1) % 32].double() * q[s, lq - 1, 0].double()).sum()) / 8
+        assert abs(float(lse[s, 0, lq - 1]) - x) <= 70 * 2.0 ** -24 * x

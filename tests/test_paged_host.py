@@ -405,3 +405,22 @@ def test_tensors_that_came_to_track_a_gradient(monkeypatch):
             cache._struct()
         with torch.no_grad():
             cache._struct()
+
+
+def test_a_replaced_tensor_is_let_go(monkeypatch):
+    import gc
+    import weakref
+
+    for name in _NAMES:
+        cache = _built(monkeypatch)
+        old = weakref.ref(getattr(cache, name))
+        setattr(cache, name, getattr(cache, name).clone())
+        gc.collect()
+        assert old() is None
+
+
+def test_dense_tokens():
+    cache = _on_host()
+    for tokens in (-1, cache.capacity + 1):
+        with pytest.raises(ValueError, match="tokens must be 0 .. 256"):
+            cache.dense(tokens=tokens)

@@ -139,6 +139,7 @@ class PagedKVCache:
         object.__setattr__(self, name, value)
         if name in _TENSORS:  # they are checked, and their C struct is made, again
             object.__setattr__(self, "_built", None)
+            object.__setattr__(self, "_reads", None)  # (which holds the tensors)
 
     @property
     def capacity(self) -> int:
